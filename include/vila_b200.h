@@ -900,6 +900,43 @@ int vila_scaled_residual_norm_rows(float* x, const void* a, int a_dtype, int64_t
                                    int b_dtype, int64_t ldb, const float* b_scale, const float* w, float eps, void* out,
                                    int out_dtype, int rows, int cols, void* stream);
 
+/* ---- Microscaled 4-bit rows ----
+ * A row is cut into blocks of 32 columns (the last one may be shorter).  A block is a scale byte b, the power of two 2^(b - 127)
+ * (255: NaN), and 32 codes of 4 bits: sign, two exponent bits, one mantissa bit, standing for 0, 0.5, 1, 1.5, 2, 3, 4, 6.
+ *   codes   [rows, 16 * blocks], blocks = ceil(cols / 32): the even column in a byte's low half, columns past the last one 0
+ *   scales  plain [rows, blocks], or tiled, the order that the products read:
+ *           [ceil(rows / 128)][2 * ceil(cols / 256)][32][4][4] bytes; row r, block j is at [r / 128][j / 4][r % 32][r / 32 % 4][j % 4],
+ *           rows and blocks past the last ones are 0
+ * Both start on 16-byte boundaries.  Unless it says plain, scales are tiled below.
+ *
+ * vila_mx4_quantize: x [rows, cols] (VILA_DT_*, row stride ldx elements) -> codes, scales.  Per block with largest magnitude m:
+ *   b = max(floor(log2 m) - 2 + 127, 0), code = x / 2^(b - 127) rounded to the nearest number, ties to the even code, +-6 beyond
+ *   6, sign kept for zeros.  A block with an infinity or a NaN: b = 255, codes 0.
+ * vila_mx4_dequantize: out[r, c] = number of the code * 2^(b - 127), rounded once to out_dtype (b = 255: NaN).
+ * vila_mx4_scales: plain <-> tiled (to_tiled 1 or 0). */
+int vila_mx4_quantize(const void* x, int x_dtype, int64_t ldx, uint8_t* codes, uint8_t* scales, int rows, int cols, void* stream);
+int vila_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, void* out, int out_dtype, int64_t ldo, int rows, int cols,
+                        void* stream);
+int vila_mx4_scales(uint8_t* plain, uint8_t* tiled, int rows, int cols, int to_tiled, void* stream);
+/* vila_mx4_linear: out[m, n] = epi(sum_k a[m, k] w[n, k] + bias[n]) in bf16, w [N, K] microscaled, fp32 sums.  a [M, K] is x (bf16,
+ * row stride ldx elements, any alignment) or, with x NULL, microscaled itself (a_codes, a_scales).  bias bf16 or NULL.  act: VILA_ACT_NONE, _GELU_TANH,
+ * _GELU_ERF, _SILU, _RELU2 or _XIELU (act_pos, act_neg); flags: one of VILA_FLAG_SWIGLU, _GEGLU, _GLU_CLAMP (act_alpha, act_limit) over interleaved weight
+ * rows as in vila_glinear, out has N / 2 columns then. */
+typedef struct vila_mx4_linear_params {
+  const void* x;
+  int64_t ldx;
+  const uint8_t* a_codes;
+  const uint8_t* a_scales;
+  const uint8_t* w_codes;
+  const uint8_t* w_scales;
+  const void* bias;
+  void* out;
+  int64_t ldo;
+  float act_alpha, act_limit, act_pos, act_neg;
+  int32_t M, N, K, act, flags;
+} vila_mx4_linear_params;
+int vila_mx4_linear(const vila_mx4_linear_params* p, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,328 @@
+"""GPU: microscaled 4-bit rows against their restatement in float64."""
+import math
+
+import pytest
+import torch
+
+from tests import mx4_reference as R
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+
+
+def rand(seed, *shape, dtype=torch.float32):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+# ---- quantisation: bit by bit -------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+@pytest.mark.parametrize("rows, cols", [(1, 1), (1, 31), (1, 32), (3, 33), (2, 255), (129, 256), (5, 257), (130, 1000), (7, 3584)])
+def test_quantise_is_the_definition(cuda, rows, cols, dtype):
+    from vila_b200 import ops
+    x = (rand(1, rows, cols) * torch.exp(2 * rand(2, 1, cols))).to(dtype)
+    codes, scales = R.quantise(x)
+    q = ops.mx4_quantize(x.to(cuda))
+    assert q.shape == (rows, cols)
+    assert torch.equal(q.codes.cpu(), codes)
+    assert torch.equal(q.scales.cpu(), R.tiled(scales, cols))       # padding rows and blocks are 0
+    got_codes, got_scales = ops.mx4_unpack(q)
+    assert torch.equal(got_codes.cpu(), codes) and torch.equal(got_scales.cpu(), scales)
+    want = R.values(codes, scales, cols)
+    assert torch.equal(ops.mx4_dequantize(q, out_dtype=torch.float32).cpu().double(), want)
+    assert torch.equal(ops.mx4_dequantize(q).cpu().double(), want)  # a 4-bit number times a power of two is a bf16 number
+
+
+def test_quantise_edges(cuda):
+    from vila_b200 import ops
+    ties = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 7.999, -0.25, -0.75, -5.0, 6.0, 4.0, -0.0, 0.0, 0.125])
+    x = torch.zeros(12, 64)
+    x[0, :16] = ties
+    x[1, :16] = ties * 2.0 ** 100
+    x[2, :16] = ties * 2.0 ** -120
+    x[3, :4] = torch.tensor([2.0 ** -149, 2.0 ** -140, 0.0, -(2.0 ** -130)])        # fp32 subnormals
+    x[4, 32:36] = torch.tensor([3.4028234e38, -3.4028234e38, 1e38, 1.0])
+    x[5, 3] = math.inf
+    x[6, 40] = math.nan
+    x[7, 3], x[7, 4] = math.nan, -math.inf
+    x[8] = 6.0
+    x[9, 0] = 2.0 ** -126
+    x[10, 0] = 2.0 ** -125
+    x[11] = -1e-45
+    codes, scales = R.quantise(x)
+    q = ops.mx4_quantize(x.to(cuda))
+    got_codes, got_scales = ops.mx4_unpack(q)
+    assert torch.equal(got_scales.cpu(), scales)
+    assert torch.equal(got_codes.cpu(), codes)
+    back = ops.mx4_dequantize(q, out_dtype=torch.float32).cpu()
+    want = R.values(codes, scales, 64).float()
+    assert torch.equal(torch.isnan(back), torch.isnan(want)) and torch.equal(back.nan_to_num(7.0), want.nan_to_num(7.0))
+    assert torch.isnan(back[5, :32]).all() and not torch.isnan(back[5, 32:]).any()
+
+
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+@pytest.mark.parametrize("gap, off", [(8, 0), (3, 0), (8, 1), (0, 3)])
+def test_quantise_views(cuda, gap, off, dtype):
+    from vila_b200 import ops
+    wide = rand(3, 70, 300 + gap + off).to(dtype)
+    x = wide[:, off:off + 300]
+    codes, scales = R.quantise(x)
+    q = ops.mx4_quantize(wide.to(cuda)[:, off:off + 300])
+    assert torch.equal(q.codes.cpu(), codes) and torch.equal(q.scales.cpu(), R.tiled(scales, 300))
+
+
+def test_quantise_broadcast_rows_no_rows_and_pack(cuda):
+    from vila_b200 import ops
+    x = rand(4, 1, 96).to(cuda)
+    q = ops.mx4_quantize(x.expand(5, 96))
+    one = R.quantise(x.cpu())
+    assert torch.equal(q.codes.cpu(), one[0].expand(5, -1)) and torch.equal(ops.mx4_unpack(q)[1].cpu(), one[1].expand(5, -1))
+    none = ops.mx4_quantize(torch.empty(0, 96, device=cuda))
+    assert none.shape == (0, 96) and ops.mx4_dequantize(none).shape == (0, 96)
+    # plain codes and scales; columns past the last one come with something in them
+    codes, scales = R.quantise(rand(5, 9, 41))
+    dirty = codes.clone()
+    dirty[:, 20] |= 0x70
+    dirty[:, 21:] = 0x55
+    kept = dirty.to(cuda)
+    p = ops.mx4_pack(kept, scales.to(cuda), 41)
+    assert torch.equal(p.codes.cpu(), codes) and torch.equal(p.scales.cpu(), R.tiled(scales, 41))
+    assert torch.equal(kept.cpu(), dirty)
+    assert torch.equal(ops.mx4_dequantize(p, out_dtype=torch.float32).cpu().double(), R.values(codes, scales, 41))
+
+
+# ---- products --------------------------------------------------------------------------------------------
+def act64(z, name, pair=None):
+    if name == "none":
+        return z
+    if name == "silu":
+        return z * torch.sigmoid(z)
+    if name == "relu2":
+        return z.clamp(min=0) ** 2
+    if name == "gelu_tanh":
+        return 0.5 * z * (1 + torch.tanh(math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3)))
+    if name == "gelu_erf":
+        return 0.5 * z * (1 + torch.erf(z / math.sqrt(2)))
+    if name == "xielu":     # act_params (0.7, 0.4)
+        return torch.where(z > 0, 0.7 * z * z + z / 2, 0.4 * (torch.exp(z.clamp(max=0)) - 1 - z) + z / 2)
+    g, u = z[:, 0::2], z[:, 1::2]
+    if name == "swiglu":
+        return g * torch.sigmoid(g) * u
+    if name == "geglu":
+        return act64(g, "gelu_tanh") * u
+    g, u = g.clamp(max=2.0), u.clamp(-2.0, 2.0)     # glu_clamp (1.5, 2.0)
+    return g * torch.sigmoid(1.5 * g) * (u + 1)
+
+
+def act_args(name):
+    from vila_b200 import ops
+    return {"none": {}, "silu": dict(act=ops.ACT_SILU), "relu2": dict(act=ops.ACT_RELU2), "gelu_tanh": dict(act=ops.ACT_GELU_TANH),
+            "gelu_erf": dict(act=ops.ACT_GELU_ERF), "xielu": dict(act=ops.ACT_XIELU, act_params=(0.7, 0.4)), "swiglu": dict(swiglu=True),
+            "geglu": dict(geglu=True), "glu_clamp": dict(glu_clamp=(1.5, 2.0))}[name]
+
+
+def check_product(got, x, w, bias, act="none"):
+    """got (bf16) against act(x w^T + bias) in float64, element by element.  Sums: a tensor-core step of 16 products truncates by
+    at most 2^-22 of the sum of magnitudes S, so does the fp32 addition behind it; with K / 16 + 8 steps dz = S (K / 16 + 8) 2^-22.
+    The activations' derivatives are at most 1.13 but for the squares (2 |z| a) and the gates (the other factor): dz enters
+    through the corners z +- dz, twice.  fp32 evaluation of the activation: 2^-20 relative; and 1 + tanh, 1 + erf and u + 1 lose up to
+    2^-22 (tanhf and erff are within 2 units of 2^-24 of a value near -1, the addition rounds once more), which the other factor,
+    z / 2 or the gate, multiplies.  Last, the rounding to bf16: 2^-8 relative."""
+    x, w = x.double().cpu(), w.double().cpu()
+    z, S = x @ w.T, x.abs() @ w.abs().T
+    if bias is not None:
+        z, S = z + bias.double().cpu(), S + bias.double().cpu().abs()
+    dz = S * ((x.shape[1] / 16 + 8) * 2.0 ** -22)
+    want = act64(z, act)
+    off = torch.zeros_like(want)
+    even = torch.zeros_like(dz)
+    even[:, 0::2] = dz[:, 0::2]
+    for a in (1, -1):
+        for b in (1, -1):
+            off = torch.maximum(off, (act64(z + a * even + b * (dz - even), act) - want).abs())
+    cancelled = torch.zeros_like(want)
+    if act in ("gelu_tanh", "gelu_erf"):
+        cancelled = z.abs() * 2.0 ** -22
+    elif act in ("geglu", "glu_clamp"):
+        cancelled = z[:, 0::2].abs() * (z[:, 1::2].abs() + 1) * 2.0 ** -22
+    bound = 2 * off + cancelled + want.abs() * (2.0 ** -8 + 2.0 ** -20) + 2.0 ** -133
+    err = (got.double().cpu() - want).abs()
+    assert got.dtype == BF and err.shape == bound.shape
+    assert (err <= bound).all(), (err / bound).max().item()
+
+
+def weight(seed, n, k, cuda, spread=0.0):
+    from vila_b200 import ops
+    w = rand(seed, n, k) / math.sqrt(k) * torch.exp(spread * rand(seed + 1, n, 1))
+    codes, scales = R.quantise(w)
+    return ops.mx4_pack(codes.to(cuda), scales.to(cuda), k), R.values(codes, scales, k)
+
+
+SIZES = [(1, 2, 32), (1, 128, 64), (1, 300, 2048), (3, 129, 95), (7, 64, 1153), (8, 1000, 512), (9, 130, 4000), (16, 256, 1024),
+         (17, 384, 300), (33, 128, 640), (64, 514, 1000), (65, 1157, 1153), (100, 640, 256), (129, 300, 2080), (200, 130, 96), (300, 770, 520),
+         (520, 258, 1056)]
+
+
+@pytest.mark.parametrize("M, N, K", SIZES)
+def test_linear(cuda, M, N, K):
+    from vila_b200 import ops
+    q, w = weight(M, N, K, cuda, spread=1.0)
+    x = (rand(7, M, K) * torch.exp(rand(8, 1, K))).to(BF)
+    bias = rand(9, N).to(BF)
+    check_product(ops.mx4_linear(x.to(cuda), q), x, w, None)
+    check_product(ops.mx4_linear(x.to(cuda), q, bias.to(cuda)), x, w, bias)
+
+
+@pytest.mark.parametrize("M, N, K", SIZES)
+def test_matmul(cuda, M, N, K):
+    from vila_b200 import ops
+    q, w = weight(M, N, K, cuda, spread=1.0)
+    x = (rand(7, M, K) * torch.exp(rand(8, 1, K))).to(BF)
+    a = ops.mx4_quantize(x.to(cuda))
+    codes, scales = R.quantise(x)
+    bias = rand(9, N).to(BF)
+    check_product(ops.mx4_matmul(a, q), R.values(codes, scales, K), w, None)
+    check_product(ops.mx4_matmul(a, q, bias.to(cuda)), R.values(codes, scales, K), w, bias)
+
+
+@pytest.mark.parametrize("M", [1, 12, 70, 300])
+@pytest.mark.parametrize("act", ["silu", "relu2", "gelu_tanh", "gelu_erf", "xielu", "swiglu", "geglu", "glu_clamp"])
+@pytest.mark.parametrize("four", [False, True])
+def test_activations(cuda, M, act, four):
+    from vila_b200 import ops
+    q, w = weight(20, 258, 320, cuda)
+    x, bias = (2 * rand(21, M, 320)).to(BF), rand(22, 258).to(BF)
+    if four:
+        got = ops.mx4_matmul(ops.mx4_quantize(x.to(cuda)), q, bias.to(cuda), **act_args(act))
+        x = R.values(*R.quantise(x), 320)
+    else:
+        got = ops.mx4_linear(x.to(cuda), q, bias.to(cuda), **act_args(act))
+    check_product(got, x, w, bias, act)
+
+
+@pytest.mark.parametrize("M", [2, 40, 300])
+@pytest.mark.parametrize("gap, off", [(8, 0), (3, 0), (8, 1), (0, 2)])
+def test_views(cuda, M, gap, off):
+    from vila_b200 import ops
+    q, w = weight(30, 200, 288, cuda)
+    wide = rand(31, M, 288 + gap + off).to(BF)
+    out = torch.full((M, 211), 7.0, dtype=BF, device=cuda)
+    got = ops.mx4_linear(wide.to(cuda)[:, off:off + 288], q, out=out[:, 5:205])
+    assert got.data_ptr() == out[:, 5:205].data_ptr()
+    check_product(got, wide[:, off:off + 288], w, None)
+    assert (out[:, :5] == 7).all() and (out[:, 205:] == 7).all()
+
+
+@pytest.mark.parametrize("M", [1, 8, 16, 50, 300])
+@pytest.mark.parametrize("four", [False, True])
+def test_scales_over_the_whole_range(cuda, M, four):
+    """blocks of one row whose sizes are 2^40 apart, rows that differ by 2^60"""
+    from vila_b200 import ops
+    N, K = 140, 512
+    sizes = torch.tensor([2.0 ** -20, 2.0 ** 20, 1.0, 2.0 ** -5]).repeat_interleave(32).repeat(K // 128)
+    rows = torch.exp2(torch.arange(N).float() % 61 - 30)
+    codes, scales = R.quantise(rand(40, N, K) * sizes * rows[:, None])
+    x = (rand(41, M, K) / sizes * torch.exp2(torch.arange(M).float() % 41 - 20)[:, None]).to(BF)
+    q, w = ops.mx4_pack(codes.to(cuda), scales.to(cuda), K), R.values(codes, scales, K)
+    if four:
+        check_product(ops.mx4_matmul(ops.mx4_quantize(x.to(cuda)), q), R.values(*R.quantise(x), K), w, None)
+    else:
+        check_product(ops.mx4_linear(x.to(cuda), q), x, w, None)
+
+
+@pytest.mark.parametrize("M", [3, 40, 300])
+@pytest.mark.parametrize("four", [False, True])
+def test_not_a_number_stays_in_its_row_and_column(cuda, M, four):
+    from vila_b200 import ops
+    N, K = 150, 416
+    codes, scales = R.quantise(rand(50, N, K))
+    scales[17, 3] = 255
+    q, w = ops.mx4_pack(codes.to(cuda), scales.to(cuda), K), R.values(codes, scales, K)
+    x = rand(51, M, K).to(BF)
+    x[1, 200] = math.nan
+    x[2, 9] = math.inf
+    got = ops.mx4_matmul(ops.mx4_quantize(x.to(cuda)), q) if four else ops.mx4_linear(x.to(cuda), q)
+    got = got.float().cpu()
+    assert torch.isnan(got[:, 17]).all() and torch.isnan(got[1]).all()
+    assert not torch.isfinite(got[2]).any()
+    rows = [m for m in range(M) if m not in (1, 2)]
+    cols = [n for n in range(N) if n != 17]
+    ref = R.values(*R.quantise(x), K) if four else x
+    check_product(got[rows][:, cols].to(BF), ref[rows], w[cols], None)
+
+
+@pytest.mark.parametrize("M", [1, 5, 30, 300])
+@pytest.mark.parametrize("four", [False, True])
+def test_same_bits_every_time_and_on_another_stream_and_in_a_graph(cuda, M, four):
+    from vila_b200 import ops
+    q, w = weight(60, 384, 1000, cuda)
+    x = rand(61, M, 1000).to(BF).to(cuda)
+    call = (lambda: ops.mx4_matmul(ops.mx4_quantize(x), q)) if four else (lambda: ops.mx4_linear(x, q))
+    first = call()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = call()
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(first, again)
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = call()
+        graphs.append((g, out))
+    x2 = rand(62, M, 1000).to(BF).to(cuda)
+    x.copy_(x2)
+    with torch.cuda.stream(side):       # both replay at once
+        side.wait_stream(torch.cuda.current_stream())
+        graphs[0][0].replay()
+    graphs[1][0].replay()
+    torch.cuda.current_stream().wait_stream(side)
+    want = call()
+    torch.cuda.synchronize()
+    assert torch.equal(graphs[0][1], want) and torch.equal(graphs[1][1], want) and not torch.equal(want, first)
+    ops.check_waits()
+
+
+def test_row_does_not_depend_on_the_rows_around_it_within_a_kernel(cuda):
+    from vila_b200 import ops
+    q, _ = weight(70, 200, 640, cuda)
+    x = rand(71, 6, 640).to(BF).to(cuda)
+    got = ops.mx4_linear(x, q)
+    x2 = x.clone()
+    x2[[0, 1, 2, 4, 5]] = 1e4
+    assert torch.equal(ops.mx4_linear(x2, q)[3], got[3])
+
+
+def test_no_rows(cuda):
+    from vila_b200 import ops
+    q, _ = weight(80, 64, 64, cuda)
+    assert ops.mx4_linear(torch.empty(0, 64, dtype=BF, device=cuda), q).shape == (0, 64)
+    assert ops.mx4_matmul(ops.mx4_quantize(torch.empty(0, 64, device=cuda)), q, swiglu=True).shape == (0, 32)
+
+
+def test_refusals(cuda):
+    from vila_b200 import ops
+    q, _ = weight(90, 65, 64, cuda)
+    x = torch.zeros(4, 64, dtype=BF, device=cuda)
+    for match, call in [
+        ("do not fit a weight", lambda: ops.mx4_linear(x[:, :32], q)),
+        ("must be torch.bfloat16", lambda: ops.mx4_linear(x.float(), q)),
+        ("must be an Mx4", lambda: ops.mx4_linear(x, x)),
+        ("consecutive columns", lambda: ops.mx4_linear(torch.zeros(64, 4, dtype=BF, device=cuda).T, q)),
+        ("even number of weight rows", lambda: ops.mx4_linear(x, q, swiglu=True)),
+        ("one gated unit", lambda: ops.mx4_linear(x, q, swiglu=True, geglu=True)),
+        ("unknown activation", lambda: ops.mx4_linear(x, q, act=ops.ACT_SOFTCAP)),
+        ("takes act_params", lambda: ops.mx4_linear(x, q, act=ops.ACT_XIELU)),
+        ("bias must be", lambda: ops.mx4_linear(x, q, torch.zeros(65, device=cuda))),
+        ("bias must be", lambda: ops.mx4_linear(x, q, torch.zeros(64, dtype=BF, device=cuda))),
+        ("out must be", lambda: ops.mx4_linear(x, q, out=torch.zeros(4, 64, dtype=BF, device=cuda))),
+        ("consecutive columns", lambda: ops.mx4_quantize(torch.zeros(64, 4, device=cuda).T)),
+        ("bfloat16 or float32", lambda: ops.mx4_quantize(torch.zeros(4, 64, device=cuda, dtype=torch.float16))),
+        ("bfloat16 or float32", lambda: ops.mx4_dequantize(q, out_dtype=torch.float16)),
+        ("scales must be", lambda: ops.mx4_pack(q.codes, torch.zeros(65, 3, dtype=torch.uint8, device=cuda), 64)),
+    ]:
+        with pytest.raises(RuntimeError, match=match):
+            call()
+    gated, _ = weight(91, 64, 64, cuda)
+    with pytest.raises(RuntimeError, match="takes no other activation"):
+        ops.mx4_linear(x, gated, swiglu=True, act=ops.ACT_SILU)

@@ -122,6 +122,15 @@ class Hgrn2Params(C.Structure):
     ]
 
 
+class Mx4LinearParams(C.Structure):
+    _fields_ = [
+        ("x", c_void_p), ("ldx", c_i64), ("a_codes", c_void_p), ("a_scales", c_void_p),
+        ("w_codes", c_void_p), ("w_scales", c_void_p), ("bias", c_void_p), ("out", c_void_p), ("ldo", c_i64),
+        ("act_alpha", c_float), ("act_limit", c_float), ("act_pos", c_float), ("act_neg", c_float),
+        ("M", C.c_int32), ("N", C.c_int32), ("K", C.c_int32), ("act", C.c_int32), ("flags", C.c_int32),
+    ]
+
+
 class GLinearExt(C.Structure):
     _fields_ = [("act_alpha", c_float), ("act_limit", c_float), ("act_pos", c_float), ("act_neg", c_float),
                 ("in_scale", c_void_p)]
@@ -347,6 +356,10 @@ SIGNATURES = {
     "vila_scaled_residual_norm_rows": [c_void_p, c_void_p, c_int, c_i64, c_void_p, c_void_p, c_int, c_i64, c_void_p,
                                        c_void_p, c_float, c_void_p, c_int, c_int, c_int, c_void_p],
     "vila_selective_scan": [C.POINTER(SelectiveScanParams), c_void_p],
+    "vila_mx4_quantize": [c_void_p, c_int, c_i64, c_void_p, c_void_p, c_int, c_int, c_void_p],
+    "vila_mx4_dequantize": [c_void_p, c_void_p, c_void_p, c_int, c_i64, c_int, c_int, c_void_p],
+    "vila_mx4_scales": [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p],
+    "vila_mx4_linear": [C.POINTER(Mx4LinearParams), c_void_p],
 }
 _RESTYPES = {"vila_last_error": C.c_char_p}
 

@@ -45,8 +45,11 @@ SOURCES = [
     "ssm.cu",
     "outer_scan.cu",
     "ssd_chunk.cu",
+    "mx4.cu",
+    "mx4_linear.cu",
+    "mx4_rows.cu",
 ]
-HEADERS = ["common.cuh", "kernels.h", "dtype_any.cuh", "glinear_epi.cuh", "paged_attn_common.cuh", "mma_bf16.cuh", "../../include/vila_b200.h"]
+HEADERS = ["common.cuh", "kernels.h", "dtype_any.cuh", "glinear_epi.cuh", "paged_attn_common.cuh", "mma_bf16.cuh", "mx4.cuh", "../../include/vila_b200.h"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

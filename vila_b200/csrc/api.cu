@@ -624,4 +624,25 @@ int vila_selective_scan(const vila_selective_scan_params* p, void* stream) {
   return vb::selective_scan(*p, st(stream));
 }
 
+int vila_mx4_quantize(const void* x, int x_dtype, int64_t ldx, uint8_t* codes, uint8_t* scales, int rows, int cols, void* stream) {
+  VB_REQUIRE_DEVICE();
+  return vb::mx4_quantize(x, x_dtype, ldx, codes, scales, rows, cols, st(stream));
+}
+
+int vila_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, void* out, int out_dtype, int64_t ldo, int rows, int cols,
+                        void* stream) {
+  VB_REQUIRE_DEVICE();
+  return vb::mx4_dequantize(codes, scales, out, out_dtype, ldo, rows, cols, st(stream));
+}
+
+int vila_mx4_scales(uint8_t* plain, uint8_t* tiled, int rows, int cols, int to_tiled, void* stream) {
+  VB_REQUIRE_DEVICE();
+  return vb::mx4_scales(plain, tiled, rows, cols, to_tiled, st(stream));
+}
+
+int vila_mx4_linear(const vila_mx4_linear_params* p, void* stream) {
+  VB_REQUIRE_DEVICE();
+  return vb::mx4_linear(*p, st(stream));
+}
+
 }  // extern "C"

@@ -284,6 +284,7 @@ struct vila_gla_scan_params;
 struct vila_decay_scan_params;
 struct vila_moe_route_params;
 struct vila_tanh_residual_params;
+struct vila_mx4_linear_params;
 namespace vb {
 int causal_conv_rows(const vila_causal_conv_params& p, cudaStream_t stream);
 int causal_conv_state(const vila_causal_conv_params& p, cudaStream_t stream);
@@ -330,5 +331,11 @@ int latent_attention(const vila_latent_attn_params& p, cudaStream_t stream);
 int latent_rope_append(const vila_latent_rope_params& p, cudaStream_t stream);
 int hgrn2_scan(const vila_hgrn2_params& p, cudaStream_t stream);
 int hgrn2_step(const vila_hgrn2_params& p, cudaStream_t stream);
+// microscaled 4-bit rows (mx4.cuh): made and read back (mx4.cu), linear layers on them (mx4_linear.cu)
+int mx4_quantize(const void* x, int dt, int64_t ldx, uint8_t* codes, uint8_t* scales, int rows, int cols, cudaStream_t stream);
+int mx4_dequantize(const uint8_t* codes, const uint8_t* scales, void* out, int dt, int64_t ldo, int rows, int cols, cudaStream_t stream);
+int mx4_scales(uint8_t* plain, uint8_t* tiled, int rows, int cols, int to_tiled, cudaStream_t stream);
+int mx4_linear(const vila_mx4_linear_params& p, cudaStream_t stream);
+int mx4_rows(const vila_mx4_linear_params& p, const vila_glinear_ext& ext, cudaStream_t stream);   // few rows (mx4_rows.cu)
 
 }  // namespace vb

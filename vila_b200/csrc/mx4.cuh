@@ -1,0 +1,58 @@
+// Microscaled 4-bit rows ("Mx4"), shared by the kernels that make and read them.
+//
+// A row is cut into blocks of 32 columns.  A block is one power of two 2^(byte - 127) and 32 numbers of 4 bits (sign, two
+// exponent bits, one mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6).
+//   codes   [rows, 16 * blocks] bytes, the even column in a byte's low half; columns past the last one are 0
+//   scales  in the order in which the tensor core wants them in TMEM, so that a stage of a product is one straight copy:
+//           [row tiles of 128][column tiles of 128, an even number][32 rows r % 32][4 row groups r / 32][4 blocks]
+//           (512 bytes a tile, a row's 4 blocks are one word).  Rows and blocks past the last ones are 0 (finite: a NaN there
+//           would meet the zeros that TMA fills in).
+#pragma once
+#include "common.cuh"
+
+namespace vb {
+
+constexpr int kMx4Block = 32;
+__host__ __device__ __forceinline__ int mx4_pitch(int cols) { return (cols + 31) / 32 * 16; }           // bytes of a row of codes
+__host__ __device__ __forceinline__ int mx4_ktiles(int cols) { return (cols + 255) / 256 * 2; }
+// where the word of row r's blocks 4 * kt .. 4 * kt + 3 starts
+__host__ __device__ __forceinline__ size_t mx4_scale_at(int r, int kt, int ktiles) {
+  return (static_cast<size_t>(r >> 7) * ktiles + kt) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4;
+}
+__host__ __device__ __forceinline__ size_t mx4_scale_bytes(int rows, int cols) {
+  return static_cast<size_t>((rows + 127) / 128) * mx4_ktiles(cols) * 512;
+}
+
+// a scale byte as a number: 2^(b - 127), 255: NaN
+__device__ __forceinline__ float mx4_scale(uint32_t b) {
+  return __uint_as_float(b == 255u ? 0x7fffffffu : (b == 0u ? 0x00400000u : b << 23));
+}
+// the two numbers of byte `i` of w as f16 (exact), the low half's first
+template <int kByte>
+__device__ __forceinline__ uint32_t mx4_pair_f16(uint32_t w) {
+  uint32_t d;
+  if (kByte == 0)
+    asm("{.reg .b8 a, b, c, e; mov.b32 {a, b, c, e}, %1; cvt.rn.f16x2.e2m1x2 %0, a;}" : "=r"(d) : "r"(w));
+  else if (kByte == 1)
+    asm("{.reg .b8 a, b, c, e; mov.b32 {a, b, c, e}, %1; cvt.rn.f16x2.e2m1x2 %0, b;}" : "=r"(d) : "r"(w));
+  else if (kByte == 2)
+    asm("{.reg .b8 a, b, c, e; mov.b32 {a, b, c, e}, %1; cvt.rn.f16x2.e2m1x2 %0, c;}" : "=r"(d) : "r"(w));
+  else
+    asm("{.reg .b8 a, b, c, e; mov.b32 {a, b, c, e}, %1; cvt.rn.f16x2.e2m1x2 %0, e;}" : "=r"(d) : "r"(w));
+  return d;
+}
+// eight numbers, already divided by their block's scale, to 4 bits each: nearest, ties to the even code, at most 6
+__device__ __forceinline__ uint32_t mx4_encode8(const float (&v)[8]) {
+  uint32_t d;
+  asm("{.reg .b8 a, b, c, e;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 e, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, e};}"
+      : "=r"(d)
+      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  return d;
+}
+
+}  // namespace vb

@@ -1250,3 +1250,155 @@ def scaled_residual_norm_rows(x: torch.Tensor, a: torch.Tensor, a_scale: torch.T
         b.stride(0) if b is not None else 0, _f32(b_scale, "b_scale"), _f32(w, "w"), eps, _p(out),
         _dt(out, "out") if out is not None else 0, rows, cols, _stream()), "vila_scaled_residual_norm_rows")
     return out
+
+
+# ---- microscaled 4-bit rows: a power of two per 32 columns, and a number of 4 bits for each ----
+class Mx4:
+    """Rows of microscaled 4-bit numbers (include/vila_b200.h has the format): codes uint8 [rows, 16 * ceil(cols / 32)] and
+    scales uint8 in the tiled order that the products read.  Made by mx4_quantize, or by mx4_pack from plain scale bytes."""
+
+    __slots__ = ("codes", "scales", "rows", "cols")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, cols: int):
+        _mx4_check(cols > 0 and codes.dim() == 2 and codes.dtype == torch.uint8 and codes.is_contiguous()
+                   and codes.shape[1] == 16 * ((cols + 31) // 32), "codes must be contiguous uint8 [rows, 16 * ceil(cols / 32)]")
+        _mx4_check(scales.dtype == torch.uint8 and scales.is_contiguous() and scales.device == codes.device
+                   and scales.numel() == _mx4_scale_bytes(codes.shape[0], cols), "scales must be contiguous uint8, in the tiled order")
+        self.codes, self.scales, self.rows, self.cols = codes, scales, codes.shape[0], cols
+
+    @property
+    def shape(self) -> Tuple[int, int]:
+        return (self.rows, self.cols)
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    @property
+    def nbytes(self) -> int:
+        return self.codes.numel() + self.scales.numel()
+
+
+def _mx4_check(ok: bool, what: str) -> None:
+    if not ok:
+        raise RuntimeError(f"vila_b200.ops: {what}")
+
+
+def _mx4_here(t: torch.Tensor, name: str) -> None:
+    """The kernels run on the current device's current stream: what they are given has to be there."""
+    if not t.is_cuda:
+        raise RuntimeError(f"vila_b200.ops: {name} must be a CUDA tensor (no CPU fallback exists)")
+    _mx4_check(t.device.index == torch._C._cuda_getDevice(), f"{name} is on {t.device}, which is not the current device")
+
+
+def _mx4_scale_bytes(rows: int, cols: int) -> int:
+    return ((rows + 127) // 128) * (2 * ((cols + 255) // 256)) * 512
+
+
+def _mx4_empty(rows: int, cols: int, device) -> Mx4:
+    return Mx4(torch.empty(rows, 16 * ((cols + 31) // 32), dtype=torch.uint8, device=device),
+               torch.empty(_mx4_scale_bytes(rows, cols), dtype=torch.uint8, device=device), cols)
+
+
+def mx4_quantize(x: torch.Tensor) -> Mx4:
+    """x [rows, cols] bf16 or fp32 (a view with a row stride is fine) -> Mx4.  Per block of 32 columns with largest magnitude m
+    the scale is 2^max(floor(log2 m) - 2, -127), and every x / scale becomes the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 (ties to
+    the even code, 6 beyond 6; signs kept).  A block with an infinity or a NaN reads as NaN."""
+    _mx4_here(x, "x")
+    _mx4_check(x.dim() == 2 and x.shape[1] > 0 and (x.stride(1) == 1 or x.shape[1] == 1), "x must be [rows, cols] with consecutive columns")
+    q = _mx4_empty(x.shape[0], x.shape[1], x.device)
+    check(_lib.load().vila_mx4_quantize(_p(x), _dt(x, "x"), x.stride(0), _p(q.codes), _p(q.scales), q.rows, q.cols, _stream()),
+          "vila_mx4_quantize")
+    return q
+
+
+def mx4_dequantize(q: Mx4, out_dtype=torch.bfloat16) -> torch.Tensor:
+    """The numbers that q stands for, [rows, cols] in bf16 or fp32."""
+    _mx4_here(q.codes, "q")
+    out = torch.empty(q.rows, q.cols, dtype=out_dtype, device=q.device)
+    check(_lib.load().vila_mx4_dequantize(_p(q.codes), _p(q.scales), _p(out), _dt(out, "out"), q.cols, q.rows, q.cols, _stream()),
+          "vila_mx4_dequantize")
+    return out
+
+
+def mx4_pack(codes: torch.Tensor, scales: torch.Tensor, cols: int) -> Mx4:
+    """codes uint8 [rows, 16 * blocks] and plain scale bytes uint8 [rows, blocks], blocks = ceil(cols / 32) (a checkpoint's) ->
+    Mx4.  The codes are kept, not copied, unless the last block is a short one: its columns past `cols` have to be 0."""
+    _mx4_here(codes, "codes")
+    _mx4_here(scales, "scales")
+    rows, blocks = codes.shape[0], (cols + 31) // 32
+    _mx4_check(cols > 0 and codes.dim() == 2 and codes.dtype == torch.uint8 and codes.shape[1] == 16 * blocks,
+               "codes must be uint8 [rows, 16 * ceil(cols / 32)]")
+    _mx4_check(scales.dtype == torch.uint8 and tuple(scales.shape) == (rows, blocks), "scales must be uint8 [rows, ceil(cols / 32)]")
+    scales = scales.contiguous()
+    if cols % 32 or not codes.is_contiguous() or codes.data_ptr() % 16:
+        codes = codes.clone(memory_format=torch.contiguous_format)
+        codes[:, (cols + 1) // 2:] = 0
+        if cols % 2:
+            codes[:, cols // 2] &= 15
+    q = Mx4(codes, torch.empty(_mx4_scale_bytes(rows, cols), dtype=torch.uint8, device=codes.device), cols)
+    check(_lib.load().vila_mx4_scales(_p(scales), _p(q.scales), rows, cols, 1, _stream()), "vila_mx4_scales")
+    return q
+
+
+def mx4_unpack(q: Mx4) -> Tuple[torch.Tensor, torch.Tensor]:
+    """-> codes uint8 [rows, 16 * blocks] (q's own) and plain scale bytes uint8 [rows, blocks]."""
+    _mx4_here(q.codes, "q")
+    plain = torch.empty(q.rows, (q.cols + 31) // 32, dtype=torch.uint8, device=q.device)
+    check(_lib.load().vila_mx4_scales(_p(plain), _p(q.scales), q.rows, q.cols, 0, _stream()), "vila_mx4_scales")
+    return q.codes, plain
+
+
+def _mx4_product(a, w: Mx4, bias, act, act_params, swiglu, geglu, glu_clamp, out) -> torch.Tensor:
+    flags = (1 if swiglu else 0) | (4 if glu_clamp is not None else 0) | (FLAG_GEGLU if geglu else 0)
+    M, N, K = a.shape[0], w.rows, w.cols
+    _mx4_here(w.codes, "w")
+    _mx4_check(act != ACT_XIELU or act_params is not None, "ACT_XIELU takes act_params")
+    _mx4_check(N > 0 and a.shape[1] == K, f"{a.shape[0]} x {a.shape[1]} rows do not fit a weight of {N} x {K}")
+    p = _lib.Mx4LinearParams()
+    if isinstance(a, Mx4):
+        _mx4_here(a.codes, "a")
+        p.a_codes, p.a_scales = _p(a.codes), _p(a.scales)
+    else:
+        p.x, p.ldx = _p(a), a.stride(0)
+    n_out = N // 2 if flags else N
+    if out is None:
+        out = torch.empty(M, n_out, dtype=torch.bfloat16, device=w.device)
+    else:
+        _chk(out, "out")
+        _mx4_here(out, "out")
+        _mx4_check(tuple(out.shape) == (M, n_out) and (out.stride(1) == 1 or n_out == 1), f"out must be [{M}, {n_out}] with consecutive columns")
+    if bias is not None:
+        _chk(bias, "bias")
+        _mx4_here(bias, "bias")
+        _mx4_check(bias.is_contiguous() and bias.numel() == N, f"bias must be contiguous [{N}]")
+    if M == 0:
+        return out
+    p.w_codes, p.w_scales, p.bias, p.out, p.ldo = _p(w.codes), _p(w.scales), _p(bias), _p(out), out.stride(0)
+    p.M, p.N, p.K, p.act, p.flags = M, N, K, act, flags
+    if glu_clamp is not None:
+        p.act_alpha, p.act_limit = float(glu_clamp[0]), float(glu_clamp[1])
+    if act_params is not None:
+        p.act_pos, p.act_neg = float(act_params[0]), float(act_params[1])
+    check(_lib.load().vila_mx4_linear(C.byref(p), _stream()), "vila_mx4_linear")
+    return out
+
+
+def mx4_linear(x: torch.Tensor, w: Mx4, bias: Optional[torch.Tensor] = None, *, act: int = ACT_NONE,
+               act_params: Optional[Tuple[float, float]] = None, swiglu: bool = False, geglu: bool = False,
+               glu_clamp: Optional[Tuple[float, float]] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """act(x [M, K] . w[N, K]^T + bias) in bf16, x bf16 (a view with a row stride is fine), w in 4 bits, fp32 sums.  The
+    weights' values enter unrounded.  Activations and gated units as in linear / glinear."""
+    _chk(x, "x")
+    _mx4_here(x, "x")
+    _mx4_check(isinstance(w, Mx4), "w must be an Mx4 (mx4_quantize, mx4_pack)")
+    _mx4_check(x.dim() == 2 and (x.stride(1) == 1 or x.shape[1] == 1), "x must be [M, K] with consecutive columns")
+    return _mx4_product(x, w, bias, act, act_params, swiglu, geglu, glu_clamp, out)
+
+
+def mx4_matmul(a: Mx4, w: Mx4, bias: Optional[torch.Tensor] = None, *, act: int = ACT_NONE,
+               act_params: Optional[Tuple[float, float]] = None, swiglu: bool = False, geglu: bool = False,
+               glu_clamp: Optional[Tuple[float, float]] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """act(a [M, K] . w[N, K]^T + bias) in bf16, both factors in 4 bits (a = mx4_quantize(x)), fp32 sums."""
+    _mx4_check(isinstance(a, Mx4) and isinstance(w, Mx4), "a and w must be Mx4 (mx4_quantize, mx4_pack)")
+    return _mx4_product(a, w, bias, act, act_params, swiglu, geglu, glu_clamp, out)
