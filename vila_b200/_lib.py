@@ -360,6 +360,7 @@ SIGNATURES = {
     "vila_mx4_dequantize": [c_void_p, c_void_p, c_void_p, c_int, c_i64, c_int, c_int, c_void_p],
     "vila_mx4_scales": [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p],
     "vila_mx4_linear": [C.POINTER(Mx4LinearParams), c_void_p],
+    "vila_mx4_linear_tries": [C.POINTER(Mx4LinearParams), c_int, c_void_p],
 }
 _RESTYPES = {"vila_last_error": C.c_char_p}
 

@@ -494,6 +494,9 @@ int make_tmap_3d_bf16(CUtensorMap* out, const void* base, uint64_t d0, uint64_t 
                       uint32_t swizzle_bytes);
 int make_tmap_nd_bf16(CUtensorMap* out, const void* base, int rank, const uint64_t* dims,
                       const uint64_t* strides_elems, const uint32_t* box, uint32_t swizzle_bytes);
+// 2D tensor of bytes [rows, cols], row pitch `ld_bytes`; box = [box_rows, box_cols]
+int make_tmap_2d_u8(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint64_t ld_bytes, uint32_t box_rows,
+                    uint32_t box_cols, uint32_t swizzle_bytes);
 int num_sms();
 bool pdl_enabled();  // programmatic dependent launch on unless VILA_B200_NO_PDL=1
 

@@ -114,4 +114,17 @@ int make_tmap_3d_bf16(CUtensorMap* out, const void* base, uint64_t d0, uint64_t 
   return make_tmap_nd_bf16(out, base, 3, dims, strides, box, swizzle_bytes);
 }
 
+int make_tmap_2d_u8(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint64_t ld_bytes, uint32_t box_rows,
+                    uint32_t box_cols, uint32_t swizzle_bytes) {
+  EncodeTiledFn fn = get_encode_fn();
+  VB_CHECK(fn != nullptr, "cuTensorMapEncodeTiled driver entry point not available");
+  const cuuint64_t gdim[2] = {cols, rows}, gstride[1] = {ld_bytes};
+  const cuuint32_t bdim[2] = {box_cols, box_rows}, estr[2] = {1, 1};
+  CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), gdim, gstride, bdim, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, swz(swizzle_bytes), CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  VB_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed (%d): [%llu, %llu] bytes, pitch %llu, box [%u, %u], base=%p", (int)r,
+           (unsigned long long)rows, (unsigned long long)cols, (unsigned long long)ld_bytes, box_rows, box_cols, base);
+  return 0;
+}
+
 }  // namespace vb

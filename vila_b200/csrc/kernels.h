@@ -335,7 +335,9 @@ int hgrn2_step(const vila_hgrn2_params& p, cudaStream_t stream);
 int mx4_quantize(const void* x, int dt, int64_t ldx, uint8_t* codes, uint8_t* scales, int rows, int cols, cudaStream_t stream);
 int mx4_dequantize(const uint8_t* codes, const uint8_t* scales, void* out, int dt, int64_t ldo, int rows, int cols, cudaStream_t stream);
 int mx4_scales(uint8_t* plain, uint8_t* tiled, int rows, int cols, int to_tiled, cudaStream_t stream);
-int mx4_linear(const vila_mx4_linear_params& p, cudaStream_t stream);
+// tries: of every wait of the tcgen05 kernels (tests), -1: their own limit
+int mx4_linear(const vila_mx4_linear_params& p, cudaStream_t stream, int tries = -1);
+int mx4_tc(const vila_mx4_linear_params& p, const vila_glinear_ext& ext, int tries, cudaStream_t stream);    // 4-bit rows on tcgen05 (mx4_tc.cu)
 int mx4_rows(const vila_mx4_linear_params& p, const vila_glinear_ext& ext, cudaStream_t stream);   // few rows (mx4_rows.cu)
 
 }  // namespace vb

@@ -10,7 +10,8 @@ namespace {
 bool on16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 }  // namespace
 
-int mx4_linear(const vila_mx4_linear_params& p, cudaStream_t stream) {
+int mx4_linear(const vila_mx4_linear_params& p, cudaStream_t stream, int tries) {
+  if (wait_status()) return 1;   // an earlier launch gave up: nothing is built on its output
   VB_CHECK(p.M >= 0 && p.N > 0 && p.K > 0 && p.M <= (1 << 30) && p.N <= (1 << 30) && p.K <= (1 << 30), "mx4_linear: M=%d N=%d K=%d", p.M, p.N, p.K);
   const int gated = p.flags & kGluFlags;
   VB_CHECK((p.flags & ~kGluFlags) == 0 && (gated & (gated - 1)) == 0, "mx4_linear: flags=%d (one gated unit at most)", p.flags);
@@ -30,6 +31,7 @@ int mx4_linear(const vila_mx4_linear_params& p, cudaStream_t stream) {
   ext.act_limit = p.act_limit;
   ext.act_pos = p.act_pos;
   ext.act_neg = p.act_neg;
+  if (p.a_codes != nullptr && p.M > 16) return mx4_tc(p, ext, tries, stream);
   return mx4_rows(p, ext, stream);
 }
 
