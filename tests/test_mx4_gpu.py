@@ -159,7 +159,7 @@ def weight(seed, n, k, cuda, spread=0.0):
 
 SIZES = [(1, 2, 32), (1, 128, 64), (1, 300, 2048), (3, 129, 95), (7, 64, 1153), (8, 1000, 512), (9, 130, 4000), (16, 256, 1024),
          (17, 384, 300), (33, 128, 640), (64, 514, 1000), (65, 1157, 1153), (100, 640, 256), (129, 300, 2080), (200, 130, 96), (300, 770, 520),
-         (520, 258, 1056)]
+         (520, 258, 1056), (2600, 2570, 800)]
 
 
 @pytest.mark.parametrize("M, N, K", SIZES)

@@ -364,6 +364,15 @@ __device__ __forceinline__ void tma_load_2d_pair(void* smem_dst, const CUtensorM
         "r"(c1)
       : "memory");
 }
+__device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const CUtensorMap* m, uint32_t bar_cluster_addr, int32_t c0, int32_t c1,
+                                                 int32_t c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];"
+      :
+      : "r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar_cluster_addr), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
 template <uint32_t kCols>
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t* smem_result) {
   asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
@@ -497,6 +506,8 @@ int make_tmap_nd_bf16(CUtensorMap* out, const void* base, int rank, const uint64
 // 2D tensor of bytes [rows, cols], row pitch `ld_bytes`; box = [box_rows, box_cols]
 int make_tmap_2d_u8(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint64_t ld_bytes, uint32_t box_rows,
                     uint32_t box_cols, uint32_t swizzle_bytes);
+// 3D tensor of 32-bit words [d2, d1, d0], consecutive, box = [b2, b1, d0], as it lies in memory
+int make_tmap_3d_u32(CUtensorMap* out, const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint32_t b1, uint32_t b2);
 int num_sms();
 bool pdl_enabled();  // programmatic dependent launch on unless VILA_B200_NO_PDL=1
 

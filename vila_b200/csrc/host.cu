@@ -127,4 +127,17 @@ int make_tmap_2d_u8(CUtensorMap* out, const void* base, uint64_t rows, uint64_t 
   return 0;
 }
 
+int make_tmap_3d_u32(CUtensorMap* out, const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint32_t b1, uint32_t b2) {
+  EncodeTiledFn fn = get_encode_fn();
+  VB_CHECK(fn != nullptr, "cuTensorMapEncodeTiled driver entry point not available");
+  const cuuint64_t gdim[3] = {d0, d1, d2}, gstride[2] = {d0 * 4, d0 * d1 * 4};
+  const cuuint32_t bdim[3] = {static_cast<cuuint32_t>(d0), b1, b2}, estr[3] = {1, 1, 1};
+  CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<void*>(base), gdim, gstride, bdim, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  VB_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed (%d): [%llu, %llu, %llu] words, box [%u, %u], base=%p", (int)r,
+           (unsigned long long)d2, (unsigned long long)d1, (unsigned long long)d0, b2, b1, base);
+  return 0;
+}
+
 }  // namespace vb

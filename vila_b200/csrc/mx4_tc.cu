@@ -235,6 +235,219 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant_
   }
 }
 
+// ---- many tokens: tiles of 256 tokens x 256 weight rows by CTA pairs (cta_group::2) ----
+// A single CTA's tile of 128 x 128 asks for 128 bytes of operands per clock of products, more than an SM takes in; the pair's, of
+// which each CTA stages half the tokens and half the weight rows, for 64.  Each CTA's TMEM holds the sums of its 128 tokens for all 256
+// weight rows, the scales of its tokens, and those of all the weight rows.
+//
+// TMEM has room for two accumulators of 256 columns, but not for the scales beside them.  So the two share kShared columns: the
+// epilogue takes those first and says so, and the next tile's products begin then, under the rest of the epilogue.  Scales have two
+// places, taken in turn; a place is free when the products of the stage before last are done.
+namespace pair {
+constexpr int kN = 256, kStages = 6, kShared = 48;
+constexpr int kPBytes = 128 * 128, kQBytes = 128 * 128, kScales = 1024 + 2048, kStage = kPBytes + kQBytes + kScales;
+constexpr int kAcc1 = kN - kShared, kScaleCol = 2 * kN - kShared, kScaleCols = 24;
+constexpr size_t kSmem = 1024 + static_cast<size_t>(kStages) * kStage + 256;
+static_assert(kScaleCol + 2 * kScaleCols <= 512 && kSmem <= 227 * 1024, "");
+
+__device__ __forceinline__ void umma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t"
+      "}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+      : "memory");
+}
+// in both CTAs, each from its own shared memory
+__device__ __forceinline__ void scales_to_tmem_pair(uint32_t taddr, uint32_t smem_addr) {
+  const uint64_t d = make_smem_desc(smem_addr, 16, 128, kLayoutNone);
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
+}
+
+__global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
+mx4_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_sp,
+                const __grid_constant__ CUtensorMap tmap_sq, const vila_mx4_linear_params p, const vila_glinear_ext x, const WaitLimit limit,
+                volatile unsigned int* failed) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + kStages * kStage);   // the first CTA's: both CTAs' loads
+  uint64_t* empty_bar = full_bar + kStages;
+  uint64_t* acc_full = empty_bar + kStages;   // [2]
+  uint64_t* shared_free = acc_full + 2;       // the first CTA's: the columns that the accumulators share, in both CTAs
+  uint64_t* drain_bar = shared_free + 1;
+  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(drain_bar + 1);
+  volatile int* gave_up = reinterpret_cast<int*>(tmem_ptr + 1);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = static_cast<int>(cluster_ctarank());
+  const int p_tiles = (p.M + 255) / 256, q_tiles = (p.N + kN - 1) / kN, total = p_tiles * q_tiles;
+  const int worker = blockIdx.x >> 1, workers = gridDim.x >> 1, nkb = (p.K + kDepth - 1) / kDepth;
+  auto tile_at = [&](int it, int& p0, int& q0) {
+    const int qt = it / p_tiles;
+    p0 = (it - qt * p_tiles) * 256 + rank * 128;
+    q0 = qt * kN;
+  };
+
+  if (tid == 0) {
+    tma_prefetch_desc(&tmap_p);
+    tma_prefetch_desc(&tmap_q);
+    tma_prefetch_desc(&tmap_sp);
+    tma_prefetch_desc(&tmap_sq);
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&full_bar[i], 1);
+      mbar_init(&empty_bar[i], 1);
+    }
+    mbar_init(&acc_full[0], 1);
+    mbar_init(&acc_full[1], 1);
+    mbar_init(shared_free, 2 * kEpi);
+    mbar_init(drain_bar, 1);
+    *gave_up = 0;
+    fence_barrier_init();
+  }
+  if (warp == kMma) tmem_alloc_pair<512>(tmem_ptr);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_ptr;
+  // a warp that gives up tells the other CTA, too
+  auto tell = [&] {
+    *gave_up = 1;
+    st_dsmem_u32(mapa_u32(smem_u32(const_cast<int*>(gave_up)), rank ^ 1), 1u);
+  };
+  bool ok = true;
+  if (limit.quits >= 0) ok = limit.quits != (warp == kTma ? 0 : warp == kMma ? 1 : 3);
+
+  if (warp == kTma) {
+    if (lane == 0) {
+      int s = 0, rounds = 0;
+      uint32_t ph = 1;
+      for (int it = worker; it < total && ok; it += workers) {
+        int p0, q0;
+        tile_at(it, p0, q0);
+        for (int kb = 0; kb < nkb; ++kb) {
+          ok = mbar_wait_limited(&empty_bar[s], ph, gave_up, limit.tries);
+          if (!ok) break;
+          uint8_t* st = smem + s * kStage;
+          const uint32_t bar = mapa_u32(smem_u32(&full_bar[s]), 0);
+          if (rank == 0) mbar_arrive_expect_tx(&full_bar[s], 2 * kStage);
+          tma_load_2d_pair(st, &tmap_p, bar, kb * 128, p0);
+          tma_load_2d_pair(st + kPBytes, &tmap_q, bar, kb * 128, q0 + rank * 128);
+          tma_load_3d_pair(st + kPBytes + kQBytes, &tmap_sp, bar, 0, 2 * kb, p0 >> 7);
+          tma_load_3d_pair(st + kPBytes + kQBytes + 1024, &tmap_sq, bar, 0, 2 * kb, q0 >> 7);
+          if (++s == kStages) {
+            s = 0;
+            ph ^= 1;
+            ++rounds;
+          }
+        }
+      }
+      if (!ok) tell();
+      // what was asked for lands before the CTAs' memory is given back (their loads report to the first one)
+      if (rank == 0)
+        for (int i = 0; i < kStages; ++i) {
+          const int round = i < s ? rounds : rounds - 1;
+          if (round >= 0) mbar_drain(&full_bar[i], round & 1);
+        }
+    }
+  } else if (warp == kMma) {
+    if (lane == 0 && rank == 0) {
+      int j = 0, k = 0;      // stages and tiles so far
+      for (int it = worker; it < total && ok; it += workers, ++k) {
+        const uint32_t acc = tmem + (k & 1) * kAcc1;
+        if (k > 0) ok = mbar_wait_limited(shared_free, (k - 1) & 1, gave_up, limit.tries);
+        tc_fence_after();
+        for (int kb = 0; kb < nkb && ok; ++kb, ++j) {
+          const int s = j % kStages;
+          ok = mbar_wait_limited(&full_bar[s], (j / kStages) & 1, gave_up, limit.tries);
+          if (ok && j >= 2) ok = mbar_wait_limited(&empty_bar[(j - 2) % kStages], ((j - 2) / kStages) & 1, gave_up, limit.tries);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t st = smem_u32(smem + s * kStage), sc = st + kPBytes + kQBytes;
+          const uint32_t ts = tmem + kScaleCol + (j & 1) * kScaleCols, tq = ts + 8;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            scales_to_tmem_pair(ts + 4 * h, sc + 512 * h);
+            scales_to_tmem_pair(tq + 8 * h, sc + 1024 + 512 * h);
+            scales_to_tmem_pair(tq + 8 * h + 4, sc + 2048 + 512 * h);
+          }
+          const uint64_t ad = make_smem_desc(st, 16, 1024, kLayoutSW128), bd = make_smem_desc(st + kPBytes, 16, 1024, kLayoutSW128);
+          const int steps = min(4, (p.K - kb * kDepth + 63) / 64);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (i >= steps) break;
+            umma(acc, ad + 2 * i, bd + 2 * i, idesc_mx4(256, kN, 2 * (i & 1)), ts + 4 * (i >> 1), tq + 8 * (i >> 1), (kb | i) != 0);
+          }
+          umma_commit_pair(&empty_bar[s]);
+        }
+        if (ok) umma_commit_pair(&acc_full[k & 1]);
+      }
+      if (!ok) tell();
+      umma_commit_pair(drain_bar);
+      mbar_drain(drain_bar, 0);
+    }
+  } else {
+    const int quad = warp & 3, half = warp >> 2;
+    const bool vec = reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.ldo % 8 == 0;
+    const uint32_t free_bar = mapa_u32(smem_u32(shared_free), 0);
+    int k = 0;
+    for (int it = worker; it < total && ok; it += workers, ++k) {
+      int p0, q0;
+      tile_at(it, p0, q0);
+      ok = __all_sync(0xffffffffu, ok && mbar_wait_limited(&acc_full[k & 1], (k >> 1) & 1, gave_up, limit.tries));
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t acc = tmem + (static_cast<uint32_t>(quad * 32) << 16) + (k & 1) * kAcc1;
+      const int row = p0 + quad * 32 + lane, first = k & 1 ? 0 : kN - kShared;
+      mx4_with_epilogue(p, [&](auto epi) {
+        constexpr int EPI = decltype(epi)::value;
+#pragma unroll 1
+        for (int i = half; i < kN / 16; i += 2) {
+          const int c = (first + 16 * i) & (kN - 1);      // the shared columns first
+          float r[16];
+          tmem_ld_32x32b_x16(acc + c, reinterpret_cast<uint32_t*>(r));
+          tmem_ld_wait();
+          if (i + 2 >= kShared / 16 && i < kShared / 16) {      // this warp's last one of them
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(free_bar);
+          }
+          if (q0 + c < p.N) mx4_store_row<EPI>(p, x, r, row, q0 + c, vec);
+        }
+      });
+    }
+    if (!ok && lane == 0) tell();
+    tc_fence_before();
+  }
+  __syncthreads();
+  cluster_sync_all();
+  if (warp == kMma) {
+    tc_fence_after();
+    tmem_dealloc_pair<512>(tmem);
+  }
+  if (tid == 0 && *gave_up) {
+    *failed = 1u;
+    __threadfence_system();
+  }
+}
+
+int launch(const vila_mx4_linear_params& p, const vila_glinear_ext& x, int tries, cudaStream_t stream) {
+  static PerDeviceOnce once;
+  if (once.first()) VB_CUDA(cudaFuncSetAttribute(mx4_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmem)));
+  const int pitch = mx4_pitch(p.K), kts = mx4_ktiles(p.K);
+  CUtensorMap tp, tq, sp, sq;
+  if (int rc = make_tmap_2d_u8(&tp, p.a_codes, p.M, pitch, pitch, 128, 128, 128)) return rc;
+  if (int rc = make_tmap_2d_u8(&tq, p.w_codes, p.N, pitch, pitch, 128, 128, 128)) return rc;
+  if (int rc = make_tmap_3d_u32(&sp, p.a_scales, 128, kts, (p.M + 127) / 128, 2, 1)) return rc;
+  if (int rc = make_tmap_3d_u32(&sq, p.w_scales, 128, kts, (p.N + 127) / 128, 2, 2)) return rc;
+  const long long tiles = static_cast<long long>((p.M + 255) / 256) * ((p.N + kN - 1) / kN), most = num_sms() / 2;
+  VB_CHECK(tiles < (1LL << 30), "mx4_linear: too many tiles (M=%d N=%d)", p.M, p.N);
+  VB_CUDA(launch_serial(mx4_pair_kernel, dim3(static_cast<unsigned>(2 * (tiles < most ? tiles : most))), dim3(kThreads), kSmem, stream, tp, tq, sp, sq, p, x,
+                        wait_limit(tries), failed_word()));
+  return 0;
+}
+}  // namespace pair
+
 template <int BN, bool kSwap>
 int launch(const vila_mx4_linear_params& p, const vila_glinear_ext& x, int tries, cudaStream_t stream) {
   using S = Shape<BN>;
@@ -262,6 +475,7 @@ int mx4_tc(const vila_mx4_linear_params& p, const vila_glinear_ext& x, int tries
   if (p.M <= 32) return launch<32, true>(p, x, tries, stream);
   if (p.M <= 64) return launch<64, true>(p, x, tries, stream);
   if (p.M <= 128) return launch<128, true>(p, x, tries, stream);
+  if (p.M > 512) return pair::launch(p, x, tries, stream);
   return launch<128, false>(p, x, tries, stream);
 }
 
