@@ -24,38 +24,40 @@ __device__ __forceinline__ void mx4_with_epilogue(const vila_mx4_linear_params& 
   }
 }
 
-// Lane = output row (token), 16 columns n .. n + 15 of the sums.  `vec`: rows of out start on 16-byte boundaries.
+// 32 bytes (a whole sector of a row) at once
+__device__ __forceinline__ void mx4_stg32(void* p, const uint32_t* h) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]), "r"(h[4]), "r"(h[5]),
+               "r"(h[6]), "r"(h[7])
+               : "memory");
+}
+
+// Lane = output row (token), 32 columns n .. n + 31 of the sums.  `wide`: rows of out start on 32-byte boundaries.
 template <int EPI>
-__device__ __forceinline__ void mx4_store_row(const vila_mx4_linear_params& p, const vila_glinear_ext& x, const float (&r)[16], int m, int n, bool vec) {
-  const __nv_bfloat16* bias = static_cast<const __nv_bfloat16*>(p.bias);
-  float z[16];
+__device__ __forceinline__ void mx4_store_row(const vila_mx4_linear_params& p, const vila_glinear_ext& x, float (&z)[32], int m, int n, bool wide) {
+  constexpr bool kGated = EPI >= kMx4Gated;
+  constexpr int kWords = kGated ? 8 : 16;
+  if (p.bias != nullptr) {
+    const __nv_bfloat16* bias = static_cast<const __nv_bfloat16*>(p.bias);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) z[i] = r[i] + (bias != nullptr && n + i < p.N ? __bfloat162float(__ldg(bias + n + i)) : 0.f);
+    for (int i = 0; i < 32; ++i) z[i] += n + i < p.N ? __bfloat162float(__ldg(bias + n + i)) : 0.f;
+  }
   if (m >= p.M) return;
-  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out) + static_cast<size_t>(m) * p.ldo;
-  if constexpr (EPI >= kMx4Gated) {
-    uint32_t h[4];
+  uint32_t h[kWords];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      h[i] = pack_bf16(glu(z[4 * i], z[4 * i + 1], EPI - kMx4Gated, x), glu(z[4 * i + 2], z[4 * i + 3], EPI - kMx4Gated, x));
-    if (vec && n + 16 <= p.N) {
-      stg_v4(out + n / 2, make_uint4(h[0], h[1], h[2], h[3]));
-    } else {
+  for (int i = 0; i < kWords; ++i) {
+    if constexpr (kGated) h[i] = pack_bf16(glu(z[4 * i], z[4 * i + 1], EPI - kMx4Gated, x), glu(z[4 * i + 2], z[4 * i + 3], EPI - kMx4Gated, x));
+    else h[i] = pack_bf16(activate(z[2 * i], EPI, x), activate(z[2 * i + 1], EPI, x));
+  }
+  const int o = kGated ? n / 2 : n, end = kGated ? p.N / 2 : p.N;
+  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out) + static_cast<size_t>(m) * p.ldo + o;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (n + 2 * i < p.N) reinterpret_cast<unsigned short*>(out)[n / 2 + i] = static_cast<unsigned short>(h[i / 2] >> (16 * (i & 1)));
-    }
-  } else {
-    uint32_t h[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) h[i] = pack_bf16(activate(z[2 * i], EPI, x), activate(z[2 * i + 1], EPI, x));
-    if (vec && n + 16 <= p.N) {
-      stg_v4(out + n, make_uint4(h[0], h[1], h[2], h[3]));
-      stg_v4(out + n + 8, make_uint4(h[4], h[5], h[6], h[7]));
+  for (int g = 0; g < kWords / 8; ++g) {
+    if (wide && o + 16 * g + 16 <= end) {
+      mx4_stg32(out + 16 * g, h + 8 * g);
     } else {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        if (n + i < p.N) reinterpret_cast<unsigned short*>(out)[n + i] = static_cast<unsigned short>(h[i / 2] >> (16 * (i & 1)));
+        if (o + 16 * g + i < end) reinterpret_cast<unsigned short*>(out)[16 * g + i] = static_cast<unsigned short>(h[8 * g + i / 2] >> (16 * (i & 1)));
     }
   }
 }

@@ -195,7 +195,7 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant_
     }
   } else {
     const int quad = warp & 3, half = warp >> 2;
-    const bool vec = reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.ldo % 8 == 0;
+    const bool wide = reinterpret_cast<uintptr_t>(p.out) % 32 == 0 && p.ldo % 16 == 0;
     int k = 0;
     for (int it = blockIdx.x; it < total && ok; it += gridDim.x, ++k) {
       int p0, q0;
@@ -209,13 +209,15 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant_
       const float bias = kSwap && p.bias && row < p.N ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[row]) : 0.f;
       mx4_with_epilogue(p, [&](auto epi) {
         constexpr int EPI = decltype(epi)::value;
+        constexpr int kChunk = kSwap ? 16 : 32;
 #pragma unroll 1
-        for (int c = 16 * half; c < cols; c += 32) {
-          float r[16];
-          tmem_ld_32x32b_x16(acc + c, reinterpret_cast<uint32_t*>(r));
+        for (int c = kChunk * half; c < cols; c += 2 * kChunk) {
+          float r[kChunk];
+          if constexpr (kSwap) tmem_ld_32x32b_x16(acc + c, reinterpret_cast<uint32_t*>(r));
+          else tmem_ld_32x32b_x32(acc + c, reinterpret_cast<uint32_t*>(r));
           tmem_ld_wait();
-          if (kSwap) mx4_store_col<EPI>(p, x, r, q0 + c, row, bias);
-          else mx4_store_row<EPI>(p, x, r, row, q0 + c, vec);
+          if constexpr (kSwap) mx4_store_col<EPI>(p, x, r, q0 + c, row, bias);
+          else mx4_store_row<EPI>(p, x, r, row, q0 + c, wide);
         }
       });
       tc_fence_before();
@@ -241,28 +243,41 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant_
 // weight rows, the scales of its tokens, and those of all the weight rows.
 //
 // TMEM has room for two accumulators of 256 columns, but not for the scales beside them.  So the two share kShared columns: the
-// epilogue takes those first and says so, and the next tile's products begin then, under the rest of the epilogue.  Scales have two
-// places, taken in turn; a place is free when the products of the stage before last are done.
+// epilogue takes those first and says so, and the next tile's products begin then, under the rest of the epilogue.  Every stage
+// has columns of its own for its scales, which are free when its shared memory is: with fewer places and a wait for the products
+// that read one last, 8192 x 8192 x 8192 took 236 us instead of 198.
 namespace pair {
-constexpr int kN = 256, kStages = 6, kShared = 48;
+constexpr int kN = 256, kStages = 5, kShared = 128;
 constexpr int kPBytes = 128 * 128, kQBytes = 128 * 128, kScales = 1024 + 2048, kStage = kPBytes + kQBytes + kScales;
 constexpr int kAcc1 = kN - kShared, kScaleCol = 2 * kN - kShared, kScaleCols = 24;
 constexpr size_t kSmem = 1024 + static_cast<size_t>(kStages) * kStage + 256;
-static_assert(kScaleCol + 2 * kScaleCols <= 512 && kSmem <= 227 * 1024, "");
+static_assert(kScaleCol + kStages * kScaleCols <= 512 && kShared % 32 == 0 && kSmem <= 227 * 1024, "");
 
-__device__ __forceinline__ void umma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t accumulate) {
+__device__ __forceinline__ void umma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t accumulate, uint32_t one) {
   asm volatile(
       "{\n\t"
-      ".reg .pred p;\n\t"
+      ".reg .pred p, q;\n\t"
       "setp.ne.b32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t"
-      "}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+      "setp.ne.b32 q, %7, 0;\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t"
+      "}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate), "r"(one)
       : "memory");
 }
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{.reg .pred P; mbarrier.test_wait.parity.shared::cta.b64 P, [%1], %2; selp.u32 %0, 1, 0, P;}"
+               : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  return ok != 0;
+}
 // in both CTAs, each from its own shared memory
-__device__ __forceinline__ void scales_to_tmem_pair(uint32_t taddr, uint32_t smem_addr) {
-  const uint64_t d = make_smem_desc(smem_addr, 16, 128, kLayoutNone);
-  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
+__device__ __forceinline__ void scales_to_tmem_pair(uint32_t taddr, uint64_t desc, uint32_t one) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred q;\n\t"
+      "setp.ne.b32 q, %2, 0;\n\t"
+      "@q tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n\t"
+      "}\n" ::"r"(taddr), "l"(desc), "r"(one)
+      : "memory");
 }
 
 __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
@@ -351,44 +366,53 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
         }
     }
   } else if (warp == kMma) {
-    if (lane == 0 && rank == 0) {
-      int j = 0, k = 0;      // stages and tiles so far
+    if (rank == 0) {
+      // The whole warp walks the loop and one lane issues: what the instructions are given stays in uniform registers.
+      const uint32_t one = elect_one() ? 1u : 0u;
+      const uint64_t ad0 = make_smem_desc(smem_u32(smem), 16, 1024, kLayoutSW128), bd0 = make_smem_desc(smem_u32(smem) + kPBytes, 16, 1024, kLayoutSW128);
+      const uint64_t sd0 = make_smem_desc(smem_u32(smem) + kPBytes + kQBytes, 16, 128, kLayoutNone);
+      int k = 0, s = 0;                   // tiles so far, stage
+      uint32_t ph = 0;
       for (int it = worker; it < total && ok; it += workers, ++k) {
         const uint32_t acc = tmem + (k & 1) * kAcc1;
-        if (k > 0) ok = mbar_wait_limited(shared_free, (k - 1) & 1, gave_up, limit.tries);
-        tc_fence_after();
-        for (int kb = 0; kb < nkb && ok; ++kb, ++j) {
-          const int s = j % kStages;
-          ok = mbar_wait_limited(&full_bar[s], (j / kStages) & 1, gave_up, limit.tries);
-          if (ok && j >= 2) ok = mbar_wait_limited(&empty_bar[(j - 2) % kStages], ((j - 2) / kStages) & 1, gave_up, limit.tries);
+        if (k > 0) ok = __all_sync(0xffffffffu, mbar_wait_limited(shared_free, (k - 1) & 1, gave_up, limit.tries));
+        bool here = mbar_test(&full_bar[s], ph);      // asked a stage ahead: the answer takes longer than a stage has
+        for (int kb = 0; kb < nkb && ok; ++kb) {
+          if (!__all_sync(0xffffffffu, here)) ok = __all_sync(0xffffffffu, mbar_wait_limited(&full_bar[s], ph, gave_up, limit.tries));
           if (!ok) break;
           tc_fence_after();
-          const uint32_t st = smem_u32(smem + s * kStage), sc = st + kPBytes + kQBytes;
-          const uint32_t ts = tmem + kScaleCol + (j & 1) * kScaleCols, tq = ts + 8;
+          const uint32_t ts = tmem + kScaleCol + s * kScaleCols, tq = ts + 8;
+          const uint64_t ad = ad0 + s * (kStage >> 4), bd = bd0 + s * (kStage >> 4), sd = sd0 + s * (kStage >> 4);
+          uint64_t* done = &empty_bar[s];
+          if (++s == kStages) {
+            s = 0;
+            ph ^= 1;
+          }
+          here = mbar_test(&full_bar[s], ph);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            scales_to_tmem_pair(ts + 4 * h, sc + 512 * h);
-            scales_to_tmem_pair(tq + 8 * h, sc + 1024 + 512 * h);
-            scales_to_tmem_pair(tq + 8 * h + 4, sc + 2048 + 512 * h);
+            scales_to_tmem_pair(ts + 4 * h, sd + 32 * h, one);
+            scales_to_tmem_pair(tq + 8 * h, sd + 64 + 32 * h, one);
+            scales_to_tmem_pair(tq + 8 * h + 4, sd + 128 + 32 * h, one);
           }
-          const uint64_t ad = make_smem_desc(st, 16, 1024, kLayoutSW128), bd = make_smem_desc(st + kPBytes, 16, 1024, kLayoutSW128);
           const int steps = min(4, (p.K - kb * kDepth + 63) / 64);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (i >= steps) break;
-            umma(acc, ad + 2 * i, bd + 2 * i, idesc_mx4(256, kN, 2 * (i & 1)), ts + 4 * (i >> 1), tq + 8 * (i >> 1), (kb | i) != 0);
-          }
-          umma_commit_pair(&empty_bar[s]);
+          for (int i = 0; i < 4; ++i)
+            umma(acc, ad + 2 * i, bd + 2 * i, idesc_mx4(256, kN, 2 * (i & 1)), ts + 4 * (i >> 1), tq + 8 * (i >> 1), (kb | i) != 0, i < steps ? one : 0u);
+          if (one) umma_commit_pair(done);
         }
-        if (ok) umma_commit_pair(&acc_full[k & 1]);
+        if (ok && one) umma_commit_pair(&acc_full[k & 1]);
       }
-      if (!ok) tell();
-      umma_commit_pair(drain_bar);
-      mbar_drain(drain_bar, 0);
+      if (one) {
+        if (!ok) tell();
+        umma_commit_pair(drain_bar);
+        mbar_drain(drain_bar, 0);
+      }
+      __syncwarp();
     }
   } else {
     const int quad = warp & 3, half = warp >> 2;
-    const bool vec = reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.ldo % 8 == 0;
+    const bool wide = reinterpret_cast<uintptr_t>(p.out) % 32 == 0 && p.ldo % 16 == 0;
     const uint32_t free_bar = mapa_u32(smem_u32(shared_free), 0);
     int k = 0;
     for (int it = worker; it < total && ok; it += workers, ++k) {
@@ -402,17 +426,17 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
       mx4_with_epilogue(p, [&](auto epi) {
         constexpr int EPI = decltype(epi)::value;
 #pragma unroll 1
-        for (int i = half; i < kN / 16; i += 2) {
-          const int c = (first + 16 * i) & (kN - 1);      // the shared columns first
-          float r[16];
-          tmem_ld_32x32b_x16(acc + c, reinterpret_cast<uint32_t*>(r));
+        for (int i = half; i < kN / 32; i += 2) {
+          const int c = (first + 32 * i) & (kN - 1);      // the shared columns first
+          float r[32];
+          tmem_ld_32x32b_x32(acc + c, reinterpret_cast<uint32_t*>(r));
           tmem_ld_wait();
-          if (i + 2 >= kShared / 16 && i < kShared / 16) {      // this warp's last one of them
+          if (i + 2 >= kShared / 32 && i < kShared / 32) {      // this warp's last one of them
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(free_bar);
           }
-          if (q0 + c < p.N) mx4_store_row<EPI>(p, x, r, row, q0 + c, vec);
+          if (q0 + c < p.N) mx4_store_row<EPI>(p, x, r, row, q0 + c, wide);
         }
       });
     }
