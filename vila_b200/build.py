@@ -49,6 +49,7 @@ SOURCES = [
     "mx4_linear.cu",
     "mx4_rows.cu",
     "mx4_tc.cu",
+    "mx4_mixed_tc.cu",
 ]
 HEADERS = ["common.cuh", "kernels.h", "dtype_any.cuh", "glinear_epi.cuh", "paged_attn_common.cuh", "mma_bf16.cuh", "mx4.cuh", "mx4_epi.cuh", "../../include/vila_b200.h"]
 

@@ -55,4 +55,11 @@ __device__ __forceinline__ uint32_t mx4_encode8(const float (&v)[8]) {
   return d;
 }
 
+// consecutive bytes (a multiple of 16, on 16-byte boundaries)
+__device__ __forceinline__ void mx4_bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src),
+               "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
 }  // namespace vb

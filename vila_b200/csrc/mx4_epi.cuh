@@ -62,9 +62,9 @@ __device__ __forceinline__ void mx4_store_row(const vila_mx4_linear_params& p, c
   }
 }
 
-// Lane = weight row n, 16 tokens m .. m + 15 of the sums.  All lanes call it.
+// Lane = weight row n, 16 tokens m .. m + 15 of the sums, those below `end`.  All lanes call it.
 template <int EPI>
-__device__ __forceinline__ void mx4_store_col(const vila_mx4_linear_params& p, const vila_glinear_ext& x, const float (&r)[16], int m, int n, float bias) {
+__device__ __forceinline__ void mx4_store_col(const vila_mx4_linear_params& p, const vila_glinear_ext& x, const float (&r)[16], int m, int end, int n, float bias) {
   __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out);
   if constexpr (EPI >= kMx4Gated) {
     // the lanes of a pair hold gate and up: of two tokens each lane finishes one
@@ -73,13 +73,13 @@ __device__ __forceinline__ void mx4_store_col(const vila_mx4_linear_params& p, c
     for (int i = 0; i < 16; i += 2) {
       const float za = r[i] + bias, zb = r[i + 1] + bias, other = __shfl_xor_sync(0xffffffffu, odd ? za : zb, 1);
       const int row = m + i + (odd ? 1 : 0);
-      if (n < p.N && row < p.M)
+      if (n < p.N && row < end)
         out[static_cast<size_t>(row) * p.ldo + n / 2] = __float2bfloat16_rn(glu(odd ? other : za, odd ? zb : other, EPI - kMx4Gated, x));
     }
   } else {
 #pragma unroll
     for (int i = 0; i < 16; ++i)
-      if (n < p.N && m + i < p.M) out[static_cast<size_t>(m + i) * p.ldo + n] = __float2bfloat16_rn(activate(r[i] + bias, EPI, x));
+      if (n < p.N && m + i < end) out[static_cast<size_t>(m + i) * p.ldo + n] = __float2bfloat16_rn(activate(r[i] + bias, EPI, x));
   }
 }
 

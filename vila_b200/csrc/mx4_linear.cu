@@ -32,6 +32,7 @@ int mx4_linear(const vila_mx4_linear_params& p, cudaStream_t stream, int tries) 
   ext.act_pos = p.act_pos;
   ext.act_neg = p.act_neg;
   if (p.a_codes != nullptr && p.M > 16) return mx4_tc(p, ext, tries, stream);
+  if (p.M > 16 && mx4_mixed_tc_takes(p)) return mx4_mixed_tc(p, ext, tries, stream);
   return mx4_rows(p, ext, stream);
 }
 

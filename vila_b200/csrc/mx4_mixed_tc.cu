@@ -1,0 +1,349 @@
+// Linear layers of bf16 rows on microscaled 4-bit weights, more rows than mx4_rows.cu is for: tcgen05.mma kind::f16 with the
+// weights unpacked into TMEM.
+//
+// A weight is code * 2^e, which bf16 holds exactly, so the products are those of bf16 operands.  The unpacked weights never see
+// memory: the M side of tcgen05.mma may lie in TMEM, lane = weight row, 32 columns = 64 weights of a row, which is what a thread that
+// unpacks its own row writes with one tcgen05.st.  Shared memory then only serves the tokens, the N side.
+//
+//   TMA warp         codes and scales, 256 columns of 128 rows at a time; tokens, 64 columns (128 bytes, swizzled) a stage
+//   8 unpack warps   two groups of four (a warp reaches the TMEM lanes of its quarter), which take the stages in turn:
+//                    a byte's two 4-bit numbers to the places of exponent and mantissa of two bf16 (as bf16 that is the number times
+//                    2^-126, its subnormal included), then one packed multiplication by 2^(126 + e)
+//   MMA warp         TMEM allocation; four tcgen05.mma of K = 16 a stage, into one of two accumulator sets
+//   8 epilogue warps TMEM lane = weight row, column = token, under the next tile's products
+//
+// Tiles of 128 weight rows x up to BT tokens.  With BT = 256 the two accumulators share kShared columns, which the epilogue takes
+// first (there is no room for both beside the unpacked weights).
+#include "../../include/vila_b200.h"
+#include "common.cuh"
+#include "kernels.h"
+#include "mx4.cuh"
+#include "mx4_epi.cuh"
+
+namespace vb {
+namespace {
+
+constexpr int kRowsW = 128, kDepth = 64, kCodeDepth = 256;
+constexpr int kEpi = 8, kUnpack = 8, kFirstUnpack = kEpi, kTma = kEpi + kUnpack, kMma = kTma + 1, kThreads = 32 * (kMma + 1);
+constexpr int kBox = 32;                              // token rows of one TMA box
+constexpr int kCodeStages = 3, kCodeBytes = kRowsW * 128, kCodeStage = kCodeBytes + 1024;
+
+template <int BT> struct Shape {
+  static constexpr int kStages = BT > 128 ? 4 : 6;              // of tokens, and of unpacked weights
+  static constexpr int kTokBytes = BT * 128;
+  static constexpr int kAcc1 = BT > 128 ? 128 : BT;             // the second accumulator's first column
+  static constexpr int kShared = BT - kAcc1;
+  static constexpr int kWeights = kAcc1 + BT;                   // first column of the unpacked weights
+  static constexpr int kCols = kWeights + kStages * 32 <= 256 ? 256 : 512;
+  static constexpr size_t kSmem = 1024 + static_cast<size_t>(kStages) * kTokBytes + kCodeStages * kCodeStage + 256;
+  static_assert(kWeights + kStages * 32 <= kCols && kSmem <= 227 * 1024 && kShared % 16 == 0, "");
+};
+
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate, uint32_t one) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(one)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+// eight codes -> four pairs of bf16, each number times 2^-126
+__device__ __forceinline__ void spread8(uint32_t w, uint32_t (&y)[4]) {
+  const uint32_t even = w & 0x0f0f0f0fu, odd = (w >> 4) & 0x0f0f0f0fu;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    // bytes: even's byte i, 0, odd's byte i, 0 (8 + n repeats the sign of byte n, which is 0)
+    uint32_t x;
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(x) : "r"(even), "r"(odd), "r"(i | (8 + i) << 4 | (4 + i) << 8 | (12 + i) << 12));
+    y[i] = (x * 0x1040u) & 0x81c081c0u;       // sign to bit 15, the other three to bits 8 .. 6
+  }
+}
+
+// Token tiles of M rows: as few as tiles of BT allow, or more where that fills the SMs, of nearly equal size
+struct Pieces {
+  int n, per;     // tiles, rows of one (a multiple of 16)
+};
+
+template <int BT>
+__global__ void __launch_bounds__(kThreads, 1)
+mx4_mixed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const vila_mx4_linear_params p,
+                 const vila_glinear_ext x, const Pieces pieces, const WaitLimit limit, volatile unsigned int* failed) {
+  using S = Shape<BT>;
+  constexpr int ST = S::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* codes_s = smem + ST * S::kTokBytes;
+  uint64_t* tok_full = reinterpret_cast<uint64_t*>(codes_s + kCodeStages * kCodeStage);
+  uint64_t* w_full = tok_full + ST;           // unpacked weights are in TMEM
+  uint64_t* empty_bar = w_full + ST;          // the products of a stage are done: its tokens and its weights
+  uint64_t* code_full = empty_bar + ST;
+  uint64_t* code_empty = code_full + kCodeStages;
+  uint64_t* acc_full = code_empty + kCodeStages;   // [2]
+  uint64_t* acc_free = acc_full + 2;               // [2]; with shared columns [0] alone, a phase a tile
+  uint64_t* drain_bar = acc_free + 2;
+  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(drain_bar + 1);
+  volatile int* gave_up = reinterpret_cast<int*>(tmem_ptr + 1);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int n_tiles = (p.N + kRowsW - 1) / kRowsW, total = n_tiles * pieces.n;
+  const int nkb = (p.K + kDepth - 1) / kDepth, nkc = (p.K + kCodeDepth - 1) / kCodeDepth;
+  auto tile_at = [&](int it, int& n0, int& m0, int& count) {
+    const int q = it / pieces.n;
+    m0 = (it - q * pieces.n) * pieces.per;
+    count = min(pieces.per, p.M - m0);
+    n0 = q * kRowsW;
+  };
+
+  if (tid == 0) {
+    tma_prefetch_desc(&tmap_w);
+    tma_prefetch_desc(&tmap_x);
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(&tok_full[i], 1);
+      mbar_init(&w_full[i], 4);
+      mbar_init(&empty_bar[i], 1);
+    }
+    for (int i = 0; i < kCodeStages; ++i) {
+      mbar_init(&code_full[i], 1);
+      mbar_init(&code_empty[i], kUnpack);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_free[i], kEpi);
+    }
+    mbar_init(drain_bar, 1);
+    *gave_up = 0;
+    fence_barrier_init();
+  }
+  if (warp == kMma) tmem_alloc<S::kCols>(tmem_ptr);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_ptr;
+  bool ok = true;
+  if (limit.quits >= 0) {
+    ok = limit.quits != (warp == kTma ? 0 : warp == kMma ? 1 : warp >= kFirstUnpack ? 2 : 3);
+    if (!ok) *gave_up = 1;
+  }
+
+  if (warp == kTma) {
+    if (lane == 0) {
+      const int kts = 2 * nkc;
+      int s = 0, rounds = 0, cs = 0, crounds = 0;      // stages, and rounds through all of them
+      uint32_t ph = 1, cph = 1;
+      for (int it = blockIdx.x; it < total && ok; it += gridDim.x) {
+        int n0, m0, count;
+        tile_at(it, n0, m0, count);
+        const int boxes = (count + kBox - 1) / kBox;
+        for (int kb = 0; kb < nkb; ++kb) {
+          if ((kb & 3) == 0) {
+            ok = mbar_wait_limited(&code_empty[cs], cph, gave_up, limit.tries);
+            if (!ok) break;
+            uint8_t* st = codes_s + cs * kCodeStage;
+            mbar_arrive_expect_tx(&code_full[cs], kCodeStage);
+            tma_load_2d(st, &tmap_w, &code_full[cs], (kb >> 2) * 128, n0);
+            mx4_bulk_load(st + kCodeBytes, p.w_scales + (static_cast<size_t>(n0 >> 7) * kts + 2 * (kb >> 2)) * 512, 1024, &code_full[cs]);
+            if (++cs == kCodeStages) {
+              cs = 0;
+              cph ^= 1;
+              ++crounds;
+            }
+          }
+          ok = mbar_wait_limited(&empty_bar[s], ph, gave_up, limit.tries);
+          if (!ok) break;
+          uint8_t* st = smem + s * S::kTokBytes;
+          mbar_arrive_expect_tx(&tok_full[s], boxes * kBox * 128);
+          for (int b = 0; b < boxes; ++b) tma_load_2d(st + b * kBox * 128, &tmap_x, &tok_full[s], kb * kDepth, m0 + b * kBox);
+          if (++s == ST) {
+            s = 0;
+            ph ^= 1;
+            ++rounds;
+          }
+        }
+      }
+      // what was asked for lands before the CTA's memory is given back, whichever warp gave up
+      for (int i = 0; i < ST; ++i) {
+        const int round = i < s ? rounds : rounds - 1;
+        if (round >= 0) mbar_drain(&tok_full[i], round & 1);
+      }
+      for (int i = 0; i < kCodeStages; ++i) {
+        const int round = i < cs ? crounds : crounds - 1;
+        if (round >= 0) mbar_drain(&code_full[i], round & 1);
+      }
+    }
+  } else if (warp == kMma) {
+    // The whole warp walks the loop and one lane issues: what the instructions are given stays in uniform registers.
+    const uint32_t one = elect_one() ? 1u : 0u;
+    const uint64_t bd0 = make_smem_desc(smem_u32(smem), 16, 1024, kLayoutSW128);
+    int k = 0, s = 0;
+    uint32_t ph = 0;
+    for (int it = blockIdx.x; it < total && ok; it += gridDim.x, ++k) {
+      int n0, m0, count;
+      tile_at(it, n0, m0, count);
+      const uint32_t idesc = make_idesc_bf16(kRowsW, (count + 15) & ~15, 0, 0), acc = tmem + (k & 1) * S::kAcc1;
+      if (S::kShared > 0) ok = k == 0 || mbar_wait_limited(&acc_free[0], (k - 1) & 1, gave_up, limit.tries);
+      else ok = mbar_wait_limited(&acc_free[k & 1], ((k >> 1) & 1) ^ 1, gave_up, limit.tries);
+      ok = __all_sync(0xffffffffu, ok);
+      for (int kb = 0; kb < nkb && ok; ++kb) {
+        ok = __all_sync(0xffffffffu, mbar_wait_limited(&tok_full[s], ph, gave_up, limit.tries) &&
+                                         mbar_wait_limited(&w_full[s], ph, gave_up, limit.tries));
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t bd = bd0 + s * (S::kTokBytes >> 4);
+        const uint32_t wa = tmem + S::kWeights + 32 * s;
+        const int steps = min(4, (p.K - kb * kDepth + 15) / 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) umma_ts(acc, wa + 8 * i, bd + 2 * i, idesc, (kb | i) != 0, i < steps ? one : 0u);
+        if (one) umma_commit(&empty_bar[s]);
+        if (++s == ST) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+      if (ok && one) umma_commit(&acc_full[k & 1]);
+    }
+    if (one) {
+      umma_commit(drain_bar);             // products under way end before TMEM and the CTA's memory are given back, too
+      mbar_drain(drain_bar, 0);
+    }
+    __syncwarp();
+  } else if (warp >= kFirstUnpack) {
+    const int group = (warp - kFirstUnpack) >> 2, quad = warp & 3, row = quad * 32 + lane;
+    int j = 0, cs = 0;                    // stages so far (all tiles), code stage
+    uint32_t cph = 0;
+    for (int it = blockIdx.x; it < total && ok; it += gridDim.x) {
+      for (int kc = 0; kc < nkc && ok; ++kc) {
+        ok = __all_sync(0xffffffffu, mbar_wait_limited(&code_full[cs], cph, gave_up, limit.tries));
+        if (!ok) break;
+        const uint8_t* st = codes_s + cs * kCodeStage;
+        const int steps = min(4, nkb - 4 * kc);
+        for (int q = 0; q < steps && ok; ++q, ++j) {
+          if ((j & 1) != group) continue;
+          const uint4 c0 = *reinterpret_cast<const uint4*>(st + row * 128 + (((2 * q) ^ (row & 7)) << 4));
+          const uint4 c1 = *reinterpret_cast<const uint4*>(st + row * 128 + (((2 * q + 1) ^ (row & 7)) << 4));
+          const uint32_t sw = *reinterpret_cast<const uint32_t*>(st + kCodeBytes + (q >> 1) * 512 + lane * 16 + quad * 4) >> (16 * (q & 1));
+          const uint32_t b0 = sw & 255u, b1 = (sw >> 8) & 255u;
+          const uint32_t w[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+          uint32_t y[32];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) spread8(w[i], *reinterpret_cast<uint32_t(*)[4]>(y + 4 * i));
+          if (__all_sync(0xffffffffu, max(b0, b1) <= 128u)) {      // 2^(126 + e) is a bf16 number
+            const uint32_t f0 = (b0 + 126u) * 0x00800080u, f1 = (b1 + 126u) * 0x00800080u;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) y[i] = mul_bf16x2(y[i], i < 16 ? f0 : f1);
+          } else {
+            const uint32_t up = 0x7e807e80u;                       // 2^126, then 2^e
+            const uint32_t f0 = b0 == 255u ? 0x7fff7fffu : (b0 == 0u ? 0x00400040u : b0 * 0x00800080u);
+            const uint32_t f1 = b1 == 255u ? 0x7fff7fffu : (b1 == 0u ? 0x00400040u : b1 * 0x00800080u);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) y[i] = mul_bf16x2(mul_bf16x2(y[i], up), i < 16 ? f0 : f1);
+          }
+          const int s = j % ST;
+          ok = __all_sync(0xffffffffu, mbar_wait_limited(&empty_bar[s], ((j / ST) & 1) ^ 1, gave_up, limit.tries));
+          if (!ok) break;
+          tc_fence_after();
+          tmem_st_32x32b_x32(tmem + (static_cast<uint32_t>(quad * 32) << 16) + S::kWeights + 32 * s, y);
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&w_full[s]);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&code_empty[cs]);
+        if (++cs == kCodeStages) {
+          cs = 0;
+          cph ^= 1;
+        }
+      }
+    }
+    tc_fence_before();
+  } else {
+    const int quad = warp & 3, half = warp >> 2;
+    int k = 0;
+    for (int it = blockIdx.x; it < total && ok; it += gridDim.x, ++k) {
+      int n0, m0, count;
+      tile_at(it, n0, m0, count);
+      // all lanes or none: the TMEM loads need the whole warp
+      ok = __all_sync(0xffffffffu, mbar_wait_limited(&acc_full[k & 1], (k >> 1) & 1, gave_up, limit.tries));
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t acc = tmem + (static_cast<uint32_t>(quad * 32) << 16) + (k & 1) * S::kAcc1;
+      const int n = n0 + quad * 32 + lane;
+      const float bias = p.bias && n < p.N ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[n]) : 0.f;
+      const int first = S::kShared > 0 && (k & 1) == 0 ? BT - S::kShared : 0;      // the shared columns first
+      bool told = false;
+      auto tell = [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acc_free[S::kShared > 0 ? 0 : k & 1]);
+        told = true;
+      };
+      mx4_with_epilogue(p, [&](auto epi) {
+        constexpr int EPI = decltype(epi)::value;
+#pragma unroll 1
+        for (int i = half; i < BT / 16; i += 2) {
+          const int c = (first + 16 * i) & (BT - 1);
+          if (S::kShared > 0 && !told && i >= S::kShared / 16) tell();
+          if (c >= count) continue;
+          float r[16];
+          tmem_ld_32x32b_x16(acc + c, reinterpret_cast<uint32_t*>(r));
+          tmem_ld_wait();
+          mx4_store_col<EPI>(p, x, r, m0 + c, m0 + count, n, bias);
+        }
+      });
+      if (!told) tell();
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (warp == kMma) {
+    tc_fence_after();
+    tmem_dealloc<S::kCols>(tmem);
+  }
+  if (tid == 0 && *gave_up) {
+    *failed = 1u;
+    __threadfence_system();
+  }
+}
+
+template <int BT>
+int launch(const vila_mx4_linear_params& p, const vila_glinear_ext& x, const Pieces& pieces, int tries, cudaStream_t stream) {
+  using S = Shape<BT>;
+  static PerDeviceOnce once;
+  if (once.first()) VB_CUDA(cudaFuncSetAttribute(mx4_mixed_kernel<BT>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::kSmem)));
+  CUtensorMap tw, tx;
+  if (int rc = make_tmap_2d_u8(&tw, p.w_codes, p.N, mx4_pitch(p.K), mx4_pitch(p.K), kRowsW, 128, 128)) return rc;
+  if (int rc = make_tmap_2d_bf16(&tx, p.x, p.M, p.K, p.ldx, kBox, kDepth, 128)) return rc;
+  const long long tiles = static_cast<long long>((p.N + kRowsW - 1) / kRowsW) * pieces.n;
+  VB_CHECK(tiles < (1LL << 31), "mx4_linear: too many tiles (M=%d N=%d)", p.M, p.N);
+  VB_CUDA(launch_serial(mx4_mixed_kernel<BT>, dim3(static_cast<unsigned>(tiles < num_sms() ? tiles : num_sms())), dim3(kThreads), S::kSmem, stream, tw, tx, p,
+                        x, pieces, wait_limit(tries), failed_word()));
+  return 0;
+}
+
+}  // namespace
+
+bool mx4_mixed_tc_takes(const vila_mx4_linear_params& p) {      // what a tensor map of x needs
+  return p.x != nullptr && reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && p.ldx % 8 == 0 && p.ldx >= p.K;
+}
+
+int mx4_mixed_tc(const vila_mx4_linear_params& p, const vila_glinear_ext& x, int tries, cudaStream_t stream) {
+  VB_CHECK(failed_word() != nullptr, "mx4_linear: no pinned host memory for the status word");
+  const int n_tiles = (p.N + kRowsW - 1) / kRowsW;
+  Pieces pc;
+  pc.n = (p.M + 255) / 256;
+  while (pc.n * n_tiles < num_sms() && (p.M + pc.n) / (pc.n + 1) >= 48) ++pc.n;      // shorter tiles where SMs would stand idle
+  pc.per = ((p.M + pc.n - 1) / pc.n + 15) & ~15;
+  pc.n = (p.M + pc.per - 1) / pc.per;
+  if (pc.per <= 64) return launch<64>(p, x, pc, tries, stream);
+  if (pc.per <= 128) return launch<128>(p, x, pc, tries, stream);
+  return launch<256>(p, x, pc, tries, stream);
+}
+
+}  // namespace vb

@@ -58,12 +58,6 @@ __device__ __forceinline__ void scales_to_tmem(uint32_t taddr, uint32_t smem_add
   const uint64_t d = make_smem_desc(smem_addr, 16, 128, kLayoutNone);
   asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
 }
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src),
-               "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
-}
-
 template <int BN, bool kSwap>
 __global__ void __launch_bounds__(kThreads, Shape<BN>::kPerSm)
 mx4_tc_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ CUtensorMap tmap_q, const vila_mx4_linear_params p,
@@ -135,9 +129,9 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant_
           tma_load_2d(st, &tmap_p, &full_bar[s], kb * 128, p0);
           tma_load_2d(st + S::kPBytes, &tmap_q, &full_bar[s], kb * 128, q0);
           uint8_t* sc = st + S::kPBytes + S::kQBytes;
-          bulk_load(sc, sp + (static_cast<size_t>(p0 >> 7) * kts + 2 * kb) * 512, 1024, &full_bar[s]);
+          mx4_bulk_load(sc, sp + (static_cast<size_t>(p0 >> 7) * kts + 2 * kb) * 512, 1024, &full_bar[s]);
           for (int q = 0; q < qts; ++q)
-            bulk_load(sc + 1024 * (1 + q), sq + (static_cast<size_t>(qt0 + q) * kts + 2 * kb) * 512, 1024, &full_bar[s]);
+            mx4_bulk_load(sc + 1024 * (1 + q), sq + (static_cast<size_t>(qt0 + q) * kts + 2 * kb) * 512, 1024, &full_bar[s]);
           if (++s == ST) {
             s = 0;
             ph ^= 1;
@@ -216,7 +210,7 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant_
           if constexpr (kSwap) tmem_ld_32x32b_x16(acc + c, reinterpret_cast<uint32_t*>(r));
           else tmem_ld_32x32b_x32(acc + c, reinterpret_cast<uint32_t*>(r));
           tmem_ld_wait();
-          if constexpr (kSwap) mx4_store_col<EPI>(p, x, r, q0 + c, row, bias);
+          if constexpr (kSwap) mx4_store_col<EPI>(p, x, r, q0 + c, p.M, row, bias);
           else mx4_store_row<EPI>(p, x, r, row, q0 + c, wide);
         }
       });
