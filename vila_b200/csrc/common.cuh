@@ -560,6 +560,24 @@ inline cudaError_t launch_serial(void (*kern)(KArgs...), dim3 grid, dim3 block, 
   cfg.numAttrs = 0;
   return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
 }
+// the same, by clusters
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_serial_cluster(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, dim3 cluster,
+                                         Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = cluster.x;
+  attr.val.clusterDim.y = cluster.y;
+  attr.val.clusterDim.z = cluster.z;
+  cfg.attrs = &attr;
+  cfg.numAttrs = cluster.x * cluster.y * cluster.z > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
+}
 const char* last_error();
 
 // One-time per-DEVICE setup guard (cudaFuncSetAttribute is per device; a process may drive several).

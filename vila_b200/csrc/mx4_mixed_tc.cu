@@ -5,15 +5,18 @@
 // memory: the M side of tcgen05.mma may lie in TMEM, lane = weight row, 32 columns = 64 weights of a row, which is what a thread that
 // unpacks its own row writes with one tcgen05.st.  Shared memory then only serves the tokens, the N side.
 //
-//   TMA warp         codes and scales, 256 columns of 128 rows at a time; tokens, 64 columns (128 bytes, swizzled) a stage
+//   TMA warp         codes and scales, 256 columns of 128 rows at a time; a stage of tokens (64 columns, 128 bytes, swizzled)
 //   8 unpack warps   two groups of four (a warp reaches the TMEM lanes of its quarter), which take the stages in turn:
 //                    a byte's two 4-bit numbers to the places of exponent and mantissa of two bf16 (as bf16 that is the number times
 //                    2^-126, its subnormal included), then one packed multiplication by 2^(126 + e)
-//   MMA warp         TMEM allocation; four tcgen05.mma of K = 16 a stage, into one of two accumulator sets
+//   MMA warp         TMEM allocation; tcgen05.mma of K = 16, four per 64 columns, into one of two accumulator sets
 //   8 epilogue warps TMEM lane = weight row, column = token, under the next tile's products
 //
-// Tiles of 128 weight rows x up to BT tokens.  With BT = 256 the two accumulators share kShared columns, which the epilogue takes
-// first (there is no room for both beside the unpacked weights).
+// Tiles of 128 weight rows x up to BT tokens; of many tokens by CTA pairs (cta_group::2), each CTA with 128 of 256 weight rows and half
+// of 256 tokens in its shared memory.  Tokens have a ring of their own, as deep as shared memory allows: from the end of a stage's
+// products to the arrival of the tokens that replace it 1.6 us pass, and with four stages of 64 columns that bound the kernel (0.4
+// us a stage of 256 tokens, whose products take 0.27).  The pair's accumulators share kShared columns, which the epilogue takes first
+// (there is no room for both beside the unpacked weights).
 #include "../../include/vila_b200.h"
 #include "common.cuh"
 #include "kernels.h"
@@ -25,29 +28,42 @@ namespace {
 
 constexpr int kRowsW = 128, kDepth = 64, kCodeDepth = 256;
 constexpr int kEpi = 8, kUnpack = 8, kFirstUnpack = kEpi, kTma = kEpi + kUnpack, kMma = kTma + 1, kThreads = 32 * (kMma + 1);
-constexpr int kBox = 32;                              // token rows of one TMA box
-constexpr int kCodeStages = 3, kCodeBytes = kRowsW * 128, kCodeStage = kCodeBytes + 1024;
+constexpr int kCodeBytes = kRowsW * 128, kCodeStage = kCodeBytes + 1024, kCodeStages = 5;
 
-template <int BT> struct Shape {
-  static constexpr int kStages = BT > 128 ? 4 : 6;              // of tokens, and of unpacked weights
-  static constexpr int kTokBytes = BT * 128;
+template <int BT, bool kPair> struct Shape {
+  static constexpr int kSub = kPair ? 1 : 2;                    // times 64 columns are a stage
+  static constexpr int kTokRows = kPair ? BT / 2 : BT;          // that a CTA holds
+  static constexpr int kTokBytes = kSub * kTokRows * 128;
+  static constexpr int kTok = 128 * 1024 / kTokBytes;           // stages of tokens
+  static constexpr int kW = 4;                                  // stages of unpacked weights
   static constexpr int kAcc1 = BT > 128 ? 128 : BT;             // the second accumulator's first column
   static constexpr int kShared = BT - kAcc1;
   static constexpr int kWeights = kAcc1 + BT;                   // first column of the unpacked weights
-  static constexpr int kCols = kWeights + kStages * 32 <= 256 ? 256 : 512;
-  static constexpr size_t kSmem = 1024 + static_cast<size_t>(kStages) * kTokBytes + kCodeStages * kCodeStage + 256;
-  static_assert(kWeights + kStages * 32 <= kCols && kSmem <= 227 * 1024 && kShared % 16 == 0, "");
+  static constexpr int kCols = 512;
+  static constexpr size_t kSmem = 1024 + static_cast<size_t>(kTok) * kTokBytes + kCodeStages * kCodeStage + 512;
+  static_assert(kWeights + kW * kSub * 32 <= kCols && kSmem <= 227 * 1024 && kShared % 16 == 0, "");
 };
 
+template <bool kPair>
 __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate, uint32_t one) {
-  asm volatile(
-      "{\n\t"
-      ".reg .pred p, q;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "setp.ne.b32 q, %5, 0;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
-      "}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(one)
-      : "memory");
+  if (kPair)
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+        "}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(one)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+        "}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(one)
+        : "memory");
 }
 __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
   uint32_t d;
@@ -68,46 +84,65 @@ __device__ __forceinline__ void spread8(uint32_t w, uint32_t (&y)[4]) {
 
 // Token tiles of M rows: as few as tiles of BT allow, or more where that fills the SMs, of nearly equal size
 struct Pieces {
-  int n, per;     // tiles, rows of one (a multiple of 16)
+  int n, per;     // tiles, rows of one (a multiple of 16, of 32 for pairs)
 };
 
-template <int BT>
+template <int BT, bool kPair>
 __global__ void __launch_bounds__(kThreads, 1)
 mx4_mixed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const vila_mx4_linear_params p,
                  const vila_glinear_ext x, const Pieces pieces, const WaitLimit limit, volatile unsigned int* failed) {
-  using S = Shape<BT>;
-  constexpr int ST = S::kStages;
+  using S = Shape<BT, kPair>;
+  constexpr int kCtas = kPair ? 2 : 1, kSteps = kCodeDepth / (kDepth * S::kSub);      // stages of 256 columns
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint8_t* codes_s = smem + ST * S::kTokBytes;
-  uint64_t* tok_full = reinterpret_cast<uint64_t*>(codes_s + kCodeStages * kCodeStage);
-  uint64_t* w_full = tok_full + ST;           // unpacked weights are in TMEM
-  uint64_t* empty_bar = w_full + ST;          // the products of a stage are done: its tokens and its weights
-  uint64_t* code_full = empty_bar + ST;
+  uint8_t* codes_s = smem + S::kTok * S::kTokBytes;
+  uint64_t* tok_full = reinterpret_cast<uint64_t*>(codes_s + kCodeStages * kCodeStage);   // a pair's: in the first CTA, of both
+  uint64_t* tok_empty = tok_full + S::kTok;
+  uint64_t* w_full = tok_empty + S::kTok;          // unpacked weights are in TMEM; a pair's: in the first CTA, of both
+  uint64_t* w_empty = w_full + S::kW;
+  uint64_t* code_full = w_empty + S::kW;
   uint64_t* code_empty = code_full + kCodeStages;
   uint64_t* acc_full = code_empty + kCodeStages;   // [2]
-  uint64_t* acc_free = acc_full + 2;               // [2]; with shared columns [0] alone, a phase a tile
+  uint64_t* acc_free = acc_full + 2;               // [2]; with shared columns [0] alone, a phase a tile; a pair's: in the first CTA
   uint64_t* drain_bar = acc_free + 2;
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(drain_bar + 1);
   volatile int* gave_up = reinterpret_cast<int*>(tmem_ptr + 1);
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int n_tiles = (p.N + kRowsW - 1) / kRowsW, total = n_tiles * pieces.n;
-  const int nkb = (p.K + kDepth - 1) / kDepth, nkc = (p.K + kCodeDepth - 1) / kCodeDepth;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = kPair ? static_cast<int>(cluster_ctarank()) : 0;
+  const int worker = kPair ? blockIdx.x >> 1 : blockIdx.x, workers = kPair ? gridDim.x >> 1 : gridDim.x;
+  const int n_tiles = (p.N + kCtas * kRowsW - 1) / (kCtas * kRowsW), total = n_tiles * pieces.n;
+  const int nkb = (p.K + kDepth * S::kSub - 1) / (kDepth * S::kSub), nkc = (p.K + kCodeDepth - 1) / kCodeDepth;
   auto tile_at = [&](int it, int& n0, int& m0, int& count) {
     const int q = it / pieces.n;
     m0 = (it - q * pieces.n) * pieces.per;
     count = min(pieces.per, p.M - m0);
-    n0 = q * kRowsW;
+    n0 = (q * kCtas + rank) * kRowsW;
+  };
+  auto in_first = [&](uint64_t* bar) { return kPair ? mapa_u32(smem_u32(bar), 0) : smem_u32(bar); };
+  auto arrive_first = [&](uint64_t* bar) {
+    if (kPair) mbar_arrive_cluster(in_first(bar));
+    else mbar_arrive(bar);
+  };
+  auto commit = [&](uint64_t* bar) {
+    if (kPair) umma_commit_pair(bar);
+    else umma_commit(bar);
+  };
+  // a warp that gives up tells the other CTA, too
+  auto tell = [&] {
+    *gave_up = 1;
+    if (kPair) st_dsmem_u32(mapa_u32(smem_u32(const_cast<int*>(gave_up)), rank ^ 1), 1u);
   };
 
   if (tid == 0) {
     tma_prefetch_desc(&tmap_w);
     tma_prefetch_desc(&tmap_x);
-    for (int i = 0; i < ST; ++i) {
+    for (int i = 0; i < S::kTok; ++i) {
       mbar_init(&tok_full[i], 1);
-      mbar_init(&w_full[i], 4);
-      mbar_init(&empty_bar[i], 1);
+      mbar_init(&tok_empty[i], 1);
+    }
+    for (int i = 0; i < S::kW; ++i) {
+      mbar_init(&w_full[i], 4 * kCtas);
+      mbar_init(&w_empty[i], 1);
     }
     for (int i = 0; i < kCodeStages; ++i) {
       mbar_init(&code_full[i], 1);
@@ -115,144 +150,172 @@ mx4_mixed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_free[i], kEpi);
+      mbar_init(&acc_free[i], kEpi * kCtas);
     }
     mbar_init(drain_bar, 1);
     *gave_up = 0;
     fence_barrier_init();
   }
-  if (warp == kMma) tmem_alloc<S::kCols>(tmem_ptr);
+  if (warp == kMma) {
+    if (kPair) tmem_alloc_pair<S::kCols>(tmem_ptr);
+    else tmem_alloc<S::kCols>(tmem_ptr);
+  }
   tc_fence_before();
   __syncthreads();
+  if (kPair) cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem = *tmem_ptr;
-  bool ok = true;
-  if (limit.quits >= 0) {
-    ok = limit.quits != (warp == kTma ? 0 : warp == kMma ? 1 : warp >= kFirstUnpack ? 2 : 3);
-    if (!ok) *gave_up = 1;
-  }
+  bool ok = limit.quits < 0 || limit.quits != (warp == kTma ? 0 : warp == kMma ? 1 : warp >= kFirstUnpack ? 2 : 3);
 
   if (warp == kTma) {
     if (lane == 0) {
-      const int kts = 2 * nkc;
+      const int kts = 2 * nkc, tok_rows = kPair ? pieces.per / 2 : pieces.per;
+      const uint32_t tok_bytes = S::kSub * pieces.per * 128;      // of both CTAs
       int s = 0, rounds = 0, cs = 0, crounds = 0;      // stages, and rounds through all of them
       uint32_t ph = 1, cph = 1;
-      for (int it = blockIdx.x; it < total && ok; it += gridDim.x) {
+      for (int it = worker; it < total && ok; it += workers) {
         int n0, m0, count;
         tile_at(it, n0, m0, count);
-        const int boxes = (count + kBox - 1) / kBox;
         for (int kb = 0; kb < nkb; ++kb) {
-          if ((kb & 3) == 0) {
+          if (kb % kSteps == 0) {
+            const int kc = kb / kSteps;
             ok = mbar_wait_limited(&code_empty[cs], cph, gave_up, limit.tries);
             if (!ok) break;
             uint8_t* st = codes_s + cs * kCodeStage;
-            mbar_arrive_expect_tx(&code_full[cs], kCodeStage);
-            tma_load_2d(st, &tmap_w, &code_full[cs], (kb >> 2) * 128, n0);
-            mx4_bulk_load(st + kCodeBytes, p.w_scales + (static_cast<size_t>(n0 >> 7) * kts + 2 * (kb >> 2)) * 512, 1024, &code_full[cs]);
+            // the second CTA's rows may begin past the last weight row: TMA fills in zeros, scales are not loaded
+            const bool scales = n0 < p.N;
+            mbar_arrive_expect_tx(&code_full[cs], kCodeBytes + (scales ? 1024 : 0));
+            tma_load_2d(st, &tmap_w, &code_full[cs], kc * 128, n0);
+            if (scales) mx4_bulk_load(st + kCodeBytes, p.w_scales + (static_cast<size_t>(n0 >> 7) * kts + 2 * kc) * 512, 1024, &code_full[cs]);
             if (++cs == kCodeStages) {
               cs = 0;
               cph ^= 1;
               ++crounds;
             }
           }
-          ok = mbar_wait_limited(&empty_bar[s], ph, gave_up, limit.tries);
+          ok = mbar_wait_limited(&tok_empty[s], ph, gave_up, limit.tries);
           if (!ok) break;
           uint8_t* st = smem + s * S::kTokBytes;
-          mbar_arrive_expect_tx(&tok_full[s], boxes * kBox * 128);
-          for (int b = 0; b < boxes; ++b) tma_load_2d(st + b * kBox * 128, &tmap_x, &tok_full[s], kb * kDepth, m0 + b * kBox);
-          if (++s == ST) {
+          if (rank == 0) mbar_arrive_expect_tx(&tok_full[s], tok_bytes);
+          // a box is a tile's rows: of boxes of 32 rows, 8 a stage, 8192 x 8192 x 8192 took 1.23 ms, and 0.72 without the tokens
+#pragma unroll
+          for (int i = 0; i < S::kSub; ++i) {
+            if (kPair) tma_load_2d_pair(st, &tmap_x, in_first(&tok_full[s]), kb * kDepth, m0 + rank * tok_rows);
+            else tma_load_2d(st + i * S::kTokRows * 128, &tmap_x, &tok_full[s], (kb * S::kSub + i) * kDepth, m0);
+          }
+          if (++s == S::kTok) {
             s = 0;
             ph ^= 1;
             ++rounds;
           }
         }
       }
-      // what was asked for lands before the CTA's memory is given back, whichever warp gave up
-      for (int i = 0; i < ST; ++i) {
-        const int round = i < s ? rounds : rounds - 1;
-        if (round >= 0) mbar_drain(&tok_full[i], round & 1);
-      }
+      if (!ok) tell();
+      // what was asked for lands before the CTA's memory is given back, whichever warp gave up (a pair's tokens report to the first CTA)
+      if (rank == 0)
+        for (int i = 0; i < S::kTok; ++i) {
+          const int round = i < s ? rounds : rounds - 1;
+          if (round >= 0) mbar_drain(&tok_full[i], round & 1);
+        }
       for (int i = 0; i < kCodeStages; ++i) {
         const int round = i < cs ? crounds : crounds - 1;
         if (round >= 0) mbar_drain(&code_full[i], round & 1);
       }
     }
   } else if (warp == kMma) {
-    // The whole warp walks the loop and one lane issues: what the instructions are given stays in uniform registers.
-    const uint32_t one = elect_one() ? 1u : 0u;
-    const uint64_t bd0 = make_smem_desc(smem_u32(smem), 16, 1024, kLayoutSW128);
-    int k = 0, s = 0;
-    uint32_t ph = 0;
-    for (int it = blockIdx.x; it < total && ok; it += gridDim.x, ++k) {
-      int n0, m0, count;
-      tile_at(it, n0, m0, count);
-      const uint32_t idesc = make_idesc_bf16(kRowsW, (count + 15) & ~15, 0, 0), acc = tmem + (k & 1) * S::kAcc1;
-      if (S::kShared > 0) ok = k == 0 || mbar_wait_limited(&acc_free[0], (k - 1) & 1, gave_up, limit.tries);
-      else ok = mbar_wait_limited(&acc_free[k & 1], ((k >> 1) & 1) ^ 1, gave_up, limit.tries);
-      ok = __all_sync(0xffffffffu, ok);
-      for (int kb = 0; kb < nkb && ok; ++kb) {
-        ok = __all_sync(0xffffffffu, mbar_wait_limited(&tok_full[s], ph, gave_up, limit.tries) &&
-                                         mbar_wait_limited(&w_full[s], ph, gave_up, limit.tries));
-        if (!ok) break;
-        tc_fence_after();
-        const uint64_t bd = bd0 + s * (S::kTokBytes >> 4);
-        const uint32_t wa = tmem + S::kWeights + 32 * s;
-        const int steps = min(4, (p.K - kb * kDepth + 15) / 16);
+    if (rank == 0) {
+      // The whole warp walks the loop and one lane issues: what the instructions are given stays in uniform registers.
+      const uint32_t one = elect_one() ? 1u : 0u;
+      const uint64_t bd0 = make_smem_desc(smem_u32(smem), 16, 1024, kLayoutSW128);
+      int k = 0, s = 0, w = 0;
+      uint32_t ph = 0, wph = 0;
+      for (int it = worker; it < total && ok; it += workers, ++k) {
+        int n0, m0, count;
+        tile_at(it, n0, m0, count);
+        const uint32_t idesc = make_idesc_bf16(kCtas * kRowsW, kPair ? pieces.per : (count + 15) & ~15, 0, 0), acc = tmem + (k & 1) * S::kAcc1;
+        if (S::kShared > 0) ok = k == 0 || mbar_wait_limited(&acc_free[0], (k - 1) & 1, gave_up, limit.tries);
+        else ok = mbar_wait_limited(&acc_free[k & 1], ((k >> 1) & 1) ^ 1, gave_up, limit.tries);
+        ok = __all_sync(0xffffffffu, ok);
+        for (int kb = 0; kb < nkb && ok; ++kb) {
+          ok = __all_sync(0xffffffffu, mbar_wait_limited(&tok_full[s], ph, gave_up, limit.tries) &&
+                                           mbar_wait_limited(&w_full[w], wph, gave_up, limit.tries));
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t bd = bd0 + s * (S::kTokBytes >> 4);
+          const uint32_t wa = tmem + S::kWeights + 32 * S::kSub * w;
+          const int steps = (p.K - kb * S::kSub * kDepth + 15) / 16;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) umma_ts(acc, wa + 8 * i, bd + 2 * i, idesc, (kb | i) != 0, i < steps ? one : 0u);
-        if (one) umma_commit(&empty_bar[s]);
-        if (++s == ST) {
-          s = 0;
-          ph ^= 1;
+          for (int i = 0; i < 4 * S::kSub; ++i)
+            umma_ts<kPair>(acc, wa + 8 * i, bd + (i / 4) * (S::kTokRows * 128 >> 4) + 2 * (i % 4), idesc, (kb | i) != 0, i < steps ? one : 0u);
+          if (one) {
+            commit(&tok_empty[s]);
+            commit(&w_empty[w]);
+          }
+          if (++s == S::kTok) {
+            s = 0;
+            ph ^= 1;
+          }
+          if (++w == S::kW) {
+            w = 0;
+            wph ^= 1;
+          }
         }
+        if (ok && one) commit(&acc_full[k & 1]);
       }
-      if (ok && one) umma_commit(&acc_full[k & 1]);
+      if (one) {
+        if (!ok) tell();
+        commit(drain_bar);             // products under way end before TMEM and the CTA's memory are given back, too
+        mbar_drain(drain_bar, 0);
+      }
+      __syncwarp();
     }
-    if (one) {
-      umma_commit(drain_bar);             // products under way end before TMEM and the CTA's memory are given back, too
-      mbar_drain(drain_bar, 0);
-    }
-    __syncwarp();
   } else if (warp >= kFirstUnpack) {
     const int group = (warp - kFirstUnpack) >> 2, quad = warp & 3, row = quad * 32 + lane;
     int j = 0, cs = 0;                    // stages so far (all tiles), code stage
     uint32_t cph = 0;
-    for (int it = blockIdx.x; it < total && ok; it += gridDim.x) {
+    for (int it = worker; it < total && ok; it += workers) {
       for (int kc = 0; kc < nkc && ok; ++kc) {
         ok = __all_sync(0xffffffffu, mbar_wait_limited(&code_full[cs], cph, gave_up, limit.tries));
         if (!ok) break;
         const uint8_t* st = codes_s + cs * kCodeStage;
-        const int steps = min(4, nkb - 4 * kc);
-        for (int q = 0; q < steps && ok; ++q, ++j) {
+        const int steps = min(kSteps, nkb - kSteps * kc);
+        for (int step = 0; step < steps && ok; ++step, ++j) {
           if ((j & 1) != group) continue;
-          const uint4 c0 = *reinterpret_cast<const uint4*>(st + row * 128 + (((2 * q) ^ (row & 7)) << 4));
-          const uint4 c1 = *reinterpret_cast<const uint4*>(st + row * 128 + (((2 * q + 1) ^ (row & 7)) << 4));
-          const uint32_t sw = *reinterpret_cast<const uint32_t*>(st + kCodeBytes + (q >> 1) * 512 + lane * 16 + quad * 4) >> (16 * (q & 1));
-          const uint32_t b0 = sw & 255u, b1 = (sw >> 8) & 255u;
-          const uint32_t w[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
-          uint32_t y[32];
+          const int w = j % S::kW;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) spread8(w[i], *reinterpret_cast<uint32_t(*)[4]>(y + 4 * i));
-          if (__all_sync(0xffffffffu, max(b0, b1) <= 128u)) {      // 2^(126 + e) is a bf16 number
-            const uint32_t f0 = (b0 + 126u) * 0x00800080u, f1 = (b1 + 126u) * 0x00800080u;
+          for (int i = 0; i < S::kSub; ++i) {
+            const int q = step * S::kSub + i;
+            const uint4 c0 = *reinterpret_cast<const uint4*>(st + row * 128 + (((2 * q) ^ (row & 7)) << 4));
+            const uint4 c1 = *reinterpret_cast<const uint4*>(st + row * 128 + (((2 * q + 1) ^ (row & 7)) << 4));
+            const uint32_t sw = *reinterpret_cast<const uint32_t*>(st + kCodeBytes + (q >> 1) * 512 + lane * 16 + quad * 4) >> (16 * (q & 1));
+            const uint32_t b0 = sw & 255u, b1 = (sw >> 8) & 255u;
+            const uint32_t c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+            uint32_t y[32];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) y[i] = mul_bf16x2(y[i], i < 16 ? f0 : f1);
-          } else {
-            const uint32_t up = 0x7e807e80u;                       // 2^126, then 2^e
-            const uint32_t f0 = b0 == 255u ? 0x7fff7fffu : (b0 == 0u ? 0x00400040u : b0 * 0x00800080u);
-            const uint32_t f1 = b1 == 255u ? 0x7fff7fffu : (b1 == 0u ? 0x00400040u : b1 * 0x00800080u);
+            for (int e = 0; e < 8; ++e) spread8(c[e], *reinterpret_cast<uint32_t(*)[4]>(y + 4 * e));
+            if (__all_sync(0xffffffffu, max(b0, b1) <= 128u)) {      // 2^(126 + e) is a bf16 number
+              const uint32_t f0 = (b0 + 126u) * 0x00800080u, f1 = (b1 + 126u) * 0x00800080u;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) y[i] = mul_bf16x2(mul_bf16x2(y[i], up), i < 16 ? f0 : f1);
+              for (int e = 0; e < 32; ++e) y[e] = mul_bf16x2(y[e], e < 16 ? f0 : f1);
+            } else {
+              const uint32_t up = 0x7e807e80u;                       // 2^126, then 2^e
+              const uint32_t f0 = b0 == 255u ? 0x7fff7fffu : (b0 == 0u ? 0x00400040u : b0 * 0x00800080u);
+              const uint32_t f1 = b1 == 255u ? 0x7fff7fffu : (b1 == 0u ? 0x00400040u : b1 * 0x00800080u);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) y[e] = mul_bf16x2(mul_bf16x2(y[e], up), e < 16 ? f0 : f1);
+            }
+            if (i == 0) {
+              ok = __all_sync(0xffffffffu, mbar_wait_limited(&w_empty[w], ((j / S::kW) & 1) ^ 1, gave_up, limit.tries));
+              if (!ok) break;
+              tc_fence_after();
+            }
+            tmem_st_32x32b_x32(tmem + (static_cast<uint32_t>(quad * 32) << 16) + S::kWeights + 32 * (S::kSub * w + i), y);
           }
-          const int s = j % ST;
-          ok = __all_sync(0xffffffffu, mbar_wait_limited(&empty_bar[s], ((j / ST) & 1) ^ 1, gave_up, limit.tries));
           if (!ok) break;
-          tc_fence_after();
-          tmem_st_32x32b_x32(tmem + (static_cast<uint32_t>(quad * 32) << 16) + S::kWeights + 32 * s, y);
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&w_full[s]);
+          if (lane == 0) arrive_first(&w_full[w]);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&code_empty[cs]);
@@ -262,11 +325,12 @@ mx4_mixed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
         }
       }
     }
+    if (!ok && lane == 0) tell();
     tc_fence_before();
   } else {
     const int quad = warp & 3, half = warp >> 2;
     int k = 0;
-    for (int it = blockIdx.x; it < total && ok; it += gridDim.x, ++k) {
+    for (int it = worker; it < total && ok; it += workers, ++k) {
       int n0, m0, count;
       tile_at(it, n0, m0, count);
       // all lanes or none: the TMEM loads need the whole warp
@@ -278,10 +342,10 @@ mx4_mixed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
       const float bias = p.bias && n < p.N ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[n]) : 0.f;
       const int first = S::kShared > 0 && (k & 1) == 0 ? BT - S::kShared : 0;      // the shared columns first
       bool told = false;
-      auto tell = [&] {
+      auto free_acc = [&] {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&acc_free[S::kShared > 0 ? 0 : k & 1]);
+        if (lane == 0) arrive_first(&acc_free[S::kShared > 0 ? 0 : k & 1]);
         told = true;
       };
       mx4_with_epilogue(p, [&](auto epi) {
@@ -289,7 +353,7 @@ mx4_mixed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
 #pragma unroll 1
         for (int i = half; i < BT / 16; i += 2) {
           const int c = (first + 16 * i) & (BT - 1);
-          if (S::kShared > 0 && !told && i >= S::kShared / 16) tell();
+          if (S::kShared > 0 && !told && i >= S::kShared / 16) free_acc();
           if (c >= count) continue;
           float r[16];
           tmem_ld_32x32b_x16(acc + c, reinterpret_cast<uint32_t*>(r));
@@ -297,14 +361,17 @@ mx4_mixed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
           mx4_store_col<EPI>(p, x, r, m0 + c, m0 + count, n, bias);
         }
       });
-      if (!told) tell();
+      if (!told) free_acc();
     }
+    if (!ok && lane == 0) tell();
     tc_fence_before();
   }
   __syncthreads();
+  if (kPair) cluster_sync_all();      // the other CTA's products and loads have been waited for, too
   if (warp == kMma) {
     tc_fence_after();
-    tmem_dealloc<S::kCols>(tmem);
+    if (kPair) tmem_dealloc_pair<S::kCols>(tmem);
+    else tmem_dealloc<S::kCols>(tmem);
   }
   if (tid == 0 && *gave_up) {
     *failed = 1u;
@@ -312,18 +379,20 @@ mx4_mixed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
   }
 }
 
-template <int BT>
+template <int BT, bool kPair>
 int launch(const vila_mx4_linear_params& p, const vila_glinear_ext& x, const Pieces& pieces, int tries, cudaStream_t stream) {
-  using S = Shape<BT>;
+  using S = Shape<BT, kPair>;
+  constexpr int kCtas = kPair ? 2 : 1;
   static PerDeviceOnce once;
-  if (once.first()) VB_CUDA(cudaFuncSetAttribute(mx4_mixed_kernel<BT>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::kSmem)));
+  if (once.first())
+    VB_CUDA(cudaFuncSetAttribute(mx4_mixed_kernel<BT, kPair>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::kSmem)));
   CUtensorMap tw, tx;
   if (int rc = make_tmap_2d_u8(&tw, p.w_codes, p.N, mx4_pitch(p.K), mx4_pitch(p.K), kRowsW, 128, 128)) return rc;
-  if (int rc = make_tmap_2d_bf16(&tx, p.x, p.M, p.K, p.ldx, kBox, kDepth, 128)) return rc;
-  const long long tiles = static_cast<long long>((p.N + kRowsW - 1) / kRowsW) * pieces.n;
-  VB_CHECK(tiles < (1LL << 31), "mx4_linear: too many tiles (M=%d N=%d)", p.M, p.N);
-  VB_CUDA(launch_serial(mx4_mixed_kernel<BT>, dim3(static_cast<unsigned>(tiles < num_sms() ? tiles : num_sms())), dim3(kThreads), S::kSmem, stream, tw, tx, p,
-                        x, pieces, wait_limit(tries), failed_word()));
+  if (int rc = make_tmap_2d_bf16(&tx, p.x, p.M, p.K, p.ldx, pieces.per / kCtas, kDepth, 128)) return rc;
+  const long long tiles = static_cast<long long>((p.N + kCtas * kRowsW - 1) / (kCtas * kRowsW)) * pieces.n, most = num_sms() / kCtas;
+  VB_CHECK(tiles < (1LL << 30), "mx4_linear: too many tiles (M=%d N=%d)", p.M, p.N);
+  VB_CUDA(launch_serial_cluster(mx4_mixed_kernel<BT, kPair>, dim3(static_cast<unsigned>(kCtas * (tiles < most ? tiles : most))), dim3(kThreads), S::kSmem, stream,
+                                dim3(kCtas), tw, tx, p, x, pieces, wait_limit(tries), failed_word()));
   return 0;
 }
 
@@ -341,9 +410,11 @@ int mx4_mixed_tc(const vila_mx4_linear_params& p, const vila_glinear_ext& x, int
   while (pc.n * n_tiles < num_sms() && (p.M + pc.n) / (pc.n + 1) >= 48) ++pc.n;      // shorter tiles where SMs would stand idle
   pc.per = ((p.M + pc.n - 1) / pc.n + 15) & ~15;
   pc.n = (p.M + pc.per - 1) / pc.per;
-  if (pc.per <= 64) return launch<64>(p, x, pc, tries, stream);
-  if (pc.per <= 128) return launch<128>(p, x, pc, tries, stream);
-  return launch<256>(p, x, pc, tries, stream);
+  if (pc.per <= 64) return launch<64, false>(p, x, pc, tries, stream);
+  if (pc.per <= 128) return launch<128, false>(p, x, pc, tries, stream);
+  pc.per = (pc.per + 31) & ~31;
+  pc.n = (p.M + pc.per - 1) / pc.per;
+  return launch<256, true>(p, x, pc, tries, stream);
 }
 
 }  // namespace vb
