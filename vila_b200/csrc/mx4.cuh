@@ -55,6 +55,27 @@ __device__ __forceinline__ uint32_t mx4_encode8(const float (&v)[8]) {
   return d;
 }
 
+// whether an mbarrier's phase is over, without waiting for it
+__device__ __forceinline__ bool mx4_mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{.reg .pred P; mbarrier.test_wait.parity.shared::cta.b64 P, [%1], %2; selp.u32 %0, 1, 0, P;}"
+               : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  return ok != 0;
+}
+// umma_commit / umma_commit_pair by the lanes whose `one` is set (one lane), with no branch around it
+__device__ __forceinline__ void mx4_commit(uint64_t* bar, uint32_t one) {
+  asm volatile(
+      "{.reg .pred q; setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];}" ::"r"(smem_u32(bar)), "r"(one)
+      : "memory");
+}
+__device__ __forceinline__ void mx4_commit_pair(uint64_t* bar, uint32_t one) {
+  asm volatile(
+      "{.reg .pred q; setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %2;}" ::"r"(smem_u32(bar)), "r"(one),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
 // consecutive bytes (a multiple of 16, on 16-byte boundaries)
 __device__ __forceinline__ void mx4_bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src),

@@ -120,12 +120,12 @@ mx4_mixed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
   };
   auto in_first = [&](uint64_t* bar) { return kPair ? mapa_u32(smem_u32(bar), 0) : smem_u32(bar); };
   auto arrive_first = [&](uint64_t* bar) {
-    if (kPair) mbar_arrive_cluster(in_first(bar));
+    if (kPair) mbar_arrive_cluster_relaxed(in_first(bar));
     else mbar_arrive(bar);
   };
-  auto commit = [&](uint64_t* bar) {
-    if (kPair) umma_commit_pair(bar);
-    else umma_commit(bar);
+  auto commit = [&](uint64_t* bar, uint32_t one) {
+    if (kPair) mx4_commit_pair(bar, one);
+    else mx4_commit(bar, one);
   };
   // a warp that gives up tells the other CTA, too
   auto tell = [&] {
@@ -236,21 +236,17 @@ mx4_mixed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
         if (S::kShared > 0) ok = k == 0 || mbar_wait_limited(&acc_free[0], (k - 1) & 1, gave_up, limit.tries);
         else ok = mbar_wait_limited(&acc_free[k & 1], ((k >> 1) & 1) ^ 1, gave_up, limit.tries);
         ok = __all_sync(0xffffffffu, ok);
+        bool tok_here = false, w_here = false;      // asked a stage ahead: the answer takes a while
         for (int kb = 0; kb < nkb && ok; ++kb) {
-          ok = __all_sync(0xffffffffu, mbar_wait_limited(&tok_full[s], ph, gave_up, limit.tries) &&
-                                           mbar_wait_limited(&w_full[w], wph, gave_up, limit.tries));
+          if (!__all_sync(0xffffffffu, tok_here && w_here))
+            ok = __all_sync(0xffffffffu, mbar_wait_limited(&tok_full[s], ph, gave_up, limit.tries) &&
+                                             mbar_wait_limited(&w_full[w], wph, gave_up, limit.tries));
           if (!ok) break;
           tc_fence_after();
           const uint64_t bd = bd0 + s * (S::kTokBytes >> 4);
           const uint32_t wa = tmem + S::kWeights + 32 * S::kSub * w;
           const int steps = (p.K - kb * S::kSub * kDepth + 15) / 16;
-#pragma unroll
-          for (int i = 0; i < 4 * S::kSub; ++i)
-            umma_ts<kPair>(acc, wa + 8 * i, bd + (i / 4) * (S::kTokRows * 128 >> 4) + 2 * (i % 4), idesc, (kb | i) != 0, i < steps ? one : 0u);
-          if (one) {
-            commit(&tok_empty[s]);
-            commit(&w_empty[w]);
-          }
+          uint64_t *tok_done = &tok_empty[s], *w_done = &w_empty[w];
           if (++s == S::kTok) {
             s = 0;
             ph ^= 1;
@@ -259,12 +255,19 @@ mx4_mixed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
             w = 0;
             wph ^= 1;
           }
+          tok_here = mx4_mbar_test(&tok_full[s], ph);
+          w_here = mx4_mbar_test(&w_full[w], wph);
+#pragma unroll
+          for (int i = 0; i < 4 * S::kSub; ++i)
+            umma_ts<kPair>(acc, wa + 8 * i, bd + (i / 4) * (S::kTokRows * 128 >> 4) + 2 * (i % 4), idesc, (kb | i) != 0, i < steps ? one : 0u);
+          commit(tok_done, one);
+          commit(w_done, one);
         }
-        if (ok && one) commit(&acc_full[k & 1]);
+        if (ok) commit(&acc_full[k & 1], one);
       }
       if (one) {
         if (!ok) tell();
-        commit(drain_bar);             // products under way end before TMEM and the CTA's memory are given back, too
+        commit(drain_bar, 1);             // products under way end before TMEM and the CTA's memory are given back, too
         mbar_drain(drain_bar, 0);
       }
       __syncwarp();

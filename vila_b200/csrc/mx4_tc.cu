@@ -257,12 +257,6 @@ __device__ __forceinline__ void umma(uint32_t d, uint64_t a, uint64_t b, uint32_
       "}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate), "r"(one)
       : "memory");
 }
-__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile("{.reg .pred P; mbarrier.test_wait.parity.shared::cta.b64 P, [%1], %2; selp.u32 %0, 1, 0, P;}"
-               : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
-  return ok != 0;
-}
 // in both CTAs, each from its own shared memory
 __device__ __forceinline__ void scales_to_tmem_pair(uint32_t taddr, uint64_t desc, uint32_t one) {
   asm volatile(
@@ -370,7 +364,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
       for (int it = worker; it < total && ok; it += workers, ++k) {
         const uint32_t acc = tmem + (k & 1) * kAcc1;
         if (k > 0) ok = __all_sync(0xffffffffu, mbar_wait_limited(shared_free, (k - 1) & 1, gave_up, limit.tries));
-        bool here = mbar_test(&full_bar[s], ph);      // asked a stage ahead: the answer takes longer than a stage has
+        bool here = mx4_mbar_test(&full_bar[s], ph);      // asked a stage ahead: the answer takes longer than a stage has
         for (int kb = 0; kb < nkb && ok; ++kb) {
           if (!__all_sync(0xffffffffu, here)) ok = __all_sync(0xffffffffu, mbar_wait_limited(&full_bar[s], ph, gave_up, limit.tries));
           if (!ok) break;
@@ -382,7 +376,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
             s = 0;
             ph ^= 1;
           }
-          here = mbar_test(&full_bar[s], ph);
+          here = mx4_mbar_test(&full_bar[s], ph);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             scales_to_tmem_pair(ts + 4 * h, sd + 32 * h, one);
@@ -393,9 +387,9 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             umma(acc, ad + 2 * i, bd + 2 * i, idesc_mx4(256, kN, 2 * (i & 1)), ts + 4 * (i >> 1), tq + 8 * (i >> 1), (kb | i) != 0, i < steps ? one : 0u);
-          if (one) umma_commit_pair(done);
+          mx4_commit_pair(done, one);
         }
-        if (ok && one) umma_commit_pair(&acc_full[k & 1]);
+        if (ok) mx4_commit_pair(&acc_full[k & 1], one);
       }
       if (one) {
         if (!ok) tell();
@@ -428,7 +422,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
           if (i + 2 >= kShared / 32 && i < kShared / 32) {      // this warp's last one of them
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(free_bar);
+            if (lane == 0) mbar_arrive_cluster_relaxed(free_bar);
           }
           if (q0 + c < p.N) mx4_store_row<EPI>(p, x, r, row, q0 + c, wide);
         }
