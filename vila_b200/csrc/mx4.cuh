@@ -27,6 +27,12 @@ __host__ __device__ __forceinline__ size_t mx4_scale_bytes(int rows, int cols) {
 __device__ __forceinline__ float mx4_scale(uint32_t b) {
   return __uint_as_float(b == 255u ? 0x7fffffffu : (b == 0u ? 0x00400000u : b << 23));
 }
+// the number of a code
+__device__ __forceinline__ float mx4_number(uint32_t c) {
+  const uint32_t e = (c >> 1) & 3u, m = c & 1u;
+  const float v = e == 0u ? 0.5f * m : __uint_as_float((126u + e) << 23 | m << 22);
+  return c & 8u ? -v : v;
+}
 // the two numbers of byte `i` of w as f16 (exact), the low half's first
 template <int kByte>
 __device__ __forceinline__ uint32_t mx4_pair_f16(uint32_t w) {
@@ -55,12 +61,23 @@ __device__ __forceinline__ uint32_t mx4_encode8(const float (&v)[8]) {
   return d;
 }
 
-// whether an mbarrier's phase is over, without waiting for it
-__device__ __forceinline__ bool mx4_mbar_test(uint64_t* bar, uint32_t parity) {
+// A warp's wait on an mbarrier that no lane leaves before the others: the warps that issue tcgen05 instructions stay converged, so that
+// what they hold in uniform registers is one value.  (Lanes that left the wait one by one, or one lane that waited for all, ended in
+// launch failures.)
+__device__ __forceinline__ bool mx4_warp_wait(uint64_t* bar, uint32_t parity, volatile int* gave_up, int tries) {
+  for (int i = 0; i < tries; ++i) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    if (__any_sync(0xffffffffu, *gave_up != 0)) return false;
+  }
+  *gave_up = 1;
+  return false;
+}
+// whether an mbarrier's phase is over, without waiting for it; the same answer for all lanes
+__device__ __forceinline__ bool mx4_warp_test(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
   asm volatile("{.reg .pred P; mbarrier.test_wait.parity.shared::cta.b64 P, [%1], %2; selp.u32 %0, 1, 0, P;}"
                : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
-  return ok != 0;
+  return __all_sync(0xffffffffu, ok != 0);
 }
 // umma_commit / umma_commit_pair by the lanes whose `one` is set (one lane), with no branch around it
 __device__ __forceinline__ void mx4_commit(uint64_t* bar, uint32_t one) {

@@ -24,6 +24,21 @@ __device__ __forceinline__ void mx4_with_epilogue(const vila_mx4_linear_params& 
   }
 }
 
+// The activations with __expf and __fdividef: their results are rounded to bf16 right after, and under the unpacking of weights
+// or a few clocks of products per output the exact ones showed (2048 x 37888 x 3584 with a gated unit: 545 us).
+template <int EPI>
+__device__ __forceinline__ float mx4_act(float z, const vila_glinear_ext& x) {
+  if (EPI == VILA_ACT_SILU) return silu_f(z);
+  if (EPI == VILA_ACT_GELU_TANH) return gelu_tanh_f(z);
+  if (EPI == VILA_ACT_XIELU) return xielu_fast_f(z, x.act_pos, x.act_neg);
+  return activate(z, EPI, x);
+}
+template <int EPI>
+__device__ __forceinline__ float mx4_glu(float g, float u, const vila_glinear_ext& x) {
+  if (EPI == kMx4Gated + VILA_FLAG_GLU_CLAMP) return glu_clamp_fast_f(g, u, x.act_alpha, x.act_limit);
+  return (EPI == kMx4Gated + VILA_FLAG_GEGLU ? gelu_tanh_f(g) : silu_f(g)) * u;
+}
+
 // 32 bytes (a whole sector of a row) at once
 __device__ __forceinline__ void mx4_stg32(void* p, const uint32_t* h) {
   asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]), "r"(h[4]), "r"(h[5]),
@@ -45,8 +60,8 @@ __device__ __forceinline__ void mx4_store_row(const vila_mx4_linear_params& p, c
   uint32_t h[kWords];
 #pragma unroll
   for (int i = 0; i < kWords; ++i) {
-    if constexpr (kGated) h[i] = pack_bf16(glu(z[4 * i], z[4 * i + 1], EPI - kMx4Gated, x), glu(z[4 * i + 2], z[4 * i + 3], EPI - kMx4Gated, x));
-    else h[i] = pack_bf16(activate(z[2 * i], EPI, x), activate(z[2 * i + 1], EPI, x));
+    if constexpr (kGated) h[i] = pack_bf16(mx4_glu<EPI>(z[4 * i], z[4 * i + 1], x), mx4_glu<EPI>(z[4 * i + 2], z[4 * i + 3], x));
+    else h[i] = pack_bf16(mx4_act<EPI>(z[2 * i], x), mx4_act<EPI>(z[2 * i + 1], x));
   }
   const int o = kGated ? n / 2 : n, end = kGated ? p.N / 2 : p.N;
   __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out) + static_cast<size_t>(m) * p.ldo + o;
@@ -74,12 +89,12 @@ __device__ __forceinline__ void mx4_store_col(const vila_mx4_linear_params& p, c
       const float za = r[i] + bias, zb = r[i + 1] + bias, other = __shfl_xor_sync(0xffffffffu, odd ? za : zb, 1);
       const int row = m + i + (odd ? 1 : 0);
       if (n < p.N && row < end)
-        out[static_cast<size_t>(row) * p.ldo + n / 2] = __float2bfloat16_rn(glu(odd ? other : za, odd ? zb : other, EPI - kMx4Gated, x));
+        out[static_cast<size_t>(row) * p.ldo + n / 2] = __float2bfloat16_rn(mx4_glu<EPI>(odd ? other : za, odd ? zb : other, x));
     }
   } else {
 #pragma unroll
     for (int i = 0; i < 16; ++i)
-      if (n < p.N && m + i < end) out[static_cast<size_t>(m + i) * p.ldo + n] = __float2bfloat16_rn(activate(r[i] + bias, EPI, x));
+      if (n < p.N && m + i < end) out[static_cast<size_t>(m + i) * p.ldo + n] = __float2bfloat16_rn(mx4_act<EPI>(r[i] + bias, x));
   }
 }
 

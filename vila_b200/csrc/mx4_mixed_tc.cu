@@ -6,17 +6,20 @@
 // unpacks its own row writes with one tcgen05.st.  Shared memory then only serves the tokens, the N side.
 //
 //   TMA warp         codes and scales, 256 columns of 128 rows at a time; a stage of tokens (64 columns, 128 bytes, swizzled)
-//   8 unpack warps   two groups of four (a warp reaches the TMEM lanes of its quarter), which take the stages in turn:
-//                    a byte's two 4-bit numbers to the places of exponent and mantissa of two bf16 (as bf16 that is the number times
-//                    2^-126, its subnormal included), then one packed multiplication by 2^(126 + e)
+//   8 unpack warps   two groups of four (a warp reaches the TMEM lanes of its quarter), which take the stages in turn: a byte of
+//                    codes (two weights) is looked up in shared memory as a pair of bf16, then multiplied by the block's 2^e
 //   MMA warp         TMEM allocation; tcgen05.mma of K = 16, four per 64 columns, into one of two accumulator sets
 //   8 epilogue warps TMEM lane = weight row, column = token, under the next tile's products
 //
+// The table has 256 entries, one copy for each lane in a bank of its own, entry v of lane l at 65536 + 256 v + 4 l: one prmt makes the
+// address, no two lanes meet in a bank.  Spreading the bits with integer instructions instead took 174 of them on the ALU per
+// 64 weights of a row, 350 clocks of each scheduler, where the products of 128 tokens take 256.
+//
 // Tiles of 128 weight rows x up to BT tokens; of many tokens by CTA pairs (cta_group::2), each CTA with 128 of 256 weight rows and half
-// of 256 tokens in its shared memory.  Tokens have a ring of their own, as deep as shared memory allows: from the end of a stage's
-// products to the arrival of the tokens that replace it 1.6 us pass, and with four stages of 64 columns that bound the kernel (0.4
-// us a stage of 256 tokens, whose products take 0.27).  The pair's accumulators share kShared columns, which the epilogue takes first
-// (there is no room for both beside the unpacked weights).
+// of 256 tokens in its shared memory: an SM takes in 54 bytes a clock, and 256 tokens of its own alone are 64 per clock of their
+// products.  Tokens have a ring of their own, as deep as shared memory allows: from the end of a stage's products to the arrival of
+// the tokens that replace it 1.6 us pass.  The pair's accumulators share kShared columns, which the epilogue takes first (there is no
+// room for both beside the unpacked weights).
 #include "../../include/vila_b200.h"
 #include "common.cuh"
 #include "kernels.h"
@@ -28,20 +31,24 @@ namespace {
 
 constexpr int kRowsW = 128, kDepth = 64, kCodeDepth = 256;
 constexpr int kEpi = 8, kUnpack = 8, kFirstUnpack = kEpi, kTma = kEpi + kUnpack, kMma = kTma + 1, kThreads = 32 * (kMma + 1);
-constexpr int kCodeBytes = kRowsW * 128, kCodeStage = kCodeBytes + 1024, kCodeStages = 5;
+constexpr int kCodeBytes = kRowsW * 128, kCodeStage = kCodeBytes + 1024, kCodeStages = 3;
+// Shared memory by addresses of the shared window: codes and barriers, the table from 64 KB on, tokens behind it
+constexpr uint32_t kTable = 0x10000, kTokens = 0x20000, kTokensBytes = 96 * 1024, kBars = kCodeStages * kCodeStage, kLow = kBars + 1024;
+constexpr uint32_t kSmemFrom = 1024;                  // where dynamic shared memory begins (the first 1 KB is the system's)
+constexpr size_t kSmem = kTokens + kTokensBytes - kSmemFrom;
+static_assert(kSmemFrom + kLow <= kTable && kSmem <= 227 * 1024, "");
 
 template <int BT, bool kPair> struct Shape {
-  static constexpr int kSub = kPair ? 1 : 2;                    // times 64 columns are a stage
+  static constexpr int kSub = BT > 64 ? 1 : 2;                  // times 64 columns are a stage
   static constexpr int kTokRows = kPair ? BT / 2 : BT;          // that a CTA holds
   static constexpr int kTokBytes = kSub * kTokRows * 128;
-  static constexpr int kTok = 128 * 1024 / kTokBytes;           // stages of tokens
-  static constexpr int kW = 4;                                  // stages of unpacked weights
+  static constexpr int kTok = kTokensBytes / kTokBytes;         // stages of tokens
+  static constexpr int kW = BT > 128 ? 4 : (BT > 64 ? 8 : 4);   // stages of unpacked weights
   static constexpr int kAcc1 = BT > 128 ? 128 : BT;             // the second accumulator's first column
   static constexpr int kShared = BT - kAcc1;
   static constexpr int kWeights = kAcc1 + BT;                   // first column of the unpacked weights
   static constexpr int kCols = 512;
-  static constexpr size_t kSmem = 1024 + static_cast<size_t>(kTok) * kTokBytes + kCodeStages * kCodeStage + 512;
-  static_assert(kWeights + kW * kSub * 32 <= kCols && kSmem <= 227 * 1024 && kShared % 16 == 0, "");
+  static_assert(kWeights + kW * kSub * 32 <= kCols && kShared % 16 == 0, "");
 };
 
 template <bool kPair>
@@ -70,15 +77,13 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
-// eight codes -> four pairs of bf16, each number times 2^-126
-__device__ __forceinline__ void spread8(uint32_t w, uint32_t (&y)[4]) {
-  const uint32_t even = w & 0x0f0f0f0fu, odd = (w >> 4) & 0x0f0f0f0fu;
+// eight codes -> four pairs of bf16 out of the table; here: this lane's column of it
+__device__ __forceinline__ void look_up8(uint32_t w, uint32_t here, uint32_t (&y)[4]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    // bytes: even's byte i, 0, odd's byte i, 0 (8 + n repeats the sign of byte n, which is 0)
-    uint32_t x;
-    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(x) : "r"(even), "r"(odd), "r"(i | (8 + i) << 4 | (4 + i) << 8 | (12 + i) << 12));
-    y[i] = (x * 0x1040u) & 0x81c081c0u;       // sign to bit 15, the other three to bits 8 .. 6
+    uint32_t at;      // bytes: here's 0, w's byte i, here's 2 and 3
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(at) : "r"(w), "r"(here), "r"(0x7604 | i << 4));
+    asm("ld.shared.u32 %0, [%1];" : "=r"(y[i]) : "r"(at));
   }
 }
 
@@ -94,9 +99,15 @@ mx4_mixed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
   using S = Shape<BT, kPair>;
   constexpr int kCtas = kPair ? 2 : 1, kSteps = kCodeDepth / (kDepth * S::kSub);      // stages of 256 columns
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint8_t* codes_s = smem + S::kTok * S::kTokBytes;
-  uint64_t* tok_full = reinterpret_cast<uint64_t*>(codes_s + kCodeStages * kCodeStage);   // a pair's: in the first CTA, of both
+  // where it lies in the shared window is known, as the kernel has no other; in a cluster the CTA's rank is in the upper bits.  (Were it
+  // somewhere else, all CTAs would leave here, and the launch be reported as one that gave up.)
+  const uint32_t window = smem_u32(smem_raw) - kSmemFrom;
+  if ((window & 0xffffffu) != 0u) {
+    if (threadIdx.x == 0) *failed = 1u;
+    return;
+  }
+  uint8_t *codes_s = smem_raw, *smem = smem_raw + (kTokens - kSmemFrom);
+  uint64_t* tok_full = reinterpret_cast<uint64_t*>(codes_s + kBars);   // a pair's: in the first CTA, of both
   uint64_t* tok_empty = tok_full + S::kTok;
   uint64_t* w_full = tok_empty + S::kTok;          // unpacked weights are in TMEM; a pair's: in the first CTA, of both
   uint64_t* w_empty = w_full + S::kW;
@@ -155,6 +166,11 @@ mx4_mixed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
     mbar_init(drain_bar, 1);
     *gave_up = 0;
     fence_barrier_init();
+  }
+  for (int v = warp; v < 256; v += kThreads / 32) {      // the table
+    const uint32_t lo = v & 15, hi = v >> 4;
+    const float a = mx4_number(lo), b = mx4_number(hi);
+    *reinterpret_cast<uint32_t*>(smem_raw + (kTable - kSmemFrom) + v * 256 + lane * 4) = pack_bf16(a, b);
   }
   if (warp == kMma) {
     if (kPair) tmem_alloc_pair<S::kCols>(tmem_ptr);
@@ -233,14 +249,12 @@ mx4_mixed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
         int n0, m0, count;
         tile_at(it, n0, m0, count);
         const uint32_t idesc = make_idesc_bf16(kCtas * kRowsW, kPair ? pieces.per : (count + 15) & ~15, 0, 0), acc = tmem + (k & 1) * S::kAcc1;
-        if (S::kShared > 0) ok = k == 0 || mbar_wait_limited(&acc_free[0], (k - 1) & 1, gave_up, limit.tries);
-        else ok = mbar_wait_limited(&acc_free[k & 1], ((k >> 1) & 1) ^ 1, gave_up, limit.tries);
-        ok = __all_sync(0xffffffffu, ok);
+        if (S::kShared > 0) ok = k == 0 || mx4_warp_wait(&acc_free[0], (k - 1) & 1, gave_up, limit.tries);
+        else ok = mx4_warp_wait(&acc_free[k & 1], ((k >> 1) & 1) ^ 1, gave_up, limit.tries);
         bool tok_here = false, w_here = false;      // asked a stage ahead: the answer takes a while
         for (int kb = 0; kb < nkb && ok; ++kb) {
-          if (!__all_sync(0xffffffffu, tok_here && w_here))
-            ok = __all_sync(0xffffffffu, mbar_wait_limited(&tok_full[s], ph, gave_up, limit.tries) &&
-                                             mbar_wait_limited(&w_full[w], wph, gave_up, limit.tries));
+          if (!tok_here) ok = mx4_warp_wait(&tok_full[s], ph, gave_up, limit.tries);
+          if (ok && !w_here) ok = mx4_warp_wait(&w_full[w], wph, gave_up, limit.tries);
           if (!ok) break;
           tc_fence_after();
           const uint64_t bd = bd0 + s * (S::kTokBytes >> 4);
@@ -255,8 +269,8 @@ mx4_mixed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
             w = 0;
             wph ^= 1;
           }
-          tok_here = mx4_mbar_test(&tok_full[s], ph);
-          w_here = mx4_mbar_test(&w_full[w], wph);
+          tok_here = mx4_warp_test(&tok_full[s], ph);
+          w_here = mx4_warp_test(&w_full[w], wph);
 #pragma unroll
           for (int i = 0; i < 4 * S::kSub; ++i)
             umma_ts<kPair>(acc, wa + 8 * i, bd + (i / 4) * (S::kTokRows * 128 >> 4) + 2 * (i % 4), idesc, (kb | i) != 0, i < steps ? one : 0u);
@@ -265,20 +279,20 @@ mx4_mixed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
         }
         if (ok) commit(&acc_full[k & 1], one);
       }
-      if (one) {
-        if (!ok) tell();
-        commit(drain_bar, 1);             // products under way end before TMEM and the CTA's memory are given back, too
-        mbar_drain(drain_bar, 0);
-      }
-      __syncwarp();
+      if (!ok && lane == 0) tell();
+      commit(drain_bar, one);      // a pair's: reports to both CTAs
     }
+    // products under way, and what they report to this CTA, end before TMEM and the CTA's memory are given back
+    if (lane == 0 && !mbar_wait_limited(drain_bar, 0, gave_up, limit.tries)) mbar_drain(drain_bar, 0);
+    __syncwarp();
   } else if (warp >= kFirstUnpack) {
     const int group = (warp - kFirstUnpack) >> 2, quad = warp & 3, row = quad * 32 + lane;
+    const uint32_t here = window + kTable + lane * 4;
     int j = 0, cs = 0;                    // stages so far (all tiles), code stage
     uint32_t cph = 0;
     for (int it = worker; it < total && ok; it += workers) {
       for (int kc = 0; kc < nkc && ok; ++kc) {
-        ok = __all_sync(0xffffffffu, mbar_wait_limited(&code_full[cs], cph, gave_up, limit.tries));
+        ok = mx4_warp_wait(&code_full[cs], cph, gave_up, limit.tries);
         if (!ok) break;
         const uint8_t* st = codes_s + cs * kCodeStage;
         const int steps = min(kSteps, nkb - kSteps * kc);
@@ -295,20 +309,14 @@ mx4_mixed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
             const uint32_t c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
             uint32_t y[32];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) spread8(c[e], *reinterpret_cast<uint32_t(*)[4]>(y + 4 * e));
-            if (__all_sync(0xffffffffu, max(b0, b1) <= 128u)) {      // 2^(126 + e) is a bf16 number
-              const uint32_t f0 = (b0 + 126u) * 0x00800080u, f1 = (b1 + 126u) * 0x00800080u;
+            for (int e = 0; e < 8; ++e) look_up8(c[e], here, *reinterpret_cast<uint32_t(*)[4]>(y + 4 * e));
+            // 2^(byte - 127) as a pair of bf16, 0: their subnormal 2^-127, 255: NaN
+            const uint32_t f0 = b0 == 255u ? 0x7fff7fffu : (b0 == 0u ? 0x00400040u : b0 * 0x00800080u);
+            const uint32_t f1 = b1 == 255u ? 0x7fff7fffu : (b1 == 0u ? 0x00400040u : b1 * 0x00800080u);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) y[e] = mul_bf16x2(y[e], e < 16 ? f0 : f1);
-            } else {
-              const uint32_t up = 0x7e807e80u;                       // 2^126, then 2^e
-              const uint32_t f0 = b0 == 255u ? 0x7fff7fffu : (b0 == 0u ? 0x00400040u : b0 * 0x00800080u);
-              const uint32_t f1 = b1 == 255u ? 0x7fff7fffu : (b1 == 0u ? 0x00400040u : b1 * 0x00800080u);
-#pragma unroll
-              for (int e = 0; e < 32; ++e) y[e] = mul_bf16x2(mul_bf16x2(y[e], up), e < 16 ? f0 : f1);
-            }
+            for (int e = 0; e < 32; ++e) y[e] = mul_bf16x2(y[e], e < 16 ? f0 : f1);
             if (i == 0) {
-              ok = __all_sync(0xffffffffu, mbar_wait_limited(&w_empty[w], ((j / S::kW) & 1) ^ 1, gave_up, limit.tries));
+              ok = mx4_warp_wait(&w_empty[w], ((j / S::kW) & 1) ^ 1, gave_up, limit.tries);
               if (!ok) break;
               tc_fence_after();
             }
@@ -337,7 +345,7 @@ mx4_mixed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
       int n0, m0, count;
       tile_at(it, n0, m0, count);
       // all lanes or none: the TMEM loads need the whole warp
-      ok = __all_sync(0xffffffffu, mbar_wait_limited(&acc_full[k & 1], (k >> 1) & 1, gave_up, limit.tries));
+      ok = mx4_warp_wait(&acc_full[k & 1], (k >> 1) & 1, gave_up, limit.tries);
       if (!ok) break;
       tc_fence_after();
       const uint32_t acc = tmem + (static_cast<uint32_t>(quad * 32) << 16) + (k & 1) * S::kAcc1;
@@ -348,7 +356,7 @@ mx4_mixed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
       auto free_acc = [&] {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) arrive_first(&acc_free[S::kShared > 0 ? 0 : k & 1]);
+        if (lane == 0 && it + workers < total) arrive_first(&acc_free[S::kShared > 0 ? 0 : k & 1]);      // someone waits for it
         told = true;
       };
       mx4_with_epilogue(p, [&](auto epi) {
@@ -388,13 +396,13 @@ int launch(const vila_mx4_linear_params& p, const vila_glinear_ext& x, const Pie
   constexpr int kCtas = kPair ? 2 : 1;
   static PerDeviceOnce once;
   if (once.first())
-    VB_CUDA(cudaFuncSetAttribute(mx4_mixed_kernel<BT, kPair>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::kSmem)));
+    VB_CUDA(cudaFuncSetAttribute(mx4_mixed_kernel<BT, kPair>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmem)));
   CUtensorMap tw, tx;
   if (int rc = make_tmap_2d_u8(&tw, p.w_codes, p.N, mx4_pitch(p.K), mx4_pitch(p.K), kRowsW, 128, 128)) return rc;
   if (int rc = make_tmap_2d_bf16(&tx, p.x, p.M, p.K, p.ldx, pieces.per / kCtas, kDepth, 128)) return rc;
   const long long tiles = static_cast<long long>((p.N + kCtas * kRowsW - 1) / (kCtas * kRowsW)) * pieces.n, most = num_sms() / kCtas;
   VB_CHECK(tiles < (1LL << 30), "mx4_linear: too many tiles (M=%d N=%d)", p.M, p.N);
-  VB_CUDA(launch_serial_cluster(mx4_mixed_kernel<BT, kPair>, dim3(static_cast<unsigned>(kCtas * (tiles < most ? tiles : most))), dim3(kThreads), S::kSmem, stream,
+  VB_CUDA(launch_serial_cluster(mx4_mixed_kernel<BT, kPair>, dim3(static_cast<unsigned>(kCtas * (tiles < most ? tiles : most))), dim3(kThreads), kSmem, stream,
                                 dim3(kCtas), tw, tx, p, x, pieces, wait_limit(tries), failed_word()));
   return 0;
 }

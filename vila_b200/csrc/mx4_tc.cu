@@ -195,7 +195,7 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant_
       int p0, q0;
       tile_at(it, p0, q0);
       // all lanes or none: the TMEM loads need the whole warp
-      ok = __all_sync(0xffffffffu, mbar_wait_limited(&acc_full[k & 1], (k >> 1) & 1, gave_up, limit.tries));
+      ok = mx4_warp_wait(&acc_full[k & 1], (k >> 1) & 1, gave_up, limit.tries);
       if (!ok) break;
       tc_fence_after();
       const uint32_t acc = tmem + (static_cast<uint32_t>(quad * 32) << 16) + (k & 1) * BN;
@@ -363,10 +363,10 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
       uint32_t ph = 0;
       for (int it = worker; it < total && ok; it += workers, ++k) {
         const uint32_t acc = tmem + (k & 1) * kAcc1;
-        if (k > 0) ok = __all_sync(0xffffffffu, mbar_wait_limited(shared_free, (k - 1) & 1, gave_up, limit.tries));
-        bool here = mx4_mbar_test(&full_bar[s], ph);      // asked a stage ahead: the answer takes longer than a stage has
+        if (k > 0) ok = mx4_warp_wait(shared_free, (k - 1) & 1, gave_up, limit.tries);
+        bool here = mx4_warp_test(&full_bar[s], ph);      // asked a stage ahead: the answer takes longer than a stage has
         for (int kb = 0; kb < nkb && ok; ++kb) {
-          if (!__all_sync(0xffffffffu, here)) ok = __all_sync(0xffffffffu, mbar_wait_limited(&full_bar[s], ph, gave_up, limit.tries));
+          if (!here) ok = mx4_warp_wait(&full_bar[s], ph, gave_up, limit.tries);
           if (!ok) break;
           tc_fence_after();
           const uint32_t ts = tmem + kScaleCol + s * kScaleCols, tq = ts + 8;
@@ -376,7 +376,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
             s = 0;
             ph ^= 1;
           }
-          here = mx4_mbar_test(&full_bar[s], ph);
+          here = mx4_warp_test(&full_bar[s], ph);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             scales_to_tmem_pair(ts + 4 * h, sd + 32 * h, one);
@@ -391,13 +391,12 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
         }
         if (ok) mx4_commit_pair(&acc_full[k & 1], one);
       }
-      if (one) {
-        if (!ok) tell();
-        umma_commit_pair(drain_bar);
-        mbar_drain(drain_bar, 0);
-      }
-      __syncwarp();
+      if (!ok && lane == 0) tell();
+      mx4_commit_pair(drain_bar, one);      // reports to both CTAs
     }
+    // products under way, and what they report to this CTA, end before TMEM and the CTA's memory are given back
+    if (lane == 0 && !mbar_wait_limited(drain_bar, 0, gave_up, limit.tries)) mbar_drain(drain_bar, 0);
+    __syncwarp();
   } else {
     const int quad = warp & 3, half = warp >> 2;
     const bool wide = reinterpret_cast<uintptr_t>(p.out) % 32 == 0 && p.ldo % 16 == 0;
@@ -406,7 +405,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
     for (int it = worker; it < total && ok; it += workers, ++k) {
       int p0, q0;
       tile_at(it, p0, q0);
-      ok = __all_sync(0xffffffffu, ok && mbar_wait_limited(&acc_full[k & 1], (k >> 1) & 1, gave_up, limit.tries));
+      ok = mx4_warp_wait(&acc_full[k & 1], (k >> 1) & 1, gave_up, limit.tries);
       if (!ok) break;
       tc_fence_after();
       const uint32_t acc = tmem + (static_cast<uint32_t>(quad * 32) << 16) + (k & 1) * kAcc1;
@@ -422,7 +421,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
           if (i + 2 >= kShared / 32 && i < kShared / 32) {      // this warp's last one of them
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive_cluster_relaxed(free_bar);
+            if (lane == 0 && it + workers < total) mbar_arrive_cluster_relaxed(free_bar);      // someone waits for it
           }
           if (q0 + c < p.N) mx4_store_row<EPI>(p, x, r, row, q0 + c, wide);
         }
