@@ -61,8 +61,8 @@ __device__ __forceinline__ uint32_t mx4_encode8(const float (&v)[8]) {
   return d;
 }
 
-// A warp's wait on an mbarrier that no lane leaves before the others: the warps that issue tcgen05 instructions stay converged, so that
-// what they hold in uniform registers is one value.  (Lanes that left the wait one by one, or one lane that waited for all, ended in
+// A warp's wait on an mbarrier that no lane leaves before the others: the warps that issue tcgen05 instructions stay converged but for
+// the one branch in which a lane issues them, so that what these take from uniform registers is one value.  (Lanes that left the wait one by one, or one lane that waited for all, ended in
 // launch failures.)
 __device__ __forceinline__ bool mx4_warp_wait(uint64_t* bar, uint32_t parity, volatile int* gave_up, int tries) {
   for (int i = 0; i < tries; ++i) {
@@ -72,26 +72,13 @@ __device__ __forceinline__ bool mx4_warp_wait(uint64_t* bar, uint32_t parity, vo
   *gave_up = 1;
   return false;
 }
-// whether an mbarrier's phase is over, without waiting for it; the same answer for all lanes
-__device__ __forceinline__ bool mx4_warp_test(uint64_t* bar, uint32_t parity) {
+// Whether an mbarrier's phase is over, without waiting for it.  The answer takes about 200 clocks: it is asked for a stage ahead, and the
+// lanes vote on it (__all_sync) when they need it.
+__device__ __forceinline__ uint32_t mx4_test(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
   asm volatile("{.reg .pred P; mbarrier.test_wait.parity.shared::cta.b64 P, [%1], %2; selp.u32 %0, 1, 0, P;}"
                : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
-  return __all_sync(0xffffffffu, ok != 0);
-}
-// umma_commit / umma_commit_pair by the lanes whose `one` is set (one lane), with no branch around it
-__device__ __forceinline__ void mx4_commit(uint64_t* bar, uint32_t one) {
-  asm volatile(
-      "{.reg .pred q; setp.ne.b32 q, %1, 0;\n\t"
-      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];}" ::"r"(smem_u32(bar)), "r"(one)
-      : "memory");
-}
-__device__ __forceinline__ void mx4_commit_pair(uint64_t* bar, uint32_t one) {
-  asm volatile(
-      "{.reg .pred q; setp.ne.b32 q, %1, 0;\n\t"
-      "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %2;}" ::"r"(smem_u32(bar)), "r"(one),
-      "h"(static_cast<uint16_t>(3))
-      : "memory");
+  return ok;
 }
 // consecutive bytes (a multiple of 16, on 16-byte boundaries)
 __device__ __forceinline__ void mx4_bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {

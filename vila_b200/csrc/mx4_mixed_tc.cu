@@ -52,24 +52,22 @@ template <int BT, bool kPair> struct Shape {
 };
 
 template <bool kPair>
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate, uint32_t one) {
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   if (kPair)
     asm volatile(
         "{\n\t"
-        ".reg .pred p, q;\n\t"
+        ".reg .pred p;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "setp.ne.b32 q, %5, 0;\n\t"
-        "@q tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t"
-        "}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(one)
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+        "}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
         : "memory");
   else
     asm volatile(
         "{\n\t"
-        ".reg .pred p, q;\n\t"
+        ".reg .pred p;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "setp.ne.b32 q, %5, 0;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
-        "}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(one)
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+        "}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
 __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
@@ -134,9 +132,9 @@ mx4_mixed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
     if (kPair) mbar_arrive_cluster_relaxed(in_first(bar));
     else mbar_arrive(bar);
   };
-  auto commit = [&](uint64_t* bar, uint32_t one) {
-    if (kPair) mx4_commit_pair(bar, one);
-    else mx4_commit(bar, one);
+  auto commit = [&](uint64_t* bar) {
+    if (kPair) umma_commit_pair(bar);
+    else umma_commit(bar);
   };
   // a warp that gives up tells the other CTA, too
   auto tell = [&] {
@@ -241,7 +239,7 @@ mx4_mixed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
   } else if (warp == kMma) {
     if (rank == 0) {
       // The whole warp walks the loop and one lane issues: what the instructions are given stays in uniform registers.
-      const uint32_t one = elect_one() ? 1u : 0u;
+      const bool one = elect_one();
       const uint64_t bd0 = make_smem_desc(smem_u32(smem), 16, 1024, kLayoutSW128);
       int k = 0, s = 0, w = 0;
       uint32_t ph = 0, wph = 0;
@@ -251,15 +249,14 @@ mx4_mixed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
         const uint32_t idesc = make_idesc_bf16(kCtas * kRowsW, kPair ? pieces.per : (count + 15) & ~15, 0, 0), acc = tmem + (k & 1) * S::kAcc1;
         if (S::kShared > 0) ok = k == 0 || mx4_warp_wait(&acc_free[0], (k - 1) & 1, gave_up, limit.tries);
         else ok = mx4_warp_wait(&acc_free[k & 1], ((k >> 1) & 1) ^ 1, gave_up, limit.tries);
-        bool tok_here = false, w_here = false;      // asked a stage ahead: the answer takes a while
+        uint32_t tok_here = 0, w_here = 0;
         for (int kb = 0; kb < nkb && ok; ++kb) {
-          if (!tok_here) ok = mx4_warp_wait(&tok_full[s], ph, gave_up, limit.tries);
-          if (ok && !w_here) ok = mx4_warp_wait(&w_full[w], wph, gave_up, limit.tries);
+          if (!__all_sync(0xffffffffu, tok_here & w_here))
+            ok = mx4_warp_wait(&tok_full[s], ph, gave_up, limit.tries) && mx4_warp_wait(&w_full[w], wph, gave_up, limit.tries);
           if (!ok) break;
           tc_fence_after();
           const uint64_t bd = bd0 + s * (S::kTokBytes >> 4);
           const uint32_t wa = tmem + S::kWeights + 32 * S::kSub * w;
-          const int steps = (p.K - kb * S::kSub * kDepth + 15) / 16;
           uint64_t *tok_done = &tok_empty[s], *w_done = &w_empty[w];
           if (++s == S::kTok) {
             s = 0;
@@ -269,18 +266,22 @@ mx4_mixed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
             w = 0;
             wph ^= 1;
           }
-          tok_here = mx4_warp_test(&tok_full[s], ph);
-          w_here = mx4_warp_test(&w_full[w], wph);
+          tok_here = mx4_test(&tok_full[s], ph);
+          w_here = mx4_test(&w_full[w], wph);
+          if (one) {      // columns past K are zeros on both sides
 #pragma unroll
-          for (int i = 0; i < 4 * S::kSub; ++i)
-            umma_ts<kPair>(acc, wa + 8 * i, bd + (i / 4) * (S::kTokRows * 128 >> 4) + 2 * (i % 4), idesc, (kb | i) != 0, i < steps ? one : 0u);
-          commit(tok_done, one);
-          commit(w_done, one);
+            for (int i = 0; i < 4 * S::kSub; ++i)
+              umma_ts<kPair>(acc, wa + 8 * i, bd + (i / 4) * (S::kTokRows * 128 >> 4) + 2 * (i % 4), idesc, (kb | i) != 0);
+            commit(tok_done);
+            commit(w_done);
+          }
+          __syncwarp();
         }
-        if (ok) commit(&acc_full[k & 1], one);
+        if (ok && one) commit(&acc_full[k & 1]);
+        __syncwarp();
       }
       if (!ok && lane == 0) tell();
-      commit(drain_bar, one);      // a pair's: reports to both CTAs
+      if (one) commit(drain_bar);      // a pair's: reports to both CTAs
     }
     // products under way, and what they report to this CTA, end before TMEM and the CTA's memory are given back
     if (lane == 0 && !mbar_wait_limited(drain_bar, 0, gave_up, limit.tries)) mbar_drain(drain_bar, 0);

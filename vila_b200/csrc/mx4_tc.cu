@@ -54,9 +54,8 @@ __device__ __forceinline__ void umma_mx4(uint32_t d, uint64_t a, uint64_t b, uin
       : "memory");
 }
 // 512 bytes (32 rows of 16) -> 4 TMEM columns, in each of the four lane quarters
-__device__ __forceinline__ void scales_to_tmem(uint32_t taddr, uint32_t smem_addr) {
-  const uint64_t d = make_smem_desc(smem_addr, 16, 128, kLayoutNone);
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
+__device__ __forceinline__ void scales_to_tmem(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 template <int BN, bool kSwap>
 __global__ void __launch_bounds__(kThreads, Shape<BN>::kPerSm)
@@ -146,47 +145,53 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant_
       }
     }
   } else if (warp == kMma) {
-    if (lane == 0) {
-      int s = 0, k = 0;
-      uint32_t ph = 0;
-      for (int it = blockIdx.x; it < total && ok; it += gridDim.x, ++k) {
-        int p0, q0;
-        tile_at(it, p0, q0);
-        const uint32_t n = kSwap ? min(BN, (Q - q0 + 15) & ~15) : BN, acc = tmem + (k & 1) * BN;
-        ok = mbar_wait_limited(&acc_free[k & 1], ((k >> 1) & 1) ^ 1, gave_up, limit.tries);
+    // The whole warp walks the loop and one lane issues: what the instructions are given stays in uniform registers.
+    const bool one = elect_one();
+    const uint64_t ad0 = make_smem_desc(smem_u32(smem), 16, 1024, kLayoutSW128), bd0 = make_smem_desc(smem_u32(smem) + S::kPBytes, 16, 1024, kLayoutSW128);
+    const uint64_t sd0 = make_smem_desc(smem_u32(smem) + S::kPBytes + S::kQBytes, 16, 128, kLayoutNone);
+    int s = 0, k = 0;
+    uint32_t ph = 0;
+    for (int it = blockIdx.x; it < total && ok; it += gridDim.x, ++k) {
+      int p0, q0;
+      tile_at(it, p0, q0);
+      const uint32_t n = kSwap ? min(BN, (Q - q0 + 15) & ~15) : BN, acc = tmem + (k & 1) * BN;
+      const uint32_t idesc = idesc_mx4(kP, n, 0), idesc2 = idesc_mx4(kP, n, 2);
+      ok = mx4_warp_wait(&acc_free[k & 1], ((k >> 1) & 1) ^ 1, gave_up, limit.tries);
+      uint32_t here = mx4_test(&full_bar[s], ph);
+      for (int kb = 0; kb < nkb && ok; ++kb) {
+        if (!__all_sync(0xffffffffu, here)) ok = mx4_warp_wait(&full_bar[s], ph, gave_up, limit.tries);
+        if (!ok) break;
         tc_fence_after();
-        for (int kb = 0; kb < nkb && ok; ++kb) {
-          ok = mbar_wait_limited(&full_bar[s], ph, gave_up, limit.tries);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t st = smem_u32(smem + s * S::kStage), sc = st + S::kPBytes + S::kQBytes;
-          // Every stage has TMEM columns of its own for its scales: P's 128 columns twice, then Q's by column tile.  They are free
-          // when the stage's shared memory is, which full_bar has said.
-          const uint32_t ts = tmem + 2 * BN + s * S::kScaleCols, tq = ts + 8;
+        // Every stage has TMEM columns of its own for its scales: P's 128 columns twice, then Q's by column tile.  They are free
+        // when the stage's shared memory is, which full_bar has said.
+        const uint32_t ts = tmem + 2 * BN + s * S::kScaleCols, tq = ts + 8;
+        const uint64_t ad = ad0 + s * (S::kStage >> 4), bd = bd0 + s * (S::kStage >> 4), sd = sd0 + s * (S::kStage >> 4);
+        uint64_t* done = &empty_bar[s];
+        if (++s == ST) {
+          s = 0;
+          ph ^= 1;
+        }
+        here = mx4_test(&full_bar[s], ph);
+        if (one) {      // columns past K are zeros on both sides
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            scales_to_tmem(ts + 4 * h, sc + 512 * h);
+            scales_to_tmem(ts + 4 * h, sd + 32 * h);
 #pragma unroll
-            for (int q = 0; q < S::kQTiles; ++q) scales_to_tmem(tq + 4 * (S::kQTiles * h + q), sc + 1024 * (1 + q) + 512 * h);
+            for (int q = 0; q < S::kQTiles; ++q) scales_to_tmem(tq + 4 * (S::kQTiles * h + q), sd + 64 * (1 + q) + 32 * h);
           }
-          const uint64_t ad = make_smem_desc(st, 16, 1024, kLayoutSW128), bd = make_smem_desc(st + S::kPBytes, 16, 1024, kLayoutSW128);
-          const int steps = min(4, (p.K - kb * kDepth + 63) / 64);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (j >= steps) break;
-            umma_mx4(acc, ad + 2 * j, bd + 2 * j, idesc_mx4(kP, n, 2 * (j & 1)), ts + 4 * (j >> 1), tq + 4 * S::kQTiles * (j >> 1), (kb | j) != 0);
-          }
-          umma_commit(&empty_bar[s]);
-          if (++s == ST) {
-            s = 0;
-            ph ^= 1;
-          }
+          for (int j = 0; j < 4; ++j)
+            umma_mx4(acc, ad + 2 * j, bd + 2 * j, j & 1 ? idesc2 : idesc, ts + 4 * (j >> 1), tq + 4 * S::kQTiles * (j >> 1), (kb | j) != 0);
+          umma_commit(done);
         }
-        if (ok) umma_commit(&acc_full[k & 1]);
+        __syncwarp();
       }
-      umma_commit(drain_bar);             // products under way end before TMEM and the CTA's memory are given back, too
-      mbar_drain(drain_bar, 0);
+      if (ok && one) umma_commit(&acc_full[k & 1]);
+      __syncwarp();
     }
+    if (one) umma_commit(drain_bar);             // products under way end before TMEM and the CTA's memory are given back, too
+    if (lane == 0) mbar_drain(drain_bar, 0);
+    __syncwarp();
   } else {
     const int quad = warp & 3, half = warp >> 2;
     const bool wide = reinterpret_cast<uintptr_t>(p.out) % 32 == 0 && p.ldo % 16 == 0;
@@ -247,25 +252,18 @@ constexpr int kAcc1 = kN - kShared, kScaleCol = 2 * kN - kShared, kScaleCols = 2
 constexpr size_t kSmem = 1024 + static_cast<size_t>(kStages) * kStage + 256;
 static_assert(kScaleCol + kStages * kScaleCols <= 512 && kShared % 32 == 0 && kSmem <= 227 * 1024, "");
 
-__device__ __forceinline__ void umma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t accumulate, uint32_t one) {
+__device__ __forceinline__ void umma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t accumulate) {
   asm volatile(
       "{\n\t"
-      ".reg .pred p, q;\n\t"
+      ".reg .pred p;\n\t"
       "setp.ne.b32 p, %6, 0;\n\t"
-      "setp.ne.b32 q, %7, 0;\n\t"
-      "@q tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t"
-      "}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate), "r"(one)
+      "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t"
+      "}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
       : "memory");
 }
 // in both CTAs, each from its own shared memory
-__device__ __forceinline__ void scales_to_tmem_pair(uint32_t taddr, uint64_t desc, uint32_t one) {
-  asm volatile(
-      "{\n\t"
-      ".reg .pred q;\n\t"
-      "setp.ne.b32 q, %2, 0;\n\t"
-      "@q tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n\t"
-      "}\n" ::"r"(taddr), "l"(desc), "r"(one)
-      : "memory");
+__device__ __forceinline__ void scales_to_tmem_pair(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 
 __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
@@ -356,7 +354,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
   } else if (warp == kMma) {
     if (rank == 0) {
       // The whole warp walks the loop and one lane issues: what the instructions are given stays in uniform registers.
-      const uint32_t one = elect_one() ? 1u : 0u;
+      const bool one = elect_one();
       const uint64_t ad0 = make_smem_desc(smem_u32(smem), 16, 1024, kLayoutSW128), bd0 = make_smem_desc(smem_u32(smem) + kPBytes, 16, 1024, kLayoutSW128);
       const uint64_t sd0 = make_smem_desc(smem_u32(smem) + kPBytes + kQBytes, 16, 128, kLayoutNone);
       int k = 0, s = 0;                   // tiles so far, stage
@@ -364,9 +362,9 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
       for (int it = worker; it < total && ok; it += workers, ++k) {
         const uint32_t acc = tmem + (k & 1) * kAcc1;
         if (k > 0) ok = mx4_warp_wait(shared_free, (k - 1) & 1, gave_up, limit.tries);
-        bool here = mx4_warp_test(&full_bar[s], ph);      // asked a stage ahead: the answer takes longer than a stage has
+        uint32_t here = mx4_test(&full_bar[s], ph);
         for (int kb = 0; kb < nkb && ok; ++kb) {
-          if (!here) ok = mx4_warp_wait(&full_bar[s], ph, gave_up, limit.tries);
+          if (!__all_sync(0xffffffffu, here)) ok = mx4_warp_wait(&full_bar[s], ph, gave_up, limit.tries);
           if (!ok) break;
           tc_fence_after();
           const uint32_t ts = tmem + kScaleCol + s * kScaleCols, tq = ts + 8;
@@ -376,23 +374,26 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
             s = 0;
             ph ^= 1;
           }
-          here = mx4_warp_test(&full_bar[s], ph);
+          here = mx4_test(&full_bar[s], ph);
+          if (one) {      // columns past K are zeros on both sides
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            scales_to_tmem_pair(ts + 4 * h, sd + 32 * h, one);
-            scales_to_tmem_pair(tq + 8 * h, sd + 64 + 32 * h, one);
-            scales_to_tmem_pair(tq + 8 * h + 4, sd + 128 + 32 * h, one);
+            for (int h = 0; h < 2; ++h) {
+              scales_to_tmem_pair(ts + 4 * h, sd + 32 * h);
+              scales_to_tmem_pair(tq + 8 * h, sd + 64 + 32 * h);
+              scales_to_tmem_pair(tq + 8 * h + 4, sd + 128 + 32 * h);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              umma(acc, ad + 2 * i, bd + 2 * i, idesc_mx4(256, kN, 2 * (i & 1)), ts + 4 * (i >> 1), tq + 8 * (i >> 1), (kb | i) != 0);
+            umma_commit_pair(done);
           }
-          const int steps = min(4, (p.K - kb * kDepth + 63) / 64);
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            umma(acc, ad + 2 * i, bd + 2 * i, idesc_mx4(256, kN, 2 * (i & 1)), ts + 4 * (i >> 1), tq + 8 * (i >> 1), (kb | i) != 0, i < steps ? one : 0u);
-          mx4_commit_pair(done, one);
+          __syncwarp();
         }
-        if (ok) mx4_commit_pair(&acc_full[k & 1], one);
+        if (ok && one) umma_commit_pair(&acc_full[k & 1]);
+        __syncwarp();
       }
       if (!ok && lane == 0) tell();
-      mx4_commit_pair(drain_bar, one);      // reports to both CTAs
+      if (one) umma_commit_pair(drain_bar);      // reports to both CTAs
     }
     // products under way, and what they report to this CTA, end before TMEM and the CTA's memory are given back
     if (lane == 0 && !mbar_wait_limited(drain_bar, 0, gave_up, limit.tries)) mbar_drain(drain_bar, 0);
