@@ -6,7 +6,7 @@
 // unpacks its own row writes with one tcgen05.st.  Shared memory then only serves the tokens, the N side.
 //
 //   TMA warp         codes and scales, 256 columns of 128 rows at a time; a stage of tokens (64 columns, 128 bytes, swizzled)
-//   8 unpack warps   two groups of four (a warp reaches the TMEM lanes of its quarter), which take the stages in turn: a byte of
+//   unpack warps     two or three groups of four (a warp reaches the TMEM lanes of its quarter), which take the stages in turn: a byte of
 //                    codes (two weights) is looked up in shared memory as a pair of bf16, then multiplied by the block's 2^e
 //   MMA warp         TMEM allocation; tcgen05.mma of K = 16, four per 64 columns, into one of two accumulator sets
 //   8 epilogue warps TMEM lane = weight row, column = token, under the next tile's products
@@ -30,7 +30,7 @@ namespace vb {
 namespace {
 
 constexpr int kRowsW = 128, kDepth = 64, kCodeDepth = 256;
-constexpr int kEpi = 8, kUnpack = 8, kFirstUnpack = kEpi, kTma = kEpi + kUnpack, kMma = kTma + 1, kThreads = 32 * (kMma + 1);
+constexpr int kEpi = 8, kFirstUnpack = kEpi;
 constexpr int kCodeBytes = kRowsW * 128, kCodeStage = kCodeBytes + 1024, kCodeStages = 3;
 // Shared memory by addresses of the shared window: codes and barriers, the table from 64 KB on, tokens behind it
 constexpr uint32_t kTable = 0x10000, kTokens = 0x20000, kTokensBytes = 96 * 1024, kBars = kCodeStages * kCodeStage, kLow = kBars + 1024;
@@ -39,11 +39,14 @@ constexpr size_t kSmem = kTokens + kTokensBytes - kSmemFrom;
 static_assert(kSmemFrom + kLow <= kTable && kSmem <= 227 * 1024, "");
 
 template <int BT, bool kPair> struct Shape {
-  static constexpr int kSub = BT > 64 ? 1 : 2;                  // times 64 columns are a stage
+  static constexpr int kGroups = kPair ? 2 : 3;                 // of four unpack warps
+  static constexpr int kUnpack = 4 * kGroups, kTma = kEpi + kUnpack, kMma = kTma + 1, kThreads = 32 * (kMma + 1);
+  // times 64 columns are a stage: of one, the issuing warp's 400 clocks a stage showed (17 rows, 3584 x 3584: 22.2 us, of two 19.1)
+  static constexpr int kSub = kPair ? 1 : 2;
   static constexpr int kTokRows = kPair ? BT / 2 : BT;          // that a CTA holds
   static constexpr int kTokBytes = kSub * kTokRows * 128;
   static constexpr int kTok = kTokensBytes / kTokBytes;         // stages of tokens
-  static constexpr int kW = BT > 128 ? 4 : (BT > 64 ? 8 : 4);   // stages of unpacked weights
+  static constexpr int kW = 4;                                  // stages of unpacked weights
   static constexpr int kAcc1 = BT > 128 ? 128 : BT;             // the second accumulator's first column
   static constexpr int kShared = BT - kAcc1;
   static constexpr int kWeights = kAcc1 + BT;                   // first column of the unpacked weights
@@ -91,10 +94,11 @@ struct Pieces {
 };
 
 template <int BT, bool kPair>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Shape<BT, kPair>::kThreads, 1)
 mx4_mixed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const vila_mx4_linear_params p,
                  const vila_glinear_ext x, const Pieces pieces, const WaitLimit limit, volatile unsigned int* failed) {
   using S = Shape<BT, kPair>;
+  constexpr int kUnpack = S::kUnpack, kTma = S::kTma, kMma = S::kMma;
   constexpr int kCtas = kPair ? 2 : 1, kSteps = kCodeDepth / (kDepth * S::kSub);      // stages of 256 columns
   extern __shared__ uint8_t smem_raw[];
   // where it lies in the shared window is known, as the kernel has no other; in a cluster the CTA's rank is in the upper bits.  (Were it
@@ -165,7 +169,7 @@ mx4_mixed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
     *gave_up = 0;
     fence_barrier_init();
   }
-  for (int v = warp; v < 256; v += kThreads / 32) {      // the table
+  for (int v = warp; v < 256; v += S::kThreads / 32) {      // the table
     const uint32_t lo = v & 15, hi = v >> 4;
     const float a = mx4_number(lo), b = mx4_number(hi);
     *reinterpret_cast<uint32_t*>(smem_raw + (kTable - kSmemFrom) + v * 256 + lane * 4) = pack_bf16(a, b);
@@ -298,7 +302,7 @@ mx4_mixed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
         const uint8_t* st = codes_s + cs * kCodeStage;
         const int steps = min(kSteps, nkb - kSteps * kc);
         for (int step = 0; step < steps && ok; ++step, ++j) {
-          if ((j & 1) != group) continue;
+          if (j % S::kGroups != group) continue;
           const int w = j % S::kW;
 #pragma unroll
           for (int i = 0; i < S::kSub; ++i) {
@@ -364,7 +368,7 @@ mx4_mixed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
         constexpr int EPI = decltype(epi)::value;
 #pragma unroll 1
         for (int i = half; i < BT / 16; i += 2) {
-          const int c = (first + 16 * i) & (BT - 1);
+          const int c = S::kShared > 0 ? (first + 16 * i) & (BT - 1) : 16 * i;
           if (S::kShared > 0 && !told && i >= S::kShared / 16) free_acc();
           if (c >= count) continue;
           float r[16];
@@ -403,7 +407,7 @@ int launch(const vila_mx4_linear_params& p, const vila_glinear_ext& x, const Pie
   if (int rc = make_tmap_2d_bf16(&tx, p.x, p.M, p.K, p.ldx, pieces.per / kCtas, kDepth, 128)) return rc;
   const long long tiles = static_cast<long long>((p.N + kCtas * kRowsW - 1) / (kCtas * kRowsW)) * pieces.n, most = num_sms() / kCtas;
   VB_CHECK(tiles < (1LL << 30), "mx4_linear: too many tiles (M=%d N=%d)", p.M, p.N);
-  VB_CUDA(launch_serial_cluster(mx4_mixed_kernel<BT, kPair>, dim3(static_cast<unsigned>(kCtas * (tiles < most ? tiles : most))), dim3(kThreads), kSmem, stream,
+  VB_CUDA(launch_serial_cluster(mx4_mixed_kernel<BT, kPair>, dim3(static_cast<unsigned>(kCtas * (tiles < most ? tiles : most))), dim3(S::kThreads), kSmem, stream,
                                 dim3(kCtas), tw, tx, p, x, pieces, wait_limit(tries), failed_word()));
   return 0;
 }
@@ -419,10 +423,11 @@ int mx4_mixed_tc(const vila_mx4_linear_params& p, const vila_glinear_ext& x, int
   const int n_tiles = (p.N + kRowsW - 1) / kRowsW;
   Pieces pc;
   pc.n = (p.M + 255) / 256;
-  while (pc.n * n_tiles < num_sms() && (p.M + pc.n) / (pc.n + 1) >= 48) ++pc.n;      // shorter tiles where SMs would stand idle
+  while ((pc.n + 1) * n_tiles <= num_sms() && (p.M + pc.n) / (pc.n + 1) >= 48) ++pc.n;      // shorter tiles where SMs would stand idle
   pc.per = ((p.M + pc.n - 1) / pc.n + 15) & ~15;
   pc.n = (p.M + pc.per - 1) / pc.per;
   if (pc.per <= 64) return launch<64, false>(p, x, pc, tries, stream);
+  if (pc.per <= 96) return launch<96, false>(p, x, pc, tries, stream);
   if (pc.per <= 128) return launch<128, false>(p, x, pc, tries, stream);
   pc.per = (pc.per + 31) & ~31;
   pc.n = (p.M + pc.per - 1) / pc.per;

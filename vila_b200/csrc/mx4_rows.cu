@@ -31,15 +31,17 @@ constexpr int kWarps = 8, kThreads = 32 * kWarps;
 constexpr int kRows = 128;                       // weight rows of a CTA
 constexpr int kStages = 6;                       // of a warp's ring, 128 columns each
 constexpr int kStage = 16 * 64 + 64;             // 16 rows of codes, their scale words
-constexpr int kChunk = 1024;                     // columns whose tokens are in shared memory at a time
-constexpr int kTokPitch = kChunk + 32;           // f16: 64 bytes off the bank of the row before
+constexpr int kTokBytes = 36 * 1024;             // of tokens that are in shared memory at a time
 
+// Columns whose tokens fit: all of a CTA's, if they do (one token: up to 16384)
+__host__ __device__ __forceinline__ int chunk_of(int tokens, int columns) {
+  const int most = (kTokBytes / tokens - 64) * 8 / 17 / 256 * 256;      // 2 bytes a column, 4 a block (and 64 bytes a row)
+  return columns < most ? (columns + 255) / 256 * 256 : most;
+}
 template <int TM> struct Smem {
-  static constexpr int kTok = TM * kTokPitch * 2;
-  static constexpr int kTokScale = TM * (kChunk / 32) * 4;
   static constexpr int kRing = kWarps * kStages * kStage;
   static constexpr int kRed = kRows * (TM + 1) * 4;
-  static constexpr int kTotal = kTok + kTokScale + kRing + kRed;
+  static constexpr int kTotal = kTokBytes + kRing + kRed;
 };
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t a0, const uint32_t a1, const uint32_t a2, const uint32_t a3,
@@ -61,11 +63,11 @@ __device__ __forceinline__ void scales2(uint32_t word, int h, float& s0, float& 
   s1 = bf_hi(d);
 }
 
-// The tokens of columns [k0, k0 + kChunk) as f16, with their scales; a warp takes 256 columns of a token, a lane 8.
+// The tokens of columns [k0, k0 + chunk) as f16, with their scales; a warp takes 256 columns of a token, a lane 8.
 template <int TM>
-__device__ __forceinline__ void stage_tokens(const vila_mx4_linear_params& p, int m0, int k0, int k1, __half* tok, float* tok_scale) {
+__device__ __forceinline__ void stage_tokens(const vila_mx4_linear_params& p, int m0, int k0, int k1, int chunk, __half* tok, float* tok_scale) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tokens = min(TM, p.M - m0);
-  const int pieces = (min(k1 - k0, kChunk) + 255) / 256;
+  const int pieces = (min(k1 - k0, chunk) + 255) / 256, pitch16 = chunk + 32;      // 64 bytes off the bank of the row before
   for (int it = warp; it < tokens * pieces; it += kWarps) {
     const int m = it / pieces, c = (it - m * pieces) * 256 + lane * 8, k = k0 + c;
     uint32_t h[4];
@@ -108,8 +110,8 @@ __device__ __forceinline__ void stage_tokens(const vila_mx4_linear_params& p, in
       }
       back = ldexpf(1.f, -up);
     }
-    *reinterpret_cast<uint4*>(tok + m * kTokPitch + c) = make_uint4(h[0], h[1], h[2], h[3]);
-    if ((lane & 3) == 0) tok_scale[(c >> 5) * TM + m] = back;
+    *reinterpret_cast<uint4*>(tok + m * pitch16 + c) = make_uint4(h[0], h[1], h[2], h[3]);
+    if ((lane & 3) == 0) tok_scale[(c >> 5) * tokens + m] = back;
   }
 }
 
@@ -118,9 +120,7 @@ __global__ void __launch_bounds__(kThreads)
 mx4_rows_kernel(const vila_mx4_linear_params p, const vila_glinear_ext ext, int split) {
   constexpr int NT = TM / 8;
   extern __shared__ __align__(128) uint8_t smem[];
-  __half* tok = reinterpret_cast<__half*>(smem);
-  float* tok_scale = reinterpret_cast<float*>(smem + Smem<TM>::kTok);
-  uint8_t* ring_all = smem + Smem<TM>::kTok + Smem<TM>::kTokScale;
+  uint8_t* ring_all = smem + kTokBytes;
   float* red = reinterpret_cast<float*>(ring_all + Smem<TM>::kRing);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -128,6 +128,9 @@ mx4_rows_kernel(const vila_mx4_linear_params p, const vila_glinear_ext ext, int 
   const int pitch = mx4_pitch(p.K), kts = mx4_ktiles(p.K), nk = (p.K + 127) / 128;
   const int kt0 = static_cast<int>(static_cast<long long>(nk) * rank / split), kt1 = static_cast<int>(static_cast<long long>(nk) * (rank + 1) / split);
   uint8_t* ring = ring_all + warp * (kStages * kStage);
+  const int tokens = min(TM, p.M - m0), chunk = chunk_of(tokens, (kt1 - kt0) * 128), tok_pitch = chunk + 32;
+  __half* tok = reinterpret_cast<__half*>(smem);
+  float* tok_scale = reinterpret_cast<float*>(smem + tokens * tok_pitch * 2);
 
   // this lane's part of a stage: two pieces of codes (rows i0, i0 + 8 of the warp's 16), lanes 0 .. 3 one of scales
   const int i0 = lane >> 2, b0 = lane & 3;
@@ -150,16 +153,24 @@ mx4_rows_kernel(const vila_mx4_linear_params p, const vila_glinear_ext ext, int 
 #pragma unroll
   for (int s = 0; s < kStages - 1; ++s) fetch(kt0 + s, s);
 
+  // this lane's token of an operand and its two of a sum; columns past the last token repeat it and are not read
+  int row[NT], col0[NT], col1[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    row[j] = min(j * 8 + g, tokens - 1) * tok_pitch;
+    col0[j] = min(j * 8 + 2 * t, tokens - 1);
+    col1[j] = min(j * 8 + 2 * t + 1, tokens - 1);
+  }
   float acc[NT][4];
 #pragma unroll
   for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
 
   int stage = 0;
-  for (int kc = kt0; kc < kt1; kc += kChunk / 128) {
+  for (int kc = kt0; kc < kt1; kc += chunk / 128) {
     if (kc != kt0) __syncthreads();
-    stage_tokens<TM>(p, m0, kc * 128, kt1 * 128, tok, tok_scale);
+    stage_tokens<TM>(p, m0, kc * 128, kt1 * 128, chunk, tok, tok_scale);
     __syncthreads();
-    const int kend = min(kt1, kc + kChunk / 128);
+    const int kend = min(kt1, kc + chunk / 128);
     for (int kt = kc; kt < kend; ++kt) {
       asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
       __syncwarp();
@@ -175,8 +186,8 @@ mx4_rows_kernel(const vila_mx4_linear_params p, const vila_glinear_ext ext, int 
       scales2(sw0, 1, ws0[2], ws0[3]);
       scales2(sw1, 0, ws1[0], ws1[1]);
       scales2(sw1, 1, ws1[2], ws1[3]);
-      const __half* tk = tok + g * kTokPitch + (kt - kc) * 128 + t * 8;
-      const float* ts = tok_scale + (kt - kc) * 4 * TM + t * 2;
+      const __half* tk = tok + (kt - kc) * 128 + t * 8;
+      const float* ts = tok_scale + (kt - kc) * 4 * tokens;
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         const uint32_t w0 = *reinterpret_cast<const uint32_t*>(st + g * 64 + ((b ^ ((g >> 1) & 3)) << 4) + t * 4);
@@ -185,11 +196,11 @@ mx4_rows_kernel(const vila_mx4_linear_params p, const vila_glinear_ext ext, int 
         const uint32_t a10 = mx4_pair_f16<0>(w1), a11 = mx4_pair_f16<1>(w1), a12 = mx4_pair_f16<2>(w1), a13 = mx4_pair_f16<3>(w1);
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          const uint4 x = *reinterpret_cast<const uint4*>(tk + j * 8 * kTokPitch + b * 32);
+          const uint4 x = *reinterpret_cast<const uint4*>(tk + row[j] + b * 32);
           float part[4];
           mma_f16_first(part, a00, a10, a01, a11, x.x, x.y);
           mma_f16(part, a02, a12, a03, a13, x.z, x.w);
-          const float2 xs = *reinterpret_cast<const float2*>(ts + b * TM + j * 8);
+          const float2 xs = make_float2(ts[b * tokens + col0[j]], ts[b * tokens + col1[j]]);
           acc[j][0] = fmaf(part[0], ws0[b] * xs.x, acc[j][0]);
           acc[j][1] = fmaf(part[1], ws0[b] * xs.y, acc[j][1]);
           acc[j][2] = fmaf(part[2], ws1[b] * xs.x, acc[j][2]);
@@ -215,7 +226,7 @@ mx4_rows_kernel(const vila_mx4_linear_params p, const vila_glinear_ext ext, int 
   }
   if (split > 1) cluster_sync_all();
   else __syncthreads();
-  const int share = kRows / split, first = rank * share, tokens = min(TM, p.M - m0);
+  const int share = kRows / split, first = rank * share;
   const uint32_t red_a = smem_u32(red);
   const bool gated = (p.flags & kGluFlags) != 0;
   __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out);

@@ -1286,18 +1286,15 @@ def _mx4_check(ok: bool, what: str) -> None:
 
 def _mx4_here(t: torch.Tensor, name: str) -> None:
     """The kernels run on the current device's current stream: what they are given has to be there."""
-    if not t.is_cuda:
+    d = t.get_device()
+    if d < 0:
         raise RuntimeError(f"vila_b200.ops: {name} must be a CUDA tensor (no CPU fallback exists)")
-    _mx4_check(t.device.index == torch._C._cuda_getDevice(), f"{name} is on {t.device}, which is not the current device")
+    if d != torch._C._cuda_getDevice():
+        raise RuntimeError(f"vila_b200.ops: {name} is on {t.device}, which is not the current device")
 
 
 def _mx4_scale_bytes(rows: int, cols: int) -> int:
     return ((rows + 127) // 128) * (2 * ((cols + 255) // 256)) * 512
-
-
-def _mx4_empty(rows: int, cols: int, device) -> Mx4:
-    return Mx4(torch.empty(rows, 16 * ((cols + 31) // 32), dtype=torch.uint8, device=device),
-               torch.empty(_mx4_scale_bytes(rows, cols), dtype=torch.uint8, device=device), cols)
 
 
 def mx4_quantize(x: torch.Tensor) -> Mx4:
@@ -1305,19 +1302,24 @@ def mx4_quantize(x: torch.Tensor) -> Mx4:
     the scale is 2^max(floor(log2 m) - 2, -127), and every x / scale becomes the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 (ties to
     the even code, 6 beyond 6; signs kept).  A block with an infinity or a NaN reads as NaN."""
     _mx4_here(x, "x")
-    _mx4_check(x.dim() == 2 and x.shape[1] > 0 and (x.stride(1) == 1 or x.shape[1] == 1), "x must be [rows, cols] with consecutive columns")
-    q = _mx4_empty(x.shape[0], x.shape[1], x.device)
-    check(_lib.load().vila_mx4_quantize(_p(x), _dt(x, "x"), x.stride(0), _p(q.codes), _p(q.scales), q.rows, q.cols, _stream()),
-          "vila_mx4_quantize")
+    if x.dim() != 2 or x.shape[1] == 0 or (x.stride(1) != 1 and x.shape[1] != 1):
+        raise RuntimeError("vila_b200.ops: x must be [rows, cols] with consecutive columns")
+    rows, cols = x.shape
+    q = Mx4.__new__(Mx4)
+    q.codes = torch.empty((rows, 16 * ((cols + 31) // 32)), dtype=torch.uint8, device=x.device)
+    q.scales = torch.empty(_mx4_scale_bytes(rows, cols), dtype=torch.uint8, device=x.device)
+    q.rows, q.cols = rows, cols
+    check(_lib.load().vila_mx4_quantize(x.data_ptr(), _dt(x, "x"), x.stride(0), q.codes.data_ptr(), q.scales.data_ptr(), rows, cols,
+                                        _stream()), "vila_mx4_quantize")
     return q
 
 
 def mx4_dequantize(q: Mx4, out_dtype=torch.bfloat16) -> torch.Tensor:
     """The numbers that q stands for, [rows, cols] in bf16 or fp32."""
     _mx4_here(q.codes, "q")
-    out = torch.empty(q.rows, q.cols, dtype=out_dtype, device=q.device)
-    check(_lib.load().vila_mx4_dequantize(_p(q.codes), _p(q.scales), _p(out), _dt(out, "out"), q.cols, q.rows, q.cols, _stream()),
-          "vila_mx4_dequantize")
+    out = torch.empty((q.rows, q.cols), dtype=out_dtype, device=q.codes.device)
+    check(_lib.load().vila_mx4_dequantize(q.codes.data_ptr(), q.scales.data_ptr(), out.data_ptr(), _dt(out, "out"), q.cols, q.rows, q.cols,
+                                          _stream()), "vila_mx4_dequantize")
     return out
 
 
@@ -1349,21 +1351,18 @@ def mx4_unpack(q: Mx4) -> Tuple[torch.Tensor, torch.Tensor]:
     return q.codes, plain
 
 
-def _mx4_product(a, w: Mx4, bias, act, act_params, swiglu, geglu, glu_clamp, out) -> torch.Tensor:
+def _mx4_product(x: Optional[torch.Tensor], a: Optional[Mx4], M: int, K: int, w: Mx4, bias, act, act_params, swiglu, geglu, glu_clamp,
+                 out) -> torch.Tensor:
+    """x or a: the rows.  (The parameters go by position: by name they took 4 us of a call.)"""
+    N, codes = w.rows, w.codes
+    _mx4_here(codes, "w")
+    if K != w.cols or N == 0:
+        raise RuntimeError(f"vila_b200.ops: {M} x {K} rows do not fit a weight of {N} x {w.cols}")
     flags = (1 if swiglu else 0) | (4 if glu_clamp is not None else 0) | (FLAG_GEGLU if geglu else 0)
-    M, N, K = a.shape[0], w.rows, w.cols
-    _mx4_here(w.codes, "w")
     _mx4_check(act != ACT_XIELU or act_params is not None, "ACT_XIELU takes act_params")
-    _mx4_check(N > 0 and a.shape[1] == K, f"{a.shape[0]} x {a.shape[1]} rows do not fit a weight of {N} x {K}")
-    p = _lib.Mx4LinearParams()
-    if isinstance(a, Mx4):
-        _mx4_here(a.codes, "a")
-        p.a_codes, p.a_scales = _p(a.codes), _p(a.scales)
-    else:
-        p.x, p.ldx = _p(a), a.stride(0)
     n_out = N // 2 if flags else N
     if out is None:
-        out = torch.empty(M, n_out, dtype=torch.bfloat16, device=w.device)
+        out = torch.empty((M, n_out), dtype=torch.bfloat16, device=codes.device)
     else:
         _chk(out, "out")
         _mx4_here(out, "out")
@@ -1374,12 +1373,11 @@ def _mx4_product(a, w: Mx4, bias, act, act_params, swiglu, geglu, glu_clamp, out
         _mx4_check(bias.is_contiguous() and bias.numel() == N, f"bias must be contiguous [{N}]")
     if M == 0:
         return out
-    p.w_codes, p.w_scales, p.bias, p.out, p.ldo = _p(w.codes), _p(w.scales), _p(bias), _p(out), out.stride(0)
-    p.M, p.N, p.K, p.act, p.flags = M, N, K, act, flags
-    if glu_clamp is not None:
-        p.act_alpha, p.act_limit = float(glu_clamp[0]), float(glu_clamp[1])
-    if act_params is not None:
-        p.act_pos, p.act_neg = float(act_params[0]), float(act_params[1])
+    alpha, limit = glu_clamp if glu_clamp is not None else (0.0, 0.0)
+    pos, neg = act_params if act_params is not None else (0.0, 0.0)
+    p = _lib.Mx4LinearParams(None if x is None else x.data_ptr(), 0 if x is None else x.stride(0), None if a is None else a.codes.data_ptr(),
+                             None if a is None else a.scales.data_ptr(), codes.data_ptr(), w.scales.data_ptr(),
+                             None if bias is None else bias.data_ptr(), out.data_ptr(), out.stride(0), alpha, limit, pos, neg, M, N, K, act, flags)
     check(_lib.load().vila_mx4_linear(C.byref(p), _stream()), "vila_mx4_linear")
     return out
 
@@ -1391,14 +1389,19 @@ def mx4_linear(x: torch.Tensor, w: Mx4, bias: Optional[torch.Tensor] = None, *, 
     weights' values enter unrounded.  Activations and gated units as in linear / glinear."""
     _chk(x, "x")
     _mx4_here(x, "x")
-    _mx4_check(isinstance(w, Mx4), "w must be an Mx4 (mx4_quantize, mx4_pack)")
-    _mx4_check(x.dim() == 2 and (x.stride(1) == 1 or x.shape[1] == 1), "x must be [M, K] with consecutive columns")
-    return _mx4_product(x, w, bias, act, act_params, swiglu, geglu, glu_clamp, out)
+    if not isinstance(w, Mx4):
+        raise RuntimeError("vila_b200.ops: w must be an Mx4 (mx4_quantize, mx4_pack)")
+    if x.dim() != 2 or (x.stride(1) != 1 and x.shape[1] != 1):
+        raise RuntimeError("vila_b200.ops: x must be [M, K] with consecutive columns")
+    M, K = x.shape
+    return _mx4_product(x, None, M, K, w, bias, act, act_params, swiglu, geglu, glu_clamp, out)
 
 
 def mx4_matmul(a: Mx4, w: Mx4, bias: Optional[torch.Tensor] = None, *, act: int = ACT_NONE,
                act_params: Optional[Tuple[float, float]] = None, swiglu: bool = False, geglu: bool = False,
                glu_clamp: Optional[Tuple[float, float]] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """act(a [M, K] . w[N, K]^T + bias) in bf16, both factors in 4 bits (a = mx4_quantize(x)), fp32 sums."""
-    _mx4_check(isinstance(a, Mx4) and isinstance(w, Mx4), "a and w must be Mx4 (mx4_quantize, mx4_pack)")
-    return _mx4_product(a, w, bias, act, act_params, swiglu, geglu, glu_clamp, out)
+    if not (isinstance(a, Mx4) and isinstance(w, Mx4)):
+        raise RuntimeError("vila_b200.ops: a and w must be Mx4 (mx4_quantize, mx4_pack)")
+    _mx4_here(a.codes, "a")
+    return _mx4_product(None, a, a.rows, a.cols, w, bias, act, act_params, swiglu, geglu, glu_clamp, out)
