@@ -934,7 +934,11 @@ typedef struct vila_mx4_linear_params {
   int64_t ldo;
   float act_alpha, act_limit, act_pos, act_neg;
   int32_t M, N, K, act, flags;
+  void* scratch;
+  int64_t scratch_bytes;
 } vila_mx4_linear_params;
+/* Bytes of scratch (on a 16-byte boundary, of this call alone until it has run) that vila_mx4_linear is faster with; 0: none. */
+int64_t vila_mx4_linear_scratch(const vila_mx4_linear_params* p);
 int vila_mx4_linear(const vila_mx4_linear_params* p, void* stream);
 /* vila_mx4_linear with waits of its tcgen05 kernels that end after `tries` tries (test hook: 0 gives up at once; -2 - r: those of
  * role r at once, the others as ever; 0 loads, 1 products, 2 unpacking, 3 epilogue).  vila_wait_status speaks for it. */

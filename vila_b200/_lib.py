@@ -128,6 +128,7 @@ class Mx4LinearParams(C.Structure):
         ("w_codes", c_void_p), ("w_scales", c_void_p), ("bias", c_void_p), ("out", c_void_p), ("ldo", c_i64),
         ("act_alpha", c_float), ("act_limit", c_float), ("act_pos", c_float), ("act_neg", c_float),
         ("M", C.c_int32), ("N", C.c_int32), ("K", C.c_int32), ("act", C.c_int32), ("flags", C.c_int32),
+        ("scratch", c_void_p), ("scratch_bytes", c_i64),
     ]
 
 
@@ -359,10 +360,11 @@ SIGNATURES = {
     "vila_mx4_quantize": [c_void_p, c_int, c_i64, c_void_p, c_void_p, c_int, c_int, c_void_p],
     "vila_mx4_dequantize": [c_void_p, c_void_p, c_void_p, c_int, c_i64, c_int, c_int, c_void_p],
     "vila_mx4_scales": [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p],
+    "vila_mx4_linear_scratch": [C.POINTER(Mx4LinearParams)],
     "vila_mx4_linear": [C.POINTER(Mx4LinearParams), c_void_p],
     "vila_mx4_linear_tries": [C.POINTER(Mx4LinearParams), c_int, c_void_p],
 }
-_RESTYPES = {"vila_last_error": C.c_char_p}
+_RESTYPES = {"vila_last_error": C.c_char_p, "vila_mx4_linear_scratch": c_i64}
 
 _lib = None
 
@@ -386,7 +388,7 @@ def load() -> C.CDLL:
     for name, argtypes in SIGNATURES.items():
         fn = getattr(lib, name)  # AttributeError if the symbol is missing
         fn.argtypes = argtypes
-        fn.restype = c_int
+        fn.restype = _RESTYPES.get(name, c_int)
     _lib = lib
     return lib
 

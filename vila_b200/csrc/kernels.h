@@ -338,6 +338,10 @@ int mx4_scales(uint8_t* plain, uint8_t* tiled, int rows, int cols, int to_tiled,
 // tries: of every wait of the tcgen05 kernels (tests), -1: their own limit
 int mx4_linear(const vila_mx4_linear_params& p, cudaStream_t stream, int tries = -1);
 int mx4_tc(const vila_mx4_linear_params& p, const vila_glinear_ext& ext, int tries, cudaStream_t stream);    // 4-bit rows on tcgen05 (mx4_tc.cu)
+// few bf16 rows, cut into 16 rows of 4-bit numbers each, on tcgen05 (mx4_tc.cu); scratch: mx4_pieces_bytes
+size_t mx4_pieces_bytes(int M, int K);
+int mx4_pieces(const vila_mx4_linear_params& p, const vila_glinear_ext& ext, int tries, cudaStream_t stream);
+size_t mx4_linear_scratch(const vila_mx4_linear_params& p);
 // bf16 rows on 16-byte boundaries, weights unpacked into TMEM (mx4_mixed_tc.cu)
 bool mx4_mixed_tc_takes(const vila_mx4_linear_params& p);
 int mx4_mixed_tc(const vila_mx4_linear_params& p, const vila_glinear_ext& ext, int tries, cudaStream_t stream);

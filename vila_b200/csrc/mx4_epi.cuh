@@ -77,6 +77,19 @@ __device__ __forceinline__ void mx4_store_row(const vila_mx4_linear_params& p, c
   }
 }
 
+// Lane = weight row n, one token m.  All lanes call it.
+template <int EPI>
+__device__ __forceinline__ void mx4_store_one(const vila_mx4_linear_params& p, const vila_glinear_ext& x, float v, int m, int n, float bias) {
+  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out) + static_cast<size_t>(m) * p.ldo;
+  const float z = v + bias;
+  if constexpr (EPI >= kMx4Gated) {
+    const float other = __shfl_xor_sync(0xffffffffu, z, 1);
+    if (n < p.N && (n & 1) == 0) out[n / 2] = __float2bfloat16_rn(mx4_glu<EPI>(z, other, x));
+  } else {
+    if (n < p.N) out[n] = __float2bfloat16_rn(mx4_act<EPI>(z, x));
+  }
+}
+
 // Lane = weight row n, 16 tokens m .. m + 15 of the sums, those below `end`.  All lanes call it.
 template <int EPI>
 __device__ __forceinline__ void mx4_store_col(const vila_mx4_linear_params& p, const vila_glinear_ext& x, const float (&r)[16], int m, int end, int n, float bias) {

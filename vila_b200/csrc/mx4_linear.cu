@@ -8,7 +8,31 @@
 namespace vb {
 namespace {
 bool on16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+constexpr int kFew = 16;      // rows
+// bf16 rows that are cut into 4-bit rows
+bool by_pieces(const vila_mx4_linear_params& p) { return p.x != nullptr && p.M <= kFew; }
+int padded(int K) { return (K + 7) & ~7; }
+
+// rows off 16-byte boundaries -> rows of padded(K) elements; a thread moves 8
+__global__ void __launch_bounds__(256) align_kernel(const uint16_t* x, int64_t ldx, uint16_t* out, int M, int K) {
+  const int groups = (K + 7) / 8;
+  const long long items = static_cast<long long>(M) * groups, step = static_cast<long long>(gridDim.x) * 256;
+  for (long long it = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; it < items; it += step) {
+    const int m = static_cast<int>(it / groups), k = static_cast<int>(it - static_cast<long long>(m) * groups) * 8;
+    const uint16_t* row = x + static_cast<size_t>(m) * ldx + k;
+    uint32_t e[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = k + i < K ? __ldg(row + i) : 0u;
+    stg_v4(out + static_cast<size_t>(m) * groups * 8 + k, make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16));
+  }
+}
 }  // namespace
+
+size_t mx4_linear_scratch(const vila_mx4_linear_params& p) {
+  if (p.M <= 0 || p.K <= 0 || p.x == nullptr) return 0;
+  if (by_pieces(p)) return mx4_pieces_bytes(p.M, p.K);
+  return mx4_mixed_tc_takes(p) ? 0 : static_cast<size_t>(p.M) * padded(p.K) * 2;
+}
 
 int mx4_linear(const vila_mx4_linear_params& p, cudaStream_t stream, int tries) {
   if (wait_status()) return 1;   // an earlier launch gave up: nothing is built on its output
@@ -31,8 +55,20 @@ int mx4_linear(const vila_mx4_linear_params& p, cudaStream_t stream, int tries) 
   ext.act_limit = p.act_limit;
   ext.act_pos = p.act_pos;
   ext.act_neg = p.act_neg;
-  if (p.a_codes != nullptr && p.M > 16) return mx4_tc(p, ext, tries, stream);
-  if (p.M > 16 && mx4_mixed_tc_takes(p)) return mx4_mixed_tc(p, ext, tries, stream);
+  if (p.a_codes != nullptr) return mx4_tc(p, ext, tries, stream);
+  if (const size_t want = mx4_linear_scratch(p); want > 0 && p.scratch != nullptr) {
+    VB_CHECK(on16(p.scratch) && p.scratch_bytes >= static_cast<int64_t>(want), "mx4_linear: %lld bytes of scratch, %lld wanted, on a 16-byte boundary",
+             static_cast<long long>(p.scratch_bytes), static_cast<long long>(want));
+    if (by_pieces(p)) return mx4_pieces(p, ext, tries, stream);
+    vila_mx4_linear_params q = p;
+    q.x = p.scratch;
+    q.ldx = padded(p.K);
+    const long long blocks = (static_cast<long long>(p.M) * (padded(p.K) / 8) + 255) / 256, most = 16ll * num_sms();
+    VB_CUDA(launch_serial(align_kernel, dim3(static_cast<unsigned>(blocks < most ? blocks : most)), dim3(256), 0, stream, static_cast<const uint16_t*>(p.x), p.ldx,
+                          static_cast<uint16_t*>(p.scratch), p.M, p.K));
+    return mx4_mixed_tc(q, ext, tries, stream);
+  }
+  if (p.M > kFew && mx4_mixed_tc_takes(p)) return mx4_mixed_tc(p, ext, tries, stream);
   return mx4_rows(p, ext, stream);
 }
 

@@ -10,8 +10,16 @@
 //   MMA warp        TMEM allocation; scales to TMEM, then four tcgen05.mma a stage, into one of two accumulator sets
 //   8 epilogue warps: bias, activation, gated unit, bf16 out, under the products of the next tile
 //
-// kSwap false: P = tokens, Q = weight rows (a lane writes 16 consecutive outputs of its token); true: P = weight rows, Q = tokens,
-// for few tokens, whose number is then a multiple of 16 or so and not of 128.
+// kSwap false: P = tokens, Q = weight rows (a lane writes 32 consecutive outputs of its token); true: P = weight rows, Q = tokens,
+// for few tokens, whose number is then a multiple of 16 and not of 128, and K is split over a cluster of up to 8 CTAs where the weight
+// rows' tiles leave SMs idle (the parts are added in rank order through distributed shared memory).
+//
+// kPieces: few bf16 tokens on 4-bit weights, by the same products.  A token is cut into 16 rows of 4-bit numbers that add up to it
+// (mx4_pieces): a block's numbers in units u_0 = 2^(floor(log2 max) - 2) are below 8, the nearest 4-bit number leaves at most 2, which are
+// at most 8 of the next row's units u_1 = u_0 / 4, and so on; what 16 rows leave is under 2^-31 of the block's largest magnitude, and of
+// bf16's 8 bits nothing at all where a number is above 2^-22 of it.  The 16 columns of a token are added in fp32.  The tensor core has
+// that to spare (128 weight rows x 16 columns x 256: about 60 clocks, their codes take 300 to arrive), while unpacking weights
+// to f16 is bound by integer instructions: mx4_rows.cu takes 20.7 us for one token on 37888 x 3584.
 #include "../../include/vila_b200.h"
 #include "common.cuh"
 #include "kernels.h"
@@ -32,7 +40,7 @@ template <int BN> struct Shape {
   static constexpr int kStages = BN == 64 ? 4 : (BN == 128 ? 6 : 5);
   static constexpr int kPerSm = BN > 64 ? 1 : 2;
   static constexpr int kScaleCols = 8 * (1 + kQTiles);          // TMEM columns of a stage's scales
-  static constexpr int kCols = 2 * BN + kStages * kScaleCols <= 256 ? 256 : 512;
+  static constexpr int kCols = 2 * BN + kStages * kScaleCols <= 128 ? 128 : (2 * BN + kStages * kScaleCols <= 256 ? 256 : 512);
   static constexpr size_t kSmem = 1024 + static_cast<size_t>(kStages) * kStage + 256;
   static_assert(2 * BN + kStages * kScaleCols <= kCols, "TMEM");
   static_assert(kCols * kPerSm <= 512, "TMEM of an SM");
@@ -57,10 +65,11 @@ __device__ __forceinline__ void umma_mx4(uint32_t d, uint64_t a, uint64_t b, uin
 __device__ __forceinline__ void scales_to_tmem(uint32_t taddr, uint64_t desc) {
   asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
-template <int BN, bool kSwap>
+constexpr int kPieceRows = 16;
+template <int BN, bool kSwap, bool kPieces>
 __global__ void __launch_bounds__(kThreads, Shape<BN>::kPerSm)
 mx4_tc_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ CUtensorMap tmap_q, const vila_mx4_linear_params p,
-              const vila_glinear_ext x, const WaitLimit limit, volatile unsigned int* failed) {
+              const vila_glinear_ext x, const int split, const WaitLimit limit, volatile unsigned int* failed) {
   using S = Shape<BN>;
   constexpr int ST = S::kStages;
   extern __shared__ uint8_t smem_raw[];
@@ -74,9 +83,12 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant_
   volatile int* gave_up = reinterpret_cast<int*>(tmem_ptr + 1);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int P = kSwap ? p.N : p.M, Q = kSwap ? p.M : p.N;
+  const int P = kSwap ? p.N : p.M, Q = kSwap ? (kPieces ? kPieceRows * p.M : p.M) : p.N;
   const int p_tiles = (P + kP - 1) / kP, q_tiles = (Q + BN - 1) / BN, total = p_tiles * q_tiles;
   const int nkb = (p.K + kDepth - 1) / kDepth, kts = 2 * nkb;
+  // a cluster's CTAs share a tile and cut K; without clusters split is 1
+  const int rank = static_cast<int>(blockIdx.x) % split, it0 = static_cast<int>(blockIdx.x) / split, it_step = static_cast<int>(gridDim.x) / split;
+  const int kb0 = static_cast<int>(static_cast<long long>(nkb) * rank / split), kb1 = static_cast<int>(static_cast<long long>(nkb) * (rank + 1) / split);
   auto tile_at = [&](int it, int& p0, int& q0) {     // the tiles that run together share their rows of Q (few of them)
     const int qt = it / p_tiles;
     p0 = (it - qt * p_tiles) * kP;
@@ -115,22 +127,36 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant_
       const int q_row_tiles = (Q + 127) / 128;
       int s = 0, rounds = 0;              // rounds: through all the stages
       uint32_t ph = 1;                    // parity to wait for on an empty barrier: the first round passes
-      for (int it = blockIdx.x; it < total && ok; it += gridDim.x) {
+      for (int it = it0; it < total && ok; it += it_step) {
         int p0, q0;
         tile_at(it, p0, q0);
         const int qt0 = q0 >> 7, qts = min(S::kQTiles, q_row_tiles - qt0);
         const uint32_t bytes = S::kPBytes + S::kQBytes + 1024 * (1 + qts);
-        for (int kb = 0; kb < nkb; ++kb) {
-          ok = mbar_wait_limited(&empty_bar[s], ph, gave_up, limit.tries);
-          if (!ok) break;
+        auto load_p = [&](int kb, int s) {
           uint8_t* st = smem + s * S::kStage;
           mbar_arrive_expect_tx(&full_bar[s], bytes);
           tma_load_2d(st, &tmap_p, &full_bar[s], kb * 128, p0);
+          mx4_bulk_load(st + S::kPBytes + S::kQBytes, sp + (static_cast<size_t>(p0 >> 7) * kts + 2 * kb) * 512, 1024, &full_bar[s]);
+        };
+        auto load_q = [&](int kb, int s) {
+          uint8_t* st = smem + s * S::kStage;
           tma_load_2d(st + S::kPBytes, &tmap_q, &full_bar[s], kb * 128, q0);
-          uint8_t* sc = st + S::kPBytes + S::kQBytes;
-          mx4_bulk_load(sc, sp + (static_cast<size_t>(p0 >> 7) * kts + 2 * kb) * 512, 1024, &full_bar[s]);
           for (int q = 0; q < qts; ++q)
-            mx4_bulk_load(sc + 1024 * (1 + q), sq + (static_cast<size_t>(qt0 + q) * kts + 2 * kb) * 512, 1024, &full_bar[s]);
+            mx4_bulk_load(st + S::kPBytes + S::kQBytes + 1024 * (1 + q), sq + (static_cast<size_t>(qt0 + q) * kts + 2 * kb) * 512, 1024, &full_bar[s]);
+        };
+        int ahead = 0;
+        if (kPieces && it == it0) {      // the first weights are asked for while the kernel before cuts the tokens
+          ahead = min(ST, kb1 - kb0);
+          for (int i = 0; i < ahead; ++i) load_p(kb0 + i, i);
+          griddep_wait();
+        }
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (kb - kb0 >= ahead) {
+            ok = mbar_wait_limited(&empty_bar[s], ph, gave_up, limit.tries);
+            if (!ok) break;
+            load_p(kb, s);
+          }
+          load_q(kb, s);
           if (++s == ST) {
             s = 0;
             ph ^= 1;
@@ -138,6 +164,7 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant_
           }
         }
       }
+      if (kPieces) griddep_wait();      // whatever became of the loads: this kernel does not end before the one before it
       // what was asked for lands before the CTA's memory is given back, whichever warp gave up
       for (int i = 0; i < ST; ++i) {
         const int round = i < s ? rounds : rounds - 1;
@@ -151,14 +178,14 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant_
     const uint64_t sd0 = make_smem_desc(smem_u32(smem) + S::kPBytes + S::kQBytes, 16, 128, kLayoutNone);
     int s = 0, k = 0;
     uint32_t ph = 0;
-    for (int it = blockIdx.x; it < total && ok; it += gridDim.x, ++k) {
+    for (int it = it0; it < total && ok; it += it_step, ++k) {
       int p0, q0;
       tile_at(it, p0, q0);
       const uint32_t n = kSwap ? min(BN, (Q - q0 + 15) & ~15) : BN, acc = tmem + (k & 1) * BN;
       const uint32_t idesc = idesc_mx4(kP, n, 0), idesc2 = idesc_mx4(kP, n, 2);
       ok = mx4_warp_wait(&acc_free[k & 1], ((k >> 1) & 1) ^ 1, gave_up, limit.tries);
       uint32_t here = mx4_test(&full_bar[s], ph);
-      for (int kb = 0; kb < nkb && ok; ++kb) {
+      for (int kb = kb0; kb < kb1 && ok; ++kb) {
         if (!__all_sync(0xffffffffu, here)) ok = mx4_warp_wait(&full_bar[s], ph, gave_up, limit.tries);
         if (!ok) break;
         tc_fence_after();
@@ -181,7 +208,7 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant_
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            umma_mx4(acc, ad + 2 * j, bd + 2 * j, j & 1 ? idesc2 : idesc, ts + 4 * (j >> 1), tq + 4 * S::kQTiles * (j >> 1), (kb | j) != 0);
+            umma_mx4(acc, ad + 2 * j, bd + 2 * j, j & 1 ? idesc2 : idesc, ts + 4 * (j >> 1), tq + 4 * S::kQTiles * (j >> 1), (kb - kb0) | j ? 1u : 0u);
           umma_commit(done);
         }
         __syncwarp();
@@ -196,7 +223,7 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant_
     const int quad = warp & 3, half = warp >> 2;
     const bool wide = reinterpret_cast<uintptr_t>(p.out) % 32 == 0 && p.ldo % 16 == 0;
     int k = 0;
-    for (int it = blockIdx.x; it < total && ok; it += gridDim.x, ++k) {
+    for (int it = it0; it < total && ok; it += it_step, ++k) {
       int p0, q0;
       tile_at(it, p0, q0);
       // all lanes or none: the TMEM loads need the whole warp
@@ -205,6 +232,7 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant_
       tc_fence_after();
       const uint32_t acc = tmem + (static_cast<uint32_t>(quad * 32) << 16) + (k & 1) * BN;
       const int row = p0 + quad * 32 + lane, cols = min(BN, Q - q0);
+      float* red = reinterpret_cast<float*>(smem);      // [column][128]; a part of a tile is all its CTA has: the stages are done with
       const float bias = kSwap && p.bias && row < p.N ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[row]) : 0.f;
       mx4_with_epilogue(p, [&](auto epi) {
         constexpr int EPI = decltype(epi)::value;
@@ -215,8 +243,22 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant_
           if constexpr (kSwap) tmem_ld_32x32b_x16(acc + c, reinterpret_cast<uint32_t*>(r));
           else tmem_ld_32x32b_x32(acc + c, reinterpret_cast<uint32_t*>(r));
           tmem_ld_wait();
-          if constexpr (kSwap) mx4_store_col<EPI>(p, x, r, q0 + c, p.M, row, bias);
-          else mx4_store_row<EPI>(p, x, r, row, q0 + c, wide);
+          if constexpr (!kSwap) {
+            mx4_store_row<EPI>(p, x, r, row, q0 + c, wide);
+          } else if constexpr (kPieces) {
+            float v = r[kPieceRows - 1];      // the smallest first
+#pragma unroll
+            for (int i = kPieceRows - 2; i >= 0; --i) v += r[i];
+            if (split > 1) red[(c / kPieceRows) * kP + quad * 32 + lane] = v;
+            else mx4_store_one<EPI>(p, x, v, (q0 + c) / kPieceRows, row, bias);
+          } else {
+            if (split > 1) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) red[(c + i) * kP + quad * 32 + lane] = r[i];
+            } else {
+              mx4_store_col<EPI>(p, x, r, q0 + c, p.M, row, bias);
+            }
+          }
         }
       });
       tc_fence_before();
@@ -229,6 +271,31 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant_
   if (warp == kMma) {
     tc_fence_after();
     tmem_dealloc<S::kCols>(tmem);
+  }
+  if (kSwap && split > 1) {      // every CTA of the cluster adds the parts of its share of the weight rows
+    cluster_sync_all();
+    int p0, q0;
+    tile_at(it0, p0, q0);
+    const int cols = kPieces ? min(BN, Q - q0) / kPieceRows : min(BN, Q - q0), m0 = kPieces ? q0 / kPieceRows : q0;
+    const bool gated = (p.flags & kGluFlags) != 0;
+    const int share = kP / split, per = gated ? share / 2 : share;
+    const uint32_t red = smem_u32(smem);
+    const __nv_bfloat16* bias = static_cast<const __nv_bfloat16*>(p.bias);
+    __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out);
+    auto sum = [&](int c, int r) {
+      float v = 0.f;
+      for (int q = 0; q < split; ++q) v += ld_dsmem_f32(mapa_u32(red + (c * kP + r) * 4, q));
+      const int n = p0 + r;
+      return bias != nullptr && n < p.N ? v + __bfloat162float(bias[n]) : v;
+    };
+    for (int i = tid; i < cols * per; i += kThreads) {
+      const int c = i / per, r = rank * share + (i - c * per) * (gated ? 2 : 1), n = p0 + r;
+      if (n >= p.N) continue;
+      const size_t o = static_cast<size_t>(m0 + c) * p.ldo;
+      if (gated) out[o + n / 2] = __float2bfloat16_rn(glu(sum(c, r), sum(c, r + 1), p.flags, x));
+      else out[o + n] = __float2bfloat16_rn(activate(sum(c, r), p.act, x));
+    }
+    cluster_sync_all();      // the others still read this CTA's parts
   }
   if (tid == 0 && *gave_up) {
     *failed = 1u;
@@ -460,23 +527,101 @@ int launch(const vila_mx4_linear_params& p, const vila_glinear_ext& x, int tries
 }
 }  // namespace pair
 
-template <int BN, bool kSwap>
+// ---- bf16 tokens to 16 rows of 4-bit numbers each ----
+// A warp takes 256 columns of a token, a lane 8.  v is what is left, in units of the row at hand; all steps are exact in fp32.
+constexpr int kPieceWarps = 4;
+__global__ void __launch_bounds__(32 * kPieceWarps)
+mx4_pieces_kernel(const __nv_bfloat16* x, int64_t ldx, uint8_t* codes, uint8_t* scales, int M, int K) {
+  griddep_launch_dependents();
+  const int lane = threadIdx.x & 31, pitch = mx4_pitch(K), kts = mx4_ktiles(K), chunks = kts / 2;
+  const int it = blockIdx.x * kPieceWarps + (threadIdx.x >> 5), m = it / chunks, ch = it - m * chunks;
+  const int rows = kPieceRows * M, padded = (rows + 127) / 128 * 128;
+  if (m * kPieceRows >= padded) return;
+  const int c0 = ch * 256 + lane * 8, at = ch * 128 + lane * 4;
+  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (m < M) {
+    const __nv_bfloat16* row = x + static_cast<size_t>(m) * ldx;
+    if (c0 + 8 <= K && ((reinterpret_cast<uintptr_t>(x) | (ldx * 2)) & 15) == 0) {
+      const uint4 a = __ldg(reinterpret_cast<const uint4*>(row + c0));
+      v[0] = bf_lo(a.x); v[1] = bf_hi(a.x); v[2] = bf_lo(a.y); v[3] = bf_hi(a.y);
+      v[4] = bf_lo(a.z); v[5] = bf_hi(a.z); v[6] = bf_lo(a.w); v[7] = bf_hi(a.w);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = c0 + i < K ? __bfloat162float(row[c0 + i]) : 0.f;
+    }
+  }
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  const bool finite = top < 0x7f800000u;
+  const uint32_t e = top >> 23, first = finite ? (e > 2 ? e - 2 : 0u) : 255u;
+  const float inv = __uint_as_float((254u - (finite ? first : 0u)) << 23);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = finite ? v[i] * inv : 0.f;
+#pragma unroll 1
+  for (int i = 0; i < kPieceRows; ++i) {
+    const int r = m * kPieceRows + i;
+    // the first row of a block that is not finite says so; units below 2^-127 do not exist, nor do rows of them
+    const uint32_t byte = i == 0 ? first : (finite && first >= 2u * i ? first - 2u * i : 0u);
+    const bool rest = i == 0 || (finite && first >= 2u * i);
+    const uint32_t c = rest && m < M ? mx4_encode8(v) : 0u;
+    const uint32_t h[4] = {mx4_pair_f16<0>(c), mx4_pair_f16<1>(c), mx4_pair_f16<2>(c), mx4_pair_f16<3>(c)};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
+      v[2 * j] = (v[2 * j] - f.x) * 4.f;
+      v[2 * j + 1] = (v[2 * j + 1] - f.y) * 4.f;
+    }
+    if (m < M && at < pitch) *reinterpret_cast<uint32_t*>(codes + static_cast<size_t>(r) * pitch + at) = c;
+    uint32_t word = m < M ? byte << (8 * ((lane >> 2) & 3)) : 0u;
+    word |= __shfl_xor_sync(0xffffffffu, word, 4);
+    word |= __shfl_xor_sync(0xffffffffu, word, 8);
+    if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(scales + mx4_scale_at(r, 2 * ch + (lane >> 4), kts)) = word;
+  }
+}
+
+template <int BN, bool kSwap, bool kPieces>
 int launch(const vila_mx4_linear_params& p, const vila_glinear_ext& x, int tries, cudaStream_t stream) {
   using S = Shape<BN>;
   static PerDeviceOnce once;
   if (once.first())
-    VB_CUDA(cudaFuncSetAttribute(mx4_tc_kernel<BN, kSwap>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::kSmem)));
-  const int pitch = mx4_pitch(p.K);
+    VB_CUDA(cudaFuncSetAttribute(mx4_tc_kernel<BN, kSwap, kPieces>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::kSmem)));
+  const int pitch = mx4_pitch(p.K), tokens = kPieces ? kPieceRows * p.M : p.M;
   const uint8_t *pc = kSwap ? p.w_codes : p.a_codes, *qc = kSwap ? p.a_codes : p.w_codes;
-  const int P = kSwap ? p.N : p.M, Q = kSwap ? p.M : p.N;
+  const int P = kSwap ? p.N : tokens, Q = kSwap ? tokens : p.N;
   CUtensorMap tp, tq;
   if (int rc = make_tmap_2d_u8(&tp, pc, P, pitch, pitch, kP, 128, 128)) return rc;
   if (int rc = make_tmap_2d_u8(&tq, qc, Q, pitch, pitch, BN, 128, 128)) return rc;
-  const long long tiles = static_cast<long long>((P + kP - 1) / kP) * ((Q + BN - 1) / BN);
-  VB_CHECK(tiles < (1LL << 31), "mx4_linear: too many tiles (M=%d N=%d)", p.M, p.N);
-  const long long most = static_cast<long long>(S::kPerSm) * num_sms();
-  VB_CUDA(launch_serial(mx4_tc_kernel<BN, kSwap>, dim3(static_cast<unsigned>(tiles < most ? tiles : most)), dim3(kThreads), S::kSmem, stream, tp, tq, p, x,
-                        wait_limit(tries), failed_word()));
+  const long long tiles = static_cast<long long>((P + kP - 1) / kP) * ((Q + BN - 1) / BN), most = static_cast<long long>(S::kPerSm) * num_sms();
+  VB_CHECK(tiles < (1LL << 28), "mx4_linear: too many tiles (M=%d N=%d)", p.M, p.N);
+  // K over a cluster where the tiles leave SMs idle, two stages a CTA at least
+  int split = 1;
+  if (kSwap)
+    while (split < 8 && tiles * split * 2 <= most && (p.K + kDepth - 1) / kDepth >= 4 * split) split *= 2;
+  const dim3 grid(static_cast<unsigned>(split > 1 ? tiles * split : (tiles < most ? tiles : most)));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (split > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = split;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (kPieces && pdl_enabled()) {      // behind mx4_pieces_kernel, which lets it begin
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  VB_CUDA(cudaLaunchKernelEx(&cfg, mx4_tc_kernel<BN, kSwap, kPieces>, tp, tq, p, x, split, wait_limit(tries), failed_word()));
   return 0;
 }
 
@@ -484,11 +629,33 @@ int launch(const vila_mx4_linear_params& p, const vila_glinear_ext& x, int tries
 
 int mx4_tc(const vila_mx4_linear_params& p, const vila_glinear_ext& x, int tries, cudaStream_t stream) {
   VB_CHECK(failed_word() != nullptr, "mx4_linear: no pinned host memory for the status word");
-  if (p.M <= 32) return launch<32, true>(p, x, tries, stream);
-  if (p.M <= 64) return launch<64, true>(p, x, tries, stream);
-  if (p.M <= 128) return launch<128, true>(p, x, tries, stream);
+  if (p.M <= 16) return launch<16, true, false>(p, x, tries, stream);
+  if (p.M <= 32) return launch<32, true, false>(p, x, tries, stream);
+  if (p.M <= 64) return launch<64, true, false>(p, x, tries, stream);
+  if (p.M <= 128) return launch<128, true, false>(p, x, tries, stream);
   if (p.M > 512) return pair::launch(p, x, tries, stream);
-  return launch<128, false>(p, x, tries, stream);
+  return launch<128, false, false>(p, x, tries, stream);
+}
+
+size_t mx4_pieces_bytes(int M, int K) {
+  return static_cast<size_t>(kPieceRows) * M * mx4_pitch(K) + mx4_scale_bytes(kPieceRows * M, K);
+}
+int mx4_pieces(const vila_mx4_linear_params& given, const vila_glinear_ext& x, int tries, cudaStream_t stream) {
+  VB_CHECK(failed_word() != nullptr, "mx4_linear: no pinned host memory for the status word");
+  vila_mx4_linear_params p = given;
+  uint8_t* codes = static_cast<uint8_t*>(p.scratch);
+  uint8_t* scales = codes + static_cast<size_t>(kPieceRows) * p.M * mx4_pitch(p.K);
+  const long long items = static_cast<long long>((kPieceRows * p.M + 127) / 128 * 128 / kPieceRows) * (mx4_ktiles(p.K) / 2);
+  VB_CUDA(launch_serial(mx4_pieces_kernel, dim3(static_cast<unsigned>((items + kPieceWarps - 1) / kPieceWarps)), dim3(32 * kPieceWarps), 0, stream,
+                        static_cast<const __nv_bfloat16*>(p.x), p.ldx, codes, scales, p.M, p.K));
+  p.x = nullptr;
+  p.a_codes = codes;
+  p.a_scales = scales;
+  const int rows = kPieceRows * p.M;
+  if (rows <= 16) return launch<16, true, true>(p, x, tries, stream);
+  if (rows <= 32) return launch<32, true, true>(p, x, tries, stream);
+  if (rows <= 64) return launch<64, true, true>(p, x, tries, stream);
+  return launch<128, true, true>(p, x, tries, stream);
 }
 
 }  // namespace vb

@@ -1306,8 +1306,8 @@ def mx4_quantize(x: torch.Tensor) -> Mx4:
         raise RuntimeError("vila_b200.ops: x must be [rows, cols] with consecutive columns")
     rows, cols = x.shape
     q = Mx4.__new__(Mx4)
-    q.codes = torch.empty((rows, 16 * ((cols + 31) // 32)), dtype=torch.uint8, device=x.device)
-    q.scales = torch.empty(_mx4_scale_bytes(rows, cols), dtype=torch.uint8, device=x.device)
+    q.codes = x.new_empty((rows, 16 * ((cols + 31) // 32)), dtype=torch.uint8)
+    q.scales = x.new_empty(_mx4_scale_bytes(rows, cols), dtype=torch.uint8)
     q.rows, q.cols = rows, cols
     check(_lib.load().vila_mx4_quantize(x.data_ptr(), _dt(x, "x"), x.stride(0), q.codes.data_ptr(), q.scales.data_ptr(), rows, cols,
                                         _stream()), "vila_mx4_quantize")
@@ -1317,7 +1317,7 @@ def mx4_quantize(x: torch.Tensor) -> Mx4:
 def mx4_dequantize(q: Mx4, out_dtype=torch.bfloat16) -> torch.Tensor:
     """The numbers that q stands for, [rows, cols] in bf16 or fp32."""
     _mx4_here(q.codes, "q")
-    out = torch.empty((q.rows, q.cols), dtype=out_dtype, device=q.codes.device)
+    out = q.codes.new_empty((q.rows, q.cols), dtype=out_dtype)
     check(_lib.load().vila_mx4_dequantize(q.codes.data_ptr(), q.scales.data_ptr(), out.data_ptr(), _dt(out, "out"), q.cols, q.rows, q.cols,
                                           _stream()), "vila_mx4_dequantize")
     return out
@@ -1362,7 +1362,7 @@ def _mx4_product(x: Optional[torch.Tensor], a: Optional[Mx4], M: int, K: int, w:
     _mx4_check(act != ACT_XIELU or act_params is not None, "ACT_XIELU takes act_params")
     n_out = N // 2 if flags else N
     if out is None:
-        out = torch.empty((M, n_out), dtype=torch.bfloat16, device=codes.device)
+        out = codes.new_empty((M, n_out), dtype=torch.bfloat16)
     else:
         _chk(out, "out")
         _mx4_here(out, "out")
@@ -1378,7 +1378,13 @@ def _mx4_product(x: Optional[torch.Tensor], a: Optional[Mx4], M: int, K: int, w:
     p = _lib.Mx4LinearParams(None if x is None else x.data_ptr(), 0 if x is None else x.stride(0), None if a is None else a.codes.data_ptr(),
                              None if a is None else a.scales.data_ptr(), codes.data_ptr(), w.scales.data_ptr(),
                              None if bias is None else bias.data_ptr(), out.data_ptr(), out.stride(0), alpha, limit, pos, neg, M, N, K, act, flags)
-    check(_lib.load().vila_mx4_linear(C.byref(p), _stream()), "vila_mx4_linear")
+    lib = _lib.load()
+    if x is not None and (M <= 16 or (p.x | 2 * p.ldx) % 16):      # a workspace of the call's own: a captured graph keeps its own, too
+        n = lib.vila_mx4_linear_scratch(C.byref(p))
+        if n:
+            scratch = codes.new_empty(n)
+            p.scratch, p.scratch_bytes = scratch.data_ptr(), n
+    check(lib.vila_mx4_linear(C.byref(p), _stream()), "vila_mx4_linear")
     return out
 
 
