@@ -87,4 +87,42 @@ __device__ __forceinline__ void mx4_bulk_load(void* dst, const void* src, uint32
                : "memory");
 }
 
+// How many clusters of a kernel the GPU holds at once, by cluster size (1, 2, 4, 8), asked for once a device: a cluster lies within a
+// group of SMs, so that 28 clusters of 5 are more than the 148 SMs take at a time, and one too many takes as long again.
+struct Mx4Clusters {
+  int most[64][4] = {};
+  template <typename K>
+  int of(K* kernel, int log2, int threads, size_t smem) {
+    int d = 0;
+    cudaGetDevice(&d);
+    if (d < 0 || d >= 64) d = 0;
+    int& n = most[d][log2];
+    if (n == 0) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(1u << log2);
+      cfg.blockDim = dim3(threads);
+      cfg.dynamicSmemBytes = smem;
+      cudaLaunchAttribute attr;
+      attr.id = cudaLaunchAttributeClusterDimension;
+      attr.val.clusterDim.x = 1u << log2;
+      attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+      cfg.attrs = &attr;
+      cfg.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+        (void)cudaGetLastError();
+        n = 0;
+      }
+      if (n <= 0) n = -1;
+    }
+    return n;
+  }
+  // the largest size (a power of two, at most 8 and `limit`) of which the GPU holds `tiles`; 1: none
+  template <typename K>
+  int split(K* kernel, int threads, size_t smem, long long tiles, long long limit) {
+    int s = 1;
+    for (int l = 1; l <= 3 && (2 << (l - 1)) <= limit && tiles <= of(kernel, l, threads, smem); ++l) s = 1 << l;
+    return s;
+  }
+};
+
 }  // namespace vb

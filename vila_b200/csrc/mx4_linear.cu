@@ -9,8 +9,12 @@ namespace vb {
 namespace {
 bool on16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 constexpr int kFew = 16;      // rows
-// bf16 rows that are cut into 4-bit rows
-bool by_pieces(const vila_mx4_linear_params& p) { return p.x != nullptr && p.M <= kFew; }
+// bf16 rows that are cut into 4-bit rows.  Small layers of up to 8 rows are faster in one launch (mx4_rows.cu), us against us: one row
+// of 2048 x 2048 5.5 and 7.6, of 3584 x 3584 7.3 and 8.3, of 8192 x 4096 13.7 and 9.7; 4 rows of 3584 x 3584 7.7 and 8.7, 16 rows
+// 12.7 and 10.5.
+bool by_pieces(const vila_mx4_linear_params& p) {
+  return p.x != nullptr && p.M <= kFew && (p.M > 8 || static_cast<long long>(p.N) * p.K > (16ll << 20));
+}
 int padded(int K) { return (K + 7) & ~7; }
 
 // rows off 16-byte boundaries -> rows of padded(K) elements; a thread moves 8
@@ -31,7 +35,7 @@ __global__ void __launch_bounds__(256) align_kernel(const uint16_t* x, int64_t l
 size_t mx4_linear_scratch(const vila_mx4_linear_params& p) {
   if (p.M <= 0 || p.K <= 0 || p.x == nullptr) return 0;
   if (by_pieces(p)) return mx4_pieces_bytes(p.M, p.K);
-  return mx4_mixed_tc_takes(p) ? 0 : static_cast<size_t>(p.M) * padded(p.K) * 2;
+  return p.M <= kFew || mx4_mixed_tc_takes(p) ? 0 : static_cast<size_t>(p.M) * padded(p.K) * 2;
 }
 
 int mx4_linear(const vila_mx4_linear_params& p, cudaStream_t stream, int tries) {

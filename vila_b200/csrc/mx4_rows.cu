@@ -262,8 +262,8 @@ int launch(const vila_mx4_linear_params& p, const vila_glinear_ext& ext, cudaStr
   if (once.first())
     VB_CUDA(cudaFuncSetAttribute(mx4_rows_kernel<TM>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<TM>::kTotal));
   const int tiles = (p.N + kRows - 1) / kRows, groups = (p.M + TM - 1) / TM, nk = (p.K + 127) / 128;
-  int split = 1;
-  while (split < 8 && static_cast<long long>(tiles) * groups * split < 2 * num_sms() && nk >= 4 * split) split *= 2;
+  static Mx4Clusters clusters;
+  const int split = clusters.split(mx4_rows_kernel<TM>, kThreads, Smem<TM>::kTotal, static_cast<long long>(tiles) * groups, nk / 2);
   VB_CHECK(groups <= 65535 && static_cast<long long>(tiles) * split < (1LL << 31), "mx4_linear: M=%d N=%d", p.M, p.N);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(tiles * split, groups, 1);

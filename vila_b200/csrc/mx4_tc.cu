@@ -278,22 +278,38 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant_
     tile_at(it0, p0, q0);
     const int cols = kPieces ? min(BN, Q - q0) / kPieceRows : min(BN, Q - q0), m0 = kPieces ? q0 / kPieceRows : q0;
     const bool gated = (p.flags & kGluFlags) != 0;
-    const int share = kP / split, per = gated ? share / 2 : share;
+    const int f0 = kP / 4 * rank / split, f1 = kP / 4 * (rank + 1) / split;      // its rows, by fours
     const uint32_t red = smem_u32(smem);
     const __nv_bfloat16* bias = static_cast<const __nv_bfloat16*>(p.bias);
     __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out);
-    auto sum = [&](int c, int r) {
-      float v = 0.f;
-      for (int q = 0; q < split; ++q) v += ld_dsmem_f32(mapa_u32(red + (c * kP + r) * 4, q));
-      const int n = p0 + r;
-      return bias != nullptr && n < p.N ? v + __bfloat162float(bias[n]) : v;
-    };
-    for (int i = tid; i < cols * per; i += kThreads) {
-      const int c = i / per, r = rank * share + (i - c * per) * (gated ? 2 : 1), n = p0 + r;
-      if (n >= p.N) continue;
+    for (int i = tid; i < cols * (f1 - f0); i += kThreads) {
+      const int c = i / (f1 - f0), r = 4 * (f0 + i - c * (f1 - f0)), n = p0 + r;
+      float4 part[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        if (q < split) part[q] = ld_dsmem_v4f(mapa_u32(red + (c * kP + r) * 4, q));
+      float z[4] = {part[0].x, part[0].y, part[0].z, part[0].w};
+#pragma unroll
+      for (int q = 1; q < 8; ++q)
+        if (q < split) {
+          z[0] += part[q].x;
+          z[1] += part[q].y;
+          z[2] += part[q].z;
+          z[3] += part[q].w;
+        }
       const size_t o = static_cast<size_t>(m0 + c) * p.ldo;
-      if (gated) out[o + n / 2] = __float2bfloat16_rn(glu(sum(c, r), sum(c, r + 1), p.flags, x));
-      else out[o + n] = __float2bfloat16_rn(activate(sum(c, r), p.act, x));
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (bias != nullptr && n + j < p.N) z[j] += __bfloat162float(bias[n + j]);
+      if (gated) {
+#pragma unroll
+        for (int j = 0; j < 4; j += 2)
+          if (n + j < p.N) out[o + (n + j) / 2] = __float2bfloat16_rn(glu(z[j], z[j + 1], p.flags, x));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n + j < p.N) out[o + n + j] = __float2bfloat16_rn(activate(z[j], p.act, x));
+      }
     }
     cluster_sync_all();      // the others still read this CTA's parts
   }
@@ -596,10 +612,9 @@ int launch(const vila_mx4_linear_params& p, const vila_glinear_ext& x, int tries
   if (int rc = make_tmap_2d_u8(&tq, qc, Q, pitch, pitch, BN, 128, 128)) return rc;
   const long long tiles = static_cast<long long>((P + kP - 1) / kP) * ((Q + BN - 1) / BN), most = static_cast<long long>(S::kPerSm) * num_sms();
   VB_CHECK(tiles < (1LL << 28), "mx4_linear: too many tiles (M=%d N=%d)", p.M, p.N);
-  // K over a cluster where the tiles leave SMs idle, two stages a CTA at least
-  int split = 1;
-  if (kSwap)
-    while (split < 8 && tiles * split * 2 <= most && (p.K + kDepth - 1) / kDepth >= 4 * split) split *= 2;
+  // K over a cluster where the tiles leave SMs idle and K is long: of 14 stages (K = 3584) the cluster's joint end cost what it saved
+  static Mx4Clusters clusters;
+  const int split = kSwap ? clusters.split(mx4_tc_kernel<BN, kSwap, kPieces>, kThreads, S::kSmem, tiles, (p.K + kDepth - 1) / kDepth / 8) : 1;
   const dim3 grid(static_cast<unsigned>(split > 1 ? tiles * split : (tiles < most ? tiles : most)));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
