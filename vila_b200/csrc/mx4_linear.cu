@@ -9,11 +9,15 @@ namespace vb {
 namespace {
 bool on16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 constexpr int kFew = 16;      // rows
-// bf16 rows that are cut into 4-bit rows.  Small layers of up to 8 rows are faster in one launch (mx4_rows.cu), us against us: one row
+// bf16 rows that are cut into 4-bit rows (mx4_tc.cu).  Small layers of up to 8 rows are faster in one launch (mx4_rows.cu), us against us: one row
 // of 2048 x 2048 5.5 and 7.6, of 3584 x 3584 7.3 and 8.3, of 8192 x 4096 13.7 and 9.7; 4 rows of 3584 x 3584 7.7 and 8.7, 16 rows
-// 12.7 and 10.5.
+// 12.7 and 10.5.  More than 16 rows are unpacked weights' (mx4_mixed_tc.cu) from about two tiles of 8 rows x 128 weight rows an SM on, us
+// against us of those: 17 rows of 3584 x 3584 (84 tiles) 9.9 and 18.3, 64 of 4608 x 3584 (288) 16.4 and 19.1, 17 of 18944 x 3584 (444)
+// 20.8 and 19.0, 279 of 1152 x 4304 (315) 31.2 and 21.5.
 bool by_pieces(const vila_mx4_linear_params& p) {
-  return p.x != nullptr && p.M <= kFew && (p.M > 8 || static_cast<long long>(p.N) * p.K > (16ll << 20));
+  if (p.x == nullptr) return false;
+  if (p.M <= kFew) return p.M > 8 || static_cast<long long>(p.N) * p.K > (16ll << 20);
+  return static_cast<long long>((p.N + 127) / 128) * ((p.M + 7) / 8) <= 2ll * num_sms();
 }
 int padded(int K) { return (K + 7) & ~7; }
 

@@ -1379,7 +1379,7 @@ def _mx4_product(x: Optional[torch.Tensor], a: Optional[Mx4], M: int, K: int, w:
                              None if a is None else a.scales.data_ptr(), codes.data_ptr(), w.scales.data_ptr(),
                              None if bias is None else bias.data_ptr(), out.data_ptr(), out.stride(0), alpha, limit, pos, neg, M, N, K, act, flags)
     lib = _lib.load()
-    if x is not None and (M <= 16 or (p.x | 2 * p.ldx) % 16):      # a workspace of the call's own: a captured graph keeps its own, too
+    if x is not None:      # a workspace of the call's own: a captured graph keeps its own, too
         n = lib.vila_mx4_linear_scratch(C.byref(p))
         if n:
             scratch = codes.new_empty(n)
