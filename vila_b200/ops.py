@@ -1257,14 +1257,46 @@ class Mx4:
     """Rows of microscaled 4-bit numbers (include/vila_b200.h has the format): codes uint8 [rows, 16 * ceil(cols / 32)] and
     scales uint8 in the tiled order that the products read.  Made by mx4_quantize, or by mx4_pack from plain scale bytes."""
 
-    __slots__ = ("codes", "scales", "rows", "cols")
+    __slots__ = ("rows", "cols", "_codes", "_scales", "_both", "_at")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, cols: int):
         _mx4_check(cols > 0 and codes.dim() == 2 and codes.dtype == torch.uint8 and codes.is_contiguous()
                    and codes.shape[1] == 16 * ((cols + 31) // 32), "codes must be contiguous uint8 [rows, 16 * ceil(cols / 32)]")
         _mx4_check(scales.dtype == torch.uint8 and scales.is_contiguous() and scales.device == codes.device
                    and scales.numel() == _mx4_scale_bytes(codes.shape[0], cols), "scales must be contiguous uint8, in the tiled order")
-        self.codes, self.scales, self.rows, self.cols = codes, scales, codes.shape[0], cols
+        self._codes, self._scales, self._both, self._at = codes, scales, None, 0
+        self.rows, self.cols = codes.shape[0], cols
+
+    @classmethod
+    def _alloc(cls, like: torch.Tensor, rows: int, cols: int) -> "Mx4":
+        """Uninitialised, codes and scales in one piece of memory on the device of `like`: the views of it are made when they are
+        asked for (an allocation takes 2 us of the host's time, a view 1)."""
+        q = cls.__new__(cls)
+        q.rows, q.cols, q._codes, q._scales = rows, cols, None, None
+        q._at = rows * 16 * ((cols + 31) // 32)
+        q._both = like.new_empty(q._at + _mx4_scale_bytes(rows, cols), dtype=torch.uint8)
+        return q
+
+    @property
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            self._codes = self._both[:self._at].view(self.rows, -1) if self.rows else self._both.new_empty((0, 16 * ((self.cols + 31) // 32)))
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            self._scales = self._both[self._at:]
+        return self._scales
+
+    def _held(self) -> torch.Tensor:
+        return self._codes if self._both is None else self._both
+
+    def _ptrs(self) -> Tuple[int, int]:
+        if self._both is not None:
+            p = self._both.data_ptr()
+            return p, p + self._at
+        return self._codes.data_ptr(), self._scales.data_ptr()
 
     @property
     def shape(self) -> Tuple[int, int]:
@@ -1272,11 +1304,11 @@ class Mx4:
 
     @property
     def device(self) -> torch.device:
-        return self.codes.device
+        return self._held().device
 
     @property
     def nbytes(self) -> int:
-        return self.codes.numel() + self.scales.numel()
+        return self.rows * 16 * ((self.cols + 31) // 32) + _mx4_scale_bytes(self.rows, self.cols)
 
 
 def _mx4_check(ok: bool, what: str) -> None:
@@ -1302,24 +1334,26 @@ def mx4_quantize(x: torch.Tensor) -> Mx4:
     the scale is 2^max(floor(log2 m) - 2, -127), and every x / scale becomes the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 (ties to
     the even code, 6 beyond 6; signs kept).  A block with an infinity or a NaN reads as NaN."""
     _mx4_here(x, "x")
-    if x.dim() != 2 or x.shape[1] == 0 or (x.stride(1) != 1 and x.shape[1] != 1):
+    if x.dim() != 2:
         raise RuntimeError("vila_b200.ops: x must be [rows, cols] with consecutive columns")
     rows, cols = x.shape
-    q = Mx4.__new__(Mx4)
-    q.codes = x.new_empty((rows, 16 * ((cols + 31) // 32)), dtype=torch.uint8)
-    q.scales = x.new_empty(_mx4_scale_bytes(rows, cols), dtype=torch.uint8)
-    q.rows, q.cols = rows, cols
-    check(_lib.load().vila_mx4_quantize(x.data_ptr(), _dt(x, "x"), x.stride(0), q.codes.data_ptr(), q.scales.data_ptr(), rows, cols,
-                                        _stream()), "vila_mx4_quantize")
+    if cols == 0 or (x.stride(1) != 1 and cols != 1):
+        raise RuntimeError("vila_b200.ops: x must be [rows, cols] with consecutive columns")
+    dt = _dt(x, "x")
+    q = Mx4._alloc(x, rows, cols)
+    codes, scales = q._ptrs()
+    check(_lib.load().vila_mx4_quantize(x.data_ptr(), dt, x.stride(0), codes, scales, rows, cols, _stream()), "vila_mx4_quantize")
     return q
 
 
 def mx4_dequantize(q: Mx4, out_dtype=torch.bfloat16) -> torch.Tensor:
     """The numbers that q stands for, [rows, cols] in bf16 or fp32."""
-    _mx4_here(q.codes, "q")
-    out = q.codes.new_empty((q.rows, q.cols), dtype=out_dtype)
-    check(_lib.load().vila_mx4_dequantize(q.codes.data_ptr(), q.scales.data_ptr(), out.data_ptr(), _dt(out, "out"), q.cols, q.rows, q.cols,
-                                          _stream()), "vila_mx4_dequantize")
+    held = q._held()
+    _mx4_here(held, "q")
+    out = held.new_empty((q.rows, q.cols), dtype=out_dtype)
+    codes, scales = q._ptrs()
+    check(_lib.load().vila_mx4_dequantize(codes, scales, out.data_ptr(), _dt(out, "out"), q.cols, q.rows, q.cols, _stream()),
+          "vila_mx4_dequantize")
     return out
 
 
@@ -1345,7 +1379,7 @@ def mx4_pack(codes: torch.Tensor, scales: torch.Tensor, cols: int) -> Mx4:
 
 def mx4_unpack(q: Mx4) -> Tuple[torch.Tensor, torch.Tensor]:
     """-> codes uint8 [rows, 16 * blocks] (q's own) and plain scale bytes uint8 [rows, blocks]."""
-    _mx4_here(q.codes, "q")
+    _mx4_here(q._held(), "q")
     plain = torch.empty(q.rows, (q.cols + 31) // 32, dtype=torch.uint8, device=q.device)
     check(_lib.load().vila_mx4_scales(_p(plain), _p(q.scales), q.rows, q.cols, 0, _stream()), "vila_mx4_scales")
     return q.codes, plain
@@ -1354,15 +1388,15 @@ def mx4_unpack(q: Mx4) -> Tuple[torch.Tensor, torch.Tensor]:
 def _mx4_product(x: Optional[torch.Tensor], a: Optional[Mx4], M: int, K: int, w: Mx4, bias, act, act_params, swiglu, geglu, glu_clamp,
                  out) -> torch.Tensor:
     """x or a: the rows.  (The parameters go by position: by name they took 4 us of a call.)"""
-    N, codes = w.rows, w.codes
-    _mx4_here(codes, "w")
+    N, held = w.rows, w._held()
+    _mx4_here(held, "w")
     if K != w.cols or N == 0:
         raise RuntimeError(f"vila_b200.ops: {M} x {K} rows do not fit a weight of {N} x {w.cols}")
     flags = (1 if swiglu else 0) | (4 if glu_clamp is not None else 0) | (FLAG_GEGLU if geglu else 0)
     _mx4_check(act != ACT_XIELU or act_params is not None, "ACT_XIELU takes act_params")
     n_out = N // 2 if flags else N
     if out is None:
-        out = codes.new_empty((M, n_out), dtype=torch.bfloat16)
+        out = held.new_empty((M, n_out), dtype=torch.bfloat16)
     else:
         _chk(out, "out")
         _mx4_here(out, "out")
@@ -1375,14 +1409,19 @@ def _mx4_product(x: Optional[torch.Tensor], a: Optional[Mx4], M: int, K: int, w:
         return out
     alpha, limit = glu_clamp if glu_clamp is not None else (0.0, 0.0)
     pos, neg = act_params if act_params is not None else (0.0, 0.0)
-    p = _lib.Mx4LinearParams(None if x is None else x.data_ptr(), 0 if x is None else x.stride(0), None if a is None else a.codes.data_ptr(),
-                             None if a is None else a.scales.data_ptr(), codes.data_ptr(), w.scales.data_ptr(),
-                             None if bias is None else bias.data_ptr(), out.data_ptr(), out.stride(0), alpha, limit, pos, neg, M, N, K, act, flags)
+    w_codes, w_scales = w._ptrs()
+    if a is None:
+        p = _lib.Mx4LinearParams(x.data_ptr(), x.stride(0), None, None, w_codes, w_scales, None if bias is None else bias.data_ptr(), out.data_ptr(),
+                                 out.stride(0), alpha, limit, pos, neg, M, N, K, act, flags)
+    else:
+        a_codes, a_scales = a._ptrs()
+        p = _lib.Mx4LinearParams(None, 0, a_codes, a_scales, w_codes, w_scales, None if bias is None else bias.data_ptr(), out.data_ptr(),
+                                 out.stride(0), alpha, limit, pos, neg, M, N, K, act, flags)
     lib = _lib.load()
     if x is not None:      # a workspace of the call's own: a captured graph keeps its own, too
         n = lib.vila_mx4_linear_scratch(C.byref(p))
         if n:
-            scratch = codes.new_empty(n)
+            scratch = held.new_empty(n, dtype=torch.uint8)
             p.scratch, p.scratch_bytes = scratch.data_ptr(), n
     check(lib.vila_mx4_linear(C.byref(p), _stream()), "vila_mx4_linear")
     return out
@@ -1409,5 +1448,5 @@ def mx4_matmul(a: Mx4, w: Mx4, bias: Optional[torch.Tensor] = None, *, act: int 
     """act(a [M, K] . w[N, K]^T + bias) in bf16, both factors in 4 bits (a = mx4_quantize(x)), fp32 sums."""
     if not (isinstance(a, Mx4) and isinstance(w, Mx4)):
         raise RuntimeError("vila_b200.ops: a and w must be Mx4 (mx4_quantize, mx4_pack)")
-    _mx4_here(a.codes, "a")
+    _mx4_here(a._held(), "a")
     return _mx4_product(None, a, a.rows, a.cols, w, bias, act, act_params, swiglu, geglu, glu_clamp, out)
