@@ -33,6 +33,7 @@ def main(argv=None) -> str:
                         help="prompt as comma-separated token ids; ';' separates several prompts")
     parser.add_argument("--max-new-tokens", type=int, default=32)
     parser.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
+    parser.add_argument("--weights", choices=["mx4"], default=None, help="hold the layers' weights in microscaled 4-bit numbers")
     parser.add_argument("--temperature", type=float, default=0.0, help="0: greedy")
     parser.add_argument("--top-k", type=int, default=0)
     parser.add_argument("--top-p", type=float, default=1.0)
@@ -43,7 +44,7 @@ def main(argv=None) -> str:
         if args.token_ids is None:
             raise SystemExit("--token-ids is required for a token-id language model")
         prompts = [[int(t) for t in p.split(",") if t.strip()] for p in args.token_ids.split(";")]
-        lm = load_language_model(args.model_path, dtype=args.dtype)
+        lm = load_language_model(args.model_path, dtype=args.dtype, weights=args.weights)
         out = lm.generate(prompts, max_new_tokens=args.max_new_tokens, do_sample=args.temperature > 0,
                           temperature=args.temperature or 1.0, top_k=args.top_k, top_p=args.top_p, seed=args.seed)
         response = ";".join(",".join(map(str, ids)) for ids in out)

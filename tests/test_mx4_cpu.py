@@ -84,3 +84,18 @@ def test_parameter_struct_follows_the_header():
             names = decl.strip().split(",")
             fields += [names[0].split()[-1].lstrip("*")] + [n.strip().lstrip("*") for n in names[1:]]
     assert fields == [f[0] for f in _lib.Mx4LinearParams._fields_]
+
+
+def test_weights_in_4_bits_are_refused_before_anything_is_loaded(tmp_path):
+    import json
+    from vila_b200.model.registry import load_language_model, quantize_weights
+    (tmp_path / "config.json").write_text(json.dumps({"architecture": "Moronex"}))
+    with pytest.raises(ValueError, match="4-bit weights are for"):
+        load_language_model(tmp_path, weights="mx4")
+    (tmp_path / "config.json").write_text(json.dumps({"architecture": "Nusovik"}))
+    with pytest.raises(ValueError, match="in bfloat16"):
+        load_language_model(tmp_path, dtype="float32", weights="mx4")
+    with pytest.raises(ValueError, match="None or 'mx4'"):
+        load_language_model(tmp_path, weights="int4")
+    with pytest.raises(ValueError, match="does not hold weights in 4 bits"):
+        quantize_weights(object())

@@ -80,6 +80,11 @@ __device__ __forceinline__ uint32_t mx4_test(uint64_t* bar, uint32_t parity) {
                : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
   return ok;
 }
+// A CTA of a pair that gives up: its tokens' loads report to the first CTA's barriers, which may have given up before it asked for its part
+// of them.  They land within a few microseconds.
+__device__ __forceinline__ void mx4_let_loads_land() {
+  for (int i = 0; i < 64; ++i) __nanosleep(1000);
+}
 // consecutive bytes (a multiple of 16, on 16-byte boundaries)
 __device__ __forceinline__ void mx4_bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src),

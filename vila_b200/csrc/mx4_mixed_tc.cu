@@ -228,7 +228,10 @@ mx4_mixed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
           }
         }
       }
-      if (!ok) tell();
+      if (!ok) {
+        tell();
+        if (kPair) mx4_let_loads_land();
+      }
       // what was asked for lands before the CTA's memory is given back, whichever warp gave up (a pair's tokens report to the first CTA)
       if (rank == 0)
         for (int i = 0; i < S::kTok; ++i) {

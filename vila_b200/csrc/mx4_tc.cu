@@ -426,7 +426,10 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
           }
         }
       }
-      if (!ok) tell();
+      if (!ok) {
+        tell();
+        mx4_let_loads_land();
+      }
       // what was asked for lands before the CTAs' memory is given back (their loads report to the first one)
       if (rank == 0)
         for (int i = 0; i < kStages; ++i) {

@@ -11,7 +11,7 @@ from .moronex import MoronexConfig, MoronexForCausalLM, MoronexLayerConfig
 from .nibelix import NibelixConfig, NibelixForCausalLM, NibelixLayerConfig
 from .nusovik import NusovikConfig, NusovikForCausalLM, NusovikLayerConfig
 from .projector import MultimodalProjector
-from .registry import LANGUAGE_MODELS, language_model_architecture, load_language_model
+from .registry import LANGUAGE_MODELS, language_model_architecture, load_language_model, quantize_weights
 from .qwen2 import GraphDecoder, MegaDecoder, PagedKVCache, Qwen2ForCausalLM
 from .vision import SiglipVisionModel, SiglipVisionTower
 

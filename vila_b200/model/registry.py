@@ -31,10 +31,46 @@ def language_model_architecture(model_dir) -> Optional[str]:
     return arch if arch in LANGUAGE_MODELS else None
 
 
-def load_language_model(model_dir, device="cuda", dtype="bfloat16"):
+# The layers' weights that linear_any alone reads, by class: these may be held in 4 bits.  Narrow projections that a recurrence's
+# step size or decay comes from stay as they are, as do embeddings, routers, experts, norms and the output head.
+MX4_WEIGHTS: Dict[str, tuple] = {
+    "Lufatar": ("qkv", "o", "side_gate", "side_proj"),
+    "Nusovik": ("qkg", "attn_o", "ssd_in", "ssd_o", "sel_in", "sel_o", "up", "down"),
+    "Ludazen": ("qkv", "in_w", "o", "up", "down", "shared_gu", "shared_down"),
+    "Bivizen": ("in_w", "o", "gu", "down"),
+    "Nibelix": ("in_w", "o", "gu", "down", "shared_up", "shared_down"),
+}
+
+
+def quantize_weights(model):
+    """Hold a bf16 language model's layer weights as microscaled 4-bit rows (ops.Mx4: 17 bytes per 32 of them instead of 64), each
+    rounded to the nearest number of its block; activations stay bf16.  In place; -> model.  state_dict and save_pretrained
+    still give the weights that were loaded."""
+    from .. import ops
+    arch = next((a for a, c in LANGUAGE_MODELS.items() if type(model) is c), None)
+    names = MX4_WEIGHTS.get(arch)
+    if names is None:
+        raise ValueError(f"{type(model).__name__} does not hold weights in 4 bits (those that do: {sorted(MX4_WEIGHTS)})")
+    if model.dtype != torch.bfloat16:
+        raise ValueError(f"4-bit weights go with bfloat16 activations, not {model.dtype}")
+    for layer in model.layers:
+        for name in names:
+            w = getattr(layer, name, None)
+            if isinstance(w, torch.Tensor) and w.dim() == 2:      # experts' weights are one tensor of three dimensions
+                setattr(layer, name, ops.mx4_quantize(w))
+    return model
+
+
+def load_language_model(model_dir, device="cuda", dtype="bfloat16", weights: Optional[str] = None):
+    """weights: None (as dtype says) or "mx4" (quantize_weights)"""
+    if weights not in (None, "mx4"):
+        raise ValueError(f"weights={weights!r}: None or 'mx4'")
     arch = language_model_architecture(model_dir)
     if arch is None:
         raise ValueError(f"{model_dir}: config.json names no registered architecture "
                          f"(known: {sorted(LANGUAGE_MODELS)})")
     dt = _DTYPES[dtype] if isinstance(dtype, str) else dtype
-    return LANGUAGE_MODELS[arch].from_pretrained(model_dir, device=device, dtype=dt)
+    if weights is not None and (arch not in MX4_WEIGHTS or dt != torch.bfloat16):      # before anything is loaded
+        raise ValueError(f"{arch} in {dt}: 4-bit weights are for {sorted(MX4_WEIGHTS)} in bfloat16")
+    model = LANGUAGE_MODELS[arch].from_pretrained(model_dir, device=device, dtype=dt)
+    return model if weights is None else quantize_weights(model)

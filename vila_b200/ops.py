@@ -703,7 +703,12 @@ def linear_any(x: torch.Tensor, w: torch.Tensor, *, swiglu: bool = False, out_dt
                act_params: Optional[Tuple[float, float]] = None,
                glu_clamp: Optional[Tuple[float, float]] = None, geglu: bool = False) -> torch.Tensor:
     """act(x [M, K] · w[N, K]^T + bias): bf16 operands with 16-byte aligned rows go to the tcgen05 GEMM,
-    everything else (fp32 tensors, odd shapes, an fp32 result) to the CUDA-core grouped kernel."""
+    everything else (fp32 tensors, odd shapes, an fp32 result) to the CUDA-core grouped kernel.  w may be an Mx4
+    (mx4_quantize): bf16 rows on 4-bit weights, a bf16 result."""
+    if isinstance(w, Mx4):
+        if out_dtype not in (None, torch.bfloat16):
+            raise RuntimeError(f"vila_b200.ops: a linear layer on 4-bit weights gives bfloat16, not {out_dtype}")
+        return mx4_linear(x, w, bias, act=act, act_params=act_params, swiglu=swiglu, geglu=geglu, glu_clamp=glu_clamp)
     N, K = w.shape
     if (x.dtype == torch.bfloat16 and w.dtype == torch.bfloat16 and out_dtype in (None, torch.bfloat16)
             and K % 8 == 0 and N % 8 == 0 and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0
