@@ -162,7 +162,13 @@ SIZES = [(1, 2, 32), (1, 128, 64), (1, 300, 2048), (3, 129, 95), (7, 64, 1153), 
          (520, 258, 1056), (2600, 2570, 800)]
 
 
-@pytest.mark.parametrize("M, N, K", SIZES)
+# more tiles than rows cut into 4-bit rows are used for: unpacked weights, by tile size (64, 96, 128 rows, pairs), rows off 16-byte
+# boundaries (odd K), K of one step, of half a stage, several rounds of the rings, several tiles a CTA
+UNPACKED = [(20, 16000, 96), (60, 12000, 520), (33, 9700, 1153), (90, 12000, 520), (96, 6300, 32), (120, 12000, 776), (200, 20000, 300),
+            (1200, 5000, 520), (700, 5001, 577), (1031, 2500, 1600)]
+
+
+@pytest.mark.parametrize("M, N, K", SIZES + UNPACKED)
 def test_linear(cuda, M, N, K):
     from vila_b200 import ops
     q, w = weight(M, N, K, cuda, spread=1.0)
@@ -199,25 +205,53 @@ def test_activations(cuda, M, act, four):
     check_product(got, x, w, bias, act)
 
 
-@pytest.mark.parametrize("M", [2, 40, 300])
-@pytest.mark.parametrize("gap, off", [(8, 0), (3, 0), (8, 1), (0, 2)])
-def test_views(cuda, M, gap, off):
+def test_few_rows_of_a_wide_layer(cuda):
+    """rows cut into 4-bit rows: several tiles of tokens (16 rows) and K over a cluster"""
     from vila_b200 import ops
-    q, w = weight(30, 200, 288, cuda)
+    for M, N, K in ((1, 20000, 1000), (3, 9000, 2080), (8, 5000, 4000), (16, 6000, 3000), (2, 384, 50000)):
+        q, w = weight(M, N, K, cuda)
+        x, bias = rand(7, M, K).to(BF), rand(9, N).to(BF)
+        check_product(ops.mx4_linear(x.to(cuda), q, bias.to(cuda)), x, w, bias)
+
+
+@pytest.mark.parametrize("act", ["silu", "relu2", "gelu_tanh", "gelu_erf", "xielu", "swiglu", "geglu", "glu_clamp"])
+@pytest.mark.parametrize("M, N", [(1, 60002), (60, 9002), (90, 9002), (120, 9002), (700, 5002)])
+def test_activations_of_wide_layers(cuda, M, N, act):
+    from vila_b200 import ops
+    q, w = weight(20, N, 320, cuda)
+    x, bias = (2 * rand(21, M, 320)).to(BF), rand(22, N).to(BF)
+    check_product(ops.mx4_linear(x.to(cuda), q, bias.to(cuda), **act_args(act)), x, w, bias, act)
+
+
+@pytest.mark.parametrize("M, N", [(2, 200), (40, 200), (300, 200), (2, 70000), (60, 9000), (700, 5000)])
+@pytest.mark.parametrize("gap, off", [(8, 0), (3, 0), (8, 1), (0, 2)])
+def test_views(cuda, M, N, gap, off):
+    from vila_b200 import ops
+    q, w = weight(30, N, 288, cuda)
     wide = rand(31, M, 288 + gap + off).to(BF)
-    out = torch.full((M, 211), 7.0, dtype=BF, device=cuda)
-    got = ops.mx4_linear(wide.to(cuda)[:, off:off + 288], q, out=out[:, 5:205])
-    assert got.data_ptr() == out[:, 5:205].data_ptr()
+    out = torch.full((M, N + 11), 7.0, dtype=BF, device=cuda)
+    got = ops.mx4_linear(wide.to(cuda)[:, off:off + 288], q, out=out[:, 5:5 + N])
+    assert got.data_ptr() == out[:, 5:].data_ptr()
     check_product(got, wide[:, off:off + 288], w, None)
-    assert (out[:, :5] == 7).all() and (out[:, 205:] == 7).all()
+    assert (out[:, :5] == 7).all() and (out[:, 5 + N:] == 7).all()
 
 
-@pytest.mark.parametrize("M", [1, 8, 16, 50, 300])
-@pytest.mark.parametrize("four", [False, True])
-def test_scales_over_the_whole_range(cuda, M, four):
+@pytest.mark.parametrize("M, N", [(3, 200), (40, 200), (3, 70000), (60, 9000), (700, 5000)])
+def test_broadcast_rows(cuda, M, N):
+    from vila_b200 import ops
+    q, w = weight(32, N, 288, cuda)
+    x = rand(33, 1, 288).to(BF)
+    got = ops.mx4_linear(x.to(cuda).expand(M, 288), q)
+    check_product(got, x.expand(M, 288), w, None)
+    assert (got == got[:1]).all()
+
+
+@pytest.mark.parametrize("M, N, four", [(M, 140, four) for M in (1, 8, 16, 50, 300) for four in (False, True)] +
+                         [(2, 40000, False), (60, 9000, False), (90, 9000, False), (700, 5000, False)])
+def test_scales_over_the_whole_range(cuda, M, N, four):
     """blocks of one row whose sizes are 2^40 apart, rows that differ by 2^60"""
     from vila_b200 import ops
-    N, K = 140, 512
+    K = 512
     sizes = torch.tensor([2.0 ** -20, 2.0 ** 20, 1.0, 2.0 ** -5]).repeat_interleave(32).repeat(K // 128)
     rows = torch.exp2(torch.arange(N).float() % 61 - 30)
     codes, scales = R.quantise(rand(40, N, K) * sizes * rows[:, None])
@@ -229,11 +263,11 @@ def test_scales_over_the_whole_range(cuda, M, four):
         check_product(ops.mx4_linear(x.to(cuda), q), x, w, None)
 
 
-@pytest.mark.parametrize("M", [3, 40, 300])
-@pytest.mark.parametrize("four", [False, True])
-def test_not_a_number_stays_in_its_row_and_column(cuda, M, four):
+@pytest.mark.parametrize("M, N, four", [(M, 150, four) for M in (3, 40, 300) for four in (False, True)] +
+                         [(3, 50000, False), (60, 9000, False), (90, 9000, False), (700, 5000, False)])
+def test_not_a_number_stays_in_its_row_and_column(cuda, M, N, four):
     from vila_b200 import ops
-    N, K = 150, 416
+    K = 416
     codes, scales = R.quantise(rand(50, N, K))
     scales[17, 3] = 255
     q, w = ops.mx4_pack(codes.to(cuda), scales.to(cuda), K), R.values(codes, scales, K)
@@ -250,11 +284,11 @@ def test_not_a_number_stays_in_its_row_and_column(cuda, M, four):
     check_product(got[rows][:, cols].to(BF), ref[rows], w[cols], None)
 
 
-@pytest.mark.parametrize("M", [1, 5, 30, 300])
-@pytest.mark.parametrize("four", [False, True])
-def test_same_bits_every_time_and_on_another_stream_and_in_a_graph(cuda, M, four):
+@pytest.mark.parametrize("M, N, four", [(M, 384, four) for M in (1, 5, 30, 300) for four in (False, True)] +
+                         [(2, 17000, False), (60, 9000, False), (700, 5000, False), (700, 5000, True)])
+def test_same_bits_every_time_and_on_another_stream_and_in_a_graph(cuda, M, N, four):
     from vila_b200 import ops
-    q, w = weight(60, 384, 1000, cuda)
+    q, w = weight(60, N, 1000, cuda)
     x = rand(61, M, 1000).to(BF).to(cuda)
     call = (lambda: ops.mx4_matmul(ops.mx4_quantize(x), q)) if four else (lambda: ops.mx4_linear(x, q))
     first = call()
