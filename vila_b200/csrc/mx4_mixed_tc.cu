@@ -5,7 +5,8 @@
 // memory: the M side of tcgen05.mma may lie in TMEM, lane = weight row, 32 columns = 64 weights of a row, which is what a thread that
 // unpacks its own row writes with one tcgen05.st.  Shared memory then only serves the tokens, the N side.
 //
-//   TMA warp         codes and scales, 256 columns of 128 rows at a time; a stage of tokens (64 columns, 128 bytes, swizzled)
+//   2 TMA warps      codes and scales, 256 columns of 128 rows at a time; a stage of tokens (64 columns, 128 bytes, swizzled).  As the MMA
+//                    warp they stay converged but for the branch that issues: one thread with both loops took 800 clocks a stage
 //   unpack warps     two or three groups of four (a warp reaches the TMEM lanes of its quarter), which take the stages in turn: a byte of
 //                    codes (two weights) is looked up in shared memory as a pair of bf16, then multiplied by the block's 2^e
 //   MMA warp         TMEM allocation; tcgen05.mma of K = 16, four per 64 columns, into one of two accumulator sets
@@ -40,7 +41,7 @@ static_assert(kSmemFrom + kLow <= kTable && kSmem <= 227 * 1024, "");
 
 template <int BT, bool kPair> struct Shape {
   static constexpr int kGroups = kPair ? 2 : 3;                 // of four unpack warps
-  static constexpr int kUnpack = 4 * kGroups, kTma = kEpi + kUnpack, kMma = kTma + 1, kThreads = 32 * (kMma + 1);
+  static constexpr int kUnpack = 4 * kGroups, kTma = kEpi + kUnpack, kCode = kTma + 1, kMma = kTma + 2, kThreads = 32 * (kMma + 1);
   // times 64 columns are a stage: of one, the issuing warp's 400 clocks a stage showed (17 rows, 3584 x 3584: 22.2 us, of two 19.1)
   static constexpr int kSub = kPair ? 1 : 2;
   static constexpr int kTokRows = kPair ? BT / 2 : BT;          // that a CTA holds
@@ -98,7 +99,7 @@ __global__ void __launch_bounds__(Shape<BT, kPair>::kThreads, 1)
 mx4_mixed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const vila_mx4_linear_params p,
                  const vila_glinear_ext x, const Pieces pieces, const WaitLimit limit, volatile unsigned int* failed) {
   using S = Shape<BT, kPair>;
-  constexpr int kUnpack = S::kUnpack, kTma = S::kTma, kMma = S::kMma;
+  constexpr int kUnpack = S::kUnpack, kTma = S::kTma, kCode = S::kCode, kMma = S::kMma;
   constexpr int kCtas = kPair ? 2 : 1, kSteps = kCodeDepth / (kDepth * S::kSub);      // stages of 256 columns
   extern __shared__ uint8_t smem_raw[];
   // where it lies in the shared window is known, as the kernel has no other; in a cluster the CTA's rank is in the upper bits.  (Were it
@@ -183,66 +184,89 @@ mx4_mixed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
   if (kPair) cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem = *tmem_ptr;
-  bool ok = limit.quits < 0 || limit.quits != (warp == kTma ? 0 : warp == kMma ? 1 : warp >= kFirstUnpack ? 2 : 3);
+  bool ok = limit.quits < 0 || limit.quits != (warp == kTma || warp == kCode ? 0 : warp == kMma ? 1 : warp >= kFirstUnpack ? 2 : 3);
 
   if (warp == kTma) {
-    if (lane == 0) {
-      const int kts = 2 * nkc, tok_rows = kPair ? pieces.per / 2 : pieces.per;
-      const uint32_t tok_bytes = S::kSub * pieces.per * 128;      // of both CTAs
-      int s = 0, rounds = 0, cs = 0, crounds = 0;      // stages, and rounds through all of them
-      uint32_t ph = 1, cph = 1;
-      for (int it = worker; it < total && ok; it += workers) {
-        int n0, m0, count;
-        tile_at(it, n0, m0, count);
-        for (int kb = 0; kb < nkb; ++kb) {
-          if (kb % kSteps == 0) {
-            const int kc = kb / kSteps;
-            ok = mbar_wait_limited(&code_empty[cs], cph, gave_up, limit.tries);
-            if (!ok) break;
-            uint8_t* st = codes_s + cs * kCodeStage;
-            // the second CTA's rows may begin past the last weight row: TMA fills in zeros, scales are not loaded
-            const bool scales = n0 < p.N;
-            mbar_arrive_expect_tx(&code_full[cs], kCodeBytes + (scales ? 1024 : 0));
-            tma_load_2d(st, &tmap_w, &code_full[cs], kc * 128, n0);
-            if (scales) mx4_bulk_load(st + kCodeBytes, p.w_scales + (static_cast<size_t>(n0 >> 7) * kts + 2 * kc) * 512, 1024, &code_full[cs]);
-            if (++cs == kCodeStages) {
-              cs = 0;
-              cph ^= 1;
-              ++crounds;
-            }
-          }
-          ok = mbar_wait_limited(&tok_empty[s], ph, gave_up, limit.tries);
-          if (!ok) break;
-          uint8_t* st = smem + s * S::kTokBytes;
-          if (rank == 0) mbar_arrive_expect_tx(&tok_full[s], tok_bytes);
+    const bool one = elect_one();
+    const int tok_rows = kPair ? pieces.per / 2 : pieces.per;
+    const uint32_t tok_bytes = S::kSub * pieces.per * 128;      // of both CTAs
+    int s = 0, rounds = 0;                // stage, and rounds through all of them
+    uint32_t ph = 1, here = 1;            // the first round passes
+    for (int it = worker; it < total && ok; it += workers) {
+      int n0, m0, count;
+      tile_at(it, n0, m0, count);
+      for (int kb = 0; kb < nkb; ++kb) {
+        if (!__all_sync(0xffffffffu, here)) ok = mx4_warp_wait(&tok_empty[s], ph, gave_up, limit.tries);
+        if (!ok) break;
+        uint8_t* st = smem + s * S::kTokBytes;
+        uint64_t* full = &tok_full[s];
+        if (++s == S::kTok) {
+          s = 0;
+          ph ^= 1;
+          ++rounds;
+        }
+        here = mx4_test(&tok_empty[s], ph);
+        if (one) {
+          if (rank == 0) mbar_arrive_expect_tx(full, tok_bytes);
           // a box is a tile's rows: of boxes of 32 rows, 8 a stage, 8192 x 8192 x 8192 took 1.23 ms, and 0.72 without the tokens
 #pragma unroll
           for (int i = 0; i < S::kSub; ++i) {
-            if (kPair) tma_load_2d_pair(st, &tmap_x, in_first(&tok_full[s]), kb * kDepth, m0 + rank * tok_rows);
-            else tma_load_2d(st + i * S::kTokRows * 128, &tmap_x, &tok_full[s], (kb * S::kSub + i) * kDepth, m0);
-          }
-          if (++s == S::kTok) {
-            s = 0;
-            ph ^= 1;
-            ++rounds;
+            if (kPair) tma_load_2d_pair(st, &tmap_x, in_first(full), kb * kDepth, m0 + rank * tok_rows);
+            else tma_load_2d(st + i * S::kTokRows * 128, &tmap_x, full, (kb * S::kSub + i) * kDepth, m0);
           }
         }
+        __syncwarp();
       }
-      if (!ok) {
-        tell();
-        if (kPair) mx4_let_loads_land();
+    }
+    if (!ok && lane == 0) {
+      tell();
+      if (kPair) mx4_let_loads_land();
+    }
+    // what was asked for lands before the CTA's memory is given back, whichever warp gave up (a pair's tokens report to the first CTA)
+    if (rank == 0 && lane == 0)
+      for (int i = 0; i < S::kTok; ++i) {
+        const int round = i < s ? rounds : rounds - 1;
+        if (round >= 0) mbar_drain(&tok_full[i], round & 1);
       }
-      // what was asked for lands before the CTA's memory is given back, whichever warp gave up (a pair's tokens report to the first CTA)
-      if (rank == 0)
-        for (int i = 0; i < S::kTok; ++i) {
-          const int round = i < s ? rounds : rounds - 1;
-          if (round >= 0) mbar_drain(&tok_full[i], round & 1);
+    __syncwarp();
+  } else if (warp == kCode) {
+    const bool one = elect_one();
+    const int kts = 2 * nkc;
+    int s = 0, rounds = 0;
+    uint32_t ph = 1, here = 1;
+    for (int it = worker; it < total && ok; it += workers) {
+      int n0, m0, count;
+      tile_at(it, n0, m0, count);
+      // the second CTA's rows may begin past the last weight row: TMA fills in zeros, scales are not loaded
+      const bool scales = n0 < p.N;
+      const uint8_t* scale = p.w_scales + static_cast<size_t>(n0 >> 7) * kts * 512;
+      for (int kc = 0; kc < nkc; ++kc) {
+        if (!__all_sync(0xffffffffu, here)) ok = mx4_warp_wait(&code_empty[s], ph, gave_up, limit.tries);
+        if (!ok) break;
+        uint8_t* st = codes_s + s * kCodeStage;
+        uint64_t* full = &code_full[s];
+        if (++s == kCodeStages) {
+          s = 0;
+          ph ^= 1;
+          ++rounds;
         }
+        here = mx4_test(&code_empty[s], ph);
+        if (one) {
+          mbar_arrive_expect_tx(full, kCodeBytes + (scales ? 1024 : 0));
+          tma_load_2d(st, &tmap_w, full, kc * 128, n0);
+          if (scales) mx4_bulk_load(st + kCodeBytes, scale + kc * 1024, 1024, full);
+        }
+        __syncwarp();
+      }
+    }
+    if (lane == 0) {
+      if (!ok) tell();
       for (int i = 0; i < kCodeStages; ++i) {
-        const int round = i < cs ? crounds : crounds - 1;
+        const int round = i < s ? rounds : rounds - 1;
         if (round >= 0) mbar_drain(&code_full[i], round & 1);
       }
     }
+    __syncwarp();
   } else if (warp == kMma) {
     if (rank == 0) {
       // The whole warp walks the loop and one lane issues: what the instructions are given stays in uniform registers.
@@ -297,16 +321,23 @@ mx4_mixed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
     const int group = (warp - kFirstUnpack) >> 2, quad = warp & 3, row = quad * 32 + lane;
     const uint32_t here = window + kTable + lane * 4;
     int j = 0, cs = 0;                    // stages so far (all tiles), code stage
-    uint32_t cph = 0;
+    uint32_t cph = 0, code_here = 0;
     for (int it = worker; it < total && ok; it += workers) {
       for (int kc = 0; kc < nkc && ok; ++kc) {
-        ok = mx4_warp_wait(&code_full[cs], cph, gave_up, limit.tries);
+        if (!__all_sync(0xffffffffu, code_here)) ok = mx4_warp_wait(&code_full[cs], cph, gave_up, limit.tries);
         if (!ok) break;
         const uint8_t* st = codes_s + cs * kCodeStage;
+        uint64_t* code_done = &code_empty[cs];
+        if (++cs == kCodeStages) {
+          cs = 0;
+          cph ^= 1;
+        }
+        code_here = mx4_test(&code_full[cs], cph);
         const int steps = min(kSteps, nkb - kSteps * kc);
         for (int step = 0; step < steps && ok; ++step, ++j) {
           if (j % S::kGroups != group) continue;
           const int w = j % S::kW;
+          const uint32_t w_free = mx4_test(&w_empty[w], ((j / S::kW) & 1) ^ 1);
 #pragma unroll
           for (int i = 0; i < S::kSub; ++i) {
             const int q = step * S::kSub + i;
@@ -324,7 +355,7 @@ mx4_mixed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
 #pragma unroll
             for (int e = 0; e < 32; ++e) y[e] = mul_bf16x2(y[e], e < 16 ? f0 : f1);
             if (i == 0) {
-              ok = mx4_warp_wait(&w_empty[w], ((j / S::kW) & 1) ^ 1, gave_up, limit.tries);
+              if (!__all_sync(0xffffffffu, w_free)) ok = mx4_warp_wait(&w_empty[w], ((j / S::kW) & 1) ^ 1, gave_up, limit.tries);
               if (!ok) break;
               tc_fence_after();
             }
@@ -337,11 +368,7 @@ mx4_mixed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
           if (lane == 0) arrive_first(&w_full[w]);
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&code_empty[cs]);
-        if (++cs == kCodeStages) {
-          cs = 0;
-          cph ^= 1;
-        }
+        if (lane == 0) mbar_arrive(code_done);
       }
     }
     if (!ok && lane == 0) tell();

@@ -122,55 +122,62 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant_
   }
 
   if (warp == kTma) {
-    if (lane == 0) {
-      const uint8_t *sp = kSwap ? p.w_scales : p.a_scales, *sq = kSwap ? p.a_scales : p.w_scales;
-      const int q_row_tiles = (Q + 127) / 128;
-      int s = 0, rounds = 0;              // rounds: through all the stages
-      uint32_t ph = 1;                    // parity to wait for on an empty barrier: the first round passes
-      for (int it = it0; it < total && ok; it += it_step) {
-        int p0, q0;
-        tile_at(it, p0, q0);
-        const int qt0 = q0 >> 7, qts = min(S::kQTiles, q_row_tiles - qt0);
-        const uint32_t bytes = S::kPBytes + S::kQBytes + 1024 * (1 + qts);
-        auto load_p = [&](int kb, int s) {
-          uint8_t* st = smem + s * S::kStage;
-          mbar_arrive_expect_tx(&full_bar[s], bytes);
-          tma_load_2d(st, &tmap_p, &full_bar[s], kb * 128, p0);
-          mx4_bulk_load(st + S::kPBytes + S::kQBytes, sp + (static_cast<size_t>(p0 >> 7) * kts + 2 * kb) * 512, 1024, &full_bar[s]);
-        };
-        auto load_q = [&](int kb, int s) {
-          uint8_t* st = smem + s * S::kStage;
-          tma_load_2d(st + S::kPBytes, &tmap_q, &full_bar[s], kb * 128, q0);
-          for (int q = 0; q < qts; ++q)
-            mx4_bulk_load(st + S::kPBytes + S::kQBytes + 1024 * (1 + q), sq + (static_cast<size_t>(qt0 + q) * kts + 2 * kb) * 512, 1024, &full_bar[s]);
-        };
-        int ahead = 0;
-        if (kPieces && it == it0) {      // the first weights are asked for while the kernel before cuts the tokens
-          ahead = min(ST, kb1 - kb0);
-          for (int i = 0; i < ahead; ++i) load_p(kb0 + i, i);
-          griddep_wait();
-        }
-        for (int kb = kb0; kb < kb1; ++kb) {
-          if (kb - kb0 >= ahead) {
-            ok = mbar_wait_limited(&empty_bar[s], ph, gave_up, limit.tries);
-            if (!ok) break;
-            load_p(kb, s);
-          }
-          load_q(kb, s);
-          if (++s == ST) {
-            s = 0;
-            ph ^= 1;
-            ++rounds;
-          }
-        }
+    const bool one = elect_one();
+    const uint8_t *sp = kSwap ? p.w_scales : p.a_scales, *sq = kSwap ? p.a_scales : p.w_scales;
+    const int q_row_tiles = (Q + 127) / 128;
+    int s = 0, rounds = 0;                // stage, rounds through all of them
+    uint32_t ph = 1, here = 1;            // parity to wait for on an empty barrier: the first round passes
+    for (int it = it0; it < total && ok; it += it_step) {
+      int p0, q0;
+      tile_at(it, p0, q0);
+      const int qt0 = q0 >> 7, qts = min(S::kQTiles, q_row_tiles - qt0);
+      const uint32_t bytes = S::kPBytes + S::kQBytes + 1024 * (1 + qts);
+      const uint8_t *scale_p = sp + static_cast<size_t>(p0 >> 7) * kts * 512, *scale_q = sq + static_cast<size_t>(qt0) * kts * 512;
+      auto load_p = [&](uint8_t* st, uint64_t* full, int kb) {
+        mbar_arrive_expect_tx(full, bytes);
+        tma_load_2d(st, &tmap_p, full, kb * 128, p0);
+        mx4_bulk_load(st + S::kPBytes + S::kQBytes, scale_p + kb * 1024, 1024, full);
+      };
+      auto load_q = [&](uint8_t* st, uint64_t* full, int kb) {
+        tma_load_2d(st + S::kPBytes, &tmap_q, full, kb * 128, q0);
+        for (int q = 0; q < qts; ++q)
+          mx4_bulk_load(st + S::kPBytes + S::kQBytes + 1024 * (1 + q), scale_q + static_cast<size_t>(q) * kts * 512 + kb * 1024, 1024, full);
+      };
+      int ahead = 0;
+      if (kPieces && it == it0) {      // the first weights are asked for while the kernel before cuts the tokens
+        ahead = min(ST, kb1 - kb0);
+        if (one)
+          for (int i = 0; i < ahead; ++i) load_p(smem + i * S::kStage, &full_bar[i], kb0 + i);
+        __syncwarp();
+        griddep_wait();
       }
-      if (kPieces) griddep_wait();      // whatever became of the loads: this kernel does not end before the one before it
-      // what was asked for lands before the CTA's memory is given back, whichever warp gave up
+      for (int kb = kb0; kb < kb1; ++kb) {
+        const bool first = kb - kb0 < ahead;      // in the first round: nothing to wait for
+        if (!__all_sync(0xffffffffu, here)) ok = mx4_warp_wait(&empty_bar[s], ph, gave_up, limit.tries);
+        if (!ok) break;
+        uint8_t* st = smem + s * S::kStage;
+        uint64_t* full = &full_bar[s];
+        if (++s == ST) {
+          s = 0;
+          ph ^= 1;
+          ++rounds;
+        }
+        here = mx4_test(&empty_bar[s], ph);
+        if (one) {
+          if (!first) load_p(st, full, kb);
+          load_q(st, full, kb);
+        }
+        __syncwarp();
+      }
+    }
+    if (kPieces) griddep_wait();      // whatever became of the loads: this kernel does not end before the one before it
+    // what was asked for lands before the CTA's memory is given back, whichever warp gave up
+    if (lane == 0)
       for (int i = 0; i < ST; ++i) {
         const int round = i < s ? rounds : rounds - 1;
         if (round >= 0) mbar_drain(&full_bar[i], round & 1);
       }
-    }
+    __syncwarp();
   } else if (warp == kMma) {
     // The whole warp walks the loop and one lane issues: what the instructions are given stays in uniform registers.
     const bool one = elect_one();
@@ -403,40 +410,45 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
   if (limit.quits >= 0) ok = limit.quits != (warp == kTma ? 0 : warp == kMma ? 1 : 3);
 
   if (warp == kTma) {
-    if (lane == 0) {
-      int s = 0, rounds = 0;
-      uint32_t ph = 1;
-      for (int it = worker; it < total && ok; it += workers) {
-        int p0, q0;
-        tile_at(it, p0, q0);
-        for (int kb = 0; kb < nkb; ++kb) {
-          ok = mbar_wait_limited(&empty_bar[s], ph, gave_up, limit.tries);
-          if (!ok) break;
-          uint8_t* st = smem + s * kStage;
-          const uint32_t bar = mapa_u32(smem_u32(&full_bar[s]), 0);
-          if (rank == 0) mbar_arrive_expect_tx(&full_bar[s], 2 * kStage);
+    const bool one = elect_one();
+    int s = 0, rounds = 0;
+    uint32_t ph = 1, here = 1;      // the first round passes
+    for (int it = worker; it < total && ok; it += workers) {
+      int p0, q0;
+      tile_at(it, p0, q0);
+      for (int kb = 0; kb < nkb; ++kb) {
+        if (!__all_sync(0xffffffffu, here)) ok = mx4_warp_wait(&empty_bar[s], ph, gave_up, limit.tries);
+        if (!ok) break;
+        uint8_t* st = smem + s * kStage;
+        uint64_t* full = &full_bar[s];
+        if (++s == kStages) {
+          s = 0;
+          ph ^= 1;
+          ++rounds;
+        }
+        here = mx4_test(&empty_bar[s], ph);
+        if (one) {
+          const uint32_t bar = mapa_u32(smem_u32(full), 0);
+          if (rank == 0) mbar_arrive_expect_tx(full, 2 * kStage);
           tma_load_2d_pair(st, &tmap_p, bar, kb * 128, p0);
           tma_load_2d_pair(st + kPBytes, &tmap_q, bar, kb * 128, q0 + rank * 128);
           tma_load_3d_pair(st + kPBytes + kQBytes, &tmap_sp, bar, 0, 2 * kb, p0 >> 7);
           tma_load_3d_pair(st + kPBytes + kQBytes + 1024, &tmap_sq, bar, 0, 2 * kb, q0 >> 7);
-          if (++s == kStages) {
-            s = 0;
-            ph ^= 1;
-            ++rounds;
-          }
         }
+        __syncwarp();
       }
-      if (!ok) {
-        tell();
-        mx4_let_loads_land();
-      }
-      // what was asked for lands before the CTAs' memory is given back (their loads report to the first one)
-      if (rank == 0)
-        for (int i = 0; i < kStages; ++i) {
-          const int round = i < s ? rounds : rounds - 1;
-          if (round >= 0) mbar_drain(&full_bar[i], round & 1);
-        }
     }
+    if (!ok && lane == 0) {
+      tell();
+      mx4_let_loads_land();
+    }
+    // what was asked for lands before the CTAs' memory is given back (their loads report to the first one)
+    if (rank == 0 && lane == 0)
+      for (int i = 0; i < kStages; ++i) {
+        const int round = i < s ? rounds : rounds - 1;
+        if (round >= 0) mbar_drain(&full_bar[i], round & 1);
+      }
+    __syncwarp();
   } else if (warp == kMma) {
     if (rank == 0) {
       // The whole warp walks the loop and one lane issues: what the instructions are given stays in uniform registers.
