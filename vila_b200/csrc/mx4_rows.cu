@@ -1,4 +1,5 @@
-// Linear layers of few rows on microscaled 4-bit weights: out[m, n] = epi(sum_k x[m, k] w[n, k] + bias[n]).
+// Linear layers of up to 8 bf16 rows on up to 16 M microscaled 4-bit weights (and of any, where the caller gives no
+// workspace or K suits no tensor map): out[m, n] = epi(sum_k x[m, k] w[n, k] + bias[n]).
 //
 // Bound by the stream of weights (17 bytes per 32 of them), or for the smallest layers by latency.  mma.sync m16n8k16 in f16: 16
 // weight rows are the M side, 8 tokens the N side; tensor-core tiles of 128 tokens would stand empty here, and the sums of
