@@ -327,6 +327,55 @@ def test_row_does_not_depend_on_the_rows_around_it_within_a_kernel(cuda):
     assert torch.equal(ops.mx4_linear(x2, q)[3], got[3])
 
 
+def product_bound(x, w):
+    """|x| . |w| of a bf16 result's rounding (2^-8 of the value) and of the fp32 sums, as in check_product"""
+    z, S = x.double() @ w.double().T, x.double().abs() @ w.double().abs().T
+    return z, z.abs() * 2.0 ** -8 + S * (x.shape[1] / 16 + 8) * 2.0 ** -22 + 1e-30
+
+
+@pytest.mark.parametrize("M, N, K", [(270000, 8192, 64), (70000, 512, 32768)])
+@pytest.mark.parametrize("four", [False, True])
+def test_offsets_past_32_bits(cuda, M, N, K, four):
+    """results, and rows, of more than 2^31 elements"""
+    from vila_b200 import ops
+    x, q = torch.randn(M, K, device=cuda, dtype=BF), ops.mx4_quantize(torch.randn(N, K, device=cuda))
+    rows = torch.tensor([0, 1, M // 2, M - 129, M - 1], device=cuda)
+    if four:
+        a = ops.mx4_quantize(x)
+        got, x = ops.mx4_matmul(a, q)[rows], ops.mx4_dequantize(a)[rows]
+    else:
+        got, x = ops.mx4_linear(x, q)[rows], x[rows]
+    z, most = product_bound(x, ops.mx4_dequantize(q, out_dtype=torch.float32))
+    assert ((got.double() - z).abs() <= most).all()
+
+
+@pytest.mark.parametrize("M", [7, 8, 9, 15, 16, 17, 127, 128, 129, 255, 256, 257])
+def test_both_sides_of_every_boundary(cuda, M):
+    from vila_b200 import ops
+    for N in (1, 2, 127, 128, 129, 4096, 4097):
+        for K in (1, 31, 32, 33, 255, 256, 257, 4096):
+            x, q = torch.randn(M, K, device=cuda, dtype=BF), ops.mx4_quantize(torch.randn(N, K, device=cuda))
+            z, most = product_bound(x, ops.mx4_dequantize(q, out_dtype=torch.float32))
+            assert ((ops.mx4_linear(x, q).double() - z).abs() <= most).all(), (N, K)
+
+
+def test_four_streams_at_once(cuda):
+    from vila_b200 import ops
+    q = ops.mx4_quantize(torch.randn(9000, 1000, device=cuda))
+    xs = [torch.randn(m, 1000, device=cuda, dtype=BF) for m in (2, 12, 60, 700)]
+    want = [ops.mx4_linear(x, q) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    for _ in range(20):
+        got = []
+        for x, stream in zip(xs, streams):
+            with torch.cuda.stream(stream):
+                got.append(ops.mx4_linear(x, q))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    ops.check_waits()
+
+
 def test_no_rows(cuda):
     from vila_b200 import ops
     q, _ = weight(80, 64, 64, cuda)

@@ -45,7 +45,8 @@ MX4_WEIGHTS: Dict[str, tuple] = {
 def quantize_weights(model):
     """Hold a bf16 language model's layer weights as microscaled 4-bit rows (ops.Mx4: 17 bytes per 32 of them instead of 64), each
     rounded to the nearest number of its block; activations stay bf16.  In place; -> model.  state_dict and save_pretrained
-    still give the weights that were loaded."""
+    still give the weights that were loaded, which the model keeps where they were: on the host after from_pretrained.  A model
+    made from tensors on the GPU keeps those there, too, and then takes more of its memory, not less."""
     from .. import ops
     arch = next((a for a, c in LANGUAGE_MODELS.items() if type(model) is c), None)
     names = MX4_WEIGHTS.get(arch)
