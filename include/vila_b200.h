@@ -941,7 +941,8 @@ typedef struct vila_mx4_linear_params {
 int64_t vila_mx4_linear_scratch(const vila_mx4_linear_params* p);
 int vila_mx4_linear(const vila_mx4_linear_params* p, void* stream);
 /* vila_mx4_linear with waits of its tcgen05 kernels that end after `tries` tries (test hook: 0 gives up at once; -2 - r: those of
- * role r at once, the others as ever; 0 loads, 1 products, 2 unpacking, 3 epilogue).  vila_wait_status speaks for it. */
+ * role r at once, the others as ever; 0 loads, 1 products, 2 unpacking, 3 epilogue; r + 4, r + 8, in kernels of CTA pairs: those of the first,
+ * of the second CTA alone).  vila_wait_status speaks for it. */
 int vila_mx4_linear_tries(const vila_mx4_linear_params* p, int tries, void* stream);
 
 #ifdef __cplusplus

@@ -447,6 +447,34 @@ def test_waits_that_run_out(cuda, monkeypatch, M, N, K, four, tries):
     assert torch.equal(call(), want)
 
 
+@pytest.mark.parametrize("role", [0, 1, 2, 3])
+@pytest.mark.parametrize("rank", [0, 1])
+@pytest.mark.parametrize("M, N, K, four", [(1500, 1300, 800, True), (1500, 1300, 5000, True), (1200, 5000, 520, False), (1200, 5000, 5000, False)])
+def test_one_cta_of_a_pair_gives_up(cuda, monkeypatch, M, N, K, four, rank, role):
+    """One CTA of every pair quits while the other has copies in flight that report to it, or expects copies that the first has not
+    asked for: the launch ends, says so, and the calls after it are right."""
+    from vila_b200 import _lib, ops
+    w = ops.mx4_quantize(torch.randn(N, K, device=cuda, generator=torch.Generator(cuda).manual_seed(1)))
+    x = torch.randn(M, K, device=cuda, generator=torch.Generator(cuda).manual_seed(2)).to(BF)
+    call = (lambda: ops.mx4_matmul(ops.mx4_quantize(x), w)) if four else (lambda: ops.mx4_linear(x, w))
+    want = call()
+    torch.cuda.synchronize()
+    ops.check_waits()
+    lib = _lib.load()
+    for _ in range(3):
+        with monkeypatch.context() as m:
+            m.setattr(lib, "vila_mx4_linear", lambda p, stream: lib.vila_mx4_linear_tries(p, -2 - (role + 4 * (rank + 1)), stream))
+            out = call()
+            torch.cuda.synchronize()
+        if (four and role == 2) or (rank == 1 and role == 1):      # no such warp: unpacking, the second CTA's products
+            assert torch.equal(out, want)
+        else:
+            with pytest.raises(RuntimeError, match="ran out of tries"):
+                ops.check_waits()
+        ops.check_waits()
+        assert torch.equal(call(), want)
+
+
 def test_nothing_is_launched_behind_a_launch_that_gave_up(cuda, monkeypatch):
     from vila_b200 import _lib, ops
     w = ops.mx4_quantize(torch.randn(300, 800, device=cuda))

@@ -150,6 +150,10 @@ __device__ __forceinline__ void mbar_arrive_expect_tx(uint64_t* bar, uint32_t by
                "r"(bytes)
                : "memory");
 }
+// takes bytes off what the current phase still waits for, as if a copy had brought them
+__device__ __forceinline__ void mbar_complete_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.complete_tx.relaxed.cluster.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -186,7 +190,8 @@ __device__ __forceinline__ bool mbar_wait_limited(uint64_t* bar, uint32_t parity
   *gave_up = 1;
   return false;
 }
-// Tries of a kernel's waits: `tries` (-1: the limit), or (tests: -2 - r) the limit, and role r gives up before its first wait.
+// Tries of a kernel's waits: `tries` (-1: the limit), or (tests: -2 - r) the limit, and role r gives up before its first wait
+// (kernels of CTA pairs on microscaled rows: role r % 4, of both CTAs, or of CTA r / 4 - 1 alone).
 // A kernel parameter, read from constant memory where a warp waits: as a register of each role it cost vila_fmha's two-tile form,
 // which has none to spare, 10 % of its time.
 struct WaitLimit {

@@ -79,10 +79,20 @@ __device__ __forceinline__ uint32_t mx4_test(uint64_t* bar, uint32_t parity) {
                : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
   return ok;
 }
-// A CTA of a pair that gives up: its tokens' loads report to the first CTA's barriers, which may have given up before it asked for its part
-// of them.  They land within a few microseconds.
-__device__ __forceinline__ void mx4_let_loads_land() {
-  for (int i = 0; i < 64; ++i) __nanosleep(1000);
+// Whether a warp of role `role` in CTA `rank` of a pair is to give up before its first wait (WaitLimit).
+__device__ __forceinline__ bool mx4_pair_quits(const WaitLimit& limit, int role, int rank) {
+  return limit.quits >= 0 && (limit.quits & 3) == role && ((limit.quits >> 2) == 0 || (limit.quits >> 2) == rank + 1);
+}
+// The end of a pair of which a warp gave up.  Both CTAs' loads of a stage report to the first CTA's barrier, which it arms for both.  Stages are
+// asked for in order, stage j by barrier j % stages, and neither CTA gets more than a round ahead of what both have asked for (a stage is free
+// once both CTAs' loads of it have been consumed).  `own` stages were asked for by the first CTA, `other` by the second; no more will be, as
+// both CTAs' warps are behind a cluster barrier.  Stages that the second alone asked for are armed for its bytes; those that the first alone
+// asked for no longer wait for the second's.  Then every barrier's last phase ends with the last byte that is on its way.
+__device__ __forceinline__ void mx4_settle_pair(uint64_t* full, int stages, int own, int other, uint32_t second_bytes) {
+  for (int j = own; j < other; ++j) mbar_arrive_expect_tx(&full[j % stages], second_bytes);
+  for (int j = other; j < own; ++j) mbar_complete_tx(&full[j % stages], second_bytes);
+  const int most = own > other ? own : other;
+  for (int j = most - stages > 0 ? most - stages : 0; j < most; ++j) mbar_drain(&full[j % stages], (j / stages) & 1);
 }
 // consecutive bytes (a multiple of 16, on 16-byte boundaries)
 __device__ __forceinline__ void mx4_bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {

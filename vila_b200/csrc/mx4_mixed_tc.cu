@@ -122,6 +122,7 @@ mx4_mixed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
   uint64_t* drain_bar = acc_free + 2;
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(drain_bar + 1);
   volatile int* gave_up = reinterpret_cast<int*>(tmem_ptr + 1);
+  volatile int* asked = gave_up + 1;               // [2]: stages of tokens that this CTA asked for; in a pair's first one also: the second did
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = kPair ? static_cast<int>(cluster_ctarank()) : 0;
   const int worker = kPair ? blockIdx.x >> 1 : blockIdx.x, workers = kPair ? gridDim.x >> 1 : gridDim.x;
@@ -185,7 +186,8 @@ mx4_mixed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
   if (kPair) cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem = *tmem_ptr;
-  bool ok = limit.quits < 0 || limit.quits != (warp == kTma || warp == kCode ? 0 : warp == kMma ? 1 : warp >= kFirstUnpack ? 2 : 3);
+  const int role = warp == kTma || warp == kCode ? 0 : warp == kMma ? 1 : warp >= kFirstUnpack ? 2 : 3;
+  bool ok = kPair ? !mx4_pair_quits(limit, role, rank) : limit.quits != role;
 
   if (warp == kTma) {
     const bool one = elect_one();
@@ -219,16 +221,16 @@ mx4_mixed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
         __syncwarp();
       }
     }
-    if (!ok && lane == 0) {
-      tell();
-      if (kPair) mx4_let_loads_land();
+    if (lane == 0) {
+      if (!ok) tell();
+      // what was asked for lands before the CTA's memory is given back, whichever warp gave up (a pair's: at its end)
+      if (kPair) asked[0] = rounds * S::kTok + s;
+      else
+        for (int i = 0; i < S::kTok; ++i) {
+          const int round = i < s ? rounds : rounds - 1;
+          if (round >= 0) mbar_drain(&tok_full[i], round & 1);
+        }
     }
-    // what was asked for lands before the CTA's memory is given back, whichever warp gave up (a pair's tokens report to the first CTA)
-    if (rank == 0 && lane == 0)
-      for (int i = 0; i < S::kTok; ++i) {
-        const int round = i < s ? rounds : rounds - 1;
-        if (round >= 0) mbar_drain(&tok_full[i], round & 1);
-      }
     __syncwarp();
   } else if (warp == kCode) {
     const bool one = elect_one();
@@ -414,7 +416,22 @@ mx4_mixed_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
     tc_fence_before();
   }
   __syncthreads();
-  if (kPair) cluster_sync_all();      // the other CTA's products and loads have been waited for, too
+  if (kPair) {
+    if (tid == 0) {
+      if (rank == 1) st_dsmem_u32(mapa_u32(smem_u32(const_cast<int*>(asked + 1)), 0), asked[0]);
+      if (*gave_up) tell();      // both CTAs take the branch below, or neither does
+    }
+    __syncwarp();
+    cluster_sync_all();
+    if (*gave_up) {      // otherwise the products have consumed what was asked for, and the epilogues the products
+      if (tid == 0) {
+        if (rank == 0) mx4_settle_pair(tok_full, S::kTok, asked[0], asked[1], S::kSub * (pieces.per / 2) * 128);
+        mbar_drain(drain_bar, 0);
+      }
+      __syncthreads();
+      cluster_sync_all();
+    }
+  }
   if (warp == kMma) {
     tc_fence_after();
     if (kPair) tmem_dealloc_pair<S::kCols>(tmem);

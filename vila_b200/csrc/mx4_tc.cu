@@ -369,6 +369,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
   uint64_t* drain_bar = shared_free + 1;
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(drain_bar + 1);
   volatile int* gave_up = reinterpret_cast<int*>(tmem_ptr + 1);
+  volatile int* asked = gave_up + 1;          // [2]: stages whose loads this CTA asked for; in the first one also: the second did
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = static_cast<int>(cluster_ctarank());
   const int p_tiles = (p.M + 255) / 256, q_tiles = (p.N + kN - 1) / kN, total = p_tiles * q_tiles;
@@ -406,8 +407,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
     *gave_up = 1;
     st_dsmem_u32(mapa_u32(smem_u32(const_cast<int*>(gave_up)), rank ^ 1), 1u);
   };
-  bool ok = true;
-  if (limit.quits >= 0) ok = limit.quits != (warp == kTma ? 0 : warp == kMma ? 1 : 3);
+  bool ok = !mx4_pair_quits(limit, warp == kTma ? 0 : warp == kMma ? 1 : 3, rank);
 
   if (warp == kTma) {
     const bool one = elect_one();
@@ -438,16 +438,10 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
         __syncwarp();
       }
     }
-    if (!ok && lane == 0) {
-      tell();
-      mx4_let_loads_land();
+    if (lane == 0) {
+      if (!ok) tell();
+      asked[0] = rounds * kStages + s;
     }
-    // what was asked for lands before the CTAs' memory is given back (their loads report to the first one)
-    if (rank == 0 && lane == 0)
-      for (int i = 0; i < kStages; ++i) {
-        const int round = i < s ? rounds : rounds - 1;
-        if (round >= 0) mbar_drain(&full_bar[i], round & 1);
-      }
     __syncwarp();
   } else if (warp == kMma) {
     if (rank == 0) {
@@ -530,7 +524,20 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
     tc_fence_before();
   }
   __syncthreads();
+  if (tid == 0) {
+    if (rank == 1) st_dsmem_u32(mapa_u32(smem_u32(const_cast<int*>(asked + 1)), 0), asked[0]);
+    if (*gave_up) tell();      // both CTAs take the branch below, or neither does
+  }
+  __syncwarp();
   cluster_sync_all();
+  if (*gave_up) {      // otherwise the products have consumed what was asked for, and the epilogues the products
+    if (tid == 0) {
+      if (rank == 0) mx4_settle_pair(full_bar, kStages, asked[0], asked[1], kStage);
+      mbar_drain(drain_bar, 0);
+    }
+    __syncthreads();
+    cluster_sync_all();
+  }
   if (warp == kMma) {
     tc_fence_after();
     tmem_dealloc_pair<512>(tmem);
