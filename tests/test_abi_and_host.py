@@ -124,3 +124,47 @@ def test_dynamic_s2_preprocess_matches_reference_fixture():
         assert [int(a.sum()) for a in arrs] == item["tile_sums"].tolist(), item["size"]
         thumbs = np.stack([a[::28, ::28, :] for a in arrs]).astype(np.uint8)
         assert np.array_equal(thumbs, item["tile_thumbs"].numpy()), item["size"]
+
+
+ONCE = r"""
+#include <chrono>
+#include <cstdio>
+#include <thread>
+#include <vector>
+#include "once.h"
+int main() {
+  for (int device : {0, 63, 64, -1}) {
+    vb::OncePerDevice once;
+    std::atomic<int> calls{0}, early{0}, failed{0};
+    std::atomic<bool> set{false};
+    std::vector<std::thread> threads;
+    for (int t = 0; t < 8; ++t)
+      threads.emplace_back([&] {
+        const int rc = once.run(device, [&] {
+          std::this_thread::sleep_for(std::chrono::milliseconds(20));
+          if (calls++ == 0) return 2;      // the first setup fails
+          set = true;
+          return 0;
+        });
+        if (rc == 2) ++failed;
+        else if (!set) ++early;            // went on before it was set up
+      });
+    for (auto& t : threads) t.join();
+    std::printf("%d %d %d\n", calls.load(), early.load(), failed.load());
+  }
+}
+"""
+
+
+def test_setup_once_per_device_is_finished_before_anyone_goes_on(tmp_path):
+    import shutil
+    import subprocess
+    gxx = shutil.which("g++")
+    if gxx is None:
+        pytest.skip("no g++")
+    (tmp_path / "once.cpp").write_text(ONCE)
+    subprocess.run([gxx, "-std=c++17", "-O2", "-pthread", f"-I{ROOT / 'vila_b200' / 'csrc'}", str(tmp_path / "once.cpp"), "-o", str(tmp_path / "once")],
+                   check=True)
+    lines = subprocess.run([str(tmp_path / "once")], check=True, capture_output=True, text=True).stdout.split("\n")
+    assert lines[:2] == ["2 0 1"] * 2          # one failure, one success, six that waited for it
+    assert lines[2:4] == ["8 0 1"] * 2         # devices that are not counted set up every time

@@ -376,6 +376,53 @@ def test_four_streams_at_once(cuda):
     ops.check_waits()
 
 
+FIRST_CALLS = """
+import threading, torch
+from vila_b200 import ops
+torch.manual_seed(0)
+cases = [(1, 2000, 2000, False), (8, 9000, 4000, False), (16, 3584, 4096, False), (60, 12000, 520, False), (90, 12000, 520, False), (1200, 5000, 520, False),
+         (16, 300, 8192, True), (100, 300, 5000, True), (300, 514, 800, True), (1500, 1300, 800, True)]
+data = [(torch.randn(M, K, device="cuda").bfloat16(), ops.mx4_quantize(torch.randn(N, K, device="cuda")), four) for M, N, K, four in cases]
+torch.cuda.synchronize()
+def call(x, w, four):
+    return ops.mx4_matmul(ops.mx4_quantize(x), w) if four else ops.mx4_linear(x, w)
+got, errors, threads = [[None] * len(data) for _ in range(8)], [], []
+start = threading.Barrier(8)
+def work(t):
+    try:
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for i in range(len(data)):
+                start.wait()
+                got[t][i] = call(*data[i])
+            torch.cuda.current_stream().synchronize()
+    except Exception as e:
+        errors.append(repr(e))
+        start.abort()
+for t in range(8):
+    threads.append(threading.Thread(target=work, args=(t,)))
+    threads[-1].start()
+for t in threads:
+    t.join()
+assert not errors, errors
+torch.cuda.synchronize()
+for i, d in enumerate(data):
+    want = call(*d)
+    assert all(torch.equal(g[i], want) for g in got), i
+ops.check_waits()
+print("agree")
+"""
+
+
+def test_first_calls_from_several_host_threads(cuda):
+    """every kernel's first launch of a process comes from eight threads at once: none is refused, and all cut K alike"""
+    import subprocess
+    import sys
+    from pathlib import Path
+    root = Path(__file__).resolve().parent.parent
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "agree" in r.stdout, r.stdout + r.stderr
+
+
 def test_no_rows(cuda):
     from vila_b200 import ops
     q, _ = weight(80, 64, 64, cuda)

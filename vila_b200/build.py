@@ -51,7 +51,7 @@ SOURCES = [
     "mx4_tc.cu",
     "mx4_mixed_tc.cu",
 ]
-HEADERS = ["common.cuh", "kernels.h", "dtype_any.cuh", "glinear_epi.cuh", "paged_attn_common.cuh", "mma_bf16.cuh", "mx4.cuh", "mx4_epi.cuh", "../../include/vila_b200.h"]
+HEADERS = ["common.cuh", "once.h", "kernels.h", "dtype_any.cuh", "glinear_epi.cuh", "paged_attn_common.cuh", "mma_bf16.cuh", "mx4.cuh", "mx4_epi.cuh", "../../include/vila_b200.h"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

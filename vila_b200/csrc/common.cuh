@@ -8,6 +8,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "once.h"
+
 namespace vb {
 
 // ----------------------------------------------------------------------------------------------
@@ -590,17 +592,27 @@ inline cudaError_t launch_serial_cluster(void (*kern)(KArgs...), dim3 grid, dim3
 }
 const char* last_error();
 
-// One-time per-DEVICE setup guard (cudaFuncSetAttribute is per device; a process may drive several).
+// One-time setup per device (cudaFuncSetAttribute is per device; a process may drive several): see once.h.
 struct PerDeviceOnce {
-  bool done[64] = {};
-  bool first() {
+  OncePerDevice once;
+  template <typename F>
+  int run(F&& f) {
     int d = 0;
     cudaGetDevice(&d);
-    if (d < 0 || d >= 64) d = 0;
-    if (done[d]) return false;
-    done[d] = true;
-    return true;
+    return once.run(d, f);
   }
 };
+// Dynamic shared memory that launches of `kern` may take, set before the first of them on a device, whichever host thread it comes from.
+template <typename K>
+int allow_smem(PerDeviceOnce& once, K* kern, size_t bytes) {
+  return once.run([&] {
+    VB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
+    return 0;
+  });
+}
+#define VB_ALLOW_SMEM(once, ...)                                         \
+  do {                                                                   \
+    if (int _rc = ::vb::allow_smem(once, __VA_ARGS__)) return _rc;       \
+  } while (0)
 
 }  // namespace vb

@@ -736,9 +736,7 @@ int gemv_bf16(const GemvParams& p, cudaStream_t stream) {
            rows_per_block);
   auto kern = gemv_kernel<8>;
   static PerDeviceOnce attr_once;
-  if (attr_once.first()) {
-    VB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
-  }
+  VB_ALLOW_SMEM(attr_once, kern, 200 * 1024);
   VB_CUDA(launch_pdl(kern, dim3(grid), dim3(kGemvThreads), smem, stream, p, rows_per_block, ksplit));
   return 0;
 }
@@ -772,9 +770,7 @@ int decode_attention(const DecodeAttnParams& p, cudaStream_t stream) {
     auto kern = use_cluster ? decode_attn_kernel<128, GG, true> : decode_attn_kernel<128, GG, false>; \
     const size_t smem = (size_t)kDaWarps * 2 * GG * (128 + 2) * sizeof(float);                  \
     static PerDeviceOnce attr_once[2];                                                          \
-    if (attr_once[use_cluster].first()) {                                                       \
-      VB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)); \
-    }                                                                                           \
+    VB_ALLOW_SMEM(attr_once[use_cluster], kern, (int)smem); \
     VB_CUDA(launch_pdl_cluster(kern, grid, dim3(kDaThreads), smem, stream,                      \
                                dim3(1, use_cluster ? p.num_splits : 1, 1), p));                 \
     break;                                                                                      \

@@ -605,9 +605,7 @@ int decode_mega(const MegaParams& pin, cudaStream_t stream) {
   case GG: {                                                                                     \
     auto kern = decode_mega_kernel<GG>;                                                          \
     static PerDeviceOnce attr_once;                                                              \
-    if (attr_once.first()) {                                                                     \
-      VB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 225 * 1024)); \
-    }                                                                                            \
+    VB_ALLOW_SMEM(attr_once, kern, 225 * 1024); \
     int occ = 0;                                                                                 \
     VB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kern, MT, smem));                \
     VB_CHECK(occ >= 1, "decode_mega: kernel does not fit on an SM");                             \

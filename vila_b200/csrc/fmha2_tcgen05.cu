@@ -605,9 +605,7 @@ int launch(const FmhaParams& p, cudaStream_t stream, int tries) {
   a.scale_log2 = p.scale * 1.4426950408889634f;
   auto kern = fmha_pipe_kernel<DP, CW, TILES, ADD>;
   static PerDeviceOnce attr_once;
-  if (attr_once.first()) {
-    VB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
-  }
+  VB_ALLOW_SMEM(attr_once, kern, C::kSmem);
   const long total = static_cast<long>(a.units) * p.Hq * p.B;
   VB_CHECK(total < (1L << 30), "fmha: too many query tiles");
   const int grid = static_cast<int>(total < num_sms() ? total : num_sms());

@@ -420,9 +420,7 @@ int launch_fmha(const FmhaParams& p, cudaStream_t stream, const SplitArgs& split
   a.split_counters = split.counters;
   auto kern = fmha_fwd_kernel<DP, CW>;
   static PerDeviceOnce attr_once;
-  if (attr_once.first()) {
-    VB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
-  }
+  VB_ALLOW_SMEM(attr_once, kern, C::kSmem);
   dim3 grid(1, p.Hq, p.B);
   VB_CUDA(launch_pdl(kern, grid, dim3(kThreads), C::kSmem, stream, tq, tk, tv, a));
   return 0;

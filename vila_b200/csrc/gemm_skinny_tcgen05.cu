@@ -727,9 +727,7 @@ int launch_skinny(const __nv_bfloat16* A, int lda, const __nv_bfloat16* W, int l
   const size_t smem = static_cast<size_t>(stages) * stage_bytes + kStgBytes + kBarBytes + 1024;
   auto kern = gemm_skinny_kernel<kPair>;
   static PerDeviceOnce attr_once;
-  if (attr_once.first()) {
-    VB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
-  }
+  VB_ALLOW_SMEM(attr_once, kern, 227 * 1024);
   // cluster split-K (single-CTA flavour): largest split count whose clusters are all co-resident
   int cluster_k = 0;
   if (!kPair && want_splits > 1) {

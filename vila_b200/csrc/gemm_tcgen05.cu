@@ -631,9 +631,7 @@ int launch_gemm(const __nv_bfloat16* A, int lda, const __nv_bfloat16* W, int ldw
   if (make_tmap_2d_bf16(&tw, W, N, K, ldw, S::kBRows, BLOCK_K, 128)) return 1;
   auto kern = gemm_bf16_tcgen05_kernel<BLOCK_N, kStages, kMode>;
   static PerDeviceOnce attr_once;
-  if (attr_once.first()) {
-    VB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kTotal));
-  }
+  VB_ALLOW_SMEM(attr_once, kern, S::kTotal);
   const int sms = num_sms();
   const int tiles = ((M + TILE_M - 1) / TILE_M) * ((N + BLOCK_N - 1) / BLOCK_N);
   if (kMode == kModeSplitK2) {

@@ -369,7 +369,7 @@ int launch_stream(const vila_glinear_params& p, const vila_glinear_ext& x, cudaS
   const long rows = static_cast<long>(p.M) * ((2 * p.K + 127) / 128 * 128 + 64);
   const int tokens = static_cast<int>(rows < kTokens ? rows : kTokens);
   static PerDeviceOnce once;
-  if (once.first()) VB_CUDA(cudaFuncSetAttribute(glinear_stream_kernel<KW, NT, SLOTS, ROUTED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStreamSmem));
+  VB_ALLOW_SMEM(once, glinear_stream_kernel<KW, NT, SLOTS, ROUTED>, kStreamSmem);
   VB_CUDA(launch_serial(glinear_stream_kernel<KW, NT, SLOTS, ROUTED>, dim3(static_cast<unsigned>(ctas < num_sms() ? ctas : num_sms())), dim3(32 * kStay),
                         kStay * SLOTS * 1024 + tokens, stream, p, x, tokens));
   return 0;

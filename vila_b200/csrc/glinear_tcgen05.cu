@@ -432,8 +432,7 @@ template <int BT, int EPI>
 int launch_epi(const CUtensorMap& tm, const CUtensorMap& ta, const vila_glinear_params& p, const vila_glinear_ext& x, int tries, cudaStream_t stream) {
   using S = Shape<BT>;
   static PerDeviceOnce once;
-  if (once.first())
-    VB_CUDA(cudaFuncSetAttribute(glinear_tc_kernel<BT, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::smem(kMaxGroups))));
+  VB_ALLOW_SMEM(once, glinear_tc_kernel<BT, EPI>, static_cast<int>(S::smem(kMaxGroups)));
   const long long tok = (p.M + BT - 1) / BT + (p.mode == 1 ? p.groups : 0);   // mode 1: upper bound of sum_g ceil(rows_g / BT)
   const long long tiles = tok * ((p.N + kRowsW - 1) / kRowsW) * (p.mode == 0 ? p.groups : 1);
   VB_CHECK(tiles < (1LL << 31), "glinear: too many tiles (M=%d N=%d groups=%d)", p.M, p.N, p.groups);

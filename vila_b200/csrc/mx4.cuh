@@ -102,15 +102,16 @@ __device__ __forceinline__ void mx4_bulk_load(void* dst, const void* src, uint32
 }
 
 // How many clusters of a kernel the GPU holds at once, by cluster size (1, 2, 4, 8), asked for once a device: a cluster lies within a
-// group of SMs, so that 28 clusters of 5 are more than the 148 SMs take at a time, and one too many takes as long again.
+// group of SMs, so that 28 clusters of 5 are more than the 148 SMs take at a time, and one too many takes as long again.  Host threads may ask
+// at the same time; a question that fails is asked again by the next call.
 struct Mx4Clusters {
-  int most[64][4] = {};
+  std::atomic<int> most[64][4] = {};      // 0: not asked yet, -1: none
   template <typename K>
   int of(K* kernel, int log2, int threads, size_t smem) {
     int d = 0;
     cudaGetDevice(&d);
     if (d < 0 || d >= 64) d = 0;
-    int& n = most[d][log2];
+    int n = most[d][log2].load(std::memory_order_relaxed);
     if (n == 0) {
       cudaLaunchConfig_t cfg = {};
       cfg.gridDim = dim3(1u << log2);
@@ -124,9 +125,10 @@ struct Mx4Clusters {
       cfg.numAttrs = 1;
       if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
         (void)cudaGetLastError();
-        n = 0;
+        return -1;
       }
       if (n <= 0) n = -1;
+      most[d][log2].store(n, std::memory_order_relaxed);
     }
     return n;
   }

@@ -448,8 +448,7 @@ int launch(const vila_mx4_linear_params& p, const vila_glinear_ext& x, const Pie
   using S = Shape<BT, kPair>;
   constexpr int kCtas = kPair ? 2 : 1;
   static PerDeviceOnce once;
-  if (once.first())
-    VB_CUDA(cudaFuncSetAttribute(mx4_mixed_kernel<BT, kPair>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmem)));
+  VB_ALLOW_SMEM(once, mx4_mixed_kernel<BT, kPair>, static_cast<int>(kSmem));
   CUtensorMap tw, tx;
   if (int rc = make_tmap_2d_u8(&tw, p.w_codes, p.N, mx4_pitch(p.K), mx4_pitch(p.K), kRowsW, 128, 128)) return rc;
   if (int rc = make_tmap_2d_bf16(&tx, p.x, p.M, p.K, p.ldx, pieces.per / kCtas, kDepth, 128)) return rc;

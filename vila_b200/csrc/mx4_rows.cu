@@ -260,8 +260,7 @@ mx4_rows_kernel(const vila_mx4_linear_params p, const vila_glinear_ext ext, int 
 template <int TM>
 int launch(const vila_mx4_linear_params& p, const vila_glinear_ext& ext, cudaStream_t stream) {
   static PerDeviceOnce once;
-  if (once.first())
-    VB_CUDA(cudaFuncSetAttribute(mx4_rows_kernel<TM>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<TM>::kTotal));
+  VB_ALLOW_SMEM(once, mx4_rows_kernel<TM>, Smem<TM>::kTotal);
   const int tiles = (p.N + kRows - 1) / kRows, groups = (p.M + TM - 1) / TM, nk = (p.K + 127) / 128;
   static Mx4Clusters clusters;
   const int split = clusters.split(mx4_rows_kernel<TM>, kThreads, Smem<TM>::kTotal, static_cast<long long>(tiles) * groups, nk / 2);

@@ -550,7 +550,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
 
 int launch(const vila_mx4_linear_params& p, const vila_glinear_ext& x, int tries, cudaStream_t stream) {
   static PerDeviceOnce once;
-  if (once.first()) VB_CUDA(cudaFuncSetAttribute(mx4_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmem)));
+  VB_ALLOW_SMEM(once, mx4_pair_kernel, static_cast<int>(kSmem));
   const int pitch = mx4_pitch(p.K), kts = mx4_ktiles(p.K);
   CUtensorMap tp, tq, sp, sq;
   if (int rc = make_tmap_2d_u8(&tp, p.a_codes, p.M, pitch, pitch, 128, 128, 128)) return rc;
@@ -624,8 +624,7 @@ template <int BN, bool kSwap, bool kPieces>
 int launch(const vila_mx4_linear_params& p, const vila_glinear_ext& x, int tries, cudaStream_t stream) {
   using S = Shape<BN>;
   static PerDeviceOnce once;
-  if (once.first())
-    VB_CUDA(cudaFuncSetAttribute(mx4_tc_kernel<BN, kSwap, kPieces>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::kSmem)));
+  VB_ALLOW_SMEM(once, mx4_tc_kernel<BN, kSwap, kPieces>, static_cast<int>(S::kSmem));
   const int pitch = mx4_pitch(p.K), tokens = kPieces ? kPieceRows * p.M : p.M;
   const uint8_t *pc = kSwap ? p.w_codes : p.a_codes, *qc = kSwap ? p.a_codes : p.w_codes;
   const int P = kSwap ? p.N : tokens, Q = kSwap ? tokens : p.N;

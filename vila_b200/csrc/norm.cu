@@ -272,10 +272,7 @@ int layernorm_bf16(const __nv_bfloat16* x, const __nv_bfloat16* w, const __nv_bf
   }
   const size_t smem = static_cast<size_t>(cols) * 2;
   static PerDeviceOnce attr_once;
-  if (attr_once.first()) {
-    VB_CUDA(cudaFuncSetAttribute(layernorm_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 96 * 1024));
-  }
+  VB_ALLOW_SMEM(attr_once, layernorm_kernel, 96 * 1024);
   VB_CUDA(launch_pdl(layernorm_kernel, dim3(rows), dim3(kNormThreads), smem, stream, x, w, b, out, cols, eps));
   return 0;
 }
@@ -296,10 +293,7 @@ int rmsnorm_bf16(__nv_bfloat16* x_inout, const __nv_bfloat16* residual_add,
   }
   const size_t smem = static_cast<size_t>(cols) * 2;
   static PerDeviceOnce attr_once;
-  if (attr_once.first()) {
-    VB_CUDA(cudaFuncSetAttribute(rmsnorm_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 96 * 1024));
-  }
+  VB_ALLOW_SMEM(attr_once, rmsnorm_kernel, 96 * 1024);
   VB_CUDA(launch_pdl(rmsnorm_kernel, dim3(rows), dim3(kNormThreads), smem, stream, x_inout, residual_add, w,
                      out, cols, eps));
   return 0;

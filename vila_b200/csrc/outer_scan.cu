@@ -639,8 +639,7 @@ int launch_scan(const ScanArgs& p, int nseq, cudaStream_t stream) {
   constexpr int SW = CPT == 4 ? 4 : 8;
   auto kern = outer_scan_kernel<MODE, R, KPT, CPT, SW>;
   static PerDeviceOnce attr_once;
-  if (smem > 48 * 1024 && attr_once.first())
-    VB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+  if (smem > 48 * 1024) VB_ALLOW_SMEM(attr_once, kern, static_cast<int>(smem));
   const dim3 grid(nseq, p.H, (p.vdim + COLS - 1) / COLS);
   VB_CHECK(grid.y <= 65535 && grid.z <= 65535, "outer_scan: H=%d vdim=%d", p.H, p.vdim);
   // below: beside the launch that has the longer sequences (other rows and slots; that one started after all before it)

@@ -435,7 +435,7 @@ template <int D, int HW, bool AFTER>
 int launch(const vila_paged_attn_params& p, cudaStream_t stream) {
   auto kernel = paged_attn_mix_kernel<D, HW, AFTER>;
   static PerDeviceOnce once;
-  if (once.first()) VB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_bytes<D>(16 * HW))));
+  VB_ALLOW_SMEM(once, kernel, static_cast<int>(smem_bytes<D>(16 * HW)));
   const long ctas = static_cast<long>(p.ntiles) * ((p.max_rows + kRows - 1) / kRows);
   VB_CHECK(ctas < (1L << 31), "paged_attention: too many tiles");
   VB_CUDA(launch_serial(kernel, dim3(static_cast<unsigned>(ctas)), dim3(32 * ((p.H + HW - 1) / HW)), smem_bytes<D>(p.H), stream, p));

@@ -433,7 +433,7 @@ int launch_kernel(const vila_paged_attn_params& p, int warps, int tpc, cudaStrea
   auto kernel = paged_attn_mma_kernel<D, MAPS, V, SETS, CAP>;
   const int smem = warps * 3 * (D / 16) * 512 + SETS * 2 * kBK * (MAPS * D + V) * 2;
   static PerDeviceOnce once;
-  if (once.first()) VB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024));
+  VB_ALLOW_SMEM(once, kernel, 224 * 1024);
   const long ctas = static_cast<long>((p.ntiles + tpc - 1) / tpc) * p.G;
   VB_CHECK(ctas < (1L << 31), "paged_attention: too many tiles");
   VB_CUDA(launch_serial(kernel, dim3(static_cast<unsigned>(ctas)), dim3(32 * warps * SETS), smem, stream, p, tpc));

@@ -542,7 +542,7 @@ int launch(const vila_paged_attn_params& p, cudaStream_t stream, int tries) {
   VB_CHECK(failed != nullptr, "paged_attention: no pinned host memory for the status word");
   auto kernel = paged_attn_tc_kernel<CAP>;
   static PerDeviceOnce once;
-  if (once.first()) VB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem + kBiasBytes));
+  VB_ALLOW_SMEM(once, kernel, kSmem + kBiasBytes);
   // Tiles of a CTA: as few as leave no CTA without an SM, otherwise as many as its 128 rows hold.  A CTA of one tile takes as long
   // as one of several tiles of a sequence, and tiles of other sequences wait for each other there: 8 sequences of 16 rows on 100 keys,
   // capped, 16 heads over 4 / over 16 / 32 over 32 19.8 / 48 / 49 us as full as they get and 11.2 / 11.6 / 16.9 so (mma.sync 12.1 / 29 /

@@ -1201,7 +1201,7 @@ int moe_route_scores(const vila_moe_route_params& p, cudaStream_t stream) {
   else if (vec && p.x_dtype == VILA_DT_BF16 && p.ldx % 8 == 0 && aligned_to(p.x, 16) && !p.gate_w && kRouteStages * kRouteStage + kRouteTok * per_tok <= 200 * 1024 && tiles_ahead()) {
     const size_t smem = kRouteStages * kRouteStage + kRouteTok * per_tok;
     static PerDeviceOnce once;
-    if (once.first()) VB_CUDA(cudaFuncSetAttribute(moe_route_tiles_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+    VB_ALLOW_SMEM(once, moe_route_tiles_kernel, 200 * 1024);
     VB_CUDA(launch_serial(moe_route_tiles_kernel, dim3((p.rows + kRouteTok - 1) / kRouteTok), dim3(256), smem, stream, p));
   } else VB_ROUTE(4, 4, 256);
 #undef VB_ROUTE_K

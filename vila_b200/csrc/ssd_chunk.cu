@@ -561,7 +561,7 @@ template <int N, int PT>
 int launch(const vila_ssd_scan_params& p, int nseq, int min_rows, cudaStream_t stream) {
   auto kernel = ssd_chunk_kernel<N, PT>;
   static PerDeviceOnce once;
-  if (once.first()) VB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<N, PT>::kSmem));
+  VB_ALLOW_SMEM(once, kernel, Shape<N, PT>::kSmem);
   VB_CUDA(launch_serial(kernel, dim3(nseq, p.H, p.P / (16 * PT)), dim3(kThreads), Shape<N, PT>::kSmem, stream, p, min_rows));
   return 0;
 }
