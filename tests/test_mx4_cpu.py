@@ -86,6 +86,41 @@ def test_parameter_struct_follows_the_header():
     assert fields == [f[0] for f in _lib.Mx4LinearParams._fields_]
 
 
+def test_captured_steps_are_dropped_with_the_weights_that_they_read():
+    from vila_b200.serving import TokenEngine
+
+    class Model:
+        device, dtype = "cpu", torch.float32
+        latent_widths = state_shapes = staticmethod(dict)
+        eager = 0
+
+        def forward_step(self, batch, cache, layer_outputs=None):
+            self.eager += 1
+            return torch.zeros(batch.T, 4)
+
+        def logits(self, x):
+            return x
+
+    class Graph:
+        replays = 0
+
+        def replay(self):
+            self.replays += 1
+
+    model, graph = Model(), Graph()
+    engine = TokenEngine(model, 64, 1)
+    engine._decode_seen[1] = 1
+    engine._decode_graphs[1] = (graph, torch.zeros(0, dtype=torch.int32), torch.zeros(1, 4), torch.zeros(1, 4))
+    engine._decode_step_graphed = lambda flat, sizes: (graph.replay(), torch.zeros(1, 4))
+    engine.step([("a", [1], [0])])
+    assert (graph.replays, model.eager) == (1, 0)
+    model.weights_version = 1
+    engine.step([("a", [2], [0])])
+    assert (graph.replays, model.eager) == (1, 1) and not engine._decode_graphs
+    engine.step([("a", [3], [0])])      # seen once: captured, then replayed again
+    assert (graph.replays, model.eager) == (2, 1)
+
+
 def test_weights_in_4_bits_are_refused_before_anything_is_loaded(tmp_path):
     import json
     from vila_b200.model.registry import load_language_model, quantize_weights

@@ -594,6 +594,37 @@ def test_language_models_on_4_bit_weights(cuda, arch):
     assert len(small.generate(toks[:9], max_new_tokens=5)[0]) == 5
 
 
+@pytest.mark.parametrize("arch", ["nusovik", "ludazen", "bivizen", "nibelix", "lufatar"])
+def test_weights_replaced_under_an_engine_that_has_captured_its_steps(cuda, arch):
+    """quantize_weights, then load_weights, between decoded tokens: an engine with graphs goes on as one without."""
+    import importlib
+    from vila_b200.model.registry import quantize_weights
+    from vila_b200.serving import TokenEngine
+    T = importlib.import_module(f"tests.test_{arch}_gpu")
+    name = "aligned" if "aligned" in T.CONFIGS else next(iter(T.CONFIGS))
+    cfg, model = T.build(name, BF, seed=3)
+    loaded = dict(model.state_dict())
+    engines = [TokenEngine(model, 256, 2), TokenEngine(model, 256, 2, graphs=False)]
+    toks = T.tokens_for(cfg, 60, 5)
+    both = [[] for _ in engines]
+
+    def decode(first, n):
+        for e, got in zip(engines, both):
+            for t in toks[first:first + n]:
+                got.append(e.step([("a", [t], [0])]))
+
+    for e in engines:
+        e.step([("a", toks[:20], [19])])
+    decode(20, 4)
+    assert engines[0]._decode_graphs
+    quantize_weights(model)
+    decode(24, 4)
+    assert engines[0]._decode_graphs
+    model.load_weights(loaded)
+    decode(28, 4)
+    assert all(torch.equal(a, b) for a, b in zip(*both))
+
+
 def test_load_and_command_line(cuda, tmp_path, capsys):
     from llava.cli import infer
     from tests import test_nusovik_gpu as T

@@ -318,6 +318,7 @@ class LudazenForCausalLM:
         self.weights = {n: tensors[n] for n in want}
         self.embed, self.head, self.final_norm = w("embed"), w("head"), f32("final.norm")
         self.layers = []
+        self.weights_version = getattr(self, "weights_version", 0) + 1   # engines' captured steps read the former ones
         for i, lc in enumerate(cfg.layers):
             p, L = f"l{i}.", _Layer()
             L.cfg, L.index = lc, i

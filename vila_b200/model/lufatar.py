@@ -255,6 +255,7 @@ class LufatarForCausalLM:
         self.loop_step = f32("loop.step") if cfg.loops else None
         self.side_embed = w("side.embed") if cfg.side_dim else None
         self.layers = []
+        self.weights_version = getattr(self, "weights_version", 0) + 1   # engines' captured steps read the former ones
         for i, lc in enumerate(cfg.layers):
             p, L = f"l{i}.", _Layer()
             L.cfg, L.index = lc, i

@@ -316,6 +316,7 @@ class NusovikForCausalLM:
         self.inv_freq = (torch.tensor(POSITION_BASE, dtype=torch.float64) **
                          (-2.0 * torch.arange(half, dtype=torch.float64) / cfg.width)).to(dev)
         self.layers = []
+        self.weights_version = getattr(self, "weights_version", 0) + 1   # engines' captured steps read the former ones
         for i, lc in enumerate(cfg.layers):
             p, L = f"l{i}.", _Layer()
             L.cfg, L.index = lc, i

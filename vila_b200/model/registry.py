@@ -46,7 +46,9 @@ def quantize_weights(model):
     """Hold a bf16 language model's layer weights as microscaled 4-bit rows (ops.Mx4: 17 bytes per 32 of them instead of 64), each
     rounded to the nearest number of its block; activations stay bf16.  In place; -> model.  state_dict and save_pretrained
     still give the weights that were loaded, which the model keeps where they were: on the host after from_pretrained.  A model
-    made from tensors on the GPU keeps those there, too, and then takes more of its memory, not less."""
+    made from tensors on the GPU keeps those there, too, and then takes more of its memory, not less.  A TokenEngine that runs the
+    model captures its decode steps anew at its next step; what it cached for its sequences stays as the former weights made it.
+    Not while another thread runs a step of the model."""
     from .. import ops
     arch = next((a for a, c in LANGUAGE_MODELS.items() if type(model) is c), None)
     names = MX4_WEIGHTS.get(arch)
@@ -54,6 +56,9 @@ def quantize_weights(model):
         raise ValueError(f"{type(model).__name__} does not hold weights in 4 bits (those that do: {sorted(MX4_WEIGHTS)})")
     if model.dtype != torch.bfloat16:
         raise ValueError(f"4-bit weights go with bfloat16 activations, not {model.dtype}")
+    if torch.device(model.device).type == "cuda":
+        torch.cuda.synchronize(model.device)      # no step that reads the replaced weights is under way, on whichever stream
+    model.weights_version = getattr(model, "weights_version", 0) + 1
     for layer in model.layers:
         for name in names:
             w = getattr(layer, name, None)

@@ -329,6 +329,7 @@ class TokenEngine:
         self.graphs = graphs
         self._decode_graphs: Dict[int, tuple] = {}
         self._decode_seen: Dict[int, int] = {}
+        self._weights = self._weights_version()        # that the graphs were captured on
         self._unread = deque()
         self._steps = 0
 
@@ -445,6 +446,18 @@ class TokenEngine:
                            v[4].view(-1, 4) if sizes[4] else None, v[5] if sizes[5] else None,
                            v[6].view(-1, 4) if sizes[6] else None, v[7], v[8], v[9])
 
+    def _weights_version(self) -> int:
+        """how often the model's layers were given other tensors (load_weights, quantize_weights)"""
+        return getattr(self.model, "weights_version", 0)
+
+    def _drop_graphs(self) -> None:
+        """The model's layers hold other tensors than when the graphs were captured: these read memory that may be someone else's."""
+        if torch.device(self.model.device).type == "cuda":
+            torch.cuda.synchronize(self.model.device)   # none of them runs any more
+        self._decode_graphs.clear()
+        self._decode_seen.clear()
+        self._weights = self._weights_version()
+
     def _decode_step_graphed(self, flat, sizes) -> Tuple[torch.Tensor, torch.Tensor]:
         """All rows are single decoded tokens: replay (or capture) the graph of this row count.
         -> (residual rows, logits of ALL rows); both are static graph outputs."""
@@ -486,6 +499,8 @@ class TokenEngine:
         return logits
 
     def _step(self, entries, layer_outputs: Optional[list]) -> Optional[torch.Tensor]:
+        if self._weights != self._weights_version():
+            self._drop_graphs()
         flat, sizes = self._build(entries)
         T, n_want = sizes[0], sizes.pop()
         arrays = flat[:flat.numel() - n_want]
