@@ -73,6 +73,12 @@ def test_entry_points_fail_without_a_device():
     assert lib.vila_mx4_linear(C.byref(_lib.Mx4LinearParams()), None) != 0
 
 
+def test_no_parameters_want_no_workspace():
+    lib = _lib.load()
+    assert lib.vila_mx4_linear_scratch(None) == 0
+    assert lib.vila_mx4_linear(None, None) != 0 and lib.vila_mx4_linear_tries(None, 5, None) != 0
+
+
 def test_parameter_struct_follows_the_header():
     import re
     from pathlib import Path

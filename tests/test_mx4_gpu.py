@@ -458,6 +458,31 @@ def test_refusals(cuda):
         ops.mx4_linear(x, gated, swiglu=True, act=ops.ACT_SILU)
 
 
+def test_pointers_that_are_refused_on_the_host(cuda):
+    """null pointers, and pointers off their elements' boundaries, reach no kernel"""
+    import ctypes as C
+    from vila_b200 import _lib, ops
+    lib = _lib.load()
+    q, _ = weight(92, 4, 64, cuda)
+    x = torch.zeros(4, 64, device=cuda)
+    codes, scales, at = q.codes.data_ptr(), q.scales.data_ptr(), x.data_ptr()
+    BF16, F32 = ops._dt(x.to(BF), "x"), ops._dt(x, "x")
+    for refused in (lib.vila_mx4_quantize(None, F32, 64, codes, scales, 4, 64, None), lib.vila_mx4_quantize(at + 2, F32, 64, codes, scales, 3, 64, None),
+                    lib.vila_mx4_quantize(at + 1, BF16, 64, codes, scales, 3, 64, None), lib.vila_mx4_quantize(at, F32, 64, None, scales, 4, 64, None),
+                    lib.vila_mx4_dequantize(codes, scales, None, F32, 64, 4, 64, None), lib.vila_mx4_dequantize(codes, scales, at + 2, F32, 64, 3, 64, None),
+                    lib.vila_mx4_dequantize(codes, scales, at, F32, 63, 4, 64, None), lib.vila_mx4_dequantize(codes, None, at, F32, 64, 4, 64, None),
+                    lib.vila_mx4_scales(None, scales, 4, 64, 0, None), lib.vila_mx4_scales(at, None, 4, 64, 0, None)):
+        assert refused == 1
+    good = dict(x=at, ldx=64, w_codes=codes, w_scales=scales, out=at, ldo=4, M=4, N=4, K=64)
+    for bad in (dict(x=None), dict(x=at + 1), dict(out=None), dict(out=at + 1), dict(bias=at + 1), dict(w_codes=None), dict(w_scales=None),
+                dict(x=None, a_codes=codes), dict(w_codes=codes + 8), dict(ldo=3)):
+        assert lib.vila_mx4_linear(C.byref(_lib.Mx4LinearParams(**{**good, **bad})), None) == 1, bad
+    assert lib.vila_mx4_linear(None, None) == 1 and lib.vila_mx4_linear_tries(None, 5, None) == 1
+    assert lib.vila_mx4_quantize(None, F32, 64, None, None, 0, 64, None) == 0      # no rows, nothing to point at
+    torch.cuda.synchronize()
+    assert not x.any()
+
+
 # ---- waits that run out ----------------------------------------------------------------------------------
 # rows, weight rows, columns, 4-bit rows: one for every tcgen05 kernel and tile
 KERNELS = [(16, 300, 800, True), (40, 300, 800, True), (100, 300, 5000, True), (300, 514, 800, True), (1500, 1300, 800, True),

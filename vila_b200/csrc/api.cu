@@ -640,15 +640,17 @@ int vila_mx4_scales(uint8_t* plain, uint8_t* tiled, int rows, int cols, int to_t
   return vb::mx4_scales(plain, tiled, rows, cols, to_tiled, st(stream));
 }
 
-int64_t vila_mx4_linear_scratch(const vila_mx4_linear_params* p) { return static_cast<int64_t>(vb::mx4_linear_scratch(*p)); }
+int64_t vila_mx4_linear_scratch(const vila_mx4_linear_params* p) { return p == nullptr ? 0 : static_cast<int64_t>(vb::mx4_linear_scratch(*p)); }
 
 int vila_mx4_linear_tries(const vila_mx4_linear_params* p, int tries, void* stream) {
   VB_REQUIRE_DEVICE();
+  VB_CHECK(p != nullptr, "mx4_linear: no parameters");
   return vb::mx4_linear(*p, st(stream), tries == -1 ? 0 : tries);
 }
 
 int vila_mx4_linear(const vila_mx4_linear_params* p, void* stream) {
   VB_REQUIRE_DEVICE();
+  VB_CHECK(p != nullptr, "mx4_linear: no parameters");
   return vb::mx4_linear(*p, st(stream));
 }
 

@@ -239,21 +239,23 @@ int by_rows(int rows, int cols, F&& f) {
   }
   return 0;
 }
-int check_rows(const char* what, int rows, int cols, const uint8_t* codes, const uint8_t* scales) {
+// x: the rows as numbers (or plain scale bytes), of `size` bytes each
+int check_rows(const char* what, int rows, int cols, const uint8_t* codes, const uint8_t* scales, const void* x, int size) {
   VB_CHECK(rows >= 0 && cols > 0 && rows <= (1 << 30) && cols <= (1 << 25), "%s: rows=%d cols=%d", what, rows, cols);
   VB_CHECK(rows == 0 || (codes != nullptr && scales != nullptr && reinterpret_cast<uintptr_t>(codes) % 16 == 0 &&
                          reinterpret_cast<uintptr_t>(scales) % 16 == 0),
            "%s: codes and scales start on 16-byte boundaries", what);
+  VB_CHECK(rows == 0 || (x != nullptr && reinterpret_cast<uintptr_t>(x) % size == 0), "%s: a null pointer, or one off its elements' boundaries", what);
   return 0;
 }
 
 }  // namespace
 
 int mx4_quantize(const void* x, int dt, int64_t ldx, uint8_t* codes, uint8_t* scales, int rows, int cols, cudaStream_t stream) {
-  if (int rc = check_rows("mx4_quantize", rows, cols, codes, scales)) return rc;
   VB_CHECK(dt == VILA_DT_BF16 || dt == VILA_DT_F32, "mx4_quantize: dtype code %d", dt);
-  if (rows == 0) return 0;
   const bool f32 = dt == VILA_DT_F32;
+  if (int rc = check_rows("mx4_quantize", rows, cols, codes, scales, x, f32 ? 4 : 2)) return rc;
+  if (rows == 0) return 0;
   const int h = how(x, ldx, f32 ? 4 : 2);
   auto k = f32 ? (h == kBy32 ? quantize_kernel<true, kBy32> : (h == kBy16 ? quantize_kernel<true, kBy16> : quantize_kernel<true, kApart>))
                : (h == kBy32 ? quantize_kernel<false, kBy32> : (h == kBy16 ? quantize_kernel<false, kBy16> : quantize_kernel<false, kApart>));
@@ -264,10 +266,11 @@ int mx4_quantize(const void* x, int dt, int64_t ldx, uint8_t* codes, uint8_t* sc
 }
 
 int mx4_dequantize(const uint8_t* codes, const uint8_t* scales, void* out, int dt, int64_t ldo, int rows, int cols, cudaStream_t stream) {
-  if (int rc = check_rows("mx4_dequantize", rows, cols, codes, scales)) return rc;
   VB_CHECK(dt == VILA_DT_BF16 || dt == VILA_DT_F32, "mx4_dequantize: dtype code %d", dt);
-  if (rows == 0) return 0;
   const bool f32 = dt == VILA_DT_F32;
+  if (int rc = check_rows("mx4_dequantize", rows, cols, codes, scales, out, f32 ? 4 : 2)) return rc;
+  VB_CHECK(rows <= 1 || ldo >= cols, "mx4_dequantize: ldo=%lld cols=%d", static_cast<long long>(ldo), cols);
+  if (rows == 0) return 0;
   const int h = how(out, ldo, f32 ? 4 : 2);
   auto k = f32 ? (h == kBy32 ? dequantize_kernel<true, kBy32> : (h == kBy16 ? dequantize_kernel<true, kBy16> : dequantize_kernel<true, kApart>))
                : (h == kBy32 ? dequantize_kernel<false, kBy32> : (h == kBy16 ? dequantize_kernel<false, kBy16> : dequantize_kernel<false, kApart>));
@@ -278,7 +281,7 @@ int mx4_dequantize(const uint8_t* codes, const uint8_t* scales, void* out, int d
 }
 
 int mx4_scales(uint8_t* plain, uint8_t* tiled, int rows, int cols, int to_tiled, cudaStream_t stream) {
-  if (int rc = check_rows("mx4_scales", rows, cols, tiled, tiled)) return rc;
+  if (int rc = check_rows("mx4_scales", rows, cols, tiled, tiled, plain, 1)) return rc;
   if (rows == 0) return 0;
   const int padded = (rows + 127) / 128 * 128;
   const int grid = grid_for((static_cast<long long>(padded) * mx4_ktiles(cols) + 31) / 32);
