@@ -263,6 +263,40 @@ def test_scales_over_the_whole_range(cuda, M, N, four):
         check_product(ops.mx4_linear(x.to(cuda), q), x, w, None)
 
 
+def ends_of_the_range(M, N, cuda, four, top=118):
+    """Rows and weights whose blocks' scales lie at the ends of the range, each block of rows against one of weights that brings the
+    products near 1 if there is one, else as near as 2^top allows.  Block 3 of the weights is zeros under the largest
+    scale, block 7 numbers of the least size under it.  -> what the product takes, and float64 values of both"""
+    from vila_b200 import ops
+    K = 512
+    base = torch.tensor([0, 1, 2, 254, 30, 127, 200, 254, 240, 250, 252, 13, 64, 190, 252, 0])
+    codes, scales = R.quantise(rand(40, N, K))
+    scales = (base + (torch.arange(N)[:, None] % 3 - 1) * ((base > 3) & (base < 251))).to(torch.uint8)
+    codes[:, 3 * 16:4 * 16] = 0
+    codes[:, 7 * 16:8 * 16] &= 0x99      # +-0, +-0.5: what 2^127 leaves in fp32's range
+    e = (127 - base).clamp(-125, top).double()
+    x = (rand(41, M, K).double() * torch.exp2(e).repeat_interleave(32) * torch.exp2(torch.arange(M).double() % 2)[:, None]).to(BF)
+    q, w = ops.mx4_pack(codes.to(cuda), scales.to(cuda), K), R.values(codes, scales, K)
+    if not four:
+        return x.to(cuda), q, x, w
+    a_codes, a_scales = R.quantise(x)
+    a_codes[:, 5 * 16:6 * 16] = 0
+    a_scales[:, 5] = 254                 # zeros under the largest scale again
+    return ops.mx4_pack(a_codes.to(cuda), a_scales.to(cuda), K), q, R.values(a_codes, a_scales, K), w
+
+
+@pytest.mark.parametrize("top", [118, 60])
+@pytest.mark.parametrize("M, N, four", [(1, 200, False), (3, 200, False), (8, 2000, False), (60, 9000, False), (90, 9000, False), (120, 9000, False),
+                                        (700, 5000, False), (3, 200, True), (40, 200, True), (100, 200, True), (300, 200, True), (700, 500, True)])
+def test_scales_at_the_ends_of_their_range(cuda, M, N, four, top):
+    """The bound is check_product's: a tensor-core step, an addition, and a rounding to bf16 whose least step is 2^-133; scales are powers
+    of two, and add nothing to it as long as no intermediate result leaves fp32's range."""
+    from vila_b200 import ops
+    x, q, x64, w = ends_of_the_range(M, N, cuda, four, top)
+    got = ops.mx4_matmul(x, q) if four else ops.mx4_linear(x, q)
+    check_product(got, x64, w, None)
+
+
 @pytest.mark.parametrize("M, N, four", [(M, 150, four) for M in (3, 40, 300) for four in (False, True)] +
                          [(3, 50000, False), (60, 9000, False), (90, 9000, False), (700, 5000, False)])
 def test_not_a_number_stays_in_its_row_and_column(cuda, M, N, four):

@@ -6,7 +6,10 @@
 // a block stay in registers, where its scale is applied.
 //
 //   weights   a 4-bit number is an f16 number as it is (cvt e2m1x2 -> f16x2); a block's 32 products per output are summed by two
-//             mma from zero, then enter the row's fp32 sum times the block's scale: acc += 2^e * part, 2^e that of the weights and of the tokens.  No weight is rounded.
+//             mma from zero, then enter the row's fp32 sum times the block's scales: acc += (part * 2^t) * 2^e, 2^t the tokens', 2^e the
+//             weights'.  No weight is rounded.  In this order, and with 2^-9 in the tokens' scale that the finished sum takes out again, no
+//             scale leaves fp32's range before its result does: |part * 2^t| is below 32 * 6 * 2^128 * 2^-9 < 2^127, and it is a multiple of
+//             2^-143 (bf16's least step, half a unit of a weight, the 2^-9), which fp32 holds.
 //   tokens    f16 too, scaled per block by a power of two that brings its largest magnitude to 2^14 .. 2^15: bf16's 8 bits
 //             fit f16's 11, and what is 2^29 times smaller than that largest is rounded to multiples of 2^-39 of it, under
 //             the rounding of the fp32 sum (a block's weights differ by 12 at most).  4-bit tokens are f16 as they are.
@@ -45,6 +48,8 @@ template <int TM> struct Smem {
   static constexpr int kTotal = kTokBytes + kRing + kRed;
 };
 
+constexpr int kUnits = 9;      // the sums are held in units of 2^kUnits
+
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t a0, const uint32_t a1, const uint32_t a2, const uint32_t a3,
                                         uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -82,7 +87,7 @@ __device__ __forceinline__ void stage_tokens(const vila_mx4_linear_params& p, in
       h[1] = mx4_pair_f16<1>(w);
       h[2] = mx4_pair_f16<2>(w);
       h[3] = mx4_pair_f16<3>(w);
-      back = mx4_scale((sw >> (8 * ((k >> 5) & 3))) & 255u);
+      back = mx4_scale((sw >> (8 * ((k >> 5) & 3))) & 255u) * 0x1p-9f;
     } else {
       const __nv_bfloat16* row = static_cast<const __nv_bfloat16*>(p.x) + static_cast<size_t>(m0 + m) * p.ldx;
       float v[8];
@@ -109,7 +114,7 @@ __device__ __forceinline__ void stage_tokens(const vila_mx4_linear_params& p, in
         const __half2 q = __floats2half2_rn(v[2 * i] * f, v[2 * i + 1] * f);
         h[i] = *reinterpret_cast<const uint32_t*>(&q);
       }
-      back = ldexpf(1.f, -up);
+      back = __uint_as_float(static_cast<uint32_t>(141 - up) << 23) * 0x1p-23f;      // 2^(-up - kUnits): 141 - up is 14 .. 254
     }
     *reinterpret_cast<uint4*>(tok + m * pitch16 + c) = make_uint4(h[0], h[1], h[2], h[3]);
     if ((lane & 3) == 0) tok_scale[(c >> 5) * tokens + m] = back;
@@ -202,10 +207,10 @@ mx4_rows_kernel(const vila_mx4_linear_params p, const vila_glinear_ext ext, int 
           mma_f16_first(part, a00, a10, a01, a11, x.x, x.y);
           mma_f16(part, a02, a12, a03, a13, x.z, x.w);
           const float2 xs = make_float2(ts[b * tokens + col0[j]], ts[b * tokens + col1[j]]);
-          acc[j][0] = fmaf(part[0], ws0[b] * xs.x, acc[j][0]);
-          acc[j][1] = fmaf(part[1], ws0[b] * xs.y, acc[j][1]);
-          acc[j][2] = fmaf(part[2], ws1[b] * xs.x, acc[j][2]);
-          acc[j][3] = fmaf(part[3], ws1[b] * xs.y, acc[j][3]);
+          acc[j][0] = fmaf(part[0] * xs.x, ws0[b], acc[j][0]);
+          acc[j][1] = fmaf(part[1] * xs.y, ws0[b], acc[j][1]);
+          acc[j][2] = fmaf(part[2] * xs.x, ws1[b], acc[j][2]);
+          acc[j][3] = fmaf(part[3] * xs.y, ws1[b], acc[j][3]);
         }
       }
       __syncwarp();       // the stage is free
@@ -233,10 +238,10 @@ mx4_rows_kernel(const vila_mx4_linear_params p, const vila_glinear_ext ext, int 
   __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out);
   const __nv_bfloat16* bias = static_cast<const __nv_bfloat16*>(p.bias);
   auto total = [&](int row, int m) {
-    if (split == 1) return red[row * (TM + 1) + m];
+    if (split == 1) return red[row * (TM + 1) + m] * static_cast<float>(1 << kUnits);
     float v = 0.f;
     for (int q = 0; q < split; ++q) v += ld_dsmem_f32(mapa_u32(red_a + (row * (TM + 1) + m) * 4, q));
-    return v;
+    return v * static_cast<float>(1 << kUnits);
   };
   const int per = gated ? share / 2 : share;
   for (int i = tid; i < per * tokens; i += kThreads) {
