@@ -318,6 +318,40 @@ def test_not_a_number_stays_in_its_row_and_column(cuda, M, N, four):
     check_product(got[rows][:, cols].to(BF), ref[rows], w[cols], None)
 
 
+@pytest.mark.parametrize("M, N, K", [(3, 150, 416), (3, 50000, 416), (12, 150, 416), (12, 300, 8200), (40, 150, 416), (60, 9000, 416), (90, 9000, 416),
+                                     (700, 5000, 416)])
+def test_infinities_and_sums_beyond_the_range(cuda, M, N, K):
+    """Whichever kernel takes the rows: products with an infinite entry are infinite, with a weight of 0 NaN, and sums of infinities of both signs
+    are NaN.  A sum beyond bf16's largest number is infinite; where the magnitudes add up to less than that, no order of the
+    sum leaves the range, and it is held to product_bound.  To that comes what a block's largest entry leaves of the others: the 16 rows that
+    an entry is cut into leave 2 units of the last one, 2 * 4^-15 of the first's, which are at most a quarter of the largest: 2^-31
+    of it (f16 with a scale per block: 2^-39 of it), times the block's weights."""
+    from vila_b200 import ops
+    codes, scales = R.quantise(rand(50, N, K))
+    codes[::7, 4] &= 0xf0               # column 8: weights of 0
+    scales[20, 3] = 255
+    q, w = ops.mx4_pack(codes.to(cuda), scales.to(cuda), K), R.values(codes, scales, K)
+    x = rand(51, M, K).to(BF)
+    x[0, 8] = math.inf
+    x[1, 8], x[1, 300] = -math.inf, math.inf
+    x[2] = 0
+    x[2, 10:14] = torch.tensor([3.3e38, -3.3e38, 3.2e38, 2.0]).to(BF)
+    got = ops.mx4_linear(x.to(cuda), q).float().cpu()
+    z = torch.stack([(x[m].double() * w).sum(1) for m in range(3)])
+    most = (x[2].double().abs() * w.abs()).sum(1)
+    assert torch.isnan(got[:, 20]).all()
+    assert torch.isinf(z[0]).any() and torch.isnan(z[0]).any() and torch.isinf(z[1]).any()
+    assert torch.equal(got[:2].nan_to_num(7.0), z[:2].float().nan_to_num(7.0)) and torch.equal(torch.isnan(got[:2]), torch.isnan(z[:2]))
+    inside, beyond = most < 3.3e38, (z[2].abs() == most) & (most > 3.5e38) & torch.isfinite(most)
+    assert inside.any() and beyond.any()
+    z2, bound = product_bound(x[2:3], w[inside])
+    assert ((got[2:3, inside] - z2).abs() <= bound + 2.0 ** -31 * 3.3e38 * w[inside, :32].abs().sum(1)).all()
+    assert torch.equal(got[2, beyond].double(), torch.sign(z[2, beyond]) * math.inf)
+    cols = [n for n in range(N) if n != 20]
+    if M > 3:
+        check_product(got[3:][:, cols].to(BF), x[3:], w[cols], None)
+
+
 @pytest.mark.parametrize("M, N, four", [(M, 384, four) for M in (1, 5, 30, 300) for four in (False, True)] +
                          [(2, 17000, False), (60, 9000, False), (700, 5000, False), (700, 5000, True)])
 def test_same_bits_every_time_and_on_another_stream_and_in_a_graph(cuda, M, N, four):

@@ -17,7 +17,8 @@
 // kPieces: few bf16 tokens on 4-bit weights, by the same products.  A token is cut into 16 rows of 4-bit numbers that add up to it
 // (mx4_pieces): a block's numbers in units u_0 = 2^(floor(log2 max) - 2) are below 8, the nearest 4-bit number leaves at most 2, which are
 // at most 8 of the next row's units u_1 = u_0 / 4, and so on; what 16 rows leave is under 2^-31 of the block's largest magnitude, and of
-// bf16's 8 bits nothing at all where a number is above 2^-22 of it.  The 16 columns of a token are added in fp32.  The tensor core has
+// bf16's 8 bits nothing at all where a number is above 2^-22 of it.  The 16 columns of a token are added in fp32; a sum that is not finite
+// is taken again from the token itself (sum_again).  The tensor core has
 // that to spare (128 weight rows x 16 columns x 256: about 60 clocks, their codes take 300 to arrive), while unpacking weights
 // to f16 is bound by integer instructions: mx4_rows.cu takes 20.7 us for one token on 37888 x 3584.
 #include "../../include/vila_b200.h"
@@ -66,6 +67,19 @@ __device__ __forceinline__ void scales_to_tmem(uint32_t taddr, uint64_t desc) {
   asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 constexpr int kPieceRows = 16;
+// One sum term by term, where the cut rows' came out infinite or NaN: of a block with an infinity or a NaN they know no more than that (its first
+// row reads as NaN), and one row's part of a sum may leave fp32's range alone.  x: the token's row, n: the weight row.
+__device__ __noinline__ float sum_again(const __nv_bfloat16* x, const uint8_t* codes, const uint8_t* scales, int n, int K) {
+  const int pitch = mx4_pitch(K), kts = mx4_ktiles(K);
+  float s = 0.f;
+  for (int k = 0; k < K && s == s; k += 32) {
+    const uint4 c4 = __ldg(reinterpret_cast<const uint4*>(codes + static_cast<size_t>(n) * pitch + k / 2));
+    const float unit = mx4_scale(__ldg(scales + mx4_scale_at(n, k >> 7, kts) + (k >> 5 & 3)));
+    const uint32_t c[4] = {c4.x, c4.y, c4.z, c4.w};
+    for (int i = 0; i < 32 && k + i < K; ++i) s = fmaf(__bfloat162float(x[k + i]), mx4_number(c[i >> 3] >> (4 * (i & 7)) & 15u) * unit, s);
+  }
+  return s;
+}
 template <int BN, bool kSwap, bool kPieces>
 __global__ void __launch_bounds__(kThreads, Shape<BN>::kPerSm)
 mx4_tc_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ CUtensorMap tmap_q, const vila_mx4_linear_params p,
@@ -256,8 +270,13 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant_
             float v = r[kPieceRows - 1];      // the smallest first
 #pragma unroll
             for (int i = kPieceRows - 2; i >= 0; --i) v += r[i];
-            if (split > 1) red[(c / kPieceRows) * kP + quad * 32 + lane] = v;
-            else mx4_store_one<EPI>(p, x, v, (q0 + c) / kPieceRows, row, bias);
+            if (split > 1) {
+              red[(c / kPieceRows) * kP + quad * 32 + lane] = v;
+            } else {
+              const int m = (q0 + c) / kPieceRows;
+              if (!isfinite(v) && row < p.N) v = sum_again(static_cast<const __nv_bfloat16*>(p.x) + static_cast<size_t>(m) * p.ldx, p.w_codes, p.w_scales, row, p.K);
+              mx4_store_one<EPI>(p, x, v, m, row, bias);
+            }
           } else {
             if (split > 1) {
 #pragma unroll
@@ -304,6 +323,12 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant_
           z[2] += part[q].z;
           z[3] += part[q].w;
         }
+      if constexpr (kPieces) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (!isfinite(z[j]) && n + j < p.N)
+            z[j] = sum_again(static_cast<const __nv_bfloat16*>(p.x) + static_cast<size_t>(m0 + c) * p.ldx, p.w_codes, p.w_scales, n + j, p.K);
+      }
       const size_t o = static_cast<size_t>(m0 + c) * p.ldo;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
@@ -684,7 +709,6 @@ int mx4_pieces(const vila_mx4_linear_params& given, const vila_glinear_ext& x, i
   const long long items = static_cast<long long>((kPieceRows * p.M + 127) / 128 * 128 / kPieceRows) * (mx4_ktiles(p.K) / 2);
   VB_CUDA(launch_serial(mx4_pieces_kernel, dim3(static_cast<unsigned>((items + kPieceWarps - 1) / kPieceWarps)), dim3(32 * kPieceWarps), 0, stream,
                         static_cast<const __nv_bfloat16*>(p.x), p.ldx, codes, scales, p.M, p.K));
-  p.x = nullptr;
   p.a_codes = codes;
   p.a_scales = scales;
   const int rows = kPieceRows * p.M;
