@@ -286,8 +286,8 @@ def ends_of_the_range(M, N, cuda, four, top=118):
 
 
 @pytest.mark.parametrize("top", [118, 60])
-@pytest.mark.parametrize("M, N, four", [(1, 200, False), (3, 200, False), (8, 2000, False), (60, 9000, False), (90, 9000, False), (120, 9000, False),
-                                        (700, 5000, False), (3, 200, True), (40, 200, True), (100, 200, True), (300, 200, True), (700, 500, True)])
+@pytest.mark.parametrize("M, N, four", [(1, 200, False), (3, 200, False), (8, 2000, False), (3, 70000, False), (12, 300, False), (40, 200, False),
+                                        (60, 9000, False), (90, 9000, False), (120, 9000, False), (700, 5000, False), (3, 200, True), (40, 200, True), (100, 200, True), (300, 200, True), (700, 500, True)])
 def test_scales_at_the_ends_of_their_range(cuda, M, N, four, top):
     """The bound is check_product's: a tensor-core step, an addition, and a rounding to bf16 whose least step is 2^-133; scales are powers
     of two, and add nothing to it as long as no intermediate result leaves fp32's range."""
@@ -295,6 +295,25 @@ def test_scales_at_the_ends_of_their_range(cuda, M, N, four, top):
     x, q, x64, w = ends_of_the_range(M, N, cuda, four, top)
     got = ops.mx4_matmul(x, q) if four else ops.mx4_linear(x, q)
     check_product(got, x64, w, None)
+
+
+@pytest.mark.parametrize("M, N, K", [(3, 150, 416), (3, 50000, 416), (12, 150, 416), (12, 300, 8200), (40, 150, 416), (60, 9000, 416), (700, 5000, 416)])
+def test_small_entries_of_rows(cuda, M, N, K):
+    """Every kernel reads small entries to their last bit: rows of 2^-100 down to bf16's least step 2^-133, on weights of 2^90, and rows that hold
+    entries at both ends.  A block's largest entry leaves 2^-31 of itself (see test_infinities_and_sums_beyond_the_range)."""
+    from vila_b200 import ops
+    codes, scales = R.quantise(rand(50, N, K))
+    scales = scales + 90
+    q, w = ops.mx4_pack(codes.to(cuda), scales.to(cuda), K), R.values(codes, scales, K)
+    x = (rand(51, M, K).double() * torch.exp2(-100 - 3.0 * (torch.arange(M) % 13).double())[:, None]).to(BF)
+    x[1] = (torch.exp2(-133.0 + (torch.arange(K) % 8).double()) * (1 - 2 * (torch.arange(K) % 3 == 0).double())).to(BF)
+    x[2, :256] = (rand(52, 256).double() * torch.exp2(-90.0 - (torch.arange(256) // 32 * 6).double())).to(BF)
+    got = ops.mx4_linear(x.to(cuda), q)
+    z, S = x.double() @ w.T, x.double().abs() @ w.abs().T
+    blocks = torch.nn.functional.pad(x.double().abs(), (0, -K % 32)).view(M, -1, 32).amax(2).repeat_interleave(32, 1)[:, :K]
+    bound = z.abs() * 2.0 ** -8 + S * ((K / 16 + 8) * 2.0 ** -22) + 2.0 ** -31 * (blocks @ w.abs().T) + 2.0 ** -133
+    err = (got.double().cpu() - z).abs()
+    assert (err <= bound).all(), (err / bound).max().item()
 
 
 @pytest.mark.parametrize("M, N, four", [(M, 150, four) for M in (3, 40, 300) for four in (False, True)] +

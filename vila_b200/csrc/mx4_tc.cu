@@ -17,8 +17,11 @@
 // kPieces: few bf16 tokens on 4-bit weights, by the same products.  A token is cut into 16 rows of 4-bit numbers that add up to it
 // (mx4_pieces): a block's numbers in units u_0 = 2^(floor(log2 max) - 2) are below 8, the nearest 4-bit number leaves at most 2, which are
 // at most 8 of the next row's units u_1 = u_0 / 4, and so on; what 16 rows leave is under 2^-31 of the block's largest magnitude, and of
-// bf16's 8 bits nothing at all where a number is above 2^-22 of it.  The 16 columns of a token are added in fp32; a sum that is not finite
-// is taken again from the token itself (sum_again).  The tensor core has
+// bf16's 8 bits nothing at all where a number is above 2^-22 of it.  That holds for small blocks, too, as the rows' scales are 2^kPieceUnits too
+// large: scale bytes end at 2^-127, units at 2^-135.  bf16 numbers are multiples of 2^-133; in the last unit but one, 2^-132 or 2^-133, what is left
+// is a multiple of a half and below 8, its nearest 4-bit number leaves 0, 1/2, 1 or 3/2, and the last row holds four times that.  Blocks
+// of 2^122 and more have no scale.  The 16 columns of a token are added in fp32, and the 2^kPieceUnits taken out; a sum that is not finite
+// (a block without a scale reads as NaN) is taken again from the token itself (sum_again).  The tensor core has
 // that to spare (128 weight rows x 16 columns x 256: about 60 clocks, their codes take 300 to arrive), while unpacking weights
 // to f16 is bound by integer instructions: mx4_rows.cu takes 20.7 us for one token on 37888 x 3584.
 #include "../../include/vila_b200.h"
@@ -66,7 +69,7 @@ __device__ __forceinline__ void umma_mx4(uint32_t d, uint64_t a, uint64_t b, uin
 __device__ __forceinline__ void scales_to_tmem(uint32_t taddr, uint64_t desc) {
   asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
-constexpr int kPieceRows = 16;
+constexpr int kPieceRows = 16, kPieceUnits = 8;
 // One sum term by term, where the cut rows' came out infinite or NaN: of a block with an infinity or a NaN they know no more than that (its first
 // row reads as NaN), and one row's part of a sum may leave fp32's range alone.  x: the token's row, n: the weight row.
 __device__ __noinline__ float sum_again(const __nv_bfloat16* x, const uint8_t* codes, const uint8_t* scales, int n, int K) {
@@ -270,6 +273,7 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant_
             float v = r[kPieceRows - 1];      // the smallest first
 #pragma unroll
             for (int i = kPieceRows - 2; i >= 0; --i) v += r[i];
+            v *= 1.f / (1 << kPieceUnits);
             if (split > 1) {
               red[(c / kPieceRows) * kP + quad * 32 + lane] = v;
             } else {
@@ -618,17 +622,18 @@ mx4_pieces_kernel(const __nv_bfloat16* x, int64_t ldx, uint8_t* codes, uint8_t* 
   for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-  const bool finite = top < 0x7f800000u;
-  const uint32_t e = top >> 23, first = finite ? (e > 2 ? e - 2 : 0u) : 255u;
-  const float inv = __uint_as_float((254u - (finite ? first : 0u)) << 23);
+  const uint32_t e = top >> 23, unit = e > 2 ? e - 2 : 0u;
+  const bool held = unit + kPieceUnits < 255u;
+  const uint32_t first = held ? unit + kPieceUnits : 255u;
+  const float inv = __uint_as_float((254u - (held ? unit : 0u)) << 23);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = finite ? v[i] * inv : 0.f;
+  for (int i = 0; i < 8; ++i) v[i] = held ? v[i] * inv : 0.f;
 #pragma unroll 1
   for (int i = 0; i < kPieceRows; ++i) {
     const int r = m * kPieceRows + i;
-    // the first row of a block that is not finite says so; units below 2^-127 do not exist, nor do rows of them
-    const uint32_t byte = i == 0 ? first : (finite && first >= 2u * i ? first - 2u * i : 0u);
-    const bool rest = i == 0 || (finite && first >= 2u * i);
+    // the first row of a block without a scale says so; bytes below 0 do not exist, nor do rows of them
+    const uint32_t byte = i == 0 ? first : (held && first >= 2u * i ? first - 2u * i : 0u);
+    const bool rest = i == 0 || (held && first >= 2u * i);
     const uint32_t c = rest && m < M ? mx4_encode8(v) : 0u;
     const uint32_t h[4] = {mx4_pair_f16<0>(c), mx4_pair_f16<1>(c), mx4_pair_f16<2>(c), mx4_pair_f16<3>(c)};
 #pragma unroll
