@@ -737,6 +737,80 @@ def test_weights_replaced_under_an_engine_that_has_captured_its_steps(cuda, arch
     assert all(torch.equal(a, b) for a, b in zip(*both))
 
 
+@pytest.mark.parametrize("arch, layer_type, name", [("bivizen", "delta", "in_w"), ("bivizen", "gla", "in_w"), ("nusovik", "parallel", "ssd_in")])
+def test_rows_of_decays_and_step_sizes_stay_exact(cuda, arch, layer_type, name):
+    """The rows that a recurrence's decay and step size come from keep the weights that were loaded, and their columns of the projection are
+    those of the bf16 model to the bound of one linear layer; the rows before them are in 4 bits."""
+    import importlib
+    from vila_b200 import ops
+    from vila_b200.model.registry import quantize_weights
+    T = importlib.import_module(f"tests.test_{arch}_gpu")
+    cfg, small = T.build("aligned" if "aligned" in T.CONFIGS else next(iter(T.CONFIGS)), BF, seed=3)
+    loaded = small.state_dict()
+    before = [getattr(L, name, None) for L in small.layers]
+    quantize_weights(small)
+    seen = 0
+    for i, (L, w) in enumerate(zip(small.layers, before)):
+        if L.cfg.type != layer_type:
+            continue
+        seen += 1
+        if arch == "bivizen":
+            parts = ("a", "b") if layer_type == "delta" else ("a1",)
+            exact = [(L.in_off[n], loaded[f"l{i}.mix.{n}"]) for n in parts]
+        else:
+            r = L.cfg.right
+            exact = [((r.inner + r.conv_channels, r.heads), loaded[f"l{i}.mix.right.in"][r.inner + r.conv_channels:])]
+        held = ops.mx4_dequantize(getattr(L, name))
+        first = exact[0][0][0]
+        x = rand(i, 5, w.shape[1]).to(BF)
+        got = ops.linear_any(x.to(cuda), getattr(L, name))
+        for (at, n), want in exact:
+            want = want.to(cuda, BF)
+            assert torch.equal(held[at:at + n], want) and torch.equal(w[at:at + n], want)
+            check_product(got[:, at:at + n], x, want, None)
+        assert torch.equal(held[first:], w[first:])
+        rows = first // 8 * 8
+        assert torch.equal(held[:rows], ops.mx4_dequantize(ops.mx4_quantize(w[:rows]))) and not torch.equal(held[:rows], w[:rows])
+        check_product(got, x, held, None)
+    assert seen
+
+
+@pytest.mark.parametrize("M", [0, 1, 12, 60, 700])
+@pytest.mark.parametrize("N, keep, K", [(200, 8, 288), (200, 7, 288), (96, 64, 100), (2, 1, 32), (640, 320, 512)])
+def test_rows_that_stay_as_they_are(cuda, M, N, keep, K):
+    from vila_b200 import ops
+    w, x, bias = (rand(1, N, K) / math.sqrt(K)).to(BF), rand(2, M, K).to(BF), rand(3, N).to(BF)
+    q = ops.mx4_quantize(w.to(cuda), keep=keep)
+    assert q.shape == (N, K) and q.device == x.to(cuda).device and q.nbytes == q.part.nbytes + keep * K * 2
+    both = ops.mx4_dequantize(q).cpu()
+    assert torch.equal(both[N - keep:], w[N - keep:]) and torch.equal(both[:N - keep], ops.mx4_dequantize(ops.mx4_quantize(w[:N - keep].to(cuda))).cpu())
+    assert torch.equal(ops.mx4_dequantize(q, out_dtype=torch.float32).cpu(), both.float())
+    out = torch.full((M, N + 5), 7.0, dtype=BF, device=cuda)
+    check = check_product if M else lambda got, *rest: None
+    check(ops.mx4_linear(x.to(cuda), q, bias.to(cuda), out=out[:, 2:2 + N]), x, both, bias)
+    assert (out[:, :2] == 7).all() and (out[:, 2 + N:] == 7).all()
+    check(ops.linear_any(x.to(cuda), q, act=ops.ACT_SILU), x, both, None, "silu")
+    if N % 2 == 0 and keep % 2 == 0:
+        check(ops.linear_any(x.to(cuda), q, bias=bias.to(cuda), swiglu=True), x, both, bias, "swiglu")
+    elif M:
+        with pytest.raises(RuntimeError, match="even number of weight rows"):
+            ops.linear_any(x.to(cuda), q, swiglu=True)
+
+
+def test_rows_kept_in_bf16_are_refused_where_codes_are_read(cuda):
+    from vila_b200 import ops
+    w = rand(1, 64, 64).to(BF).to(cuda)
+    q, a = ops.mx4_quantize(w, keep=8), ops.mx4_quantize(w)
+    for call in (lambda: ops.mx4_matmul(a, q), lambda: ops.mx4_matmul(q, a), lambda: ops.mx4_unpack(q), lambda: q.codes, lambda: q.scales):
+        with pytest.raises(RuntimeError, match="kept in bf16"):
+            call()
+    for bad in (64, 65, -1):
+        with pytest.raises(RuntimeError, match="not all of them"):
+            ops.mx4_quantize(w, keep=bad)
+    with pytest.raises(RuntimeError, match="not all of them"):
+        ops.mx4_quantize(w.float(), keep=8)
+
+
 def test_load_and_command_line(cuda, tmp_path, capsys):
     from llava.cli import infer
     from tests import test_nusovik_gpu as T

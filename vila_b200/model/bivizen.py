@@ -258,6 +258,7 @@ class BivizenForCausalLM:
             elif lc.type == "delta":
                 L.in_w, L.in_off = stack_rows([("qkv", torch.cat([w(q + "q"), w(q + "k"), w(q + "v")])), ("g", w(q + "g")),
                                                ("a", w(q + "a")), ("b", w(q + "b"))])
+                L.exact_from = {"in_w": L.in_off["a"][0]}      # decay | step size (registry.quantize_weights)
                 L.conv = torch.cat([f32(q + "q.conv"), f32(q + "k.conv"), f32(q + "v.conv")]).contiguous()
                 L.A_log, L.dt_bias, L.norm = f32(q + "A_log"), f32(q + "dt_bias"), f32(q + "norm")
             else:
@@ -265,6 +266,7 @@ class BivizenForCausalLM:
                 if tensors[q + "a2"].shape[1] != rank:
                     raise ValueError(f"{q}a2: {tensors[q + 'a2'].shape[1]} columns for a rank of {rank}")
                 L.in_w, L.in_off = stack_rows([(n, w(q + n)) for n in ("q", "k", "v", "g", "a1")])
+                L.exact_from = {"in_w": L.in_off["a1"][0]}     # low-rank decay
                 L.a2, _ = stack_rows([("a2", w(q + "a2"))])
                 L.a2_b, L.norm = f32(q + "a2.b"), f32(q + "norm")
             if lc.ff:

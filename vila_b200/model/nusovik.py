@@ -337,6 +337,7 @@ class NusovikForCausalLM:
                 L.attn_o = w(q + "o")
                 q = p + "mix.right."
                 L.ssd_in = _pad_rows(w(q + "in"))
+                L.exact_from = {"ssd_in": lc.right.inner + lc.right.conv_channels}     # step sizes (registry.quantize_weights)
                 L.ssd_conv, L.ssd_conv_b = f32(q + "conv"), f32(q + "conv.b")
                 L.dt_bias, L.A_log, L.D = f32(q + "dt_bias"), f32(q + "A_log"), f32(q + "D")
                 L.ssd_norm, L.ssd_o = f32(q + "norm"), w(q + "o")

@@ -31,8 +31,9 @@ def language_model_architecture(model_dir) -> Optional[str]:
     return arch if arch in LANGUAGE_MODELS else None
 
 
-# The layers' weights that linear_any alone reads, by class: these may be held in 4 bits.  Narrow projections that a recurrence's
-# step size or decay comes from stay as they are, as do embeddings, routers, experts, norms and the output head.
+# The layers' weights that linear_any alone reads, by class: these may be held in 4 bits.  Projections that a recurrence's step size or
+# decay comes from stay as they are (an error in them compounds over the state), as do embeddings, routers, experts, norms and the output
+# head.  Where such rows end a fused weight, the layer's `exact_from` says from which row on.
 MX4_WEIGHTS: Dict[str, tuple] = {
     "Lufatar": ("qkv", "o", "side_gate", "side_proj"),
     "Nusovik": ("qkg", "attn_o", "ssd_in", "ssd_o", "sel_in", "sel_o", "up", "down"),
@@ -44,8 +45,8 @@ MX4_WEIGHTS: Dict[str, tuple] = {
 
 def quantize_weights(model):
     """Hold a bf16 language model's layer weights as microscaled 4-bit rows (ops.Mx4: 17 bytes per 32 of them instead of 64), each
-    rounded to the nearest number of its block; activations stay bf16.  In place; -> model.  state_dict and save_pretrained
-    still give the weights that were loaded, which the model keeps where they were: on the host after from_pretrained.  A model
+    rounded to the nearest number of its block; rows that step sizes and decays come from, and activations, stay bf16.  In place; -> model.
+    state_dict and save_pretrained still give the weights that were loaded, which the model keeps where they were: on the host after from_pretrained.  A model
     made from tensors on the GPU keeps those there, too, and then takes more of its memory, not less.  A TokenEngine that runs the
     model captures its decode steps anew at its next step; what it cached for its sequences stays as the former weights made it.
     Not while another thread runs a step of the model."""
@@ -63,7 +64,10 @@ def quantize_weights(model):
         for name in names:
             w = getattr(layer, name, None)
             if isinstance(w, torch.Tensor) and w.dim() == 2:      # experts' weights are one tensor of three dimensions
-                setattr(layer, name, ops.mx4_quantize(w))
+                first = getattr(layer, "exact_from", {}).get(name, w.shape[0])
+                first = first // 8 * 8 if first < w.shape[0] else first      # the kept rows' results start on a 16-byte boundary
+                if first > 0:
+                    setattr(layer, name, ops.mx4_quantize(w, keep=w.shape[0] - first))
     return model
 
 

@@ -709,12 +709,18 @@ def linear_any(x: torch.Tensor, w: torch.Tensor, *, swiglu: bool = False, out_dt
         if out_dtype not in (None, torch.bfloat16):
             raise RuntimeError(f"vila_b200.ops: a linear layer on 4-bit weights gives bfloat16, not {out_dtype}")
         return mx4_linear(x, w, bias, act=act, act_params=act_params, swiglu=swiglu, geglu=geglu, glu_clamp=glu_clamp)
+    return _linear_rows(x, w, None, swiglu=swiglu, out_dtype=out_dtype, bias=bias, act=act, act_params=act_params, glu_clamp=glu_clamp, geglu=geglu)
+
+
+def _linear_rows(x, w, out, *, swiglu=False, out_dtype=None, bias=None, act=ACT_NONE, act_params=None, glu_clamp=None, geglu=False) -> torch.Tensor:
+    """linear_any on a plain weight, into `out` (columns of a wider tensor, say) if there is one"""
     N, K = w.shape
     if (x.dtype == torch.bfloat16 and w.dtype == torch.bfloat16 and out_dtype in (None, torch.bfloat16)
             and K % 8 == 0 and N % 8 == 0 and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0
+            and (out is None or (out.stride(0) % 8 == 0 and out.data_ptr() % 16 == 0))
             and (not (swiglu or glu_clamp or geglu) or N % 32 == 0)):
-        return linear(x, w, bias, act=act, swiglu=swiglu, static_w=True, act_params=act_params, glu_clamp=glu_clamp, geglu=geglu)
-    return glinear(x, w, swiglu=swiglu, out_dtype=out_dtype, bias=bias, act=act, act_params=act_params, glu_clamp=glu_clamp,
+        return linear(x, w, bias, act=act, swiglu=swiglu, static_w=True, act_params=act_params, glu_clamp=glu_clamp, geglu=geglu, out=out)
+    return glinear(x, w, out=out, swiglu=swiglu, out_dtype=out_dtype, bias=bias, act=act, act_params=act_params, glu_clamp=glu_clamp,
                    geglu=geglu)
 
 
@@ -1316,6 +1322,29 @@ class Mx4:
         return self.rows * 16 * ((self.cols + 31) // 32) + _mx4_scale_bytes(self.rows, self.cols)
 
 
+class Mx4Kept(Mx4):
+    """Rows of which the last ones stay the bf16 numbers that they were (mx4_quantize's keep): `part` the 4-bit rows before them, `kept` the
+    others [keep, cols].  A weight of mx4_linear and linear_any; it has no codes and scales of its own."""
+
+    __slots__ = ("part", "kept")
+
+    def __init__(self, part: Mx4, kept: torch.Tensor):
+        self.part, self.kept = part, kept
+        self.rows, self.cols = part.rows + kept.shape[0], part.cols
+
+    def _held(self) -> torch.Tensor:
+        return self.part._held()
+
+    def _ptrs(self):
+        raise RuntimeError("vila_b200.ops: rows kept in bf16 have no codes and scales (mx4_linear and mx4_dequantize take them)")
+
+    codes = scales = property(_ptrs)
+
+    @property
+    def nbytes(self) -> int:
+        return self.part.nbytes + self.kept.numel() * 2
+
+
 def _mx4_check(ok: bool, what: str) -> None:
     if not ok:
         raise RuntimeError(f"vila_b200.ops: {what}")
@@ -1334,10 +1363,11 @@ def _mx4_scale_bytes(rows: int, cols: int) -> int:
     return ((rows + 127) // 128) * (2 * ((cols + 255) // 256)) * 512
 
 
-def mx4_quantize(x: torch.Tensor) -> Mx4:
+def mx4_quantize(x: torch.Tensor, keep: int = 0) -> Mx4:
     """x [rows, cols] bf16 or fp32 (a view with a row stride is fine) -> Mx4.  Per block of 32 columns with largest magnitude m
     the scale is 2^max(floor(log2 m) - 2, -127), and every x / scale becomes the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 (ties to
-    the even code, 6 beyond 6; signs kept).  A block with an infinity or a NaN reads as NaN."""
+    the even code, 6 beyond 6; signs kept).  A block with an infinity or a NaN reads as NaN.
+    keep: the last rows of a bf16 weight that stay as they are, copied (Mx4Kept)."""
     _mx4_here(x, "x")
     if x.dim() != 2:
         raise RuntimeError("vila_b200.ops: x must be [rows, cols] with consecutive columns")
@@ -1345,6 +1375,9 @@ def mx4_quantize(x: torch.Tensor) -> Mx4:
     if cols == 0 or (x.stride(1) != 1 and cols != 1):
         raise RuntimeError("vila_b200.ops: x must be [rows, cols] with consecutive columns")
     dt = _dt(x, "x")
+    if keep:
+        _mx4_check(0 < keep < rows and x.dtype == torch.bfloat16, f"keep={keep}: some of {rows} bf16 rows, not all of them")
+        return Mx4Kept(mx4_quantize(x[:rows - keep]), x[rows - keep:].clone(memory_format=torch.contiguous_format))
     q = Mx4._alloc(x, rows, cols)
     codes, scales = q._ptrs()
     check(_lib.load().vila_mx4_quantize(x.data_ptr(), dt, x.stride(0), codes, scales, rows, cols, _stream()), "vila_mx4_quantize")
@@ -1356,8 +1389,12 @@ def mx4_dequantize(q: Mx4, out_dtype=torch.bfloat16) -> torch.Tensor:
     held = q._held()
     _mx4_here(held, "q")
     out = held.new_empty((q.rows, q.cols), dtype=out_dtype)
-    codes, scales = q._ptrs()
-    check(_lib.load().vila_mx4_dequantize(codes, scales, out.data_ptr(), _dt(out, "out"), q.cols, q.rows, q.cols, _stream()),
+    part = q
+    if isinstance(q, Mx4Kept):
+        part = q.part
+        out[part.rows:].copy_(q.kept)
+    codes, scales = part._ptrs()
+    check(_lib.load().vila_mx4_dequantize(codes, scales, out.data_ptr(), _dt(out, "out"), q.cols, part.rows, q.cols, _stream()),
           "vila_mx4_dequantize")
     return out
 
@@ -1411,6 +1448,18 @@ def _mx4_product(x: Optional[torch.Tensor], a: Optional[Mx4], M: int, K: int, w:
         _mx4_here(bias, "bias")
         _mx4_check(bias.is_contiguous() and bias.numel() == N, f"bias must be contiguous [{N}]")
     if M == 0:
+        return out
+    if isinstance(w, Mx4Kept):
+        n = w.part.rows
+        _mx4_check(a is None, "a product of two 4-bit factors takes no rows kept in bf16")
+        _mx4_check(not flags or (n % 2 == 0 and N % 2 == 0), "a gated unit has an even number of weight rows, in 4 bits and kept")
+        cut = n // 2 if flags else n
+        _mx4_product(x, None, M, K, w.part, None if bias is None else bias[:n], act, act_params, swiglu, geglu, glu_clamp, out[:, :cut])
+        rest = None if bias is None else bias[n:]
+        if act == ACT_NONE and not flags:
+            _linear_rows(x, w.kept, out[:, cut:], bias=rest)
+        else:      # rounds once, behind the activation, as the 4-bit rows' kernels do; linear rounds before it, too
+            glinear(x, w.kept, out=out[:, cut:], bias=rest, act=act, act_params=act_params, swiglu=swiglu, geglu=geglu, glu_clamp=glu_clamp)
         return out
     alpha, limit = glu_clamp if glu_clamp is not None else (0.0, 0.0)
     pos, neg = act_params if act_params is not None else (0.0, 0.0)
