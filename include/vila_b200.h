@@ -937,7 +937,9 @@ typedef struct vila_mx4_linear_params {
   void* scratch;
   int64_t scratch_bytes;
 } vila_mx4_linear_params;
-/* Bytes of scratch (on a 16-byte boundary, of this call alone until it has run) that vila_mx4_linear is faster with; 0: none. */
+/* Bytes of scratch (on a 16-byte boundary, of this call alone until it has run) that vila_mx4_linear is faster with; 0: none.  Without it, rows
+ * that it would cut into 4-bit rows, or copy to 16-byte boundaries, are taken by slower kernels: 16 at a time on mma.sync, or, more
+ * than 16 rows on 16-byte boundaries, by unpacked weights. */
 int64_t vila_mx4_linear_scratch(const vila_mx4_linear_params* p);
 int vila_mx4_linear(const vila_mx4_linear_params* p, void* stream);
 /* vila_mx4_linear with waits of its tcgen05 kernels that end after `tries` tries (test hook: 0 gives up at once; -2 - r: those of

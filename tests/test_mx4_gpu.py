@@ -436,6 +436,28 @@ def test_offsets_past_32_bits(cuda, M, N, K, four):
     assert ((got.double() - z).abs() <= most).all()
 
 
+@pytest.mark.parametrize("M, N, K", [(8, 500, 32768), (7, 500, 32737), (5, 130, 99999), (3, 129, 60000), (1, 100, 131072), (8, 128, 4096)])
+def test_more_columns_than_tokens_fit_in_shared_memory(cuda, M, N, K):
+    """few rows, small layers: the tokens of a CTA's part of K come in several portions"""
+    from vila_b200 import ops
+    x, q = torch.randn(M, K, device=cuda, dtype=BF), ops.mx4_quantize(torch.randn(N, K, device=cuda))
+    z, most = product_bound(x, ops.mx4_dequantize(q, out_dtype=torch.float32))
+    assert ((ops.mx4_linear(x, q).double() - z).abs() <= most).all()
+
+
+@pytest.mark.parametrize("M", [1, 8, 9, 16, 17, 40])
+@pytest.mark.parametrize("N, K", [(300, 1000), (129, 33000), (3000, 8193)])
+@pytest.mark.parametrize("gap", [0, 3])
+def test_callers_without_a_workspace(cuda, monkeypatch, M, N, K, gap):
+    from vila_b200 import _lib, ops
+    x, q = torch.randn(M, K + gap, device=cuda, dtype=BF)[:, :K], ops.mx4_quantize(torch.randn(N, K, device=cuda))
+    bias = torch.randn(N, device=cuda, dtype=BF)
+    monkeypatch.setattr(_lib.load(), "vila_mx4_linear_scratch", lambda p: 0)
+    z, most = product_bound(torch.cat([x, x.new_ones(M, 1)], 1), torch.cat([ops.mx4_dequantize(q, out_dtype=torch.float32), bias.float()[:, None]], 1))
+    assert ((ops.mx4_linear(x, q, bias).double() - z).abs() <= most).all()
+    ops.check_waits()
+
+
 @pytest.mark.parametrize("M", [7, 8, 9, 15, 16, 17, 127, 128, 129, 255, 256, 257])
 def test_both_sides_of_every_boundary(cuda, M):
     from vila_b200 import ops

@@ -1,5 +1,5 @@
-// Linear layers of up to 8 bf16 rows on up to 16 M microscaled 4-bit weights (and of any, where the caller gives no
-// workspace or K suits no tensor map): out[m, n] = epi(sum_k x[m, k] w[n, k] + bias[n]).
+// Linear layers of up to 8 bf16 rows on up to 16 M microscaled 4-bit weights (and, by tiles of 16 rows, of up to 16 on any, and of
+// any off 16-byte boundaries, where the caller gives no workspace): out[m, n] = epi(sum_k x[m, k] w[n, k] + bias[n]).
 //
 // Bound by the stream of weights (17 bytes per 32 of them), or for the smallest layers by latency.  mma.sync m16n8k16 in f16: 16
 // weight rows are the M side, 8 tokens the N side; tensor-core tiles of 128 tokens would stand empty here, and the sums of
@@ -12,7 +12,7 @@
 //             2^-143 (bf16's least step, half a unit of a weight, the 2^-9), which fp32 holds.
 //   tokens    f16 too, scaled per block by a power of two that brings its largest magnitude to 2^14 .. 2^15: bf16's 8 bits
 //             fit f16's 11, and what is 2^29 times smaller than that largest is rounded to multiples of 2^-39 of it, under
-//             the rounding of the fp32 sum (a block's weights differ by 12 at most).  4-bit tokens are f16 as they are.
+//             the rounding of the fp32 sum (a block's weights differ by 12 at most).
 //   columns   lane t of a quad takes columns 8 t .. 8 t + 7 of a block, of weights and tokens alike (the order within a sum is
 //             free): one word of codes per row and block, one 16-byte load of tokens
 //   warps     a warp owns 16 rows of a tile of 128 (rows r % 32 = 4 w .. 4 w + 3: their scale words are 64 consecutive bytes) and
@@ -77,45 +77,32 @@ __device__ __forceinline__ void stage_tokens(const vila_mx4_linear_params& p, in
   for (int it = warp; it < tokens * pieces; it += kWarps) {
     const int m = it / pieces, c = (it - m * pieces) * 256 + lane * 8, k = k0 + c;
     uint32_t h[4];
-    float back;
-    if (p.a_codes) {
-      const int pitch = mx4_pitch(p.K);
-      const uint32_t w = k / 2 < pitch ? __ldg(reinterpret_cast<const uint32_t*>(p.a_codes + static_cast<size_t>(m0 + m) * pitch + k / 2)) : 0u;
-      const int kt = k >> 7;
-      const uint32_t sw = kt < mx4_ktiles(p.K) ? __ldg(reinterpret_cast<const uint32_t*>(p.a_scales + mx4_scale_at(m0 + m, kt, mx4_ktiles(p.K)))) : 0u;
-      h[0] = mx4_pair_f16<0>(w);
-      h[1] = mx4_pair_f16<1>(w);
-      h[2] = mx4_pair_f16<2>(w);
-      h[3] = mx4_pair_f16<3>(w);
-      back = mx4_scale((sw >> (8 * ((k >> 5) & 3))) & 255u) * 0x1p-9f;
+    const __nv_bfloat16* row = static_cast<const __nv_bfloat16*>(p.x) + static_cast<size_t>(m0 + m) * p.ldx;
+    float v[8];
+    if (k + 8 <= p.K && ((reinterpret_cast<uintptr_t>(p.x) | (p.ldx * 2)) & 15) == 0) {
+      const uint4 a = __ldg(reinterpret_cast<const uint4*>(row + k));
+      v[0] = bf_lo(a.x); v[1] = bf_hi(a.x); v[2] = bf_lo(a.y); v[3] = bf_hi(a.y);
+      v[4] = bf_lo(a.z); v[5] = bf_hi(a.z); v[6] = bf_lo(a.w); v[7] = bf_hi(a.w);
     } else {
-      const __nv_bfloat16* row = static_cast<const __nv_bfloat16*>(p.x) + static_cast<size_t>(m0 + m) * p.ldx;
-      float v[8];
-      if (k + 8 <= p.K && ((reinterpret_cast<uintptr_t>(p.x) | (p.ldx * 2)) & 15) == 0) {
-        const uint4 a = __ldg(reinterpret_cast<const uint4*>(row + k));
-        v[0] = bf_lo(a.x); v[1] = bf_hi(a.x); v[2] = bf_lo(a.y); v[3] = bf_hi(a.y);
-        v[4] = bf_lo(a.z); v[5] = bf_hi(a.z); v[6] = bf_lo(a.w); v[7] = bf_hi(a.w);
-      } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = k + i < p.K ? __bfloat162float(row[k + i]) : 0.f;
-      }
-      uint32_t top = 0;      // of the finite ones: infinities and NaN stay what they are
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t a = __float_as_uint(v[i]) & 0x7fffffffu;
-        top = max(top, a < 0x7f800000u ? a : 0u);
-      }
-#pragma unroll
-      for (int o = 1; o < 4; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const int up = min(127, 14 + 127 - static_cast<int>(top >> 23));    // >= -113
-      const float f = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const __half2 q = __floats2half2_rn(v[2 * i] * f, v[2 * i + 1] * f);
-        h[i] = *reinterpret_cast<const uint32_t*>(&q);
-      }
-      back = __uint_as_float(static_cast<uint32_t>(141 - up) << 23) * 0x1p-23f;      // 2^(-up - kUnits): 141 - up is 14 .. 254
+      for (int i = 0; i < 8; ++i) v[i] = k + i < p.K ? __bfloat162float(row[k + i]) : 0.f;
     }
+    uint32_t top = 0;      // of the finite ones: infinities and NaN stay what they are
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t a = __float_as_uint(v[i]) & 0x7fffffffu;
+      top = max(top, a < 0x7f800000u ? a : 0u);
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const int up = min(127, 14 + 127 - static_cast<int>(top >> 23));    // >= -113
+    const float f = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __half2 q = __floats2half2_rn(v[2 * i] * f, v[2 * i + 1] * f);
+      h[i] = *reinterpret_cast<const uint32_t*>(&q);
+    }
+    const float back = __uint_as_float(static_cast<uint32_t>(141 - up) << 23) * 0x1p-23f;      // 2^(-up - kUnits): 141 - up is 14 .. 254
     *reinterpret_cast<uint4*>(tok + m * pitch16 + c) = make_uint4(h[0], h[1], h[2], h[3]);
     if ((lane & 3) == 0) tok_scale[(c >> 5) * tokens + m] = back;
   }
