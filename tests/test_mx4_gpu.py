@@ -236,6 +236,23 @@ def test_views(cuda, M, N, gap, off):
     assert (out[:, :5] == 7).all() and (out[:, 5 + N:] == 7).all()
 
 
+@pytest.mark.parametrize("N, K, four", [(200, 288, False), (70000, 288, False), (200, 288, True)])
+def test_one_row_of_any_stride(cuda, N, K, four):
+    """a single row, whose stride means nothing, as it comes out of a transposed column"""
+    from vila_b200 import ops
+    q, w = weight(34, N, K, cuda)
+    x, out = torch.empty(K, 1, dtype=BF, device=cuda).T, torch.full((N, 1), 7.0, dtype=BF, device=cuda)
+    row = rand(35, 1, K).to(BF)
+    x.copy_(row)
+    assert x.stride(0) == 1 and out.T.stride(0) == 1
+    if four:
+        ops.mx4_matmul(ops.mx4_quantize(x), q, out=out.T)
+        row = R.values(*R.quantise(row), K)
+    else:
+        ops.mx4_linear(x, q, out=out.T)
+    check_product(out.T, row, w, None)
+
+
 @pytest.mark.parametrize("M, N", [(3, 200), (40, 200), (3, 70000), (60, 9000), (700, 5000)])
 def test_broadcast_rows(cuda, M, N):
     from vila_b200 import ops

@@ -59,7 +59,7 @@ int mx4_linear(const vila_mx4_linear_params& p, cudaStream_t stream, int tries) 
   VB_CHECK(on16(p.w_codes) && on16(p.w_scales) && on16(p.a_codes) && on16(p.a_scales), "mx4_linear: codes and scales start on 16-byte boundaries");
   VB_CHECK(reinterpret_cast<uintptr_t>(p.x) % 2 == 0 && reinterpret_cast<uintptr_t>(p.out) % 2 == 0 && reinterpret_cast<uintptr_t>(p.bias) % 2 == 0,
            "mx4_linear: x, out or bias off its elements' boundaries");
-  VB_CHECK(p.ldo >= (gated ? p.N / 2 : p.N), "mx4_linear: ldo=%lld N=%d", static_cast<long long>(p.ldo), p.N);
+  VB_CHECK(p.M == 1 || p.ldo >= (gated ? p.N / 2 : p.N), "mx4_linear: ldo=%lld N=%d", static_cast<long long>(p.ldo), p.N);
   vila_glinear_ext ext = {};
   ext.act_alpha = p.act_alpha;
   ext.act_limit = p.act_limit;
