@@ -61,8 +61,11 @@ __device__ __forceinline__ uint32_t mx4_encode8(const float (&v)[8]) {
   return d;
 }
 
-// A warp's wait on an mbarrier that no lane leaves before the others: the warps that issue tcgen05 instructions stay converged but for
-// the one branch in which a lane issues them, which takes less time than issuing from a lane on its own (8192 x 8192 x 8192 in 4 bits: 186 us and 254).
+// A warp's wait on an mbarrier: every lane asks, and none leaves before the others.  Both are needed.  What a phase's end makes visible (bytes that
+// TMA wrote, sums in TMEM) it makes visible to the lane that saw it, so that a lane which reads such bytes has to have asked itself.  And tcgen05's
+// .sync.aligned instructions behind the wait are undefined for a warp that has parted, as it has where one lane polls in a loop of its own.
+// Warps that issue tcgen05 instructions stay converged but for the one branch in which a lane issues them, which also takes less time than
+// issuing from a lane on its own (8192 x 8192 x 8192 in 4 bits: 186 us and 254).
 __device__ __forceinline__ bool mx4_warp_wait(uint64_t* bar, uint32_t parity, volatile int* gave_up, int tries) {
   for (int i = 0; i < tries; ++i) {
     if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
