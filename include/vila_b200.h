@@ -907,7 +907,8 @@ int vila_scaled_residual_norm_rows(float* x, const void* a, int a_dtype, int64_t
  *   scales  plain [rows, blocks], or tiled, the order that the products read:
  *           [ceil(rows / 128)][2 * ceil(cols / 256)][32][4][4] bytes; row r, block j is at [r / 128][j / 4][r % 32][r / 32 % 4][j % 4],
  *           rows and blocks past the last ones are 0
- * Both start on 16-byte boundaries.  Unless it says plain, scales are tiled below.
+ * Both start on 16-byte boundaries.  Unless it says plain, scales are tiled below.  Scale bytes 253 and 254 (quantisation makes none) can bring a
+ * number to 2^128 or more, beyond bf16's range and fp32's: read back it is an infinity, and in a product it may count as one.
  *
  * vila_mx4_quantize: x [rows, cols] (VILA_DT_*, row stride ldx elements) -> codes, scales.  Per block with largest magnitude m:
  *   b = max(floor(log2 m) - 2 + 127, 0), code = x / 2^(b - 127) rounded to the nearest number, ties to the even code, +-6 beyond

@@ -836,6 +836,25 @@ def test_rows_that_stay_as_they_are(cuda, M, N, keep, K):
             ops.linear_any(x.to(cuda), q, swiglu=True)
 
 
+@pytest.mark.parametrize("M", [1, 12, 300])
+def test_rows_that_stay_as_they_are_under_views_and_broadcast_rows(cuda, M):
+    from vila_b200 import ops
+    N, K, keep = 200, 288, 24
+    w = (rand(1, N, K) / math.sqrt(K)).to(BF)
+    q = ops.mx4_quantize(w.to(cuda), keep=keep)
+    both = ops.mx4_dequantize(q)
+    for gap, off in ((8, 0), (3, 0), (8, 1), (0, 2), (8, 8)):
+        wide = rand(2, M, K + gap + off).to(BF).to(cuda)
+        check_product(ops.mx4_linear(wide[:, off:off + K], q), wide[:, off:off + K], both, None)
+    one = rand(3, 1, K).to(BF).to(cuda).expand(M, K)
+    check_product(ops.linear_any(one, q), one, both, None)
+    if M == 1:
+        column, out = torch.empty(K, 1, dtype=BF, device=cuda), torch.empty(N, 1, dtype=BF, device=cuda)
+        column.copy_(one.T)
+        check_product(ops.mx4_linear(column.T, q, out=out.T), one, both, None)
+        assert out.any()
+
+
 def test_rows_kept_in_bf16_are_refused_where_codes_are_read(cuda):
     from vila_b200 import ops
     w = rand(1, 64, 64).to(BF).to(cuda)

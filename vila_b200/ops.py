@@ -709,18 +709,12 @@ def linear_any(x: torch.Tensor, w: torch.Tensor, *, swiglu: bool = False, out_dt
         if out_dtype not in (None, torch.bfloat16):
             raise RuntimeError(f"vila_b200.ops: a linear layer on 4-bit weights gives bfloat16, not {out_dtype}")
         return mx4_linear(x, w, bias, act=act, act_params=act_params, swiglu=swiglu, geglu=geglu, glu_clamp=glu_clamp)
-    return _linear_rows(x, w, None, swiglu=swiglu, out_dtype=out_dtype, bias=bias, act=act, act_params=act_params, glu_clamp=glu_clamp, geglu=geglu)
-
-
-def _linear_rows(x, w, out, *, swiglu=False, out_dtype=None, bias=None, act=ACT_NONE, act_params=None, glu_clamp=None, geglu=False) -> torch.Tensor:
-    """linear_any on a plain weight, into `out` (columns of a wider tensor, say) if there is one"""
     N, K = w.shape
     if (x.dtype == torch.bfloat16 and w.dtype == torch.bfloat16 and out_dtype in (None, torch.bfloat16)
             and K % 8 == 0 and N % 8 == 0 and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0
-            and (out is None or (out.stride(0) % 8 == 0 and out.data_ptr() % 16 == 0))
             and (not (swiglu or glu_clamp or geglu) or N % 32 == 0)):
-        return linear(x, w, bias, act=act, swiglu=swiglu, static_w=True, act_params=act_params, glu_clamp=glu_clamp, geglu=geglu, out=out)
-    return glinear(x, w, out=out, swiglu=swiglu, out_dtype=out_dtype, bias=bias, act=act, act_params=act_params, glu_clamp=glu_clamp,
+        return linear(x, w, bias, act=act, swiglu=swiglu, static_w=True, act_params=act_params, glu_clamp=glu_clamp, geglu=geglu)
+    return glinear(x, w, swiglu=swiglu, out_dtype=out_dtype, bias=bias, act=act, act_params=act_params, glu_clamp=glu_clamp,
                    geglu=geglu)
 
 
@@ -1455,11 +1449,12 @@ def _mx4_product(x: Optional[torch.Tensor], a: Optional[Mx4], M: int, K: int, w:
         _mx4_check(not flags or (n % 2 == 0 and N % 2 == 0), "a gated unit has an even number of weight rows, in 4 bits and kept")
         cut = n // 2 if flags else n
         _mx4_product(x, None, M, K, w.part, None if bias is None else bias[:n], act, act_params, swiglu, geglu, glu_clamp, out[:, :cut])
-        rest = None if bias is None else bias[n:]
-        if act == ACT_NONE and not flags:
-            _linear_rows(x, w.kept, out[:, cut:], bias=rest)
-        else:      # rounds once, behind the activation, as the 4-bit rows' kernels do; linear rounds before it, too
-            glinear(x, w.kept, out=out[:, cut:], bias=rest, act=act, act_params=act_params, swiglu=swiglu, geglu=geglu, glu_clamp=glu_clamp)
+        kept, rest, to = w.kept, None if bias is None else bias[n:], out[:, cut:]
+        if (act == ACT_NONE and not flags and K % 8 == 0 and (N - n) % 8 == 0 and x.stride(0) % 8 == 0 and x.stride(0) >= K
+                and x.data_ptr() % 16 == 0 and to.stride(0) % 8 == 0 and to.data_ptr() % 16 == 0):
+            linear(x, kept, rest, static_w=True, out=to)
+        else:      # with an activation: glinear rounds once, behind it, as the 4-bit rows' kernels do; linear rounds before it, too
+            glinear(x, kept, out=to, bias=rest, act=act, act_params=act_params, swiglu=swiglu, geglu=geglu, glu_clamp=glu_clamp)
         return out
     alpha, limit = glu_clamp if glu_clamp is not None else (0.0, 0.0)
     pos, neg = act_params if act_params is not None else (0.0, 0.0)
