@@ -279,6 +279,7 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant_
             } else {
               const int m = (q0 + c) / kPieceRows;
               if (!isfinite(v) && row < p.N) v = sum_again(static_cast<const __nv_bfloat16*>(p.x) + static_cast<size_t>(m) * p.ldx, p.w_codes, p.w_scales, row, p.K);
+              __syncwarp();      // the next TMEM load needs the whole warp
               mx4_store_one<EPI>(p, x, v, m, row, bias);
             }
           } else {
@@ -347,6 +348,7 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant_
           if (n + j < p.N) out[o + n + j] = __float2bfloat16_rn(activate(z[j], p.act, x));
       }
     }
+    __syncwarp();
     cluster_sync_all();      // the others still read this CTA's parts
   }
   if (tid == 0 && *gave_up) {
