@@ -948,6 +948,62 @@ int vila_mx4_linear(const vila_mx4_linear_params* p, void* stream);
  * of the second CTA alone).  vila_wait_status speaks for it. */
 int vila_mx4_linear_tries(const vila_mx4_linear_params* p, int tries, void* stream);
 
+/* ---- 8-bit floating point rows with a scale per block of 128 ----
+ * An element is an e4m3 number (sign, four exponent bits, three mantissa bits, at most 448) times the fp32 scale of its block.  A block is 128
+ * columns (the last one may be shorter) of one row (block_rows 1: activations) or of 128 rows (block_rows 128: weights; the last rows' blocks
+ * may be shorter).
+ *   codes   bytes, rows `ldc` bytes apart (a multiple of 16, at least cols; no matter beyond cols), on a 16-byte boundary
+ *   scales  block_rows 1:   [ceil(cols / 128)][lds], a block column's rows beside one another; lds a multiple of 4, at least rows; on a
+ *                           16-byte boundary
+ *           block_rows 128: [ceil(rows / 128)][lds], lds at least ceil(cols / 128)
+ *
+ * vila_fp8_quantize: x [rows, cols] (VILA_DT_*, row stride ldx elements) -> codes, scales.  Per block with largest magnitude m: scale =
+ *   max(m / 448, 2^-126), code = x * (1 / scale) rounded to the nearest e4m3 number, ties to even (quotients and product rounded to fp32).  A
+ *   block with an infinity or a NaN: a NaN for its scale, codes 0.
+ * vila_fp8_dequantize: out[r, c] = number of the code * scale, rounded once to out_dtype (code 0x7f or 0xff: NaN).
+ * vila_fp8_rmsnorm: the norm before a layer whose rows are 8-bit numbers.  s = x + residual, rounded to x's type (residual NULL: s = x); codes
+ *   and scales (block_rows 1) of s / sqrt(mean(s^2) + eps) * w, unrounded fp32 (w NULL: 1).  With a residual s is written to sum (x's type, row
+ *   stride ld_sum; it may be x itself, in place).  At most 32768 columns. */
+int vila_fp8_quantize(const void* x, int x_dtype, int64_t ldx, void* codes, int64_t ldc, float* scales, int64_t lds, int rows, int cols,
+                      int block_rows, void* stream);
+int vila_fp8_dequantize(const void* codes, int64_t ldc, const float* scales, int64_t lds, void* out, int out_dtype, int64_t ldo, int rows,
+                        int cols, int block_rows, void* stream);
+int vila_fp8_rmsnorm(const void* x, int x_dtype, int64_t ldx, const void* residual, int residual_dtype, int64_t ldr, void* sum,
+                     int64_t ld_sum, const void* w, int w_dtype, float eps, void* codes, int64_t ldc, float* scales, int64_t lds, int rows,
+                     int cols, void* stream);
+/* vila_fp8_linear: out[m, n] = epi(sum_k a[m, k] w[n, k] + bias[n]), a [M, K] with block_rows 1, w [N, K] with block_rows 128.  Products of a
+ * block's numbers and their sum in fp32, times the product of both scales (fp32, cut at fp32's largest number), added in fp32 in the order of the
+ * blocks (K over a cluster: each CTA's, then the CTAs').  Scales are finite, not negative, or NaN.  bias bf16 or NULL.  act, flags and their parameters as in
+ * vila_mx4_linear; with a gated unit the result has N / 2 columns.  The result goes to out in bf16 (row stride ldo), or, with out NULL,
+ * unrounded to o_codes and o_scales (block_rows 1). */
+typedef struct vila_fp8_linear_params {
+  const void* a_codes;
+  int64_t lda;
+  const float* a_scales;
+  int64_t ld_as;
+  const void* w_codes;
+  int64_t ldw;
+  const float* w_scales;
+  int64_t ld_ws;
+  const void* bias;
+  void* out;
+  int64_t ldo;
+  void* o_codes;
+  int64_t ld_oc;
+  float* o_scales;
+  int64_t ld_os;
+  float act_alpha, act_limit, act_pos, act_neg;
+  int32_t M, N, K, act, flags;
+  void* scratch;
+  int64_t scratch_bytes;
+} vila_fp8_linear_params;
+/* Bytes of scratch (on a 16-byte boundary, of this call alone until it has run) that vila_fp8_linear needs; 0: none. */
+int64_t vila_fp8_linear_scratch(const vila_fp8_linear_params* p);
+int vila_fp8_linear(const vila_fp8_linear_params* p, void* stream);
+/* vila_fp8_linear with waits that end after `tries` tries (test hook, as vila_mx4_linear_tries; there is no role 2).  vila_wait_status speaks
+ * for it. */
+int vila_fp8_linear_tries(const vila_fp8_linear_params* p, int tries, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,499 @@
+"""GPU: 8-bit rows with a scale per block of 128 against their restatement in float64."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+from tests import fp8_reference as R
+from tests.test_mx4_gpu import act64, act_args, check_product
+
+pytestmark = pytest.mark.gpu
+BF, E4M3 = torch.bfloat16, torch.float8_e4m3fn
+
+
+def rand(seed, *shape, dtype=torch.float32):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+def same(q, x, block_rows=1):
+    """q is the 8-bit form of x, bit by bit"""
+    codes, scales = R.quantise(x, block_rows)
+    assert q.shape == tuple(x.shape) and q.codes.dtype == E4M3 and q.scales.dtype == torch.float32 and q.scales.shape == scales.shape
+    assert torch.equal(q.codes.cpu().double(), codes)
+    assert torch.equal(q.scales.cpu().nan_to_num(-1.0), scales.nan_to_num(-1.0))
+
+
+# ---- quantisation: bit by bit -------------------------------------------------------------------------
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+@pytest.mark.parametrize("rows, cols", [(1, 1), (1, 15), (1, 16), (3, 17), (2, 127), (129, 128), (5, 129), (130, 1000), (257, 256), (7, 3584), (300, 401)])
+def test_quantise_is_the_definition(cuda, rows, cols, dtype, block_rows):
+    from vila_b200 import ops
+    x = (rand(1, rows, cols) * torch.exp(2 * rand(2, 1, cols))).to(dtype)
+    q = ops.fp8_quantize(x.to(cuda), block_rows=block_rows)
+    same(q, x, block_rows)
+    want = R.values(*R.quantise(x, block_rows), block_rows)
+    assert torch.equal(ops.fp8_dequantize(q, out_dtype=torch.float32).cpu(), want.float())      # one rounding of the product
+    assert torch.equal(ops.fp8_dequantize(q).cpu(), want.float().to(BF))
+
+
+def test_every_number_comes_back(cuda):
+    from vila_b200 import ops
+    codes = torch.arange(256, dtype=torch.uint8).view(E4M3).view(2, 128)
+    q = ops.fp8_pack(codes.to(cuda), torch.tensor([[1.0], [2.0]], device=cuda), block_rows=1)
+    got = ops.fp8_dequantize(q, out_dtype=torch.float32).cpu()
+    want = codes.float() * torch.tensor([[1.0], [2.0]])
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(7.0), want.nan_to_num(7.0))
+
+
+@pytest.mark.parametrize("block_rows", [1, 128])
+def test_quantise_edges(cuda, block_rows):
+    from vila_b200 import ops
+    x = torch.zeros(12 * block_rows, 256)
+    at = x[::block_rows]
+    ties = torch.tensor([448.0, 17.0, 19.0, -17.0, -19.0, 2.0 ** -10, 3 * 2.0 ** -10, -0.0, 0.0, 447.9, 432.0, 440.0, 1.0625, -1.1875])
+    at[0, :14] = ties
+    at[1, :14] = ties * 2.0 ** 100
+    at[2, :14] = ties * 2.0 ** -120
+    at[3, :4] = torch.tensor([2.0 ** -149, 2.0 ** -140, 0.0, -(2.0 ** -130)])        # fp32 subnormals
+    at[4, 128:132] = torch.tensor([3.4028234e38, -3.4028234e38, 1e38, 1.0])
+    at[5, 3] = math.inf
+    at[6, 140] = math.nan
+    at[7, 3], at[7, 4] = math.nan, -math.inf
+    at[8] = 6.0
+    at[9, 0] = 2.0 ** -126 * 448
+    at[10, 0] = 2.0 ** -125 * 448
+    at[11] = -1e-45
+    q = ops.fp8_quantize(x.to(cuda), block_rows=block_rows)
+    same(q, x, block_rows)
+    back = ops.fp8_dequantize(q, out_dtype=torch.float32).cpu()[::block_rows]
+    assert back[5, :128].isnan().all() and not back[5, 128:].isnan().any() and back[6, 128:].isnan().all() and back[7, :128].isnan().all()
+    assert back.isnan().sum() == 3 * 128
+
+
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+@pytest.mark.parametrize("gap, off", [(16, 0), (8, 0), (3, 0), (8, 1), (0, 3), (8, 8)])
+def test_quantise_views(cuda, gap, off, dtype, block_rows):
+    from vila_b200 import ops
+    wide = rand(3, 140, 300 + gap + off).to(dtype)
+    same(ops.fp8_quantize(wide.to(cuda)[:, off:off + 300], block_rows=block_rows), wide[:, off:off + 300], block_rows)
+
+
+def test_quantise_broadcast_rows_one_column_and_no_rows(cuda):
+    from vila_b200 import ops
+    x = rand(4, 1, 96)
+    for block_rows in (1, 128):
+        same(ops.fp8_quantize(x.to(cuda).expand(5, 96), block_rows=block_rows), x.expand(5, 96), block_rows)
+        same(ops.fp8_quantize(rand(5, 7, 9).to(cuda)[:, 4:5], block_rows=block_rows), rand(5, 7, 9)[:, 4:5], block_rows)
+        none = ops.fp8_quantize(torch.empty(0, 96, device=cuda), block_rows=block_rows)
+        assert none.shape == (0, 96) and none.codes.shape == (0, 96) and none.scales.shape == (0, 1) and ops.fp8_dequantize(none).shape == (0, 96)
+
+
+def test_pack_keeps_what_lies_well_and_copies_the_rest(cuda):
+    from vila_b200 import ops
+    codes, scales = (rand(6, 200, 288) * 50).to(E4M3).to(cuda), rand(7, 2, 3).abs().to(cuda)
+    want = R.values(codes.cpu().double(), scales.cpu(), 128).float()
+    q = ops.fp8_pack(codes, scales)
+    assert q.codes.data_ptr() == codes.data_ptr() and q.scales.data_ptr() == scales.data_ptr()
+    odd = codes.new_empty(200, 291)
+    odd[:, 2:290] = codes
+    inner = codes.new_empty(200, 320)
+    inner[:, 16:304] = codes
+    for c, s, kept in ((odd[:, 2:290], scales, False), (codes.T.contiguous().T, scales, False), (codes, scales.T.contiguous().T, False),
+                       (inner[:, 16:304], scales, True)):
+        q = ops.fp8_pack(c, s)
+        assert (q.codes.data_ptr() == c.data_ptr()) == kept
+        assert torch.equal(ops.fp8_dequantize(q, out_dtype=torch.float32).cpu(), want)
+    rows = rand(8, 200, 3).abs().to(cuda)       # a scale per row
+    q = ops.fp8_pack(codes, rows, block_rows=1)
+    assert torch.equal(q.scales, rows) and torch.equal(ops.fp8_dequantize(q, out_dtype=torch.float32).cpu(), R.values(codes.cpu().double(), rows.cpu(), 1).float())
+    again = ops.fp8_pack(q.codes, q.scales, block_rows=1)
+    assert again.scales.data_ptr() == q.scales.data_ptr() and again.codes.data_ptr() == q.codes.data_ptr()
+
+
+# ---- the norm ----------------------------------------------------------------------------------------------
+def check_norm(q, x, w, eps):
+    """q against quantise(x / sqrt(mean(x^2) + eps) * w) in float64.  The sum of squares: a thread adds at most 64 squares one after another
+    and 10 sums join, each rounded (2^-24): 75 roundings, half of that behind the root; mean, eps, root, reciprocal, two products and
+    the format's quotients and product: 9 more.  d = 48 * 2^-24 relative.  Then the number: half a step, 2^-4 of it, or of those below
+    2^-6 2^-10, in units of the scale."""
+    x = x.double().cpu()
+    y = x / torch.sqrt((x * x).mean(1, keepdim=True) + eps)
+    if w is not None:
+        y = y * w.double().cpu()
+    d = 48 * 2.0 ** -24
+    top = torch.from_numpy(abs(R.blocks(y.numpy(), 1)).max((1, 3)))
+    scales = q.scales.cpu().double()
+    want = (top / 448).clamp(min=2.0 ** -126)
+    assert scales.shape == want.shape and ((scales - want).abs() <= want * (d + 2.0 ** -23)).all()
+    s = R.per_element(scales, 1, *y.shape)
+    v = q.codes.cpu().double() * s
+    assert ((v - y).abs() <= torch.maximum(v.abs() * 2.0 ** -4, s * 2.0 ** -10) * (1 + 2 * d) + y.abs() * d).all()
+
+
+@pytest.mark.parametrize("dtype, r_dtype, w_dtype", [(BF, BF, BF), (torch.float32, BF, torch.float32), (BF, torch.float32, None), (torch.float32, torch.float32, BF)])
+@pytest.mark.parametrize("rows, cols", [(1, 1), (1, 3584), (3, 17), (70, 128), (5, 1153), (9, 4301), (2, 8192), (2, 8209), (2, 16384), (3, 18944), (2, 32768)])
+def test_norm(cuda, rows, cols, dtype, r_dtype, w_dtype):
+    from vila_b200 import ops
+    x, r = (3 * rand(10, rows, cols) * torch.exp(rand(11, 1, cols))).to(dtype), rand(12, rows, cols).to(r_dtype)
+    w = None if w_dtype is None else (1 + 0.2 * rand(13, cols)).to(w_dtype)
+    xc, rc, wc = x.to(cuda), r.to(cuda), None if w is None else w.to(cuda)
+    q, s = ops.fp8_rmsnorm(xc, wc, 1e-6)
+    assert s is xc and torch.equal(xc.cpu(), x)
+    check_norm(q, x, w, 1e-6)
+    total = (x.float() + r.float()).to(dtype)
+    q, s = ops.fp8_rmsnorm(xc, wc, 1e-6, residual=rc)
+    assert torch.equal(s.cpu(), total) and torch.equal(xc.cpu(), x) and torch.equal(rc.cpu(), r)
+    check_norm(q, total, w, 1e-6)
+    same_codes, same_scales = q.codes.clone(), q.scales.clone()
+    q, s = ops.fp8_rmsnorm(xc, wc, 1e-6, residual=rc, out=xc)
+    assert s is xc and torch.equal(xc.cpu(), total) and torch.equal(q.codes.float(), same_codes.float()) and torch.equal(q.scales, same_scales)
+
+
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+@pytest.mark.parametrize("gap, off", [(16, 0), (8, 8), (3, 0), (0, 1)])
+def test_norm_of_views(cuda, gap, off, dtype):
+    from vila_b200 import ops
+    cols = 520
+    wide, more, w = rand(14, 33, cols + gap + off).to(dtype), rand(15, 33, cols + gap + off).to(BF), rand(16, cols + 1).to(BF)
+    out = torch.full((33, cols + gap + off + 2), 7.0, dtype=dtype, device=cuda)
+    view = slice(off, off + cols)
+    q, s = ops.fp8_rmsnorm(wide.to(cuda)[:, view], w.to(cuda)[1:], 1e-5, residual=more.to(cuda)[:, view], out=out[:, 1:1 + cols])
+    total = (wide[:, view].float() + more[:, view].float()).to(dtype)
+    assert torch.equal(s.cpu(), total) and s.data_ptr() == out[:, 1:].data_ptr() and (out[:, :1] == 7).all() and (out[:, 1 + cols:] == 7).all()
+    check_norm(q, total, w[1:], 1e-5)
+    one = rand(17, 1, cols).to(dtype)
+    check_norm(ops.fp8_rmsnorm(one.to(cuda).expand(6, cols), None, 1e-5)[0], one.expand(6, cols), None, 1e-5)
+
+
+def test_norm_of_zeros_infinities_and_nan(cuda):
+    from vila_b200 import ops
+    x = rand(18, 5, 300)
+    x[0] = 0
+    x[1, 200] = math.nan
+    x[2, 5] = math.inf
+    x[3] = 0
+    x[3, 299] = 1e-30
+    q, _ = ops.fp8_rmsnorm(x.to(cuda), None, 0.0)
+    back = ops.fp8_dequantize(q, out_dtype=torch.float32).cpu()
+    assert back[0].isnan().all() and back[1].isnan().all()              # 0 / 0 with eps = 0, as the formula has it
+    assert back[2, :128].isnan().all() and (back[2, 128:] == 0).all()   # infinity / infinity, and what is divided by infinity
+    check_norm(ops.fp8_rmsnorm(x[4:].to(cuda), None, 0.0)[0], x[4:], None, 0.0)
+    zero = ops.fp8_rmsnorm(torch.zeros(3, 200, device=cuda), None, 1e-6)[0]
+    assert (ops.fp8_dequantize(zero) == 0).all() and (zero.scales == 2.0 ** -126).all()
+    assert ops.fp8_rmsnorm(torch.empty(0, 200, device=cuda), None, 1e-6)[0].shape == (0, 200)
+
+
+# ---- products --------------------------------------------------------------------------------------------
+def weight(seed, n, k, cuda, spread=0.0):
+    from vila_b200 import ops
+    w = rand(seed, n, k) / math.sqrt(k) * torch.exp(spread * rand(seed + 1, n, 1))
+    codes, scales = R.quantise(w, 128)
+    return ops.fp8_pack(codes.to(E4M3).to(cuda), scales.to(cuda)), R.values(codes, scales, 128)
+
+
+def rows8(x, cuda):
+    """8-bit rows of x and what they stand for"""
+    from vila_b200 import ops
+    codes, scales = R.quantise(x, 1)
+    return ops.fp8_pack(codes.to(E4M3).to(cuda), scales.to(cuda), block_rows=1), R.values(codes, scales, 1)
+
+
+def check_rows8(q, x, w, bias, act="none"):
+    """q (Fp8) against quantise(act(x w^T + bias)) in float64: check_product's bound for the sums and the activation (without the
+    rounding to bf16), then the format's own half step."""
+    x, w = x.double().cpu(), w.double().cpu()
+    z, S = x @ w.T, x.abs() @ w.abs().T
+    if bias is not None:
+        z, S = z + bias.double().cpu(), S + bias.double().cpu().abs()
+    dz = S * ((x.shape[1] / 16 + 8) * 2.0 ** -22)
+    want = act64(z, act)
+    off = torch.zeros_like(want)
+    even = torch.zeros_like(dz)
+    even[:, 0::2] = dz[:, 0::2]
+    for a in (1, -1):
+        for b in (1, -1):
+            off = torch.maximum(off, (act64(z + a * even + b * (dz - even), act) - want).abs())
+    off = 2 * off + want.abs() * 2.0 ** -20
+    if act in ("gelu_tanh", "gelu_erf"):
+        off = off + z.abs() * 2.0 ** -22
+    elif act in ("geglu", "glu_clamp"):
+        off = off + z[:, 0::2].abs() * (z[:, 1::2].abs() + 1) * 2.0 ** -22
+    top, most = (torch.from_numpy(abs(R.blocks(t.numpy(), 1)).max((1, 3))) for t in (want, off))
+    scales = q.scales.cpu().double()
+    assert q.shape == tuple(want.shape) and ((scales - (top / 448).clamp(min=2.0 ** -126)).abs() <= most / 448 + top / 448 * 2.0 ** -23).all()
+    s = R.per_element(scales, 1, *want.shape)
+    v = q.codes.cpu().double() * s
+    assert ((v - want).abs() <= torch.maximum(v.abs() * 2.0 ** -4, s * 2.0 ** -10) * (1 + 2.0 ** -20) + off).all()
+
+
+SIZES = [(1, 2, 32), (1, 128, 64), (1, 300, 2048), (3, 129, 95), (7, 64, 1153), (8, 1000, 512), (9, 130, 4000), (16, 256, 1024),
+         (17, 384, 300), (33, 128, 640), (64, 514, 1000), (65, 1157, 1153), (100, 640, 256), (129, 300, 2080), (200, 130, 96), (300, 770, 520),
+         (520, 258, 1056), (2600, 2570, 800), (1, 40000, 130), (40, 20000, 257), (31, 258, 20000)]
+
+
+@pytest.mark.parametrize("M, N, K", SIZES)
+def test_linear(cuda, M, N, K):
+    from vila_b200 import ops
+    q, w = weight(M, N, K, cuda, spread=1.0)
+    a, x = rows8(rand(7, M, K) * torch.exp(rand(8, 1, K)), cuda)
+    bias = rand(9, N).to(BF)
+    check_product(ops.fp8_linear(a, q), x, w, None)
+    check_product(ops.fp8_linear(a, q, bias.to(cuda)), x, w, bias)
+    check_rows8(ops.fp8_linear(a, q, bias.to(cuda), to8=True), x, w, bias)
+
+
+@pytest.mark.parametrize("M", [1, 20, 70, 300, 1100])
+@pytest.mark.parametrize("act", ["silu", "relu2", "gelu_tanh", "gelu_erf", "xielu", "swiglu", "geglu", "glu_clamp"])
+def test_activations(cuda, M, act):
+    from vila_b200 import ops
+    q, w = weight(20, 770, 320, cuda)
+    a, x = rows8(2 * rand(21, M, 320), cuda)
+    bias = rand(22, 770).to(BF)
+    check_product(ops.fp8_linear(a, q, bias.to(cuda), **act_args(act)), x, w, bias, act)
+    check_rows8(ops.fp8_linear(a, q, bias.to(cuda), to8=True, **act_args(act)), x, w, bias, act)
+
+
+@pytest.mark.parametrize("act", ["silu", "swiglu"])
+@pytest.mark.parametrize("M", [1, 40, 100])
+def test_activations_behind_a_cluster(cuda, M, act):
+    from vila_b200 import ops
+    q, w = weight(24, 258, 5000, cuda)
+    a, x = rows8(rand(25, M, 5000), cuda)
+    check_product(ops.fp8_linear(a, q, **act_args(act)), x, w, None, act)
+    check_rows8(ops.fp8_linear(a, q, to8=True, **act_args(act)), x, w, None, act)
+
+
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+@pytest.mark.parametrize("M", [1, 40, 300])
+def test_rows_as_they_come(cuda, M, dtype):
+    from vila_b200 import ops
+    q, w = weight(26, 200, 300, cuda)
+    wide = rand(27, M, 311).to(dtype)
+    check_product(ops.fp8_linear(wide.to(cuda)[:, 3:303], q), R.values(*R.quantise(wide[:, 3:303])), w, None)
+
+
+@pytest.mark.parametrize("M, N", [(2, 200), (40, 200), (300, 200), (2, 40000), (700, 5000)])
+def test_views(cuda, M, N):
+    from vila_b200 import ops
+    q, w = weight(30, N, 288, cuda)
+    a, x = rows8(rand(31, M, 288), cuda)
+    out = torch.full((M, N + 11), 7.0, dtype=BF, device=cuda)
+    got = ops.fp8_linear(a, q, out=out[:, 5:5 + N])
+    assert got.data_ptr() == out[:, 5:].data_ptr()
+    check_product(got, x, w, None)
+    assert (out[:, :5] == 7).all() and (out[:, 5 + N:] == 7).all()
+    # codes of rows inside wider ones, with numbers beside them that must not count; scales of more rows than there are
+    wide = torch.full((M, 320), 448.0).to(E4M3).to(cuda)
+    wide[:, 16:304] = a.codes
+    scales = torch.full((3, M + 13 - (M + 1) % 4), math.nan, device=cuda)
+    scales = scales[:, :scales.shape[1] // 4 * 4].contiguous()
+    scales[:, :M] = a.scales.T
+    b = ops.Fp8(wide[:, 16:304], scales[:, :M].T, 1)
+    assert b._lds >= M and b._ldc == 320
+    check_product(ops.fp8_linear(b, q), x, w, None)
+    row = torch.full((N, 1), 7.0, dtype=BF, device=cuda)
+    check_product(ops.fp8_linear(rows8(rand(31, M, 288)[:1], cuda)[0], q, out=row.T), x[:1], w, None)
+
+
+@pytest.mark.parametrize("M, N", [(1, 300), (12, 300), (40, 300), (100, 300), (300, 300), (700, 5000)])
+def test_scales_over_the_whole_range(cuda, M, N):
+    """Blocks of one row whose sizes are 2^40 apart, rows that differ by 2^60; and blocks of zeros under the largest scales."""
+    from vila_b200 import ops
+    K = 1024
+    sizes = torch.tensor([2.0 ** -20, 2.0 ** 20, 1.0, 2.0 ** -5]).repeat_interleave(128).repeat(K // 512)
+    block_rows = torch.exp2(torch.arange(N).float() // 128 % 5 * 15 - 30)
+    codes, scales = R.quantise(rand(40, N, K) * sizes * block_rows[:, None], 128)
+    a_codes, a_scales = R.quantise(rand(41, M, K) / sizes * torch.exp2(torch.arange(M).float() % 41 - 20)[:, None])
+    codes[:, 256:384] = 0
+    scales[:, 2] = 3e38
+    a_codes[:, 640:768] = 0
+    a_scales[:, 5] = 3e38
+    a_scales[:, 2] = a_scales[:, 2].clamp(max=448.0 * 1e3)
+    scales[:, 5] = scales[:, 5].clamp(max=448.0 * 1e3)
+    q, a = ops.fp8_pack(codes.to(E4M3).to(cuda), scales.to(cuda)), ops.fp8_pack(a_codes.to(E4M3).to(cuda), a_scales.to(cuda), block_rows=1)
+    check_product(ops.fp8_linear(a, q), R.values(a_codes, a_scales), R.values(codes, scales, 128), None)
+
+
+@pytest.mark.parametrize("to8", [False, True])
+@pytest.mark.parametrize("M, N, K", [(1, 300, 700), (40, 300, 700), (300, 300, 700), (2, 300, 9000), (700, 5000, 700)])
+def test_nan_blocks(cuda, M, N, K, to8):
+    """A row with an infinity reads as NaN, as does a weight row's output with a NaN code (in 8 bits: its block); nothing else does."""
+    from vila_b200 import ops
+    x, w = rand(50, M, K), rand(51, N, K) / math.sqrt(K)
+    x[M // 2, K - 1] = math.inf
+    codes, scales = R.quantise(w, 128)
+    codes[N // 3, 5] = math.nan
+    q = ops.fp8_pack(codes.to(E4M3).to(cuda), scales.to(cuda))
+    a = ops.fp8_quantize(x.to(cuda))
+    got = ops.fp8_linear(a, q, to8=to8)
+    bad = (ops.fp8_dequantize(got, out_dtype=torch.float32) if to8 else got).isnan().cpu()
+    want = torch.zeros(M, N, dtype=torch.bool)
+    want[M // 2] = True
+    want[:, N // 3] = True
+    if to8:
+        want[:, N // 3 // 128 * 128:N // 3 // 128 * 128 + 128] = True
+    assert torch.equal(bad, want)
+
+
+def test_sizes_of_nothing_and_gates_of_odd_rows(cuda):
+    from vila_b200 import ops
+    q, _ = weight(60, 65, 64, cuda)
+    none = ops.fp8_quantize(torch.empty(0, 64, device=cuda))
+    assert ops.fp8_linear(none, q).shape == (0, 65) and ops.fp8_linear(none, q, to8=True).shape == (0, 65)
+    a = ops.fp8_quantize(rand(61, 3, 64).to(cuda))
+    with pytest.raises(RuntimeError, match="even number of weight rows"):
+        ops.fp8_linear(a, q, swiglu=True)
+
+
+def test_refusals(cuda):
+    from vila_b200 import _lib, ops
+    q, _ = weight(62, 64, 64, cuda)
+    x = rand(63, 3, 64).to(cuda)
+    a = ops.fp8_quantize(x)
+    for call, text in ((lambda: ops.fp8_linear(a, ops.fp8_quantize(rand(1, 64, 65).to(cuda), block_rows=128)), "do not fit"),
+                       (lambda: ops.fp8_linear(q, q), "a must be Fp8 rows"), (lambda: ops.fp8_linear(a, a), "a must be Fp8 rows"),
+                       (lambda: ops.fp8_linear(a, q, rand(1, 64).to(cuda)), "bias must be torch.bfloat16"),
+                       (lambda: ops.fp8_linear(a, q, rand(1, 63).to(BF).to(cuda)), "bias must be contiguous"),
+                       (lambda: ops.fp8_linear(a, q, act=ops.ACT_SOFTCAP), "unknown activation"),
+                       (lambda: ops.fp8_linear(a, q, act=ops.ACT_XIELU), "takes act_params"),
+                       (lambda: ops.fp8_linear(a, q, swiglu=True, geglu=True), "one gated unit"),
+                       (lambda: ops.fp8_linear(a, q, swiglu=True, act=ops.ACT_SILU), "no other activation"),
+                       (lambda: ops.fp8_linear(a, q, out=torch.empty(3, 63, dtype=BF, device=cuda)), "out must be"),
+                       (lambda: ops.fp8_linear(a, q, out=torch.empty(3, 64, device=cuda)), "out must be torch.bfloat16"),
+                       (lambda: ops.fp8_linear(a, q, to8=True, out=torch.empty(3, 64, dtype=BF, device=cuda)), "takes no out"),
+                       (lambda: ops.fp8_quantize(x, block_rows=64), "1 or 128"), (lambda: ops.fp8_quantize(x.half()), "bfloat16 or float32"),
+                       (lambda: ops.fp8_quantize(x.T), "consecutive columns"), (lambda: ops.fp8_quantize(x[:, :0]), "consecutive columns"),
+                       (lambda: ops.fp8_rmsnorm(x, rand(1, 63).to(cuda), 1e-6), "w must be"),
+                       (lambda: ops.fp8_rmsnorm(x, None, 1e-6, residual=x[:2]), "residual must be"),
+                       (lambda: ops.fp8_rmsnorm(x, None, 1e-6, out=x), "goes with a residual"),
+                       (lambda: ops.fp8_rmsnorm(x, None, 1e-6, residual=x, out=x.to(BF)), "out must be"),
+                       (lambda: ops.fp8_rmsnorm(x, None, -1.0), "eps="),
+                       (lambda: ops.fp8_rmsnorm(x, None, math.nan), "eps="),
+                       (lambda: ops.fp8_rmsnorm(x[:1].expand(3, 64), None, 1e-6, residual=x, out=x[:1].expand(3, 64)), "ld_sum=0"),
+                       (lambda: ops.fp8_rmsnorm(torch.zeros(1, 32769, device=cuda), None, 1e-6), "at most 32768"),
+                       (lambda: ops.fp8_dequantize(a, out_dtype=torch.float16), "bfloat16 or float32")):
+        with pytest.raises(RuntimeError, match=text):
+            call()
+    # the C entries: null pointers, pointers off their boundaries, strides that do not hold a row
+    lib = _lib.load()
+    codes, scales = a._ptrs()
+    good = (x.data_ptr(), 1, 64, codes, 64, scales, 4, 3, 64, 1)
+    for at, bad in ((0, None), (0, x.data_ptr() + 2), (1, 5), (3, None), (3, codes + 8), (4, 56), (4, 48), (5, None), (5, scales + 4), (6, 2), (6, 6), (7, -1), (8, 0), (9, 2)):
+        args = list(good)
+        args[at] = bad
+        assert lib.vila_fp8_quantize(*args, None) == 1, (at, bad)
+    w_codes, w_scales = q._ptrs()
+    out = torch.full((3, 64), 7.0, dtype=BF, device=cuda)
+    fields = dict(a_codes=codes, lda=64, a_scales=scales, ld_as=4, w_codes=w_codes, ldw=64, w_scales=w_scales, ld_ws=1, out=out.data_ptr(), ldo=64, M=3, N=64, K=64)
+    for name, bad in (("a_codes", None), ("a_codes", codes + 8), ("lda", 72), ("lda", 48), ("a_scales", None), ("a_scales", scales + 4), ("ld_as", 3), ("ld_as", 0),
+                      ("w_codes", None), ("w_codes", w_codes + 1), ("ldw", 65), ("w_scales", w_scales + 2), ("ld_ws", 0), ("out", None), ("out", out.data_ptr() + 1),
+                      ("ldo", 63), ("N", 0), ("K", -1), ("M", -1), ("flags", 16), ("bias", out.data_ptr() + 1), ("o_codes", codes)):
+        p = _lib.Fp8LinearParams(**{**fields, name: bad})
+        assert lib.vila_fp8_linear(C.byref(p), None) == 1, (name, bad)
+    p = _lib.Fp8LinearParams(**{**fields, "out": None, "o_codes": codes, "ld_oc": 64, "o_scales": scales, "ld_os": 4})
+    if lib.vila_fp8_linear_scratch(C.byref(p)):
+        assert lib.vila_fp8_linear(C.byref(p), None) == 1      # no workspace
+    torch.cuda.synchronize()
+    assert (out == 7).all()
+
+
+# ---- streams, graphs, waits that run out ---------------------------------------------------------------------
+KERNELS = [(1, 300, 700), (1, 300, 9000), (20, 300, 700), (40, 300, 700), (100, 300, 9000), (300, 770, 520), (1500, 1300, 800)]
+
+
+def test_four_streams_at_once(cuda):
+    from vila_b200 import ops
+    jobs = []
+    for i, (M, N, K) in enumerate(KERNELS):
+        q, w = weight(70 + i, N, K, cuda)
+        a, x = rows8(rand(80 + i, M, K), cuda)
+        jobs.append((a, q, ops.fp8_linear(a, q), ops.fp8_linear(a, q, to8=True)))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    got = []
+    for r in range(3):
+        for i, (a, q, *_) in enumerate(jobs):
+            with torch.cuda.stream(streams[(i + r) % 4]):
+                got.append((i, ops.fp8_linear(a, q), ops.fp8_linear(a, q, to8=True)))
+    torch.cuda.synchronize()
+    for i, y, y8 in got:
+        assert torch.equal(y, jobs[i][2]) and torch.equal(y8.codes.float(), jobs[i][3].codes.float()) and torch.equal(y8.scales, jobs[i][3].scales)
+
+
+@pytest.mark.parametrize("M", [1, 40, 300, 1500])
+def test_captured_layer(cuda, M):
+    """norm, gate / up with a result in 8 bits, down: captured twice, replayed in turn on new rows"""
+    from vila_b200 import ops
+    gu, down = weight(90, 512, 384, cuda)[0], weight(92, 384, 256, cuda)[0]
+    w = rand(93, 384).to(BF).to(cuda)
+    x, r = torch.zeros(M, 384, dtype=BF, device=cuda), torch.zeros(M, 384, dtype=BF, device=cuda)
+
+    def layer():
+        h, s = ops.fp8_rmsnorm(x, w, 1e-6, residual=r)
+        return ops.fp8_linear(ops.fp8_linear(h, gu, swiglu=True, to8=True), down), s
+
+    layer()
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            graphs.append((g, layer()))
+    for i in range(4):
+        x.copy_(rand(94 + i, M, 384).to(BF))
+        r.copy_(rand(104 + i, M, 384).to(BF))
+        want = layer()
+        g, got = graphs[i % 2]
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("tries", [0, 1, -2, -3, -5])
+@pytest.mark.parametrize("M, N, K", KERNELS)
+def test_waits_that_run_out(cuda, monkeypatch, M, N, K, tries):
+    """The launch ends, the next status says so once, and the call after that is right."""
+    from vila_b200 import _lib, ops
+    w = ops.fp8_quantize(rand(1, N, K).to(cuda), block_rows=128)
+    a = ops.fp8_quantize(rand(2, M, K).to(cuda))
+    want = ops.fp8_linear(a, w)
+    torch.cuda.synchronize()
+    ops.check_waits()
+    lib = _lib.load()
+    with monkeypatch.context() as m:
+        m.setattr(lib, "vila_fp8_linear", lambda p, stream: lib.vila_fp8_linear_tries(p, tries, stream))
+        out = ops.fp8_linear(a, w)
+        torch.cuda.synchronize()
+    if tries <= 0 or not torch.equal(out, want):
+        with pytest.raises(RuntimeError, match="ran out of tries"):
+            ops.check_waits()
+    else:
+        try:      # a warp may have given up behind the last wait that its output needs
+            ops.check_waits()
+        except RuntimeError:
+            pass
+    ops.check_waits()
+    assert torch.equal(ops.fp8_linear(a, w), want)
+
+
+# ---- together, as they are used -----------------------------------------------------------------------------
+@pytest.mark.parametrize("M", [1, 12, 40, 300, 1100])
+def test_feed_forward_block(cuda, M):
+    """norm with the residual, gate / up with a gated unit and a result in 8 bits, down, the next norm: each step from what the one before gave"""
+    from vila_b200 import ops
+    gu, gu64 = weight(100, 1024, 384, cuda)
+    down, down64 = weight(102, 384, 512, cuda)
+    x, r, w = rand(104, M, 384).to(BF).to(cuda), rand(105, M, 384).to(BF).to(cuda), (1 + 0.1 * rand(106, 384)).to(BF).to(cuda)
+    h, s = ops.fp8_rmsnorm(x, w, 1e-6, residual=r)
+    check_norm(h, s, w, 1e-6)
+    h64 = R.values(h.codes.cpu(), h.scales.cpu())
+    g = ops.fp8_linear(h, gu, swiglu=True, to8=True)
+    check_rows8(g, h64, gu64, None, "swiglu")
+    y = ops.fp8_linear(g, down)
+    check_product(y, R.values(g.codes.cpu(), g.scales.cpu()), down64, None)
+    n, t = ops.fp8_rmsnorm(s, w, 1e-6, residual=y)
+    assert torch.equal(t, (s.float() + y.float()).to(BF))
+    check_norm(n, t, w, 1e-6)

@@ -132,6 +132,18 @@ class Mx4LinearParams(C.Structure):
     ]
 
 
+class Fp8LinearParams(C.Structure):
+    _fields_ = [
+        ("a_codes", c_void_p), ("lda", c_i64), ("a_scales", c_void_p), ("ld_as", c_i64),
+        ("w_codes", c_void_p), ("ldw", c_i64), ("w_scales", c_void_p), ("ld_ws", c_i64),
+        ("bias", c_void_p), ("out", c_void_p), ("ldo", c_i64),
+        ("o_codes", c_void_p), ("ld_oc", c_i64), ("o_scales", c_void_p), ("ld_os", c_i64),
+        ("act_alpha", c_float), ("act_limit", c_float), ("act_pos", c_float), ("act_neg", c_float),
+        ("M", C.c_int32), ("N", C.c_int32), ("K", C.c_int32), ("act", C.c_int32), ("flags", C.c_int32),
+        ("scratch", c_void_p), ("scratch_bytes", c_i64),
+    ]
+
+
 class GLinearExt(C.Structure):
     _fields_ = [("act_alpha", c_float), ("act_limit", c_float), ("act_pos", c_float), ("act_neg", c_float),
                 ("in_scale", c_void_p)]
@@ -363,8 +375,15 @@ SIGNATURES = {
     "vila_mx4_linear_scratch": [C.POINTER(Mx4LinearParams)],
     "vila_mx4_linear": [C.POINTER(Mx4LinearParams), c_void_p],
     "vila_mx4_linear_tries": [C.POINTER(Mx4LinearParams), c_int, c_void_p],
+    "vila_fp8_quantize": [c_void_p, c_int, c_i64, c_void_p, c_i64, c_void_p, c_i64, c_int, c_int, c_int, c_void_p],
+    "vila_fp8_dequantize": [c_void_p, c_i64, c_void_p, c_i64, c_void_p, c_int, c_i64, c_int, c_int, c_int, c_void_p],
+    "vila_fp8_rmsnorm": [c_void_p, c_int, c_i64, c_void_p, c_int, c_i64, c_void_p, c_i64, c_void_p, c_int, c_float, c_void_p,
+                         c_i64, c_void_p, c_i64, c_int, c_int, c_void_p],
+    "vila_fp8_linear_scratch": [C.POINTER(Fp8LinearParams)],
+    "vila_fp8_linear": [C.POINTER(Fp8LinearParams), c_void_p],
+    "vila_fp8_linear_tries": [C.POINTER(Fp8LinearParams), c_int, c_void_p],
 }
-_RESTYPES = {"vila_last_error": C.c_char_p, "vila_mx4_linear_scratch": c_i64}
+_RESTYPES = {"vila_last_error": C.c_char_p, "vila_mx4_linear_scratch": c_i64, "vila_fp8_linear_scratch": c_i64}
 
 _lib = None
 

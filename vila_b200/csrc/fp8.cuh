@@ -1,0 +1,56 @@
+// 8-bit floating point rows with an fp32 scale per block of 128 ("Fp8"), shared by the kernels that make and read them.
+//
+// A block is 128 columns of one row (activations) or of 128 rows (weights): scale s = max(largest magnitude / 448, 2^-126), element = e4m3
+// number nearest to x * (1 / s).  2^-126 keeps both quotients among the normal numbers.  include/vila_b200.h has the layouts.
+#pragma once
+#include <cuda_fp16.h>
+#include "common.cuh"
+
+namespace vb {
+
+constexpr int kFp8Block = 128;
+constexpr int kFp8Chunk = 16;      // columns of a lane: 16 bytes of codes; 8 neighbouring lanes hold a block
+
+__host__ __device__ __forceinline__ int fp8_blocks(int n) { return (n + kFp8Block - 1) / kFp8Block; }
+
+// A block's scale and what its elements are multiplied with, from its largest magnitude's bits (magnitudes order as integers, NaN above infinity).
+struct Fp8Scale {
+  float scale, inv;
+  bool fine;      // otherwise the block has an infinity or a NaN: its scale is a NaN, its codes are 0
+};
+__device__ __forceinline__ Fp8Scale fp8_scale(uint32_t top) {
+  Fp8Scale s;
+  s.fine = top < 0x7f800000u;
+  const float v = fmaxf(__fdiv_rn(__uint_as_float(top), 448.f), 1.17549435e-38f);
+  s.scale = s.fine ? v : __uint_as_float(0x7fffffffu);
+  s.inv = s.fine ? __frcp_rn(v) : 0.f;
+  return s;
+}
+// the largest magnitude of the 8 lanes that hold a block
+__device__ __forceinline__ uint32_t fp8_top8(uint32_t top) {
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  return max(top, __shfl_xor_sync(0xffffffffu, top, 4));
+}
+// two numbers to e4m3, nearest, ties to even, at most 448; the first in the low byte
+__device__ __forceinline__ uint32_t fp8_encode2(float lo, float hi) {
+  uint16_t d;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ uint32_t fp8_encode4(float a, float b, float c, float d) { return fp8_encode2(a, b) | fp8_encode2(c, d) << 16; }
+// 16 numbers of a block to codes
+__device__ __forceinline__ uint4 fp8_encode16(const float (&v)[16], const Fp8Scale& s) {
+  uint32_t c[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c[i] = fp8_encode4(v[4 * i] * s.inv, v[4 * i + 1] * s.inv, v[4 * i + 2] * s.inv, v[4 * i + 3] * s.inv);
+  return s.fine ? make_uint4(c[0], c[1], c[2], c[3]) : make_uint4(0u, 0u, 0u, 0u);
+}
+// the two numbers of a pair of codes
+__device__ __forceinline__ float2 fp8_decode2(uint32_t pair) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(pair)));
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+}  // namespace vb

@@ -9,8 +9,8 @@ namespace vb {
 // An activation (VILA_ACT_*), or kMx4Gated + the flag of a gated unit, as a template parameter: the choice is made once a tile.
 constexpr int kMx4Gated = 64;
 template <int EPI> struct Mx4Epi { static constexpr int value = EPI; };
-template <typename F>
-__device__ __forceinline__ void mx4_with_epilogue(const vila_mx4_linear_params& p, F&& f) {
+template <typename P, typename F>
+__device__ __forceinline__ void mx4_with_epilogue(const P& p, F&& f) {      // P: parameters with flags and act
   if (p.flags & VILA_FLAG_GLU_CLAMP) return f(Mx4Epi<kMx4Gated + VILA_FLAG_GLU_CLAMP>());
   if (p.flags & VILA_FLAG_GEGLU) return f(Mx4Epi<kMx4Gated + VILA_FLAG_GEGLU>());
   if (p.flags & VILA_FLAG_SWIGLU) return f(Mx4Epi<kMx4Gated + VILA_FLAG_SWIGLU>());

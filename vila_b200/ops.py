@@ -1499,3 +1499,246 @@ def mx4_matmul(a: Mx4, w: Mx4, bias: Optional[torch.Tensor] = None, *, act: int 
         raise RuntimeError("vila_b200.ops: a and w must be Mx4 (mx4_quantize, mx4_pack)")
     _mx4_here(a._held(), "a")
     return _mx4_product(None, a, a.rows, a.cols, w, bias, act, act_params, swiglu, geglu, glu_clamp, out)
+
+
+# ---- 8-bit floating point rows with a scale per block of 128 (include/vila_b200.h has the format) ----
+_E4M3 = torch.float8_e4m3fn
+FP8_BLOCK = 128
+
+
+class Fp8:
+    """A matrix of e4m3 numbers with an fp32 scale per block of 128 columns of one row (block_rows 1: activations) or of 128 rows (block_rows
+    128: weights).  Made by fp8_quantize, fp8_rmsnorm and fp8_linear(to8=True), or by fp8_pack from a checkpoint's tensors."""
+
+    __slots__ = ("rows", "cols", "block_rows", "_codes", "_ldc", "_scales", "_lds", "_both", "_at")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, block_rows: int):
+        """codes [rows, cols] float8_e4m3fn, rows a multiple of 16 bytes apart, on a 16-byte boundary; scales fp32, with block_rows 128
+        [ceil(rows / 128), ceil(cols / 128)] with consecutive columns, with block_rows 1 the same transposed: [rows, blocks] with consecutive
+        rows, columns a multiple of 4 apart (and that much memory to the end), on a 16-byte boundary."""
+        _fp8_shape(codes, scales, block_rows)
+        self.rows, self.cols = codes.shape
+        self.block_rows, self._codes, self._scales, self._both, self._at = block_rows, codes, scales, None, 0
+        blocks = scales.shape[1]
+        self._ldc = _fp8_pitch(self.cols) if self.rows <= 1 else codes.stride(0)
+        if block_rows == 1:
+            self._lds = _fp8_lds(self.rows) if blocks <= 1 else scales.stride(1)
+            ok = (self.rows <= 1 or scales.stride(0) == 1) and self._lds % 4 == 0 and self._lds >= self.rows and scales.data_ptr() % 16 == 0
+            ok = ok and scales.untyped_storage().nbytes() >= 4 * (scales.storage_offset() + blocks * self._lds)
+        else:
+            self._lds = blocks if scales.shape[0] <= 1 else scales.stride(0)
+            ok = (blocks <= 1 or scales.stride(1) == 1) and self._lds >= blocks
+        _fp8_check(ok, "the scales do not lie as the kernels read them (fp8_pack copies those that do not)")
+        _fp8_check((self.cols <= 1 or codes.stride(1) == 1) and self._ldc % 16 == 0 and self._ldc >= self.cols and codes.data_ptr() % 16 == 0
+                   and codes.untyped_storage().nbytes() >= codes.storage_offset() + max(self.rows - 1, 0) * self._ldc + (_fp8_pitch(self.cols) if self.rows else 0),
+                   "rows of codes must start on 16-byte boundaries and have whole 16 bytes of memory (fp8_pack copies those that do not)")
+
+    @classmethod
+    def _alloc(cls, like: torch.Tensor, rows: int, cols: int, block_rows: int) -> "Fp8":
+        """Uninitialised, codes and scales in one piece of memory on the device of `like`: the views of it are made when they are asked for."""
+        q = cls.__new__(cls)
+        q.rows, q.cols, q.block_rows, q._codes, q._scales = rows, cols, block_rows, None, None
+        q._ldc = (cols + 15) // 16 * 16
+        blocks = (cols + 127) // 128
+        if block_rows == 1:
+            q._lds = (rows + 3) // 4 * 4
+            n = blocks * q._lds
+        else:
+            q._lds = blocks
+            n = (rows + 127) // 128 * blocks
+        q._at = rows * q._ldc
+        q._both = like.new_empty(q._at + 4 * n, dtype=torch.uint8)
+        return q
+
+    @property
+    def codes(self) -> torch.Tensor:
+        """float8_e4m3fn [rows, cols]"""
+        if self._codes is None:
+            self._codes = self._both[:self._at].view(_E4M3).view(self.rows, self._ldc)[:, :self.cols]
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        """fp32 [rows or ceil(rows / 128), ceil(cols / 128)]"""
+        if self._scales is None:
+            s = self._both[self._at:].view(torch.float32)
+            self._scales = s.view(-1, self._lds) if self.block_rows != 1 else s.view((self.cols + 127) // 128, self._lds)[:, :self.rows].T
+        return self._scales
+
+    def _held(self) -> torch.Tensor:
+        return self._codes if self._both is None else self._both
+
+    def _ptrs(self) -> Tuple[int, int]:
+        if self._both is not None:
+            p = self._both.data_ptr()
+            return p, p + self._at
+        return self._codes.data_ptr(), self._scales.data_ptr()
+
+    @property
+    def shape(self) -> Tuple[int, int]:
+        return (self.rows, self.cols)
+
+    @property
+    def device(self) -> torch.device:
+        return self._held().device
+
+    @property
+    def nbytes(self) -> int:
+        return self.rows * self._ldc + 4 * self._lds * ((self.cols + 127) // 128 if self.block_rows == 1 else (self.rows + 127) // 128)
+
+
+def _fp8_check(ok: bool, what: str) -> None:
+    if not ok:
+        raise RuntimeError(f"vila_b200.ops: {what}")
+
+
+def _fp8_pitch(cols: int) -> int:
+    return (cols + 15) // 16 * 16
+
+
+def _fp8_lds(rows: int) -> int:
+    return (rows + 3) // 4 * 4
+
+
+def _fp8_shape(codes: torch.Tensor, scales: torch.Tensor, block_rows: int) -> None:
+    _fp8_check(block_rows in (1, FP8_BLOCK), f"block_rows={block_rows}: 1 or 128")
+    _fp8_check(codes.dim() == 2 and codes.dtype == _E4M3 and codes.shape[1] > 0, "codes must be float8_e4m3fn [rows, cols]")
+    want = (-(-codes.shape[0] // block_rows), -(-codes.shape[1] // FP8_BLOCK))
+    _fp8_check(scales.dtype == torch.float32 and tuple(scales.shape) == want and scales.device == codes.device,
+               f"scales must be float32 {list(want)} on the codes' device")
+
+
+def fp8_quantize(x: torch.Tensor, block_rows: int = 1) -> Fp8:
+    """x [rows, cols] bf16 or fp32 (a view with a row stride is fine) -> Fp8.  Per block of 128 columns of block_rows rows (1: activations,
+    128: weights) with largest magnitude m the scale is s = max(m / 448, 2^-126), and x * (1 / s) becomes the nearest e4m3 number, ties to
+    even.  A block with an infinity or a NaN reads as NaN."""
+    _mx4_here(x, "x")
+    if x.dim() != 2 or x.shape[1] == 0 or (x.stride(1) != 1 and x.shape[1] != 1):
+        raise RuntimeError("vila_b200.ops: x must be [rows, cols] with consecutive columns")
+    if block_rows != 1 and block_rows != FP8_BLOCK:
+        raise RuntimeError(f"vila_b200.ops: block_rows={block_rows}: 1 or 128")
+    dt = _dt(x, "x")
+    rows, cols = x.shape
+    q = Fp8._alloc(x, rows, cols, block_rows)
+    codes, scales = q._ptrs()
+    check(_lib.load().vila_fp8_quantize(x.data_ptr(), dt, x.stride(0), codes, q._ldc, scales, q._lds, rows, cols, block_rows, _stream()),
+          "vila_fp8_quantize")
+    return q
+
+
+def fp8_dequantize(q: Fp8, out_dtype=torch.bfloat16) -> torch.Tensor:
+    """The numbers that q stands for, [rows, cols] in bf16 or fp32."""
+    held = q._held()
+    _mx4_here(held, "q")
+    out = held.new_empty((q.rows, q.cols), dtype=out_dtype)
+    codes, scales = q._ptrs()
+    check(_lib.load().vila_fp8_dequantize(codes, q._ldc, scales, q._lds, out.data_ptr(), _dt(out, "out"), q.cols, q.rows, q.cols, q.block_rows,
+                                          _stream()), "vila_fp8_dequantize")
+    return out
+
+
+def fp8_pack(codes: torch.Tensor, scales: torch.Tensor, block_rows: int = FP8_BLOCK) -> Fp8:
+    """codes float8_e4m3fn [rows, cols] and the factors fp32 [ceil(rows / block_rows), ceil(cols / 128)] that their blocks are multiplied with (a
+    checkpoint's) -> Fp8.  Both are kept, not copied, where they lie as the kernels read them: rows of codes on 16-byte boundaries, a
+    weight's scales with consecutive columns."""
+    _mx4_here(codes, "codes")
+    _mx4_here(scales, "scales")
+    _fp8_shape(codes, scales, block_rows)
+    rows, cols = codes.shape
+    try:
+        return Fp8(codes, scales, block_rows)
+    except RuntimeError:
+        q = Fp8._alloc(codes, rows, cols, block_rows)
+        q.codes.copy_(codes)
+        q.scales.copy_(scales)
+        return q
+
+
+def fp8_rmsnorm(x: torch.Tensor, w: Optional[torch.Tensor], eps: float, *, residual: Optional[torch.Tensor] = None,
+                out: Optional[torch.Tensor] = None) -> Tuple[Fp8, torch.Tensor]:
+    """The norm before a layer on 8-bit rows: s = x + residual (rounded to x's type), s / sqrt(mean(s^2) + eps) * w in 8 bits (block_rows 1).
+    -> (Fp8, s); without a residual s is x.  x, residual [rows, cols] bf16 or fp32 (views with a row stride are fine), w [cols] bf16 or fp32
+    or None.  out: where s goes, x itself for an update in place."""
+    _mx4_here(x, "x")
+    if x.dim() != 2 or x.shape[1] == 0 or (x.stride(1) != 1 and x.shape[1] != 1):
+        raise RuntimeError("vila_b200.ops: x must be [rows, cols] with consecutive columns")
+    rows, cols = x.shape
+    dt, w_ptr, w_dt, r_ptr, r_dt, ldr, s_ptr, ld_sum, total = _dt(x, "x"), None, 0, None, 0, 0, None, 0, x
+    if w is not None:
+        _mx4_here(w, "w")
+        w_ptr, w_dt = w.data_ptr(), _dt(w, "w")
+        _fp8_check(w.numel() == cols and w.is_contiguous(), f"w must be contiguous [{cols}]")
+    if residual is not None:
+        _mx4_here(residual, "residual")
+        _fp8_check(residual.shape == x.shape and (residual.stride(1) == 1 or cols == 1), f"residual must be [{rows}, {cols}] with consecutive columns")
+        r_ptr, r_dt, ldr = residual.data_ptr(), _dt(residual, "residual"), residual.stride(0)
+        if out is None:
+            total = x.new_empty((rows, cols))
+        else:
+            _mx4_here(out, "out")
+            _fp8_check(out.shape == x.shape and out.dtype == x.dtype and (out.stride(1) == 1 or cols == 1), f"out must be [{rows}, {cols}] of x's type")
+            total = out
+        s_ptr, ld_sum = total.data_ptr(), total.stride(0)
+    elif out is not None:
+        raise RuntimeError("vila_b200.ops: out goes with a residual")
+    q = Fp8._alloc(x, rows, cols, 1)
+    codes, scales = q._ptrs()
+    check(_lib.load().vila_fp8_rmsnorm(x.data_ptr(), dt, x.stride(0), r_ptr, r_dt, ldr, s_ptr, ld_sum, w_ptr, w_dt, eps, codes, q._ldc, scales,
+                                       q._lds, rows, cols, _stream()), "vila_fp8_rmsnorm")
+    return q, total
+
+
+def fp8_linear(a, w: Fp8, bias: Optional[torch.Tensor] = None, *, act: int = ACT_NONE, act_params: Optional[Tuple[float, float]] = None,
+               swiglu: bool = False, geglu: bool = False, glu_clamp: Optional[Tuple[float, float]] = None, out: Optional[torch.Tensor] = None,
+               to8: bool = False):
+    """act(a [M, K] . w[N, K]^T + bias) in bf16, or with to8 as Fp8 rows (quantised unrounded: what the next layer reads).  a: Fp8 with
+    block_rows 1, or bf16 / fp32 rows, which are quantised first; w: Fp8 with block_rows 128.  fp32 sums.  Activations and gated units as
+    in linear / glinear."""
+    if isinstance(a, torch.Tensor):
+        a = fp8_quantize(a)
+    if not (isinstance(a, Fp8) and isinstance(w, Fp8) and a.block_rows == 1 and w.block_rows == FP8_BLOCK):
+        raise RuntimeError("vila_b200.ops: a must be Fp8 rows (block_rows 1) or a tensor, w an Fp8 weight (block_rows 128)")
+    held = w._held()
+    _mx4_here(held, "w")
+    _mx4_here(a._held(), "a")
+    M, K, N = a.rows, a.cols, w.rows
+    if K != w.cols or N == 0:
+        raise RuntimeError(f"vila_b200.ops: {M} x {K} rows do not fit a weight of {N} x {w.cols}")
+    flags = (1 if swiglu else 0) | (4 if glu_clamp is not None else 0) | (FLAG_GEGLU if geglu else 0)
+    _fp8_check(act != ACT_XIELU or act_params is not None, "ACT_XIELU takes act_params")
+    n_out = N // 2 if flags else N
+    _fp8_check(n_out > 0, f"a gated unit has an even number of weight rows (N={N})")
+    if bias is not None:
+        _chk(bias, "bias")
+        _mx4_here(bias, "bias")
+        _fp8_check(bias.is_contiguous() and bias.numel() == N, f"bias must be contiguous [{N}]")
+    o_codes, ld_oc, o_scales, ld_os, o_ptr, ldo = None, 0, None, 0, None, 0
+    if to8:
+        _fp8_check(out is None, "a result in 8 bits takes no out")
+        y = Fp8._alloc(held, M, n_out, 1)
+        o_codes, o_scales = y._ptrs()
+        ld_oc, ld_os = y._ldc, y._lds
+    else:
+        if out is None:
+            out = held.new_empty((M, n_out), dtype=torch.bfloat16)
+        else:
+            _chk(out, "out")
+            _mx4_here(out, "out")
+            _fp8_check(tuple(out.shape) == (M, n_out) and (out.stride(1) == 1 or n_out == 1), f"out must be [{M}, {n_out}] with consecutive columns")
+        o_ptr, ldo, y = out.data_ptr(), out.stride(0), out
+    if M == 0:
+        return y
+    alpha, limit = glu_clamp if glu_clamp is not None else (0.0, 0.0)
+    pos, neg = act_params if act_params is not None else (0.0, 0.0)
+    a_codes, a_scales = a._ptrs()
+    w_codes, w_scales = w._ptrs()
+    p = _lib.Fp8LinearParams(a_codes, a._ldc, a_scales, a._lds, w_codes, w._ldc, w_scales, w._lds, None if bias is None else bias.data_ptr(), o_ptr, ldo,
+                             o_codes, ld_oc, o_scales, ld_os, alpha, limit, pos, neg, M, N, K, act, flags)
+    lib = _lib.load()
+    if to8:      # a workspace of the call's own: a captured graph keeps its own, too
+        n = lib.vila_fp8_linear_scratch(C.byref(p))
+        if n:
+            scratch = held.new_empty(n, dtype=torch.uint8)
+            p.scratch, p.scratch_bytes = scratch.data_ptr(), n
+    check(lib.vila_fp8_linear(C.byref(p), _stream()), "vila_fp8_linear")
+    return y
