@@ -231,7 +231,7 @@ def check_rows8(q, x, w, bias, act="none"):
 
 SIZES = [(1, 2, 32), (1, 128, 64), (1, 300, 2048), (3, 129, 95), (7, 64, 1153), (8, 1000, 512), (9, 130, 4000), (16, 256, 1024),
          (17, 384, 300), (33, 128, 640), (64, 514, 1000), (65, 1157, 1153), (100, 640, 256), (129, 300, 2080), (200, 130, 96), (300, 770, 520),
-         (520, 258, 1056), (2600, 2570, 800), (1, 40000, 130), (40, 20000, 257), (31, 258, 20000)]
+         (520, 258, 1056), (2600, 2570, 800), (513, 255, 129), (700, 129, 5000), (5000, 5001, 300), (1, 40000, 130), (40, 20000, 257), (31, 258, 20000)]
 
 
 @pytest.mark.parametrize("M, N, K", SIZES)
@@ -477,6 +477,34 @@ def test_waits_that_run_out(cuda, monkeypatch, M, N, K, tries):
             pass
     ops.check_waits()
     assert torch.equal(ops.fp8_linear(a, w), want)
+
+
+@pytest.mark.parametrize("role", [0, 1, 3])
+@pytest.mark.parametrize("rank", [0, 1])
+@pytest.mark.parametrize("M, N, K", [(1500, 1300, 800), (1500, 1300, 5000), (5000, 5000, 700)])
+@pytest.mark.parametrize("to8", [False, True])
+def test_one_cta_of_a_pair_gives_up(cuda, monkeypatch, M, N, K, to8, rank, role):
+    """One CTA of every pair quits while the other has copies in flight that report to it, or expects copies that the first has not
+    asked for: the launch ends, says so, and the calls after it are right."""
+    from vila_b200 import _lib, ops
+    w = ops.fp8_quantize(rand(1, N, K).to(cuda), block_rows=128)
+    a = ops.fp8_quantize(rand(2, M, K).to(cuda))
+    call = lambda: (lambda y: ops.fp8_dequantize(y) if to8 else y)(ops.fp8_linear(a, w, to8=to8, swiglu=to8))  # noqa: E731
+    want = call()
+    torch.cuda.synchronize()
+    ops.check_waits()
+    lib = _lib.load()
+    with monkeypatch.context() as m:
+        m.setattr(lib, "vila_fp8_linear", lambda p, stream: lib.vila_fp8_linear_tries(p, -2 - (role + 4 * (rank + 1)), stream))
+        out = ops.fp8_linear(a, w, to8=to8, swiglu=to8)
+        torch.cuda.synchronize()
+    if rank == 1 and role == 1:      # no such warp: the second CTA's products
+        assert torch.equal(ops.fp8_dequantize(out) if to8 else out, want)
+    else:
+        with pytest.raises(RuntimeError, match="ran out of tries"):
+            ops.check_waits()
+    ops.check_waits()
+    assert torch.equal(call(), want)
 
 
 # ---- together, as they are used -----------------------------------------------------------------------------

@@ -53,6 +53,7 @@ SOURCES = [
     "fp8.cu",
     "fp8_linear.cu",
     "fp8_tc.cu",
+    "fp8_pair.cu",
 ]
 HEADERS = ["common.cuh", "once.h", "kernels.h", "dtype_any.cuh", "glinear_epi.cuh", "paged_attn_common.cuh", "mma_bf16.cuh", "mx4.cuh", "mx4_epi.cuh", "fp8.cuh", "../../include/vila_b200.h"]
 

@@ -53,4 +53,21 @@ __device__ __forceinline__ float2 fp8_decode2(uint32_t pair) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
+// ---- products ----
+// kind::f8f6f4, e4m3 x e4m3 -> fp32: [4,6) D is F32 (1)  [7,10) A, [10,13) B: E4M3 (0)  [17,23) N >> 3  [24,29) M >> 4
+__host__ __device__ constexpr uint32_t fp8_idesc(uint32_t M, uint32_t N) { return (1u << 4) | ((N >> 3) << 17) | ((M >> 4) << 24); }
+// d += a b, two numbers at a time
+__device__ __forceinline__ void fp8_fma2(float& d0, float& d1, float a0, float a1, float b0, float b1) {
+  asm("{.reg .b64 ra, rb, rd; mov.b64 ra, {%2,%3}; mov.b64 rb, {%4,%5}; mov.b64 rd, {%0,%1}; fma.rn.f32x2 rd, ra, rb, rd; "
+      "mov.b64 {%0,%1}, rd;}"
+      : "+f"(d0), "+f"(d1)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+
+// Both scales of a block's products.  Their product is cut at fp32's largest number: sums that are zero stay zero.  A NaN stays one.
+__device__ __forceinline__ float fp8_both_scales(float a, float b) {
+  const float s = a * b;
+  return s > 3.40282347e38f ? 3.40282347e38f : s;
+}
+
 }  // namespace vb

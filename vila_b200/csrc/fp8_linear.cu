@@ -12,7 +12,7 @@ int width(const vila_fp8_linear_params& p) { return p.flags & kGluFlags ? p.N / 
 
 // an unrounded result, quantised by a launch of its own
 size_t fp8_linear_scratch(const vila_fp8_linear_params& p) {
-  if (p.M <= 0 || p.N <= 0 || p.o_codes == nullptr) return 0;
+  if (p.M <= 0 || p.N <= 0 || p.K <= 0 || p.o_codes == nullptr || fp8_pair_takes(p)) return 0;
   return static_cast<size_t>(p.M) * width(p) * 4;
 }
 
@@ -43,11 +43,12 @@ int fp8_linear(const vila_fp8_linear_params& p, cudaStream_t stream, int tries) 
   const int n = width(p);
   if (p.out != nullptr) {
     VB_CHECK(on(p.out, 2) && (p.M == 1 || p.ldo >= n), "fp8_linear: out off its elements' boundaries, or ldo=%lld for %d columns", static_cast<long long>(p.ldo), n);
-    return fp8_tc(p, ext, nullptr, tries, stream);
+    return fp8_pair_takes(p) ? fp8_pair(p, ext, tries, stream) : fp8_tc(p, ext, nullptr, tries, stream);
   }
   VB_CHECK(p.o_scales != nullptr && on(p.o_codes, 16) && p.ld_oc % 16 == 0 && p.ld_oc >= n && on(p.o_scales, 16) && p.ld_os % 4 == 0 && p.ld_os >= p.M,
            "fp8_linear: the result's codes and scales start on 16-byte boundaries, ld_oc=%lld ld_os=%lld for %d rows of %d", static_cast<long long>(p.ld_oc),
            static_cast<long long>(p.ld_os), p.M, n);
+  if (fp8_pair_takes(p)) return fp8_pair(p, ext, tries, stream);
   const size_t want = fp8_linear_scratch(p);
   VB_CHECK(want == 0 || (p.scratch != nullptr && on(p.scratch, 16) && p.scratch_bytes >= static_cast<int64_t>(want)),
            "fp8_linear: %lld bytes of scratch, %lld wanted, on a 16-byte boundary", static_cast<long long>(p.scratch_bytes), static_cast<long long>(want));

@@ -27,8 +27,6 @@ namespace {
 constexpr int kRows = 128;                    // weight rows of a tile
 constexpr int kAcc = 4;                       // accumulators in TMEM
 
-// kind::f8f6f4, e4m3 x e4m3 -> fp32: [4,6) D is F32 (1)  [7,10) A, [10,13) B: E4M3 (0)  [17,23) N >> 3  [24,29) M >> 4
-__host__ __device__ constexpr uint32_t idesc_fp8(uint32_t M, uint32_t N) { return (1u << 4) | ((N >> 3) << 17) | ((M >> 4) << 24); }
 __device__ __forceinline__ void umma_fp8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t"
@@ -38,20 +36,6 @@ __device__ __forceinline__ void umma_fp8(uint32_t d, uint64_t a, uint64_t b, uin
       "}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// d += a b, two numbers at a time
-__device__ __forceinline__ void fma2(float& d0, float& d1, float a0, float a1, float b0, float b1) {
-  asm("{.reg .b64 ra, rb, rd; mov.b64 ra, {%2,%3}; mov.b64 rb, {%4,%5}; mov.b64 rd, {%0,%1}; fma.rn.f32x2 rd, ra, rb, rd; "
-      "mov.b64 {%0,%1}, rd;}"
-      : "+f"(d0), "+f"(d1)
-      : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
-}
-
-// Both scales of a block's products.  Their product is cut at fp32's largest number: sums that are zero stay zero.  A NaN stays one.
-__device__ __forceinline__ float both_scales(float a, float b) {
-  const float s = a * b;
-  return s > 3.40282347e38f ? 3.40282347e38f : s;
-}
-
 template <int BN> struct Shape {
   static constexpr int kEpi = BN > 32 ? 8 : 4;                  // epilogue warps: a quarter of the lanes each; two share a quarter's columns
   static constexpr int kTma = kEpi, kMma = kEpi + 1, kThreads = 32 * (kEpi + 2);
@@ -187,7 +171,7 @@ fp8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ C
     // The whole warp walks the loop and one lane issues: what the instructions are given stays in uniform registers.
     const bool one = elect_one();
     const uint64_t pd0 = make_smem_desc(smem_u32(smem), 16, 1024, kLayoutSW128), qd0 = make_smem_desc(smem_u32(smem) + S::kPBytes, 16, 1024, kLayoutSW128);
-    const uint32_t idesc = idesc_fp8(kRows, bn);
+    const uint32_t idesc = fp8_idesc(kRows, bn);
     int s = 0, a = 0;
     uint32_t ph = 0, aph = 1;             // the first round of accumulators passes
     for (int it = it0; it < total && ok; it += it_step) {
@@ -238,7 +222,7 @@ fp8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ C
         ok = mx4_warp_wait(&full_bar[s], ph, gave_up, limit.tries);
         if (!ok) break;
 #pragma unroll
-        for (int i = lane; i < S::kColumns; i += 32) mine[i] = both_scales(scales[s * BN + c0 + i], wb);
+        for (int i = lane; i < S::kColumns; i += 32) mine[i] = fp8_both_scales(scales[s * BN + c0 + i], wb);
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty_bar[s]);
         ok = mx4_warp_wait(&acc_full[a], aph, gave_up, limit.tries);
@@ -253,8 +237,8 @@ fp8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ C
 #pragma unroll
           for (int i = 0; i < 16; i += 4) {
             const float4 f = both[(c + i) / 4];
-            fma2(sum[c + i], sum[c + i + 1], r[i], r[i + 1], f.x, f.y);
-            fma2(sum[c + i + 2], sum[c + i + 3], r[i + 2], r[i + 3], f.z, f.w);
+            fp8_fma2(sum[c + i], sum[c + i + 1], r[i], r[i + 1], f.x, f.y);
+            fp8_fma2(sum[c + i + 2], sum[c + i + 3], r[i + 2], r[i + 3], f.z, f.w);
           }
         }
         tc_fence_before();

@@ -358,5 +358,7 @@ int fp8_rmsnorm(const void* x, int x_dt, int64_t ldx, const void* residual, int 
 size_t fp8_linear_scratch(const vila_fp8_linear_params& p);
 int fp8_linear(const vila_fp8_linear_params& p, cudaStream_t stream, int tries = -1);
 int fp8_tc(const vila_fp8_linear_params& p, const vila_glinear_ext& ext, float* out32, int tries, cudaStream_t stream);   // fp8_tc.cu
+bool fp8_pair_takes(const vila_fp8_linear_params& p);      // many rows, by CTA pairs (fp8_pair.cu)
+int fp8_pair(const vila_fp8_linear_params& p, const vila_glinear_ext& ext, int tries, cudaStream_t stream);
 
 }  // namespace vb

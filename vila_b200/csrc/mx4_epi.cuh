@@ -47,8 +47,8 @@ __device__ __forceinline__ void mx4_stg32(void* p, const uint32_t* h) {
 }
 
 // Lane = output row (token), 32 columns n .. n + 31 of the sums.  `wide`: rows of out start on 32-byte boundaries.
-template <int EPI>
-__device__ __forceinline__ void mx4_store_row(const vila_mx4_linear_params& p, const vila_glinear_ext& x, float (&z)[32], int m, int n, bool wide) {
+template <int EPI, typename P>
+__device__ __forceinline__ void mx4_store_row(const P& p, const vila_glinear_ext& x, float (&z)[32], int m, int n, bool wide) {
   constexpr bool kGated = EPI >= kMx4Gated;
   constexpr int kWords = kGated ? 8 : 16;
   if (p.bias != nullptr) {

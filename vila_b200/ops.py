@@ -1554,15 +1554,16 @@ class Fp8:
     def codes(self) -> torch.Tensor:
         """float8_e4m3fn [rows, cols]"""
         if self._codes is None:
-            self._codes = self._both[:self._at].view(_E4M3).view(self.rows, self._ldc)[:, :self.cols]
+            self._codes = self._both.view(_E4M3).as_strided((self.rows, self.cols), (self._ldc, 1))
         return self._codes
 
     @property
     def scales(self) -> torch.Tensor:
         """fp32 [rows or ceil(rows / 128), ceil(cols / 128)]"""
         if self._scales is None:
-            s = self._both[self._at:].view(torch.float32)
-            self._scales = s.view(-1, self._lds) if self.block_rows != 1 else s.view((self.cols + 127) // 128, self._lds)[:, :self.rows].T
+            blocks, one = (self.cols + 127) // 128, self.block_rows == 1
+            self._scales = self._both.view(torch.float32).as_strided((self.rows if one else (self.rows + 127) // 128, blocks),
+                                                                     (1, self._lds) if one else (self._lds, 1), self._at // 4)
         return self._scales
 
     def _held(self) -> torch.Tensor:
