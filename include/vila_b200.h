@@ -975,8 +975,11 @@ int vila_fp8_rmsnorm(const void* x, int x_dtype, int64_t ldx, const void* residu
  * block's numbers and their sum in fp32, times the product of both scales (fp32, cut at fp32's largest number), added in fp32 in the order of the
  * blocks (K over a cluster: each CTA's, then the CTAs').  Scales are finite, not negative, or NaN.  bias bf16 or NULL.  act, flags and their parameters as in
  * vila_mx4_linear; with a gated unit the result has N / 2 columns.  The result goes to out in bf16 (row stride ldo), or, with out NULL,
- * unrounded to o_codes and o_scales (block_rows 1). */
+ * unrounded to o_codes and o_scales (block_rows 1).  Rows as they come: x (VILA_DT_*, row stride ldx) instead of a_codes and a_scales, quantised
+ * into the scratch first. */
 typedef struct vila_fp8_linear_params {
+  const void* x;
+  int64_t ldx;
   const void* a_codes;
   int64_t lda;
   const float* a_scales;
@@ -993,7 +996,7 @@ typedef struct vila_fp8_linear_params {
   float* o_scales;
   int64_t ld_os;
   float act_alpha, act_limit, act_pos, act_neg;
-  int32_t M, N, K, act, flags;
+  int32_t M, N, K, act, flags, x_dtype;
   void* scratch;
   int64_t scratch_bytes;
 } vila_fp8_linear_params;

@@ -33,7 +33,9 @@ def main(argv=None) -> str:
                         help="prompt as comma-separated token ids; ';' separates several prompts")
     parser.add_argument("--max-new-tokens", type=int, default=32)
     parser.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
-    parser.add_argument("--weights", choices=["mx4"], default=None, help="hold the layers' weights in microscaled 4-bit numbers")
+    parser.add_argument("--weights", choices=["mx4", "fp8"], default=None,
+                        help="hold the layers' weights in microscaled 4-bit numbers, or in 8-bit floating point; for a VILA "
+                             "checkpoint fp8 runs prompts in 8 bits")
     parser.add_argument("--temperature", type=float, default=0.0, help="0: greedy")
     parser.add_argument("--top-k", type=int, default=0)
     parser.add_argument("--top-p", type=float, default=1.0)
@@ -59,7 +61,11 @@ def main(argv=None) -> str:
     else:
         response_format = ResponseFormat(type="json_schema", json_schema=JsonSchemaResponseFormat(
             schema=get_schema_from_python_path(args.json_schema)))
+    if args.weights == "mx4":
+        raise SystemExit("--weights mx4 is for token-id language models")
     model = llava.load(args.model_path, model_base=None)
+    if args.weights == "fp8":
+        model.llm.prefill_in_fp8()
     if args.num_video_frames > 0:
         model.config.num_video_frames = args.num_video_frames
     if args.video_max_tiles > 0:

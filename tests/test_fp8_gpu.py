@@ -525,3 +525,172 @@ def test_feed_forward_block(cuda, M):
     n, t = ops.fp8_rmsnorm(s, w, 1e-6, residual=y)
     assert torch.equal(t, (s.float() + y.float()).to(BF))
     check_norm(n, t, w, 1e-6)
+
+
+@pytest.mark.parametrize("M", [0, 1, 12, 60, 700])
+@pytest.mark.parametrize("N, keep, K", [(200, 8, 288), (200, 7, 288), (96, 64, 100), (2, 1, 32), (640, 320, 512)])
+def test_rows_that_stay_as_they_are(cuda, M, N, keep, K):
+    from vila_b200 import ops
+    w, x, bias = (rand(1, N, K) / math.sqrt(K)).to(BF), rand(2, M, K).to(BF), rand(3, N).to(BF)
+    q = ops.fp8_quantize(w.to(cuda), block_rows=128, keep=keep)
+    assert q.shape == (N, K) and q.device == x.to(cuda).device and q.nbytes == q.part.nbytes + keep * K * 2
+    both = ops.fp8_dequantize(q, out_dtype=torch.float32).cpu()
+    eight = R.quantise(w[:N - keep], 128)
+    assert torch.equal(both[N - keep:], w[N - keep:].float()) and torch.equal(both[:N - keep], R.values(*eight, 128).float())
+    x8 = R.values(*R.quantise(x))
+    out = torch.full((M, N + 5), 7.0, dtype=BF, device=cuda)
+
+    def check(got, bias, act="none"):      # the 8-bit rows read quantised rows, the kept ones the rows themselves
+        if M:
+            n = N - keep
+            cut = n // 2 if act == "swiglu" else n
+            check_product(got[:, :cut], x8, both[:n], None if bias is None else bias[:n], act)
+            check_product(got[:, cut:], x, both[n:], None if bias is None else bias[n:], act)
+
+    check(ops.fp8_linear(x.to(cuda), q, bias.to(cuda), out=out[:, 2:2 + N]), bias)
+    assert (out[:, :2] == 7).all() and (out[:, 2 + N:] == 7).all()
+    check(ops.linear_any(x.to(cuda), q, act=ops.ACT_SILU), None, "silu")
+    if N % 2 == 0 and keep % 2 == 0:
+        check(ops.linear_any(x.to(cuda), q, bias=bias.to(cuda), swiglu=True), bias, "swiglu")
+    elif M:
+        with pytest.raises(RuntimeError, match="even number of weight rows"):
+            ops.linear_any(x.to(cuda), q, swiglu=True)
+    if M:
+        with pytest.raises(RuntimeError, match="bf16 rows and a bf16 result"):
+            ops.fp8_linear(ops.fp8_quantize(x.to(cuda)), q)
+    for call in (lambda: q.codes, lambda: q.scales, lambda: ops.fp8_linear(ops.fp8_quantize(w.to(cuda)), q, to8=True)):
+        with pytest.raises(RuntimeError, match="kept in bf16"):
+            call()
+    for bad in (N, N + 1, -1):
+        with pytest.raises(RuntimeError, match="not all of them"):
+            ops.fp8_quantize(w.to(cuda), block_rows=128, keep=bad)
+    with pytest.raises(RuntimeError, match="gives bfloat16"):
+        ops.linear_any(x.to(cuda), q, out_dtype=torch.float32)
+
+
+@pytest.mark.parametrize("arch", ["nusovik", "ludazen", "bivizen", "nibelix", "lufatar"])
+def test_language_models_on_8_bit_weights(cuda, arch, monkeypatch):
+    """Every linear layer on 8-bit weights that a model runs, prompts, portions and decoded tokens, against float64 on the rows that it was
+    given; and captured steps against eager ones.  (Whole models are not compared with a second computation: where two of them differ by one
+    bf16 rounding, 2^-8, a number lands on the other side of an e4m3 boundary, 2^-3 away, one time in 16 or so.)"""
+    import importlib
+    from vila_b200 import ops
+    from vila_b200.model.registry import MX4_WEIGHTS, quantize_weights
+    from vila_b200.serving import TokenEngine
+    T = importlib.import_module(f"tests.test_{arch}_gpu")
+    name = "aligned" if "aligned" in T.CONFIGS else next(iter(T.CONFIGS))
+    cfg, small = T.build(name, BF, seed=3)
+    before = {k: v.clone() for k, v in small.state_dict().items()}
+    assert quantize_weights(small, "fp8") is small
+    names = MX4_WEIGHTS[type(small).__name__.replace("ForCausalLM", "")]
+    held = sum(isinstance(getattr(layer, n, None), ops.Fp8) for layer in small.layers for n in names)
+    assert held >= len(small.layers)
+    assert all(torch.equal(v, before[k]) for k, v in small.state_dict().items())
+    linear_any, seen = ops.linear_any, []
+    acts = {ops.ACT_NONE: "none", ops.ACT_SILU: "silu", ops.ACT_RELU2: "relu2", ops.ACT_GELU_TANH: "gelu_tanh", ops.ACT_GELU_ERF: "gelu_erf"}
+
+    def checked(x, w, *, bias=None, act=ops.ACT_NONE, swiglu=False, geglu=False, glu_clamp=None, **more):
+        got = linear_any(x, w, bias=bias, act=act, swiglu=swiglu, geglu=geglu, glu_clamp=glu_clamp, **more)
+        if isinstance(w, ops.Fp8) and act in acts and glu_clamp is None:      # the others' parameters are not what act64 has
+            seen.append(x.shape[0])
+            kind = "swiglu" if swiglu else "geglu" if geglu else acts[act]
+            n = w.part.rows if isinstance(w, ops.Fp8Kept) else w.rows
+            values = ops.fp8_dequantize(w, out_dtype=torch.float32).cpu()
+            check_product(got[:, :n // 2 if swiglu or geglu else n], R.values(*R.quantise(x)), values[:n], None if bias is None else bias[:n], kind)
+            if n < w.rows:
+                check_product(got[:, n:], x, values[n:], None if bias is None else bias[n:], kind)
+        return got
+
+    eager, captured = TokenEngine(small, 256, 2, graphs=False), TokenEngine(small, 256, 2)
+    toks = T.tokens_for(cfg, 60, 5)
+    for entries in ([("a", toks[:40], [0, 39]), ("b", toks[:7], [6])], [("a", toks[40:41], [0]), ("b", toks[7:30], [22])],
+                    *[[("a", [toks[41 + i]], [0]), ("b", [toks[30 + i]], [0])] for i in range(4)]):
+        got = captured.step(entries)
+        with monkeypatch.context() as m:
+            m.setattr(ops, "linear_any", checked)
+            want = eager.step(entries)
+        assert torch.equal(got, want)
+    assert {47, 24, 2} <= set(seen)
+    assert len(small.generate(toks[:9], max_new_tokens=5)[0]) == 5
+
+
+def test_load_and_command_line(cuda, tmp_path, capsys):
+    from llava.cli import infer
+    from tests import test_nusovik_gpu as T
+    from vila_b200 import ops
+    from vila_b200.model import load_language_model
+    cfg, model = T.build("aligned", BF, seed=8)
+    model.save_pretrained(tmp_path / "m")
+    small = load_language_model(tmp_path / "m", weights="fp8")
+    assert isinstance(small.layers[0].sel_in, ops.Fp8)
+    prompt = T.tokens_for(cfg, 9, 4)
+    text = infer.main(["--model-path", str(tmp_path / "m"), "--token-ids", ",".join(map(str, prompt)), "--max-new-tokens", "5", "--weights", "fp8"])
+    assert [int(t) for t in text.split(",")] == small.generate(prompt, max_new_tokens=5)[0]
+    assert text in capsys.readouterr().out
+
+
+# ---- prompts in 8 bits -----------------------------------------------------------------------------------------
+def qwen(seed=0, layers=3):
+    from vila_b200.model.configuration import Qwen2Config
+    from vila_b200.model.qwen2 import Qwen2ForCausalLM
+    cfg = Qwen2Config(hidden_size=512, intermediate_size=1104, num_hidden_layers=layers, num_attention_heads=4, num_key_value_heads=2, vocab_size=1000)
+    llm = Qwen2ForCausalLM(cfg, device="cuda")
+    g = torch.Generator().manual_seed(seed)
+    with torch.no_grad():
+        for name, p in llm.state_dict().items():
+            v = torch.randn(p.shape, generator=g)
+            p.copy_(1 + 0.1 * v if "norm" in name else v / math.sqrt(p.shape[-1]))
+    return llm
+
+
+def hidden(llm, emb, parts=None, graphed=False):
+    cache = llm.new_cache(emb.shape[0])
+    run = llm.prefill_hidden_graphed if graphed else llm.prefill_hidden
+    return torch.cat([run(e, cache).clone() for e in (emb.split(parts) if parts else [emb])])
+
+
+@pytest.mark.parametrize("S", [1, 40, 300, 1100])
+def test_prompts_in_8_bits(cuda, S):
+    """The hidden states of a prompt are the bf16 path's but for the numbers' rounding: an e4m3 number is off by 2^-4 of itself at most, 3.6 % in
+    the mean square for any distribution, both factors of a product 5.1 %, and a sum of products of independent signs as much of its own size.  A
+    gated unit's product has both of its factors' and one rounding more, 5.1 sqrt 2 + 3.6 < 11 %.  The residual stream adds such errors up
+    with the contributions that they belong to: 15 % of the whole, with what earlier layers' errors make of later ones."""
+    llm = qwen()
+    emb = rand(3, S, 512).to(BF).to(cuda)
+    plain = hidden(llm, emb).float()
+    assert llm.prefill_in_fp8() is llm
+    got = hidden(llm, emb).float()
+    off = ((got - plain).norm() / plain.norm()).item()
+    assert 1e-4 < off < 0.15
+    assert torch.equal(hidden(llm, emb, graphed=True).float(), got) and torch.equal(hidden(llm, emb, graphed=True).float(), got)
+    assert torch.equal(hidden(llm.prefill_in_fp8(False), emb).float(), plain)
+    assert torch.equal(hidden(llm, emb, graphed=True).float(), plain)
+
+
+def test_prompts_in_8_bits_are_the_operators_in_turn(cuda):
+    """portions of a prompt, a packed batch and changed weights"""
+    from vila_b200 import ops
+    llm = qwen().prefill_in_fp8()
+    emb = rand(4, 90, 512).to(BF).to(cuda)
+    whole = hidden(llm, emb).float()
+    parted = hidden(llm, emb, parts=40).float()      # rows are quantised one by one: only sums' order and the attention's tiles differ
+    assert ((parted - whole).norm() / whole.norm()).item() < 0.02
+    # two sequences of a packed row
+    logits = llm.forward_packed(emb[None], torch.ones(1, 90, device=cuda), torch.cat([torch.arange(50), torch.arange(40)])[None], torch.tensor([50, 40]))
+    for a, b in ((0, 50), (50, 90)):
+        want = llm.logits_from_hidden(hidden(llm, emb[a:b])).float()
+        assert ((logits[0, a:b].float() - want).norm() / want.norm()).item() < 0.02
+    # weights changed in place, as a checkpoint's are copied in: captured prompts are not replayed on the former ones
+    before = hidden(llm, emb, graphed=True).clone()
+    other = qwen(seed=1)
+    with torch.no_grad():
+        for p, q in zip(llm.state_dict().values(), other.state_dict().values()):
+            p.copy_(q)
+    want = hidden(other.prefill_in_fp8(), emb)
+    assert torch.equal(hidden(llm, emb, graphed=True), want) and torch.equal(hidden(llm, emb), want) and not torch.equal(want, before)
+    ids = llm.generate(inputs_embeds=emb[None], max_new_tokens=4, eos_token_id=None)
+    assert ids.shape == (1, 4)
+    x = emb.clone()
+    layer, eights = llm.model.layers[0], llm._fp8_weights()[0]
+    h, x = ops.fp8_rmsnorm(x, layer.input_layernorm.weight, llm.config.rms_norm_eps)
+    check_product(ops.fp8_linear(h, eights[0], layer._qkv_b), R.values(h.codes.cpu(), h.scales.cpu()), R.values(*(t.cpu() for t in (eights[0].codes, eights[0].scales)), 128), layer._qkv_b)

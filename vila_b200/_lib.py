@@ -134,13 +134,13 @@ class Mx4LinearParams(C.Structure):
 
 class Fp8LinearParams(C.Structure):
     _fields_ = [
-        ("a_codes", c_void_p), ("lda", c_i64), ("a_scales", c_void_p), ("ld_as", c_i64),
+        ("x", c_void_p), ("ldx", c_i64), ("a_codes", c_void_p), ("lda", c_i64), ("a_scales", c_void_p), ("ld_as", c_i64),
         ("w_codes", c_void_p), ("ldw", c_i64), ("w_scales", c_void_p), ("ld_ws", c_i64),
         ("bias", c_void_p), ("out", c_void_p), ("ldo", c_i64),
         ("o_codes", c_void_p), ("ld_oc", c_i64), ("o_scales", c_void_p), ("ld_os", c_i64),
         ("act_alpha", c_float), ("act_limit", c_float), ("act_pos", c_float), ("act_neg", c_float),
         ("M", C.c_int32), ("N", C.c_int32), ("K", C.c_int32), ("act", C.c_int32), ("flags", C.c_int32),
-        ("scratch", c_void_p), ("scratch_bytes", c_i64),
+        ("x_dtype", C.c_int32), ("scratch", c_void_p), ("scratch_bytes", c_i64),
     ]
 
 

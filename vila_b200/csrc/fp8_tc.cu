@@ -55,9 +55,9 @@ __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 template <int BN, bool kSwap> struct Shape {
-  static constexpr int kEpi = BN > 64 ? 8 : 4;                  // epilogue warps: a quarter of the lanes each; two share a quarter's columns
+  static constexpr int kEpi = BN > 64 ? 16 : 4;                 // epilogue warps: a quarter of the lanes each; four share a quarter's columns
   static constexpr int kTma = kEpi, kMma = kEpi + 1, kScale = kEpi + 2, kThreads = 32 * (kEpi + 3);
-  static constexpr int kColumns = BN > 64 ? BN / 2 : BN;        // columns of a thread
+  static constexpr int kColumns = BN > 64 ? BN / 4 : BN;        // columns of a thread
   static constexpr int kPBytes = kRows * 128, kQBytes = BN * 128, kStage = kPBytes + kQBytes;
   static constexpr int kStages = BN == 16 ? 5 : 4;
   static constexpr int kPerSm = BN > 64 ? 1 : 2;

@@ -155,6 +155,7 @@ class Qwen2ForCausalLM(nn.Module):
         self.generation_config = None
         self._decoder = None
         self._prefill_graphs = {}
+        self._fp8 = None      # prefill_in_fp8: per layer (qkv, o, gate / up, down) as ops.Fp8, and the versions of what they were made from
 
     # ---- HF-style accessors ----
     @property
@@ -172,6 +173,25 @@ class Qwen2ForCausalLM(nn.Module):
         return self.lm_head
 
     # ---- prefill ----
+    def prefill_in_fp8(self, on: bool = True) -> "Qwen2ForCausalLM":
+        """Run prompts' projections in 8 bits: weights held a second time as e4m3 numbers with a scale per 128 x 128, rows quantised by the norm
+        before them, by the gated unit, or (the attention's output) by the projection itself.  Attention, cache, residual stream and decoded
+        tokens' steps stay bf16.  Changed weights are quantised anew at the next prompt.  Sequence-parallel prompts stay bf16.  In place; -> self."""
+        self._prefill_graphs.clear()
+        self._fp8 = ([], None) if on else None
+        return self
+
+    def _fp8_weights(self):
+        """The layers' 8-bit weights, or None."""
+        if self._fp8 is None:
+            return None
+        held = [(layer._qkv_w, layer.self_attn.o_proj.weight, layer._gu_w, layer.mlp.down_proj.weight) for layer in self.model.layers]
+        now = [(w.data_ptr(), None if w.is_inference() else w._version) for ws in held for w in ws]
+        if self._fp8[1] != now:
+            self._prefill_graphs.clear()      # they read the former ones
+            self._fp8 = ([tuple(ops.fp8_quantize(w, block_rows=ops.FP8_BLOCK) for w in ws) for ws in held], now)
+        return self._fp8[0]
+
     def new_cache(self, max_tokens: int, page_order=None) -> PagedKVCache:
         return PagedKVCache(self.config, max_tokens, self.device, self.dtype, page_order)
 
@@ -181,6 +201,7 @@ class Qwen2ForCausalLM(nn.Module):
         per-kernel host work, so PDL overlap is not throttled by Python.  The returned tensor is a
         static graph output: consume it before the next call with the same key."""
         S = inputs_embeds.shape[0]
+        self._fp8_weights()
         if cache.length != 0 or S == 0 or S > 4096:
             # long prompts (video) are not launch-bound, and a captured graph would pin GBs of
             # intermediates in its private pool
@@ -230,13 +251,22 @@ class Qwen2ForCausalLM(nn.Module):
         fused_rope = D == 128 and 0 < S <= 384
         # cos / sin once per request (shared by all layers and heads)
         table = ops.rope_table(position_ids, D, self.inv_freq) if S > 0 and D % 16 == 0 else None
+        eights, y = self._fp8_weights() if S > 0 else None, None      # y: what the next norm adds to x
         for li, layer in enumerate(self.model.layers):
-            h = ops.rmsnorm(x, layer.input_layernorm.weight, cfg.rms_norm_eps)
-            # short chunks: projection + RoPE + cache append in one kernel; else two kernels
-            qkv = ops.linear_qkv_rope(h, layer._qkv_w, layer._qkv_b, table, Hq, Hkv, D, cache.k(li),
-                                      cache.v(li), cache.page_table, p0, static_w=True) if fused_rope else None
-            if qkv is None:
-                qkv = ops.linear(h, layer._qkv_w, layer._qkv_b, static_w=True)
+            qkv = None
+            if eights is not None:
+                h, x = ops.fp8_rmsnorm(x, layer.input_layernorm.weight, cfg.rms_norm_eps, residual=y, out=None if y is None else x)
+                qkv = ops.fp8_linear(h, eights[li][0], layer._qkv_b)
+            else:
+                h = ops.rmsnorm(x, layer.input_layernorm.weight, cfg.rms_norm_eps)
+                # short chunks: projection + RoPE + cache append in one kernel; else two kernels
+                if fused_rope:
+                    qkv = ops.linear_qkv_rope(h, layer._qkv_w, layer._qkv_b, table, Hq, Hkv, D, cache.k(li),
+                                              cache.v(li), cache.page_table, p0, static_w=True)
+            appended = eights is None and qkv is not None
+            if not appended:
+                if qkv is None:
+                    qkv = ops.linear(h, layer._qkv_w, layer._qkv_b, static_w=True)
                 if table is not None:
                     ops.rope_kv_append_table(qkv, table, Hq, Hkv, D, cache.k(li), cache.v(li),
                                              cache.page_table, p0)
@@ -246,12 +276,23 @@ class Qwen2ForCausalLM(nn.Module):
             q = qkv.view(S, Hq + 2 * Hkv, D)[:, :Hq]
             attn = ops.fmha(q, cache.k(li), cache.v(li), B=1, Sq=S, Sk=p0 + S, causal=True,
                             scale=D ** -0.5, page_table=cache.page_table)
+            if eights is not None:
+                y = self._fp8_rest(layer, eights[li], x, attn.view(S, Hq * D))
+                continue
             ops.linear(attn.view(S, Hq * D), layer.self_attn.o_proj.weight, residual=x, out=x, static_w=True)
             h = ops.rmsnorm(x, layer.post_attention_layernorm.weight, cfg.rms_norm_eps)
             a = ops.linear(h, layer._gu_w, swiglu=True, static_w=True)
             ops.linear(a, layer.mlp.down_proj.weight, residual=x, out=x, static_w=True)
+        if y is not None:
+            x.add_(y)
         cache.length = p0 + S
         return x
+
+    def _fp8_rest(self, layer, eights, x: torch.Tensor, attn: torch.Tensor) -> torch.Tensor:
+        """x += the attention's projection, in place; -> the feed-forward's result, which the next norm adds."""
+        y = ops.fp8_linear(attn, eights[1])
+        h, _ = ops.fp8_rmsnorm(x, layer.post_attention_layernorm.weight, self.config.rms_norm_eps, residual=y, out=x)
+        return ops.fp8_linear(ops.fp8_linear(h, eights[2], swiglu=True, to8=True), eights[3])
 
     def logits_from_hidden(self, hidden: torch.Tensor) -> torch.Tensor:
         """final RMSNorm + lm_head for the given rows [R, hidden] -> [R, V] (bf16 like HF)."""
@@ -275,9 +316,14 @@ class Qwen2ForCausalLM(nn.Module):
         lens = [int(n) for n in seqlens_in_batch.tolist()]
         assert sum(lens) <= T, "seqlens_in_batch exceed the packed length"
         pos = position_ids[0].to(device=self.device, dtype=torch.int32).clamp(min=0).contiguous()
-        for layer in self.model.layers:
-            h = ops.rmsnorm(x, layer.input_layernorm.weight, cfg.rms_norm_eps)
-            qkv = ops.linear(h, layer._qkv_w, layer._qkv_b, static_w=True)
+        eights, y = self._fp8_weights() if T > 0 else None, None
+        for li, layer in enumerate(self.model.layers):
+            if eights is not None:
+                h, x = ops.fp8_rmsnorm(x, layer.input_layernorm.weight, cfg.rms_norm_eps, residual=y, out=None if y is None else x)
+                qkv = ops.fp8_linear(h, eights[li][0], layer._qkv_b)
+            else:
+                h = ops.rmsnorm(x, layer.input_layernorm.weight, cfg.rms_norm_eps)
+                qkv = ops.linear(h, layer._qkv_w, layer._qkv_b, static_w=True)
             ops.rope_kv_append(qkv, pos, Hq, Hkv, D, self.inv_freq)  # RoPE in place, no cache
             q3 = qkv.view(T, Hq + 2 * Hkv, D)
             attn = torch.zeros(T, Hq, D, dtype=self.dtype, device=self.device)
@@ -287,10 +333,15 @@ class Qwen2ForCausalLM(nn.Module):
                     ops.fmha(q3[o:o + n, :Hq], q3[o:o + n, Hq:Hq + Hkv], q3[o:o + n, Hq + Hkv:], B=1,
                              Sq=n, Sk=n, causal=True, scale=D ** -0.5, out=attn[o:o + n])
                 o += n
+            if eights is not None:
+                y = self._fp8_rest(layer, eights[li], x, attn.view(T, Hq * D))
+                continue
             ops.linear(attn.view(T, Hq * D), layer.self_attn.o_proj.weight, residual=x, out=x, static_w=True)
             h = ops.rmsnorm(x, layer.post_attention_layernorm.weight, cfg.rms_norm_eps)
             a = ops.linear(h, layer._gu_w, swiglu=True, static_w=True)
             ops.linear(a, layer.mlp.down_proj.weight, residual=x, out=x, static_w=True)
+        if y is not None:
+            x.add_(y)
         return self.logits_from_hidden(x)[None]
 
     def forward(self, inputs_embeds: torch.Tensor, attention_mask: Optional[torch.Tensor] = None,

@@ -31,7 +31,7 @@ def language_model_architecture(model_dir) -> Optional[str]:
     return arch if arch in LANGUAGE_MODELS else None
 
 
-# The layers' weights that linear_any alone reads, by class: these may be held in 4 bits.  Projections that a recurrence's step size or
+# The layers' weights that linear_any alone reads, by class: these may be held in 4 or 8 bits.  Projections that a recurrence's step size or
 # decay comes from stay as they are (an error in them compounds over the state), as do embeddings, routers, experts, norms and the output
 # head.  Where such rows end a fused weight, the layer's `exact_from` says from which row on.
 MX4_WEIGHTS: Dict[str, tuple] = {
@@ -43,20 +43,26 @@ MX4_WEIGHTS: Dict[str, tuple] = {
 }
 
 
-def quantize_weights(model):
-    """Hold a bf16 language model's layer weights as microscaled 4-bit rows (ops.Mx4: 17 bytes per 32 of them instead of 64), each
-    rounded to the nearest number of its block; rows that step sizes and decays come from, and activations, stay bf16.  In place; -> model.
+WEIGHT_BITS = {"mx4": 4, "fp8": 8}
+
+
+def quantize_weights(model, to: str = "mx4"):
+    """Hold a bf16 language model's layer weights as microscaled 4-bit rows (to="mx4"; ops.Mx4: 17 bytes per 32 of them instead of 64) or as e4m3
+    numbers with a scale per 128 x 128 (to="fp8"; ops.Fp8: half the bytes), each rounded to the nearest number of its block; rows that step
+    sizes and decays come from, and activations, stay bf16 (on 8-bit weights a layer's rows are quantised within the layer).  In place; -> model.
     state_dict and save_pretrained still give the weights that were loaded, which the model keeps where they were: on the host after from_pretrained.  A model
     made from tensors on the GPU keeps those there, too, and then takes more of its memory, not less.  A TokenEngine that runs the
     model captures its decode steps anew at its next step; what it cached for its sequences stays as the former weights made it.
     Not while another thread runs a step of the model."""
     from .. import ops
+    if to not in WEIGHT_BITS:
+        raise ValueError(f"to={to!r}: one of {sorted(WEIGHT_BITS)}")
     arch = next((a for a, c in LANGUAGE_MODELS.items() if type(model) is c), None)
     names = MX4_WEIGHTS.get(arch)
     if names is None:
-        raise ValueError(f"{type(model).__name__} does not hold weights in 4 bits (those that do: {sorted(MX4_WEIGHTS)})")
+        raise ValueError(f"{type(model).__name__} does not hold weights in {WEIGHT_BITS[to]} bits (those that do: {sorted(MX4_WEIGHTS)})")
     if model.dtype != torch.bfloat16:
-        raise ValueError(f"4-bit weights go with bfloat16 activations, not {model.dtype}")
+        raise ValueError(f"{WEIGHT_BITS[to]}-bit weights go with bfloat16 activations, not {model.dtype}")
     if torch.device(model.device).type == "cuda":
         torch.cuda.synchronize(model.device)      # no step that reads the replaced weights is under way, on whichever stream
     model.weights_version = getattr(model, "weights_version", 0) + 1
@@ -67,20 +73,21 @@ def quantize_weights(model):
                 first = getattr(layer, "exact_from", {}).get(name, w.shape[0])
                 first = first // 8 * 8 if first < w.shape[0] else first      # the kept rows' results start on a 16-byte boundary
                 if first > 0:
-                    setattr(layer, name, ops.mx4_quantize(w, keep=w.shape[0] - first))
+                    keep = w.shape[0] - first
+                    setattr(layer, name, ops.mx4_quantize(w, keep=keep) if to == "mx4" else ops.fp8_quantize(w, block_rows=ops.FP8_BLOCK, keep=keep))
     return model
 
 
 def load_language_model(model_dir, device="cuda", dtype="bfloat16", weights: Optional[str] = None):
-    """weights: None (as dtype says) or "mx4" (quantize_weights)"""
-    if weights not in (None, "mx4"):
-        raise ValueError(f"weights={weights!r}: None or 'mx4'")
+    """weights: None (as dtype says), "mx4" or "fp8" (quantize_weights)"""
+    if weights is not None and weights not in WEIGHT_BITS:
+        raise ValueError(f"weights={weights!r}: None or 'mx4' or 'fp8'")
     arch = language_model_architecture(model_dir)
     if arch is None:
         raise ValueError(f"{model_dir}: config.json names no registered architecture "
                          f"(known: {sorted(LANGUAGE_MODELS)})")
     dt = _DTYPES[dtype] if isinstance(dtype, str) else dtype
     if weights is not None and (arch not in MX4_WEIGHTS or dt != torch.bfloat16):      # before anything is loaded
-        raise ValueError(f"{arch} in {dt}: 4-bit weights are for {sorted(MX4_WEIGHTS)} in bfloat16")
+        raise ValueError(f"{arch} in {dt}: {WEIGHT_BITS[weights]}-bit weights are for {sorted(MX4_WEIGHTS)} in bfloat16")
     model = LANGUAGE_MODELS[arch].from_pretrained(model_dir, device=device, dtype=dt)
-    return model if weights is None else quantize_weights(model)
+    return model if weights is None else quantize_weights(model, weights)

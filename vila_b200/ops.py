@@ -704,7 +704,12 @@ def linear_any(x: torch.Tensor, w: torch.Tensor, *, swiglu: bool = False, out_dt
                glu_clamp: Optional[Tuple[float, float]] = None, geglu: bool = False) -> torch.Tensor:
     """act(x [M, K] · w[N, K]^T + bias): bf16 operands with 16-byte aligned rows go to the tcgen05 GEMM,
     everything else (fp32 tensors, odd shapes, an fp32 result) to the CUDA-core grouped kernel.  w may be an Mx4
-    (mx4_quantize): bf16 rows on 4-bit weights, a bf16 result."""
+    (mx4_quantize): bf16 rows on 4-bit weights, a bf16 result; or an Fp8 (fp8_quantize with block_rows 128): rows that are quantised
+    first, on 8-bit weights, a bf16 result."""
+    if isinstance(w, Fp8):
+        if out_dtype not in (None, torch.bfloat16):
+            raise RuntimeError(f"vila_b200.ops: a linear layer on 8-bit weights gives bfloat16, not {out_dtype}")
+        return fp8_linear(x, w, bias, act=act, act_params=act_params, swiglu=swiglu, geglu=geglu, glu_clamp=glu_clamp)
     if isinstance(w, Mx4):
         if out_dtype not in (None, torch.bfloat16):
             raise RuntimeError(f"vila_b200.ops: a linear layer on 4-bit weights gives bfloat16, not {out_dtype}")
@@ -1547,14 +1552,14 @@ class Fp8:
             q._lds = blocks
             n = (rows + 127) // 128 * blocks
         q._at = rows * q._ldc
-        q._both = like.new_empty(q._at + 4 * n, dtype=torch.uint8)
+        q._both = like.new_empty(q._at + 4 * n, dtype=_E4M3)
         return q
 
     @property
     def codes(self) -> torch.Tensor:
         """float8_e4m3fn [rows, cols]"""
         if self._codes is None:
-            self._codes = self._both.view(_E4M3).as_strided((self.rows, self.cols), (self._ldc, 1))
+            self._codes = self._both.as_strided((self.rows, self.cols), (self._ldc, 1))
         return self._codes
 
     @property
@@ -1588,6 +1593,29 @@ class Fp8:
         return self.rows * self._ldc + 4 * self._lds * ((self.cols + 127) // 128 if self.block_rows == 1 else (self.rows + 127) // 128)
 
 
+class Fp8Kept(Fp8):
+    """An 8-bit weight of which the last rows stay the bf16 numbers that they were (fp8_quantize's keep): `part` the 8-bit rows before them, `kept`
+    the others [keep, cols].  A weight of fp8_linear and linear_any with bf16 rows; it has no codes and scales of its own."""
+
+    __slots__ = ("part", "kept")
+
+    def __init__(self, part: Fp8, kept: torch.Tensor):
+        self.part, self.kept = part, kept
+        self.rows, self.cols, self.block_rows = part.rows + kept.shape[0], part.cols, part.block_rows
+
+    def _held(self) -> torch.Tensor:
+        return self.part._held()
+
+    def _ptrs(self):
+        raise RuntimeError("vila_b200.ops: rows kept in bf16 have no codes and scales (fp8_linear and fp8_dequantize take them)")
+
+    codes = scales = property(_ptrs)
+
+    @property
+    def nbytes(self) -> int:
+        return self.part.nbytes + self.kept.numel() * 2
+
+
 def _fp8_check(ok: bool, what: str) -> None:
     if not ok:
         raise RuntimeError(f"vila_b200.ops: {what}")
@@ -1609,20 +1637,32 @@ def _fp8_shape(codes: torch.Tensor, scales: torch.Tensor, block_rows: int) -> No
                f"scales must be float32 {list(want)} on the codes' device")
 
 
-def fp8_quantize(x: torch.Tensor, block_rows: int = 1) -> Fp8:
+def _fp8_rows(x: torch.Tensor, name: str) -> int:
+    """Checks of rows of numbers; -> their type's code."""
+    _mx4_here(x, name)
+    if x.dim() != 2 or x.shape[1] == 0 or (x.stride(1) != 1 and x.shape[1] != 1):
+        raise RuntimeError(f"vila_b200.ops: {name} must be [rows, cols] with consecutive columns")
+    dt = _DT.get(x.dtype)
+    if dt is None:
+        raise RuntimeError(f"vila_b200.ops: {name} must be bfloat16 or float32, got {x.dtype}")
+    return dt
+
+
+def fp8_quantize(x: torch.Tensor, block_rows: int = 1, keep: int = 0) -> Fp8:
     """x [rows, cols] bf16 or fp32 (a view with a row stride is fine) -> Fp8.  Per block of 128 columns of block_rows rows (1: activations,
     128: weights) with largest magnitude m the scale is s = max(m / 448, 2^-126), and x * (1 / s) becomes the nearest e4m3 number, ties to
-    even.  A block with an infinity or a NaN reads as NaN."""
-    _mx4_here(x, "x")
-    if x.dim() != 2 or x.shape[1] == 0 or (x.stride(1) != 1 and x.shape[1] != 1):
-        raise RuntimeError("vila_b200.ops: x must be [rows, cols] with consecutive columns")
+    even.  A block with an infinity or a NaN reads as NaN.
+    keep: the last rows of a bf16 weight that stay as they are, copied (Fp8Kept)."""
+    dt = _fp8_rows(x, "x")
     if block_rows != 1 and block_rows != FP8_BLOCK:
         raise RuntimeError(f"vila_b200.ops: block_rows={block_rows}: 1 or 128")
-    dt = _dt(x, "x")
     rows, cols = x.shape
+    if keep:
+        _fp8_check(block_rows == FP8_BLOCK and 0 < keep < rows and x.dtype == torch.bfloat16, f"keep={keep}: some of {rows} bf16 rows of a weight, not all of them")
+        return Fp8Kept(fp8_quantize(x[:rows - keep], FP8_BLOCK), x[rows - keep:].clone(memory_format=torch.contiguous_format))
     q = Fp8._alloc(x, rows, cols, block_rows)
-    codes, scales = q._ptrs()
-    check(_lib.load().vila_fp8_quantize(x.data_ptr(), dt, x.stride(0), codes, q._ldc, scales, q._lds, rows, cols, block_rows, _stream()),
+    codes = q._both.data_ptr()
+    check(_lib.load().vila_fp8_quantize(x.data_ptr(), dt, x.stride(0), codes, q._ldc, codes + q._at, q._lds, rows, cols, block_rows, _stream()),
           "vila_fp8_quantize")
     return q
 
@@ -1632,6 +1672,9 @@ def fp8_dequantize(q: Fp8, out_dtype=torch.bfloat16) -> torch.Tensor:
     held = q._held()
     _mx4_here(held, "q")
     out = held.new_empty((q.rows, q.cols), dtype=out_dtype)
+    if isinstance(q, Fp8Kept):
+        out[q.part.rows:].copy_(q.kept)
+        q = q.part
     codes, scales = q._ptrs()
     check(_lib.load().vila_fp8_dequantize(codes, q._ldc, scales, q._lds, out.data_ptr(), _dt(out, "out"), q.cols, q.rows, q.cols, q.block_rows,
                                           _stream()), "vila_fp8_dequantize")
@@ -1660,31 +1703,30 @@ def fp8_rmsnorm(x: torch.Tensor, w: Optional[torch.Tensor], eps: float, *, resid
     """The norm before a layer on 8-bit rows: s = x + residual (rounded to x's type), s / sqrt(mean(s^2) + eps) * w in 8 bits (block_rows 1).
     -> (Fp8, s); without a residual s is x.  x, residual [rows, cols] bf16 or fp32 (views with a row stride are fine), w [cols] bf16 or fp32
     or None.  out: where s goes, x itself for an update in place."""
-    _mx4_here(x, "x")
-    if x.dim() != 2 or x.shape[1] == 0 or (x.stride(1) != 1 and x.shape[1] != 1):
-        raise RuntimeError("vila_b200.ops: x must be [rows, cols] with consecutive columns")
+    dt = _fp8_rows(x, "x")
     rows, cols = x.shape
-    dt, w_ptr, w_dt, r_ptr, r_dt, ldr, s_ptr, ld_sum, total = _dt(x, "x"), None, 0, None, 0, 0, None, 0, x
+    w_ptr, w_dt, r_ptr, r_dt, ldr, s_ptr, ld_sum, total = None, 0, None, 0, 0, None, 0, x
     if w is not None:
         _mx4_here(w, "w")
         w_ptr, w_dt = w.data_ptr(), _dt(w, "w")
-        _fp8_check(w.numel() == cols and w.is_contiguous(), f"w must be contiguous [{cols}]")
+        _fp8_check(w.shape == (cols,) and w.is_contiguous(), f"w must be contiguous [{cols}]")
     if residual is not None:
-        _mx4_here(residual, "residual")
-        _fp8_check(residual.shape == x.shape and (residual.stride(1) == 1 or cols == 1), f"residual must be [{rows}, {cols}] with consecutive columns")
-        r_ptr, r_dt, ldr = residual.data_ptr(), _dt(residual, "residual"), residual.stride(0)
+        r_dt = _fp8_rows(residual, "residual")
+        _fp8_check(residual.shape == x.shape, f"residual must be [{rows}, {cols}]")
+        r_ptr, ldr = residual.data_ptr(), residual.stride(0)
         if out is None:
             total = x.new_empty((rows, cols))
+            ld_sum = cols
         else:
-            _mx4_here(out, "out")
-            _fp8_check(out.shape == x.shape and out.dtype == x.dtype and (out.stride(1) == 1 or cols == 1), f"out must be [{rows}, {cols}] of x's type")
-            total = out
-        s_ptr, ld_sum = total.data_ptr(), total.stride(0)
+            _fp8_rows(out, "out")
+            _fp8_check(out.shape == x.shape and out.dtype == x.dtype, f"out must be [{rows}, {cols}] of x's type")
+            total, ld_sum = out, out.stride(0)
+        s_ptr = total.data_ptr()
     elif out is not None:
         raise RuntimeError("vila_b200.ops: out goes with a residual")
     q = Fp8._alloc(x, rows, cols, 1)
-    codes, scales = q._ptrs()
-    check(_lib.load().vila_fp8_rmsnorm(x.data_ptr(), dt, x.stride(0), r_ptr, r_dt, ldr, s_ptr, ld_sum, w_ptr, w_dt, eps, codes, q._ldc, scales,
+    codes = q._both.data_ptr()
+    check(_lib.load().vila_fp8_rmsnorm(x.data_ptr(), dt, x.stride(0), r_ptr, r_dt, ldr, s_ptr, ld_sum, w_ptr, w_dt, eps, codes, q._ldc, codes + q._at,
                                        q._lds, rows, cols, _stream()), "vila_fp8_rmsnorm")
     return q, total
 
@@ -1695,14 +1737,21 @@ def fp8_linear(a, w: Fp8, bias: Optional[torch.Tensor] = None, *, act: int = ACT
     """act(a [M, K] . w[N, K]^T + bias) in bf16, or with to8 as Fp8 rows (quantised unrounded: what the next layer reads).  a: Fp8 with
     block_rows 1, or bf16 / fp32 rows, which are quantised first; w: Fp8 with block_rows 128.  fp32 sums.  Activations and gated units as
     in linear / glinear."""
-    if isinstance(a, torch.Tensor):
-        a = fp8_quantize(a)
-    if not (isinstance(a, Fp8) and isinstance(w, Fp8) and a.block_rows == 1 and w.block_rows == FP8_BLOCK):
+    if not isinstance(w, Fp8) or w.block_rows != FP8_BLOCK or not (isinstance(a, torch.Tensor) or (isinstance(a, Fp8) and a.block_rows == 1)):
         raise RuntimeError("vila_b200.ops: a must be Fp8 rows (block_rows 1) or a tensor, w an Fp8 weight (block_rows 128)")
     held = w._held()
     _mx4_here(held, "w")
-    _mx4_here(a._held(), "a")
-    M, K, N = a.rows, a.cols, w.rows
+    x_ptr, ldx, x_dt, a_codes, lda, a_scales, ld_as = None, 0, 0, None, 0, None, 0
+    if isinstance(a, Fp8):
+        _mx4_here(a._held(), "a")
+        M, K = a.rows, a.cols
+        a_codes, a_scales = a._ptrs()
+        lda, ld_as = a._ldc, a._lds
+    else:
+        x_dt = _fp8_rows(a, "a")
+        M, K = a.shape
+        x_ptr, ldx = a.data_ptr(), a.stride(0)
+    N = w.rows
     if K != w.cols or N == 0:
         raise RuntimeError(f"vila_b200.ops: {M} x {K} rows do not fit a weight of {N} x {w.cols}")
     flags = (1 if swiglu else 0) | (4 if glu_clamp is not None else 0) | (FLAG_GEGLU if geglu else 0)
@@ -1729,14 +1778,27 @@ def fp8_linear(a, w: Fp8, bias: Optional[torch.Tensor] = None, *, act: int = ACT
         o_ptr, ldo, y = out.data_ptr(), out.stride(0), out
     if M == 0:
         return y
+    if isinstance(w, Fp8Kept):
+        n = w.part.rows
+        _fp8_check(isinstance(a, torch.Tensor) and a.dtype == torch.bfloat16 and not to8, "rows kept in bf16 go with bf16 rows and a bf16 result")
+        _fp8_check(not flags or (n % 2 == 0 and N % 2 == 0), "a gated unit has an even number of weight rows, in 8 bits and kept")
+        cut = n // 2 if flags else n
+        more = dict(act=act, act_params=act_params, swiglu=swiglu, geglu=geglu, glu_clamp=glu_clamp)
+        fp8_linear(a, w.part, None if bias is None else bias[:n], out=out[:, :cut], **more)
+        rest, to = None if bias is None else bias[n:], out[:, cut:]
+        if (act == ACT_NONE and not flags and K % 8 == 0 and (N - n) % 8 == 0 and a.stride(0) % 8 == 0 and a.stride(0) >= K and a.data_ptr() % 16 == 0
+                and to.stride(0) % 8 == 0 and to.data_ptr() % 16 == 0):
+            linear(a, w.kept, rest, static_w=True, out=to)
+        else:      # with an activation: glinear rounds once, behind it, as the 8-bit rows' kernels do
+            glinear(a, w.kept, out=to, bias=rest, **more)
+        return out
     alpha, limit = glu_clamp if glu_clamp is not None else (0.0, 0.0)
     pos, neg = act_params if act_params is not None else (0.0, 0.0)
-    a_codes, a_scales = a._ptrs()
     w_codes, w_scales = w._ptrs()
-    p = _lib.Fp8LinearParams(a_codes, a._ldc, a_scales, a._lds, w_codes, w._ldc, w_scales, w._lds, None if bias is None else bias.data_ptr(), o_ptr, ldo,
-                             o_codes, ld_oc, o_scales, ld_os, alpha, limit, pos, neg, M, N, K, act, flags)
+    p = _lib.Fp8LinearParams(x_ptr, ldx, a_codes, lda, a_scales, ld_as, w_codes, w._ldc, w_scales, w._lds, None if bias is None else bias.data_ptr(), o_ptr,
+                             ldo, o_codes, ld_oc, o_scales, ld_os, alpha, limit, pos, neg, M, N, K, act, flags, x_dt)
     lib = _lib.load()
-    if to8:      # a workspace of the call's own: a captured graph keeps its own, too
+    if to8 or x_ptr is not None:      # a workspace of the call's own: a captured graph keeps its own, too
         n = lib.vila_fp8_linear_scratch(C.byref(p))
         if n:
             scratch = held.new_empty(n, dtype=torch.uint8)
