@@ -53,8 +53,9 @@ __device__ __forceinline__ void mx4_store_row(const P& p, const vila_glinear_ext
   constexpr int kWords = kGated ? 8 : 16;
   if (p.bias != nullptr) {
     const __nv_bfloat16* bias = static_cast<const __nv_bfloat16*>(p.bias);
+    // Not by __ldg: of bf16 it is assembly without a side effect, which the compiler may run where the condition does not hold.
 #pragma unroll
-    for (int i = 0; i < 32; ++i) z[i] += n + i < p.N ? __bfloat162float(__ldg(bias + n + i)) : 0.f;
+    for (int i = 0; i < 32; ++i) z[i] += n + i < p.N ? __bfloat162float(bias[n + i]) : 0.f;
   }
   if (m >= p.M) return;
   uint32_t h[kWords];
