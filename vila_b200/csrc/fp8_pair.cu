@@ -239,7 +239,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
         if (p.bias != nullptr) {
           const __nv_bfloat16* bias = static_cast<const __nv_bfloat16*>(p.bias);
 #pragma unroll
-          for (int i = 0; i < 128; ++i) z[i] += n0 + i < p.N ? __bfloat162float(__ldg(bias + n0 + i)) : 0.f;
+          for (int i = 0; i < 128; ++i) z[i] += n0 + i < p.N ? __bfloat162float(bias[n0 + i]) : 0.f;
         }
         mx4_with_epilogue(p, [&](auto epi) {
           constexpr int EPI = decltype(epi)::value;

@@ -11,13 +11,12 @@
 //   epilogue warps  two blocks at a time: scales times accumulators, added up
 //
 // Up to 32 tokens (kSwap): weight rows are the 128 lanes of a tile, tokens its columns, of which there are only as many as needed; bound by the
-// weights' bytes.  More tokens: these are the lanes, 128 weight rows the columns, so that a thread's scale is one number a block (as one a column
+// weights' bytes.  More tokens: these are the lanes, 64 or 128 weight rows the columns, so that a thread's scale is one number a block (as one a column
 // it took four loads from shared memory per 16 columns, in line with the loads from TMEM: 0.43 us a block instead of 0.3).  There a block
 // costs what an epilogue warp does for it one after another: a wait takes 150 - 250 clocks even if it is over, 16 columns of TMEM 70.
 //
 // A CTA takes one tile, or, where the tiles leave SMs idle, a share of its blocks: a cluster of up to 8 CTAs splits K, every CTA sends
-// its sums to the CTAs that finish them, by rows, and these add them in rank order.  Sums go through shared memory in any case, and a
-// loop of few instructions finishes them (written out for every register of a thread, what a launch of few blocks took was fetching it).
+// its sums to the CTAs that finish them, by rows, and these add them in rank order.
 //
 // A launch may begin before the one before it has ended: the first weights are asked for while that one ends, everything else comes behind
 // griddepcontrol.wait.  (Weights come from launches that do not let others begin early.)
@@ -27,14 +26,14 @@
 #include "glinear_epi.cuh"
 #include "kernels.h"
 #include "mx4.cuh"
+#include "mx4_epi.cuh"
 
 namespace vb {
 namespace {
 
 constexpr int kRows = 128;                    // lanes of a tile
 constexpr int kAcc = 4, kVisit = 2;            // accumulators in TMEM, and how many of them change hands together
-constexpr int kTogether = 8;                  // blocks whose scales change hands together
-static_assert(kTogether % kVisit == 0 && kAcc == 2 * kVisit, "");
+static_assert(kAcc == 2 * kVisit, "");
 
 __device__ __forceinline__ void umma_fp8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -48,32 +47,33 @@ __device__ __forceinline__ void umma_fp8(uint32_t d, uint64_t a, uint64_t b, uin
 __device__ __forceinline__ void st_dsmem_f32(uint32_t cluster_addr, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
 }
-__device__ __forceinline__ void st_dsmem_v4f(uint32_t cluster_addr, const float* v) {
-  asm volatile("st.shared::cluster.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(cluster_addr), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]) : "memory");
-}
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 template <int BN, bool kSwap> struct Shape {
-  static constexpr int kEpi = BN > 64 ? 16 : 4;                 // epilogue warps: a quarter of the lanes each; four share a quarter's columns
+  static constexpr int kEpi = BN > 64 ? 16 : (BN > 32 ? 8 : 4);      // epilogue warps: a quarter of the lanes each; the others share its columns
   static constexpr int kTma = kEpi, kMma = kEpi + 1, kScale = kEpi + 2, kThreads = 32 * (kEpi + 3);
-  static constexpr int kColumns = BN > 64 ? BN / 4 : BN;        // columns of a thread
+  static constexpr int kColumns = 4 * BN / kEpi;                 // columns of a thread
   static constexpr int kPBytes = kRows * 128, kQBytes = BN * 128, kStage = kPBytes + kQBytes;
-  static constexpr int kStages = BN == 16 ? 5 : 4;
-  static constexpr int kPerSm = BN > 64 ? 1 : 2;
+  static constexpr int kStages = BN == 16 ? 5 : (BN == 64 ? 3 : 4);
+  static constexpr int kTogether = BN == 64 ? 4 : 8;             // blocks whose scales change hands together
+  static constexpr int kPerSm = BN > 64 ? 1 : 2;                 // two: a launch's first weights come while the one before it ends
   static constexpr int kCols = kAcc * BN;                        // of TMEM
   static constexpr int kTokens = kSwap ? BN : kRows;             // of a tile
-  static constexpr int kPitch = kSwap ? 0 : BN + 4;              // of a token's sums, so that lanes with a token each meet different banks
-  static constexpr int kSums = kSwap ? BN * kRows : kRows * kPitch;
-  static constexpr size_t kSmem = 1024 + static_cast<size_t>(kStages) * kStage + (2 * kTogether * kTokens + kSums) * 4 + 256;
+  static constexpr size_t kSmem = 1024 + static_cast<size_t>(kStages) * kStage + (2 * kTogether * kTokens + BN * (kRows + (kSwap ? 0 : 8))) * 4 + 256;
   static_assert(kCols == 64 || kCols == 128 || kCols == 256 || kCols == 512, "TMEM");
   static_assert(kCols * kPerSm <= 512, "TMEM of an SM");
   static_assert((kSmem + 1024) * kPerSm <= 228 * 1024, "shared memory");
+  static_assert(kTogether % kVisit == 0 && (kSwap || kColumns == 32), "");
+  static_assert(kSwap || (kEpi * 1024 <= BN * kRows && kThreads / 32 * 4096 <= kStages * kStage), "slabs");
 };
 
-// What becomes of the sums of token m, weight rows n .. n + 3 (n a multiple of 4).  out32: unrounded, rows of ld32 columns.  `wide`: four
+// kSwap: what becomes of the sums of token m, weight rows n .. n + 3 (n a multiple of 4).  out32: unrounded, rows of ld32 columns.  `wide`: four
 // results of out lie on an 8-byte boundary.  The fast exponentials are off by some 2^-21, under either rounding that follows.
+template <int EPI>
 __device__ __forceinline__ void finish(const vila_fp8_linear_params& p, const vila_glinear_ext& x, float* out32, int ld32, bool wide, int m, int n, float4 sums) {
+  constexpr bool kGated = EPI >= kMx4Gated;
+  constexpr int kOut = kGated ? 2 : 4;
   if (m >= p.M || n >= p.N) return;
   float z[4] = {sums.x, sums.y, sums.z, sums.w};
   if (p.bias != nullptr) {
@@ -82,39 +82,69 @@ __device__ __forceinline__ void finish(const vila_fp8_linear_params& p, const vi
     for (int j = 0; j < 4; ++j)
       if (n + j < p.N) z[j] += __bfloat162float(bias[j]);
   }
-  const bool gated = (p.flags & kGluFlags) != 0;
-  if (gated) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const float g = z[2 * j], u = z[2 * j + 1];
-      z[j] = p.flags & VILA_FLAG_GLU_CLAMP ? glu_clamp_fast_f(g, u, x.act_alpha, x.act_limit) : (p.flags & VILA_FLAG_GEGLU ? gelu_tanh_f(g) : silu_f(g)) * u;
-    }
-  } else if (p.act != VILA_ACT_NONE) {
-#pragma unroll 1
-    for (int j = 0; j < 4; ++j) {
-      const float v = z[0];      // in turn, so that the activations are there once
-      z[0] = z[1];
-      z[1] = z[2];
-      z[2] = z[3];
-      z[3] = p.act == VILA_ACT_SILU ? silu_f(v) : (p.act == VILA_ACT_GELU_TANH ? gelu_tanh_f(v) : (p.act == VILA_ACT_XIELU ? xielu_fast_f(v, x.act_pos, x.act_neg) : activate(v, p.act, x)));
-    }
-  }
-  const int cols = gated ? p.N / 2 : p.N, o = gated ? n / 2 : n, count = gated ? 2 : 4;
+  for (int j = 0; j < kOut; ++j) z[j] = kGated ? mx4_glu<EPI>(z[2 * j % 4], z[(2 * j + 1) % 4], x) : mx4_act<EPI>(z[j], x);
+  const int cols = kGated ? p.N / 2 : p.N, o = kGated ? n / 2 : n;
   if (out32 != nullptr) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (j < count && o + j < cols) out32[static_cast<size_t>(m) * ld32 + o + j] = z[j];
+    for (int j = 0; j < kOut; ++j)
+      if (o + j < cols) out32[static_cast<size_t>(m) * ld32 + o + j] = z[j];
     return;
   }
   __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out) + static_cast<size_t>(m) * p.ldo + o;
-  if (wide && o + count <= cols) {
-    if (gated) *reinterpret_cast<uint32_t*>(out) = pack_bf16(z[0], z[1]);
+  if (wide && o + kOut <= cols) {
+    if (kGated) *reinterpret_cast<uint32_t*>(out) = pack_bf16(z[0], z[1]);
     else *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(z[0], z[1]), pack_bf16(z[2], z[3]));
   } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (j < count && o + j < cols) out[j] = __float2bfloat16_rn(z[j]);
+    for (int j = 0; j < kOut; ++j)
+      if (o + j < cols) out[j] = __float2bfloat16_rn(z[j]);
   }
+}
+// Without kSwap: of 32 tokens, a lane's m, those below `end`, and weight rows n .. n + 31.  All lanes call it.  `wide`: rows of out lie on 32-byte
+// boundaries, and a lane writes its own; other rows change hands in `slab` (32 x 32, of this warp), so that neighbouring lanes write
+// neighbouring columns (77 rows of 1157 columns, one block: 8.9 us if each lane writes 2 bytes of a row of its own at a time).
+__device__ __forceinline__ void finish_rows(const vila_fp8_linear_params& p, const vila_glinear_ext& x, float* out32, int ld32, bool wide, int m, int end, int n,
+                                            float (&z)[32], float* slab) {
+  if (n >= p.N) return;
+  mx4_with_epilogue(p, [&](auto epi) {
+    constexpr int EPI = decltype(epi)::value;
+    constexpr bool kGated = EPI >= kMx4Gated;
+    constexpr int kOut = kGated ? 16 : 32, kRowsAtOnce = 32 / kOut;
+    const int cols = kGated ? p.N / 2 : p.N, o = kGated ? n / 2 : n, lane = threadIdx.x & 31;
+    if (p.bias != nullptr) {
+      const __nv_bfloat16* bias = static_cast<const __nv_bfloat16*>(p.bias);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) z[i] += n + i < p.N ? __bfloat162float(bias[n + i]) : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < kOut; ++i) z[i] = kGated ? mx4_glu<EPI>(z[2 * i % 32], z[(2 * i + 1) % 32], x) : mx4_act<EPI>(z[i], x);
+    if (out32 == nullptr && wide && o + kOut <= cols) {
+      if (m < end) {
+        uint32_t h[kOut / 2];
+#pragma unroll
+        for (int i = 0; i < kOut / 2; ++i) h[i] = pack_bf16(z[2 * i], z[2 * i + 1]);
+        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out) + static_cast<size_t>(m) * p.ldo + o;
+#pragma unroll
+        for (int i = 0; i < kOut; i += 16) mx4_stg32(out + i, h + i / 2);
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < kOut; ++i) slab[lane * 32 + (i ^ lane)] = z[i];
+    __syncwarp();
+    const int m0 = m - lane, c = lane % kOut;
+#pragma unroll 4
+    for (int r0 = 0; r0 < 32; r0 += kRowsAtOnce) {
+      const int r = r0 + lane / kOut;
+      const float v = slab[r * 32 + (c ^ r)];
+      if (m0 + r < end && o + c < cols) {
+        if (out32 != nullptr) out32[static_cast<size_t>(m0 + r) * ld32 + o + c] = v;
+        else static_cast<__nv_bfloat16*>(p.out)[static_cast<size_t>(m0 + r) * p.ldo + o + c] = __float2bfloat16_rn(v);
+      }
+    }
+    __syncwarp();
+  });
 }
 
 // bn: columns of a tile, with kSwap a multiple of 16, at most BN.  split: CTAs of a cluster, which share a tile and cut K.
@@ -127,8 +157,8 @@ fp8_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ C
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   float* scales = reinterpret_cast<float*>(smem + ST * S::kStage);      // [2][kTogether][token]: both scales of a token's block
-  float* sums = scales + 2 * kTogether * S::kTokens;      // of this CTA's share of the rows, by rank: [rank][column][row], or [rank][row][column]
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(sums + S::kSums);
+  float* sums = scales + 2 * S::kTogether * S::kTokens;      // of this CTA's share of the rows, by rank: [rank][column][row], without kSwap a column one longer
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(sums + BN * (kRows + (kSwap ? 0 : 8)));
   uint64_t* empty_bar = full_bar + ST;
   uint64_t* acc_full = empty_bar + ST;   // [2]: of up to kVisit blocks
   uint64_t* acc_free = acc_full + 2;     // [2]
@@ -170,7 +200,7 @@ fp8_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ C
   tc_fence_after();
   const uint32_t tmem = *tmem_ptr;
   const int ld32 = p.flags & kGluFlags ? p.N / 2 : p.N;
-  const bool wide = reinterpret_cast<uintptr_t>(p.out) % 8 == 0 && p.ldo % 4 == 0;
+  const bool wide = kSwap ? reinterpret_cast<uintptr_t>(p.out) % 8 == 0 && p.ldo % 4 == 0 : reinterpret_cast<uintptr_t>(p.out) % 32 == 0 && p.ldo % 16 == 0;
   bool ok = true;
   if (limit.quits >= 0) {
     ok = limit.quits != (warp == S::kTma ? 0 : warp == S::kMma ? 1 : warp == S::kScale ? 2 : 3);
@@ -257,11 +287,11 @@ fp8_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ C
     const float* sa = p.a_scales + (there ? t0 + lane * 4 : 0);
     const float* sw = p.w_scales + (n0 / kFp8Block) * p.ld_ws;
     int g = 0;
-    for (int kb = kb0; kb < kb1 && ok; kb += kTogether, ++g) {
-      float4 a[kTogether];
-      float w[kTogether];
+    for (int kb = kb0; kb < kb1 && ok; kb += S::kTogether, ++g) {
+      float4 a[S::kTogether];
+      float w[S::kTogether];
 #pragma unroll
-      for (int i = 0; i < kTogether; ++i) {
+      for (int i = 0; i < S::kTogether; ++i) {
         const bool in = there && kb + i < kb1;
         a[i] = in ? __ldg(reinterpret_cast<const float4*>(sa + (kb + i) * p.ld_as)) : make_float4(0.f, 0.f, 0.f, 0.f);
         w[i] = in ? __ldg(sw + kb + i) : 0.f;
@@ -270,8 +300,8 @@ fp8_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ C
       if (!ok) break;
       if (lane * 4 < S::kTokens) {
 #pragma unroll
-        for (int i = 0; i < kTogether; ++i)
-          *reinterpret_cast<float4*>(scales + ((g & 1) * kTogether + i) * S::kTokens + lane * 4) =
+        for (int i = 0; i < S::kTogether; ++i)
+          *reinterpret_cast<float4*>(scales + ((g & 1) * S::kTogether + i) * S::kTokens + lane * 4) =
               make_float4(fp8_both_scales(a[i].x, w[i]), fp8_both_scales(a[i].y, w[i]), fp8_both_scales(a[i].z, w[i]), fp8_both_scales(a[i].w, w[i]));
       }
       __syncwarp();
@@ -288,7 +318,7 @@ fp8_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ C
     for (int i = 0; i < S::kColumns; ++i) sum[i] = 0.f;
 #pragma unroll 1
     for (int kb = kb0; kb < kb1 && ok; kb += kVisit, ++v) {
-      const int in_group = (kb - kb0) % kTogether;
+      const int in_group = (kb - kb0) % S::kTogether;
       if (in_group == 0) {
         if (kb > kb0) {      // all lanes have read the group before: the warp has met since
           if (lane == 0) mbar_arrive(&scale_free[g & 1]);
@@ -297,7 +327,7 @@ fp8_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ C
         ok = mx4_warp_wait(&scale_full[g & 1], (g >> 1) & 1, gave_up, limit.tries);
         if (!ok) break;
       }
-      const float* both = scales + ((g & 1) * kTogether + in_group) * S::kTokens + (kSwap ? c0 : row);
+      const float* both = scales + ((g & 1) * S::kTogether + in_group) * S::kTokens + (kSwap ? c0 : row);
       float mine[kVisit];
 #pragma unroll
       for (int i = 0; i < kVisit; ++i) mine[i] = kSwap ? 0.f : both[i * S::kTokens];      // ahead of the loads from TMEM, which they would queue behind
@@ -332,24 +362,19 @@ fp8_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ C
     tc_fence_before();
     if (split == 1) {      // a warp finishes what it has summed up
       if (ok) {
-        if constexpr (kSwap) {
+        if constexpr (kSwap) {      // by a short loop: written out for every register, what a launch of few blocks took was fetching the code
 #pragma unroll
           for (int c = 0; c < S::kColumns; ++c) sums[(c0 + c) * kRows + row] = sum[c];
           __syncwarp();
+          mx4_with_epilogue(p, [&](auto epi) {
 #pragma unroll 1
-          for (int i = lane; i < S::kColumns * 8; i += 32) {
-            const int c = c0 + i / 8, r = quad * 32 + 4 * (i % 8);
-            if (c < bn) finish(p, x, out32, ld32, wide, t0 + c, n0 + r, *reinterpret_cast<const float4*>(sums + c * kRows + r));
-          }
+            for (int i = lane; i < S::kColumns * 8; i += 32) {
+              const int c = c0 + i / 8, r = quad * 32 + 4 * (i % 8);
+              if (c < bn) finish<decltype(epi)::value>(p, x, out32, ld32, wide, t0 + c, n0 + r, *reinterpret_cast<const float4*>(sums + c * kRows + r));
+            }
+          });
         } else {
-#pragma unroll
-          for (int c = 0; c < S::kColumns; c += 4) *reinterpret_cast<float4*>(sums + row * S::kPitch + c0 + c) = make_float4(sum[c], sum[c + 1], sum[c + 2], sum[c + 3]);
-          __syncwarp();
-#pragma unroll 1
-          for (int i = lane; i < 32 * S::kColumns / 4; i += 32) {
-            const int r = quad * 32 + i / (S::kColumns / 4), c = c0 + 4 * (i % (S::kColumns / 4));
-            finish(p, x, out32, ld32, wide, t0 + r, n0 + c, *reinterpret_cast<const float4*>(sums + r * S::kPitch + c));
-          }
+          finish_rows(p, x, out32, ld32, wide, t0 + row, p.M, n0 + c0, sum, sums + warp * 1024);      // nobody else's sums are there
         }
       }
     } else {               // the rows' sums to the CTAs that finish them
@@ -357,13 +382,8 @@ fp8_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ C
       const int share = kRows / split, owner = row / share, at = row - owner * share;
       const uint32_t to = mapa_u32(smem_u32(sums), owner);
       if (ok) {
-        if constexpr (kSwap) {
 #pragma unroll
-          for (int c = 0; c < S::kColumns; ++c) st_dsmem_f32(to + ((rank * BN + c0 + c) * share + at) * 4, sum[c]);
-        } else {
-#pragma unroll
-          for (int c = 0; c < S::kColumns; c += 4) st_dsmem_v4f(to + ((rank * share + at) * S::kPitch + c0 + c) * 4, sum + c);
-        }
+        for (int c = 0; c < S::kColumns; ++c) st_dsmem_f32(to + ((rank * BN + c0 + c) * (share + (kSwap ? 0 : 1)) + at) * 4, sum[c]);
       }
       __syncwarp();
     }
@@ -379,16 +399,65 @@ fp8_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ C
     cluster_arrive();                         // behind this CTA's sums
     cluster_wait();
     const int share = kRows / split;
-    const int fours = (kSwap ? share : BN) / 4, lines = kSwap ? min(bn, p.M - q0) : share;
+    if constexpr (kSwap) {
+      const int fours = share / 4, items = min(bn, p.M - q0) * fours;
+      mx4_with_epilogue(p, [&](auto epi) {
 #pragma unroll 1
-    for (int i = tid; i < lines * fours; i += S::kThreads) {
-      const int l = i / fours, f = 4 * (i - l * fours);
-      float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int q = 0; q < split; ++q) {
-        const float4 part = *reinterpret_cast<const float4*>(sums + (kSwap ? (q * BN + l) * share + f : (q * share + l) * S::kPitch + f));
-        z = make_float4(z.x + part.x, z.y + part.y, z.z + part.z, z.w + part.w);
+        for (int i = tid; i < items; i += S::kThreads) {
+          const int c = i / fours, r = 4 * (i - c * fours);
+          float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int q = 0; q < split; ++q) {
+            const float4 part = *reinterpret_cast<const float4*>(sums + (q * BN + c) * share + r);
+            z = make_float4(z.x + part.x, z.y + part.y, z.z + part.z, z.w + part.w);
+          }
+          finish<decltype(epi)::value>(p, x, out32, ld32, wide, t0 + c, n0 + rank * share + r, z);
+        }
+      });
+    } else if (wide && out32 == nullptr) {      // a warp takes 32 rows by 32 columns
+      const int groups = (share + 31) / 32;
+#pragma unroll 1
+      for (int i = warp; i < groups * (BN / 32); i += S::kThreads / 32) {
+        const int r = i % groups * 32 + lane, c = i / groups * 32;
+        float z[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) z[j] = 0.f;
+#pragma unroll 1
+        for (int q = 0; q < split && r < share; ++q) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) z[j] += sums[(q * BN + c + j) * (share + 1) + r];
+        }
+        __syncwarp();
+        finish_rows(p, x, out32, ld32, wide, t0 + rank * share + r, min(p.M, t0 + (rank + 1) * share), n0 + c, z,
+                    reinterpret_cast<float*>(smem) + warp * 1024);      // the stages are done with
       }
-      finish(p, x, out32, ld32, wide, kSwap ? t0 + l : t0 + rank * share + l, kSwap ? n0 + rank * share + f : n0 + f, z);
+    } else {      // a warp takes 32 neighbouring results of a token at a time
+      mx4_with_epilogue(p, [&](auto epi) {
+        constexpr int EPI = decltype(epi)::value;
+        constexpr bool kGated = EPI >= kMx4Gated;
+        constexpr int kParts = kGated ? BN / 64 : BN / 32;
+        const int cols = kGated ? p.N / 2 : p.N, rows = min(share, p.M - t0 - rank * share);
+        const __nv_bfloat16* bias = static_cast<const __nv_bfloat16*>(p.bias);
+#pragma unroll 2
+        for (int i = warp; i < rows * kParts; i += S::kThreads / 32) {
+          const int r = i / kParts, c = (i - r * kParts) * 32 + lane, m = t0 + rank * share + r, o = (kGated ? n0 / 2 : n0) + c;
+          float z[2] = {0.f, 0.f};
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+#pragma unroll
+            for (int j = 0; j < (kGated ? 2 : 1); ++j)
+              if (q < split) z[j] += sums[(q * BN + (kGated ? 2 * c + j : c)) * (share + 1) + r];
+          }
+          if (o < cols) {
+            if (bias != nullptr) {
+#pragma unroll
+              for (int j = 0; j < (kGated ? 2 : 1); ++j) z[j] += __bfloat162float(bias[kGated ? 2 * o + j : o]);
+            }
+            const float v = kGated ? mx4_glu<EPI>(z[0], z[1], x) : mx4_act<EPI>(z[0], x);
+            if (out32 != nullptr) out32[static_cast<size_t>(m) * ld32 + o] = v;
+            else static_cast<__nv_bfloat16*>(p.out)[static_cast<size_t>(m) * p.ldo + o] = __float2bfloat16_rn(v);
+          }
+        }
+      });
     }
   }
   if (tid == 0 && *gave_up) {
@@ -406,10 +475,11 @@ int launch(const vila_fp8_linear_params& p, const vila_glinear_ext& x, float* ou
   CUtensorMap tw, ta;
   if (int rc = make_tmap_2d_u8(&tw, p.w_codes, p.N, p.K, p.ldw, kSwap ? kRows : BN, 128, 128)) return rc;
   if (int rc = make_tmap_2d_u8(&ta, p.a_codes, p.M, p.K, p.lda, kSwap ? bn : kRows, 128, 128)) return rc;
-  const long long tiles = static_cast<long long>((p.N + kRows - 1) / kRows) * (kSwap ? 1 : (p.M + kRows - 1) / kRows);
+  const long long tiles = kSwap ? (p.N + kRows - 1) / kRows : static_cast<long long>((p.N + BN - 1) / BN) * ((p.M + kRows - 1) / kRows);
   VB_CHECK(tiles < (1LL << 27), "fp8_linear: too many tiles (M=%d N=%d)", p.M, p.N);
   static Mx4Clusters clusters;
-  const int split = clusters.split(fp8_kernel<BN, kSwap>, S::kThreads, S::kSmem, tiles, fp8_blocks(p.K) / 2);
+  // of 4 blocks a cluster's joint end costs what it saves (77 rows of 1157 x 512: 7.2 us by two, 6.2 alone; x 1024 by 4 7.1, by 2 8.0)
+  const int blocks = fp8_blocks(p.K), split = clusters.split(fp8_kernel<BN, kSwap>, S::kThreads, S::kSmem, tiles, blocks < 8 ? 1 : blocks / 2);
   VB_CUDA(launch_pdl_cluster(fp8_kernel<BN, kSwap>, dim3(static_cast<unsigned>(tiles * split)), dim3(S::kThreads), S::kSmem, stream, dim3(split),
                              kSwap ? tw : ta, kSwap ? ta : tw, p, x, out32, bn, split, wait_limit(tries), failed_word()));
   return 0;
@@ -421,6 +491,8 @@ int fp8_tc(const vila_fp8_linear_params& p, const vila_glinear_ext& ext, float* 
   VB_CHECK(failed_word() != nullptr, "fp8_linear: no pinned host memory for the status word");
   if (p.M <= 16) return launch<16, true>(p, ext, out32, tries, stream);
   if (p.M <= 32) return launch<32, true>(p, ext, out32, tries, stream);
+  // Up to 128 tokens tiles of 64 weight rows, two CTAs an SM; beyond, tokens would be read too often.
+  if (p.M <= 128) return launch<64, false>(p, ext, out32, tries, stream);
   return launch<128, false>(p, ext, out32, tries, stream);
 }
 
