@@ -1,5 +1,6 @@
 """GPU: 8-bit rows with a scale per block of 128 against their restatement in float64."""
 import ctypes as C
+import gc
 import math
 
 import pytest
@@ -10,6 +11,13 @@ from tests.test_mx4_gpu import act64, act_args, check_product
 
 pytestmark = pytest.mark.gpu
 BF, E4M3 = torch.bfloat16, torch.float8_e4m3fn
+
+
+@pytest.fixture(autouse=True)
+def nothing_left_behind():
+    """Models and their captured steps refer to one another: they go here, and not while a later test captures."""
+    yield
+    gc.collect()
 
 
 def rand(seed, *shape, dtype=torch.float32):
