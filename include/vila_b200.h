@@ -968,9 +968,22 @@ int vila_fp8_quantize(const void* x, int x_dtype, int64_t ldx, void* codes, int6
                       int block_rows, void* stream);
 int vila_fp8_dequantize(const void* codes, int64_t ldc, const float* scales, int64_t lds, void* out, int out_dtype, int64_t ldo, int rows,
                         int cols, int block_rows, void* stream);
-int vila_fp8_rmsnorm(const void* x, int x_dtype, int64_t ldx, const void* residual, int residual_dtype, int64_t ldr, void* sum,
-                     int64_t ld_sum, const void* w, int w_dtype, float eps, void* codes, int64_t ldc, float* scales, int64_t lds, int rows,
-                     int cols, void* stream);
+typedef struct vila_fp8_rmsnorm_params {
+  const void* x;
+  int64_t ldx;
+  const void* residual;
+  int64_t ldr;
+  void* sum;
+  int64_t ld_sum;
+  const void* w;
+  void* codes;
+  int64_t ldc;
+  float* scales;
+  int64_t lds;
+  float eps;
+  int32_t rows, cols, x_dtype, residual_dtype, w_dtype;
+} vila_fp8_rmsnorm_params;
+int vila_fp8_rmsnorm(const vila_fp8_rmsnorm_params* p, void* stream);
 /* vila_fp8_linear: out[m, n] = epi(sum_k a[m, k] w[n, k] + bias[n]), a [M, K] with block_rows 1, w [N, K] with block_rows 128.  Products of a
  * block's numbers and their sum in fp32, times the product of both scales (fp32, cut at fp32's largest number), added in fp32 in the order of the
  * blocks (K over a cluster: each CTA's, then the CTAs').  Scales are finite, not negative, or NaN.  bias bf16 or NULL.  act, flags and their parameters as in

@@ -93,22 +93,23 @@ def test_entry_points_fail_without_a_device():
     lib = _lib.load()
     assert lib.vila_fp8_quantize(None, 0, 0, None, 0, None, 0, 1, 32, 1, None) != 0 and b"no CUDA device" in lib.vila_last_error()
     assert lib.vila_fp8_dequantize(None, 0, None, 0, None, 0, 0, 1, 32, 1, None) != 0
-    assert lib.vila_fp8_rmsnorm(None, 0, 0, None, 0, 0, None, 0, None, 0, 1e-6, None, 0, None, 0, 1, 32, None) != 0
+    assert lib.vila_fp8_rmsnorm(_lib.Fp8RmsnormParams(rows=1, cols=32), None) != 0
     assert lib.vila_fp8_linear(C.byref(_lib.Fp8LinearParams()), None) != 0
 
 
 def test_no_parameters_want_no_workspace():
     lib = _lib.load()
     assert lib.vila_fp8_linear_scratch(None) == 0 and lib.vila_fp8_linear_scratch(C.byref(_lib.Fp8LinearParams())) == 0
-    assert lib.vila_fp8_linear(None, None) != 0 and lib.vila_fp8_linear_tries(None, 5, None) != 0
+    assert lib.vila_fp8_rmsnorm(None, None) != 0 and lib.vila_fp8_linear(None, None) != 0 and lib.vila_fp8_linear_tries(None, 5, None) != 0
 
 
-def test_parameter_struct_follows_the_header():
+@pytest.mark.parametrize("name, struct", [("vila_fp8_linear_params", _lib.Fp8LinearParams), ("vila_fp8_rmsnorm_params", _lib.Fp8RmsnormParams)])
+def test_parameter_structs_follow_the_header(name, struct):
     text = (Path(__file__).resolve().parent.parent / "include" / "vila_b200.h").read_text()
-    body = re.search(r"typedef struct vila_fp8_linear_params \{(.*?)\} vila_fp8_linear_params;", text, flags=re.S).group(1)
+    body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), text, flags=re.S).group(1)
     fields = []
     for decl in re.sub(r"/\*.*?\*/", "", body, flags=re.S).split(";"):
         if decl.strip():
             names = decl.strip().split(",")
             fields += [names[0].split()[-1].lstrip("*")] + [n.strip().lstrip("*") for n in names[1:]]
-    assert fields == [f[0] for f in _lib.Fp8LinearParams._fields_]
+    assert fields == [f[0] for f in struct._fields_]

@@ -144,6 +144,14 @@ class Fp8LinearParams(C.Structure):
     ]
 
 
+class Fp8RmsnormParams(C.Structure):
+    _fields_ = [
+        ("x", c_void_p), ("ldx", c_i64), ("residual", c_void_p), ("ldr", c_i64), ("sum", c_void_p), ("ld_sum", c_i64), ("w", c_void_p),
+        ("codes", c_void_p), ("ldc", c_i64), ("scales", c_void_p), ("lds", c_i64), ("eps", c_float),
+        ("rows", C.c_int32), ("cols", C.c_int32), ("x_dtype", C.c_int32), ("residual_dtype", C.c_int32), ("w_dtype", C.c_int32),
+    ]
+
+
 class GLinearExt(C.Structure):
     _fields_ = [("act_alpha", c_float), ("act_limit", c_float), ("act_pos", c_float), ("act_neg", c_float),
                 ("in_scale", c_void_p)]
@@ -377,8 +385,7 @@ SIGNATURES = {
     "vila_mx4_linear_tries": [C.POINTER(Mx4LinearParams), c_int, c_void_p],
     "vila_fp8_quantize": [c_void_p, c_int, c_i64, c_void_p, c_i64, c_void_p, c_i64, c_int, c_int, c_int, c_void_p],
     "vila_fp8_dequantize": [c_void_p, c_i64, c_void_p, c_i64, c_void_p, c_int, c_i64, c_int, c_int, c_int, c_void_p],
-    "vila_fp8_rmsnorm": [c_void_p, c_int, c_i64, c_void_p, c_int, c_i64, c_void_p, c_i64, c_void_p, c_int, c_float, c_void_p,
-                         c_i64, c_void_p, c_i64, c_int, c_int, c_void_p],
+    "vila_fp8_rmsnorm": [C.POINTER(Fp8RmsnormParams), c_void_p],
     "vila_fp8_linear_scratch": [C.POINTER(Fp8LinearParams)],
     "vila_fp8_linear": [C.POINTER(Fp8LinearParams), c_void_p],
     "vila_fp8_linear_tries": [C.POINTER(Fp8LinearParams), c_int, c_void_p],

@@ -666,12 +666,10 @@ int vila_fp8_dequantize(const void* codes, int64_t ldc, const float* scales, int
   return vb::fp8_dequantize(codes, ldc, scales, lds, out, out_dtype, ldo, rows, cols, block_rows, st(stream));
 }
 
-int vila_fp8_rmsnorm(const void* x, int x_dtype, int64_t ldx, const void* residual, int residual_dtype, int64_t ldr, void* sum,
-                     int64_t ld_sum, const void* w, int w_dtype, float eps, void* codes, int64_t ldc, float* scales, int64_t lds, int rows,
-                     int cols, void* stream) {
+int vila_fp8_rmsnorm(const vila_fp8_rmsnorm_params* p, void* stream) {
   VB_REQUIRE_DEVICE();
-  return vb::fp8_rmsnorm(x, x_dtype, ldx, residual, residual_dtype, ldr, sum, ld_sum, w, w_dtype, eps, codes, ldc, scales, lds, rows, cols,
-                         st(stream));
+  VB_CHECK(p != nullptr, "fp8_rmsnorm: no parameters");
+  return vb::fp8_rmsnorm(*p, st(stream));
 }
 
 int64_t vila_fp8_linear_scratch(const vila_fp8_linear_params* p) { return p == nullptr ? 0 : static_cast<int64_t>(vb::fp8_linear_scratch(*p)); }

@@ -346,50 +346,49 @@ int fp8_dequantize(const void* codes, int64_t ldc, const float* scales, int64_t 
   });
 }
 
-int fp8_rmsnorm(const void* x, int x_dt, int64_t ldx, const void* residual, int r_dt, int64_t ldr, void* sum, int64_t ld_sum, const void* w,
-                int w_dt, float eps, void* codes, int64_t ldc, float* scales, int64_t lds, int rows, int cols, cudaStream_t stream) {
-  if (int rc = check_form("fp8_rmsnorm", codes, ldc, scales, lds, rows, cols, 1)) return rc;
-  VB_CHECK(cols <= 32768, "fp8_rmsnorm: cols=%d (at most 32768)", cols);
-  VB_CHECK(eps >= 0.f, "fp8_rmsnorm: eps=%g", eps);
-  if (rows == 0) return 0;
-  if (int rc = check_numbers("fp8_rmsnorm", x, x_dt)) return rc;
-  if (w != nullptr)
-    if (int rc = check_numbers("fp8_rmsnorm", w, w_dt)) return rc;
-  if (residual != nullptr) {
-    if (int rc = check_numbers("fp8_rmsnorm", residual, r_dt)) return rc;
-    if (int rc = check_numbers("fp8_rmsnorm", sum, x_dt)) return rc;
-    VB_CHECK(rows == 1 || ld_sum >= cols, "fp8_rmsnorm: ld_sum=%lld cols=%d", static_cast<long long>(ld_sum), cols);
-    VB_CHECK(sum != x || rows == 1 || ld_sum == ldx, "fp8_rmsnorm: the sum in x's place has x's stride");
+int fp8_rmsnorm(const vila_fp8_rmsnorm_params& a, cudaStream_t stream) {
+  if (int rc = check_form("fp8_rmsnorm", a.codes, a.ldc, a.scales, a.lds, a.rows, a.cols, 1)) return rc;
+  VB_CHECK(a.cols <= 32768, "fp8_rmsnorm: cols=%d (at most 32768)", a.cols);
+  VB_CHECK(a.eps >= 0.f, "fp8_rmsnorm: eps=%g", a.eps);
+  if (a.rows == 0) return 0;
+  if (int rc = check_numbers("fp8_rmsnorm", a.x, a.x_dtype)) return rc;
+  if (a.w != nullptr)
+    if (int rc = check_numbers("fp8_rmsnorm", a.w, a.w_dtype)) return rc;
+  if (a.residual != nullptr) {
+    if (int rc = check_numbers("fp8_rmsnorm", a.residual, a.residual_dtype)) return rc;
+    if (int rc = check_numbers("fp8_rmsnorm", a.sum, a.x_dtype)) return rc;
+    VB_CHECK(a.rows == 1 || a.ld_sum >= a.cols, "fp8_rmsnorm: ld_sum=%lld cols=%d", static_cast<long long>(a.ld_sum), a.cols);
+    VB_CHECK(a.sum != a.x || a.rows == 1 || a.ld_sum == a.ldx, "fp8_rmsnorm: the sum in x's place has x's stride");
   }
   Norm p = {};
-  p.x = x;
-  p.ldx = ldx;
-  p.x_how = how(x, ldx, size_of(x_dt));
-  p.residual = residual;
-  if (residual != nullptr) {
-    p.sum = sum;
-    p.ldr = ldr;
-    p.ld_sum = ld_sum;
-    p.r_f32 = r_dt == VILA_DT_F32;
-    p.r_how = how(residual, ldr, size_of(r_dt));
-    p.sum_how = how(sum, ld_sum, size_of(x_dt));
+  p.x = a.x;
+  p.ldx = a.ldx;
+  p.x_how = how(a.x, a.ldx, size_of(a.x_dtype));
+  p.residual = a.residual;
+  if (a.residual != nullptr) {
+    p.sum = a.sum;
+    p.ldr = a.ldr;
+    p.ld_sum = a.ld_sum;
+    p.r_f32 = a.residual_dtype == VILA_DT_F32;
+    p.r_how = how(a.residual, a.ldr, size_of(a.residual_dtype));
+    p.sum_how = how(a.sum, a.ld_sum, size_of(a.x_dtype));
   }
-  p.w = w;
-  p.w_f32 = w != nullptr && w_dt == VILA_DT_F32;
-  p.w_how = how(w, 0, 1);
-  p.codes = static_cast<uint8_t*>(codes);
-  p.ldc = ldc;
-  p.scales = scales;
-  p.lds = lds;
-  p.eps = eps;
-  p.cols = cols;
+  p.w = a.w;
+  p.w_f32 = a.w != nullptr && a.w_dtype == VILA_DT_F32;
+  p.w_how = how(a.w, 0, 1);
+  p.codes = static_cast<uint8_t*>(a.codes);
+  p.ldc = a.ldc;
+  p.scales = a.scales;
+  p.lds = a.lds;
+  p.eps = a.eps;
+  p.cols = a.cols;
   // as many threads as the row has chunks, one each up to 512 threads, then two, then four
-  const int chunks = fp8_blocks(cols) * (kFp8Block / kFp8Chunk), iter = chunks <= 512 ? 1 : (chunks <= 1024 ? 2 : 4);
+  const int chunks = fp8_blocks(a.cols) * (kFp8Block / kFp8Chunk), iter = chunks <= 512 ? 1 : (chunks <= 1024 ? 2 : 4);
   const int threads = ((chunks + iter - 1) / iter + 31) / 32 * 32;
-  const bool f32 = x_dt == VILA_DT_F32;
+  const bool f32 = a.x_dtype == VILA_DT_F32;
   auto k = iter == 1 ? (f32 ? norm_kernel<true, 1> : norm_kernel<false, 1>)
                      : (iter == 2 ? (f32 ? norm_kernel<true, 2> : norm_kernel<false, 2>) : (f32 ? norm_kernel<true, 4> : norm_kernel<false, 4>));
-  VB_CUDA(launch_pdl(k, dim3(rows), dim3(threads), 0, stream, p));
+  VB_CUDA(launch_pdl(k, dim3(a.rows), dim3(threads), 0, stream, p));
   return 0;
 }
 

@@ -286,6 +286,7 @@ struct vila_moe_route_params;
 struct vila_tanh_residual_params;
 struct vila_mx4_linear_params;
 struct vila_fp8_linear_params;
+struct vila_fp8_rmsnorm_params;
 namespace vb {
 int causal_conv_rows(const vila_causal_conv_params& p, cudaStream_t stream);
 int causal_conv_state(const vila_causal_conv_params& p, cudaStream_t stream);
@@ -353,8 +354,7 @@ int fp8_quantize(const void* x, int dt, int64_t ldx, void* codes, int64_t ldc, f
                  cudaStream_t stream);
 int fp8_dequantize(const void* codes, int64_t ldc, const float* scales, int64_t lds, void* out, int dt, int64_t ldo, int rows, int cols,
                    int block_rows, cudaStream_t stream);
-int fp8_rmsnorm(const void* x, int x_dt, int64_t ldx, const void* residual, int r_dt, int64_t ldr, void* sum, int64_t ld_sum, const void* w,
-                int w_dt, float eps, void* codes, int64_t ldc, float* scales, int64_t lds, int rows, int cols, cudaStream_t stream);
+int fp8_rmsnorm(const vila_fp8_rmsnorm_params& p, cudaStream_t stream);
 size_t fp8_linear_scratch(const vila_fp8_linear_params& p);
 int fp8_linear(const vila_fp8_linear_params& p, cudaStream_t stream, int tries = -1);
 int fp8_tc(const vila_fp8_linear_params& p, const vila_glinear_ext& ext, float* out32, int tries, cudaStream_t stream);   // fp8_tc.cu

@@ -1709,14 +1709,16 @@ def fp8_rmsnorm(x: torch.Tensor, w: Optional[torch.Tensor], eps: float, *, resid
     if w is not None:
         _mx4_here(w, "w")
         w_ptr, w_dt = w.data_ptr(), _dt(w, "w")
-        _fp8_check(w.shape == (cols,) and w.is_contiguous(), f"w must be contiguous [{cols}]")
+        if w.shape != (cols,) or not w.is_contiguous():
+            raise RuntimeError(f"vila_b200.ops: w must be contiguous [{cols}]")
     if residual is not None:
         r_dt = _fp8_rows(residual, "residual")
-        _fp8_check(residual.shape == x.shape, f"residual must be [{rows}, {cols}]")
+        if residual.shape != x.shape:
+            raise RuntimeError(f"vila_b200.ops: residual must be [{rows}, {cols}]")
         r_ptr, ldr = residual.data_ptr(), residual.stride(0)
         if out is None:
-            total = x.new_empty((rows, cols))
-            ld_sum = cols
+            total = torch.empty_like(x)
+            ld_sum = total.stride(0)
         else:
             _fp8_rows(out, "out")
             _fp8_check(out.shape == x.shape and out.dtype == x.dtype, f"out must be [{rows}, {cols}] of x's type")
@@ -1726,8 +1728,9 @@ def fp8_rmsnorm(x: torch.Tensor, w: Optional[torch.Tensor], eps: float, *, resid
         raise RuntimeError("vila_b200.ops: out goes with a residual")
     q = Fp8._alloc(x, rows, cols, 1)
     codes = q._both.data_ptr()
-    check(_lib.load().vila_fp8_rmsnorm(x.data_ptr(), dt, x.stride(0), r_ptr, r_dt, ldr, s_ptr, ld_sum, w_ptr, w_dt, eps, codes, q._ldc, codes + q._at,
-                                       q._lds, rows, cols, _stream()), "vila_fp8_rmsnorm")
+    p = _lib.Fp8RmsnormParams(x.data_ptr(), x.stride(0), r_ptr, ldr, s_ptr, ld_sum, w_ptr, codes, q._ldc, codes + q._at, q._lds, eps, rows, cols, dt, r_dt,
+                              w_dt)      # by position, and handed over as it is: by name, or one by one, they took 2 us more
+    check(_lib.load().vila_fp8_rmsnorm(p, _stream()), "vila_fp8_rmsnorm")
     return q, total
 
 
