@@ -306,7 +306,15 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
 
 }  // namespace
 
-bool fp8_pair_takes(const vila_fp8_linear_params& p) { return p.M > 512; }
+// By rounds through the GPU: of 3584 columns a round of pairs takes 17.5 us, one of single CTAs' tiles of 128 x 128 (fp8_tc.cu) 13.4, us against us:
+// 600 rows of 1152 weight rows 19.6 and 11.6, 512 of 4608 20.5 and 14.7 (one round each), 600 of 4608 20.8 and 26.7 (one and two), 300 of 18944
+// 39.3 and 43.5, 1536 of 3584 37.2 and 40.5 (two and three), 1024 of 18944 73.6 and 112.8.
+bool fp8_pair_takes(const vila_fp8_linear_params& p) {
+  if (p.M <= 128) return false;
+  const long long sms = num_sms(), singles = ((p.M + 127ll) / 128 * ((p.N + 127) / 128) + sms - 1) / sms;
+  const long long pairs = ((p.M + 255ll) / 256 * ((p.N + kN - 1) / kN) + sms / 2 - 1) / (sms / 2);
+  return 4 * pairs < 3 * singles;
+}
 
 int fp8_pair(const vila_fp8_linear_params& p, const vila_glinear_ext& x, int tries, cudaStream_t stream) {
   VB_CHECK(failed_word() != nullptr, "fp8_linear: no pinned host memory for the status word");

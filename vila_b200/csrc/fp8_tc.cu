@@ -491,7 +491,7 @@ int fp8_tc(const vila_fp8_linear_params& p, const vila_glinear_ext& ext, float* 
   VB_CHECK(failed_word() != nullptr, "fp8_linear: no pinned host memory for the status word");
   if (p.M <= 16) return launch<16, true>(p, ext, out32, tries, stream);
   if (p.M <= 32) return launch<32, true>(p, ext, out32, tries, stream);
-  // Up to 128 tokens tiles of 64 weight rows, two CTAs an SM; beyond, tokens would be read too often.
+  // fp8_pair_takes has the rule for tiles that are many.  Up to 128 tokens tiles of 64 weight rows, two CTAs an SM; beyond, tokens would be read too often.
   if (p.M <= 128) return launch<64, false>(p, ext, out32, tries, stream);
   return launch<128, false>(p, ext, out32, tries, stream);
 }
