@@ -478,8 +478,13 @@ int launch(const vila_fp8_linear_params& p, const vila_glinear_ext& x, float* ou
   const long long tiles = kSwap ? (p.N + kRows - 1) / kRows : static_cast<long long>((p.N + BN - 1) / BN) * ((p.M + kRows - 1) / kRows);
   VB_CHECK(tiles < (1LL << 27), "fp8_linear: too many tiles (M=%d N=%d)", p.M, p.N);
   static Mx4Clusters clusters;
-  // of 4 blocks a cluster's joint end costs what it saves (77 rows of 1157 x 512: 7.2 us by two, 6.2 alone; x 1024 by 4 7.1, by 2 8.0)
-  const int blocks = fp8_blocks(p.K), split = clusters.split(fp8_kernel<BN, kSwap>, S::kThreads, S::kSmem, tiles, blocks < 8 ? 1 : blocks / 2);
+  // As many CTAs a tile, a power of two up to 8, as the GPU holds clusters for at once.  The occupancy that CUDA reports counts one CTA an SM
+  // where two fit (15 clusters of 8); the GPU holds both (64 rows of 3584 x 18944 by 8: 25.5 us, by 4, as reported, 33.6).
+  // Of 4 blocks a cluster's joint end costs what it saves (77 rows of 1157 x 512: 7.2 us by two, 6.2 alone; x 1024 by 4 7.1, by 2 8.0).
+  const int blocks = fp8_blocks(p.K), limit = blocks < 8 ? 1 : blocks / 2;
+  int split = 1;
+  for (int l = 1; l <= 3 && (1 << l) <= limit && tiles <= static_cast<long long>(S::kPerSm) * clusters.of(fp8_kernel<BN, kSwap>, l, S::kThreads, S::kSmem); ++l)
+    split = 1 << l;
   VB_CUDA(launch_pdl_cluster(fp8_kernel<BN, kSwap>, dim3(static_cast<unsigned>(tiles * split)), dim3(S::kThreads), S::kSmem, stream, dim3(split),
                              kSwap ? tw : ta, kSwap ? ta : tw, p, x, out32, bn, split, wait_limit(tries), failed_word()));
   return 0;
