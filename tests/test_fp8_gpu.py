@@ -109,14 +109,20 @@ def test_pack_keeps_what_lies_well_and_copies_the_rest(cuda):
     odd[:, 2:290] = codes
     inner = codes.new_empty(200, 320)
     inner[:, 16:304] = codes
-    for c, s, kept in ((odd[:, 2:290], scales, False), (codes.T.contiguous().T, scales, False), (codes, scales.T.contiguous().T, False),
+    for c, s, kept in ((odd[:, 2:290], scales, False), (codes.T.contiguous().T, scales, False), (codes, scales.T.contiguous().T, True),
                        (inner[:, 16:304], scales, True)):
         q = ops.fp8_pack(c, s)
         assert (q.codes.data_ptr() == c.data_ptr()) == kept
         assert torch.equal(ops.fp8_dequantize(q, out_dtype=torch.float32).cpu(), want)
     rows = rand(8, 200, 3).abs().to(cuda)       # a scale per row
     q = ops.fp8_pack(codes, rows, block_rows=1)
+    assert q.codes.data_ptr() == codes.data_ptr()
     assert torch.equal(q.scales, rows) and torch.equal(ops.fp8_dequantize(q, out_dtype=torch.float32).cpu(), R.values(codes.cpu().double(), rows.cpu(), 1).float())
+    for n, k in ((1, 17), (1, 300), (3, 1), (0, 40), (5, 128)):
+        few, per = (rand(9, n, k) * 50).to(E4M3).to(cuda), rand(10, n, -(-k // 128)).abs().to(cuda)
+        p = ops.fp8_pack(few, per, block_rows=1)
+        assert p.shape == (n, k) and torch.equal(p.scales, per) and torch.equal(p.codes.float(), few.float())
+        assert torch.equal(ops.fp8_dequantize(p, out_dtype=torch.float32).cpu(), R.values(few.cpu().double(), per.cpu(), 1).float())
     again = ops.fp8_pack(q.codes, q.scales, block_rows=1)
     assert again.scales.data_ptr() == q.scales.data_ptr() and again.codes.data_ptr() == q.codes.data_ptr()
 

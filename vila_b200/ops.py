@@ -1524,19 +1524,9 @@ class Fp8:
         _fp8_shape(codes, scales, block_rows)
         self.rows, self.cols = codes.shape
         self.block_rows, self._codes, self._scales, self._both, self._at = block_rows, codes, scales, None, 0
-        blocks = scales.shape[1]
-        self._ldc = _fp8_pitch(self.cols) if self.rows <= 1 else codes.stride(0)
-        if block_rows == 1:
-            self._lds = _fp8_lds(self.rows) if blocks <= 1 else scales.stride(1)
-            ok = (self.rows <= 1 or scales.stride(0) == 1) and self._lds % 4 == 0 and self._lds >= self.rows and scales.data_ptr() % 16 == 0
-            ok = ok and scales.untyped_storage().nbytes() >= 4 * (scales.storage_offset() + blocks * self._lds)
-        else:
-            self._lds = blocks if scales.shape[0] <= 1 else scales.stride(0)
-            ok = (blocks <= 1 or scales.stride(1) == 1) and self._lds >= blocks
-        _fp8_check(ok, "the scales do not lie as the kernels read them (fp8_pack copies those that do not)")
-        _fp8_check((self.cols <= 1 or codes.stride(1) == 1) and self._ldc % 16 == 0 and self._ldc >= self.cols and codes.data_ptr() % 16 == 0
-                   and codes.untyped_storage().nbytes() >= codes.storage_offset() + max(self.rows - 1, 0) * self._ldc + (_fp8_pitch(self.cols) if self.rows else 0),
-                   "rows of codes must start on 16-byte boundaries and have whole 16 bytes of memory (fp8_pack copies those that do not)")
+        self._ldc, self._lds = _fp8_ldc_of(codes), _fp8_lds_of(scales, block_rows)
+        _fp8_check(self._lds > 0, "the scales do not lie as the kernels read them (fp8_pack copies those that do not)")
+        _fp8_check(self._ldc > 0, "rows of codes must start on 16-byte boundaries and have whole 16 bytes of memory (fp8_pack copies those that do not)")
 
     @classmethod
     def _alloc(cls, like: torch.Tensor, rows: int, cols: int, block_rows: int) -> "Fp8":
@@ -1629,6 +1619,28 @@ def _fp8_lds(rows: int) -> int:
     return (rows + 3) // 4 * 4
 
 
+def _fp8_ldc_of(codes: torch.Tensor) -> int:
+    """The stride of rows of codes that lie as the kernels read them, 0 of others."""
+    rows, cols = codes.shape
+    ldc = _fp8_pitch(cols) if rows <= 1 else codes.stride(0)
+    ok = ((cols <= 1 or codes.stride(1) == 1) and ldc % 16 == 0 and ldc >= cols and codes.data_ptr() % 16 == 0
+          and codes.untyped_storage().nbytes() >= codes.storage_offset() + max(rows - 1, 0) * ldc + (_fp8_pitch(cols) if rows else 0))
+    return ldc if ok else 0
+
+
+def _fp8_lds_of(scales: torch.Tensor, block_rows: int) -> int:
+    """The stride of scales that lie as the kernels read them, 0 of others."""
+    rows, blocks = scales.shape
+    if block_rows == 1:
+        lds = max(4, _fp8_lds(rows)) if blocks <= 1 else scales.stride(1)
+        ok = ((rows <= 1 or scales.stride(0) == 1) and lds % 4 == 0 and lds >= rows and scales.data_ptr() % 16 == 0
+              and (rows == 0 or scales.untyped_storage().nbytes() >= 4 * (scales.storage_offset() + blocks * lds)))
+    else:
+        lds = blocks if rows <= 1 else scales.stride(0)
+        ok = (blocks <= 1 or scales.stride(1) == 1) and lds >= blocks
+    return lds if ok else 0
+
+
 def _fp8_shape(codes: torch.Tensor, scales: torch.Tensor, block_rows: int) -> None:
     _fp8_check(block_rows in (1, FP8_BLOCK), f"block_rows={block_rows}: 1 or 128")
     _fp8_check(codes.dim() == 2 and codes.dtype == _E4M3 and codes.shape[1] > 0, "codes must be float8_e4m3fn [rows, cols]")
@@ -1683,19 +1695,19 @@ def fp8_dequantize(q: Fp8, out_dtype=torch.bfloat16) -> torch.Tensor:
 
 def fp8_pack(codes: torch.Tensor, scales: torch.Tensor, block_rows: int = FP8_BLOCK) -> Fp8:
     """codes float8_e4m3fn [rows, cols] and the factors fp32 [ceil(rows / block_rows), ceil(cols / 128)] that their blocks are multiplied with (a
-    checkpoint's) -> Fp8.  Both are kept, not copied, where they lie as the kernels read them: rows of codes on 16-byte boundaries, a
-    weight's scales with consecutive columns."""
+    checkpoint's) -> Fp8.  Both are kept, not copied, each where it lies as the kernels read it: rows of codes on 16-byte boundaries, a
+    weight's scales with consecutive columns, rows' scales with consecutive rows."""
     _mx4_here(codes, "codes")
     _mx4_here(scales, "scales")
     _fp8_shape(codes, scales, block_rows)
-    rows, cols = codes.shape
-    try:
-        return Fp8(codes, scales, block_rows)
-    except RuntimeError:
-        q = Fp8._alloc(codes, rows, cols, block_rows)
-        q.codes.copy_(codes)
-        q.scales.copy_(scales)
-        return q
+    if not _fp8_ldc_of(codes):
+        rows, cols = codes.shape
+        codes = codes.new_empty((rows, _fp8_pitch(cols)))[:, :cols].copy_(codes)
+    if not _fp8_lds_of(scales, block_rows):
+        rows, blocks = scales.shape
+        to = scales.new_empty((blocks, _fp8_lds(rows)))[:, :rows].T if block_rows == 1 else scales.new_empty((rows, blocks))
+        scales = to.copy_(scales)
+    return Fp8(codes, scales, block_rows)
 
 
 def fp8_rmsnorm(x: torch.Tensor, w: Optional[torch.Tensor], eps: float, *, residual: Optional[torch.Tensor] = None,
