@@ -18,8 +18,8 @@
 // A CTA takes one tile, or, where the tiles leave SMs idle, a share of its blocks: a cluster of up to 8 CTAs splits K, every CTA sends
 // its sums to the CTAs that finish them, by rows, and these add them in rank order.
 //
-// A launch may begin before the one before it has ended: the first weights are asked for while that one ends, everything else comes behind
-// griddepcontrol.wait.  (Weights come from launches that do not let others begin early.)
+// A launch may begin before the one before it has ended: TMEM and the first weights are asked for while that one ends, everything else comes
+// behind griddepcontrol.wait.  (Weights come from launches that do not let others begin early.)
 #include "../../include/vila_b200.h"
 #include "common.cuh"
 #include "fp8.cuh"
@@ -175,29 +175,40 @@ fp8_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ C
   const int qt = tile / p_tiles, p0 = (tile - qt * p_tiles) * kRows, q0 = qt * bn;      // tiles that run together share their columns' rows
   const int t0 = kSwap ? q0 : p0, n0 = kSwap ? p0 : q0;                                 // first token, first weight row
 
-  griddep_launch_dependents();
   if (split > 1) cluster_arrive();      // this CTA runs: others may write to its shared memory
-  if (tid == 0) {
-    tma_prefetch_desc(&tmap_p);
-    tma_prefetch_desc(&tmap_q);
-    for (int i = 0; i < ST; ++i) {
-      mbar_init(&full_bar[i], 1);
-      mbar_init(&empty_bar[i], 1);
+  const uint32_t bytes = S::kPBytes + bn * 128;                                // of a stage
+  const int ahead = limit.quits == 0 ? 0 : min(ST, kb1 - kb0);                 // stages whose weights are asked for before the launch before has ended
+  if (warp == S::kTma) {
+    if (lane == 0) {
+      tma_prefetch_desc(&tmap_p);
+      tma_prefetch_desc(&tmap_q);
+      for (int i = 0; i < ST; ++i) {
+        mbar_init(&full_bar[i], 1);
+        mbar_init(&empty_bar[i], 1);
+      }
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&acc_full[i], 1);
+        mbar_init(&acc_free[i], S::kEpi);
+        mbar_init(&scale_full[i], 1);
+        mbar_init(&scale_free[i], S::kEpi);
+      }
+      mbar_init(drain_bar, 1);
+      *gave_up = 0;
+      fence_barrier_init();
+      for (int i = 0; i < ahead; ++i) {
+        mbar_arrive_expect_tx(&full_bar[i], bytes);
+        tma_load_2d(smem + i * S::kStage + (kSwap ? 0 : S::kPBytes), kSwap ? &tmap_p : &tmap_q, &full_bar[i], (kb0 + i) * 128, n0);
+      }
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_free[i], S::kEpi);
-      mbar_init(&scale_full[i], 1);
-      mbar_init(&scale_free[i], S::kEpi);
-    }
-    mbar_init(drain_bar, 1);
-    *gave_up = 0;
-    fence_barrier_init();
+    __syncwarp();
   }
   if (warp == S::kMma) tmem_alloc<S::kCols>(tmem_ptr);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // Behind TMEM: the next launch's CTAs may ask for theirs and then wait for this one to end, on an SM that both fit on.  Were they there first,
+  // both would wait for good.
+  griddep_launch_dependents();
   const uint32_t tmem = *tmem_ptr;
   const int ld32 = p.flags & kGluFlags ? p.N / 2 : p.N;
   const bool wide = kSwap ? reinterpret_cast<uintptr_t>(p.out) % 8 == 0 && p.ldo % 4 == 0 : reinterpret_cast<uintptr_t>(p.out) % 32 == 0 && p.ldo % 16 == 0;
@@ -211,14 +222,6 @@ fp8_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ C
     const bool one = elect_one();
     const CUtensorMap *tw = kSwap ? &tmap_p : &tmap_q, *ta = kSwap ? &tmap_q : &tmap_p;
     const int w_at = kSwap ? 0 : S::kPBytes, a_at = kSwap ? S::kPBytes : 0;
-    const uint32_t bytes = S::kPBytes + bn * 128;
-    const int ahead = ok ? min(ST, kb1 - kb0) : 0;      // stages whose weights are asked for before the launch before has ended
-    if (one)
-      for (int i = 0; i < ahead; ++i) {
-        mbar_arrive_expect_tx(&full_bar[i], bytes);
-        tma_load_2d(smem + i * S::kStage + w_at, tw, &full_bar[i], (kb0 + i) * 128, n0);
-      }
-    __syncwarp();
     griddep_wait();
     int s = 0, rounds = 0;                // stage, rounds through all of them
     uint32_t ph = 1;                      // parity to wait for on an empty barrier: the first round passes
