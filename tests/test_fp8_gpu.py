@@ -504,6 +504,26 @@ def test_waits_that_run_out(cuda, monkeypatch, M, N, K, tries):
     assert torch.equal(ops.fp8_linear(a, w), want)
 
 
+@pytest.mark.parametrize("M", [1, 20, 40])
+def test_a_long_launch_before_takes_no_tries(cuda, monkeypatch, M):
+    """The launch before lets this one begin and runs for milliseconds: waits are counted from its end."""
+    from vila_b200 import _lib, ops
+    K = 1 << 24
+    long_a, long_w = ops.fp8_quantize(torch.ones(1, K, dtype=BF, device=cuda)), ops.fp8_quantize(torch.ones(8, K, dtype=BF, device=cuda), block_rows=128)
+    w, a = ops.fp8_quantize(rand(1, 300, 700).to(cuda), block_rows=128), ops.fp8_quantize(rand(2, M, 700).to(cuda))
+    want = ops.fp8_linear(a, w)
+    torch.cuda.synchronize()
+    ops.check_waits()
+    lib = _lib.load()
+    ops.fp8_linear(long_a, long_w)
+    with monkeypatch.context() as m:
+        m.setattr(lib, "vila_fp8_linear", lambda p, stream: lib.vila_fp8_linear_tries(p, 256, stream))
+        got = ops.fp8_linear(a, w)
+    torch.cuda.synchronize()
+    ops.check_waits()
+    assert torch.equal(got, want)
+
+
 @pytest.mark.parametrize("role", [0, 1, 3])
 @pytest.mark.parametrize("rank", [0, 1])
 @pytest.mark.parametrize("M, N, K", [(2000, 2400, 800), (2000, 2400, 5000), (5000, 5000, 700)])

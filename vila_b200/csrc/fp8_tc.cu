@@ -256,6 +256,7 @@ fp8_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ C
     const bool one = elect_one();
     const uint64_t pd0 = make_smem_desc(smem_u32(smem), 16, 1024, kLayoutSW128), qd0 = make_smem_desc(smem_u32(smem) + S::kPBytes, 16, 1024, kLayoutSW128);
     const uint32_t idesc = fp8_idesc(kRows, bn);
+    griddep_wait();                       // or the tries of the first wait would be spent on the launch before
     int s = 0, v = 0;                     // stage, visits of the epilogue warps so far
     uint32_t ph = 0;
     for (int kb = kb0; kb < kb1 && ok; kb += kVisit, ++v) {
