@@ -504,6 +504,24 @@ def test_waits_that_run_out(cuda, monkeypatch, M, N, K, tries):
     assert torch.equal(ops.fp8_linear(a, w), want)
 
 
+@pytest.mark.parametrize("M", [1, 40, 300, 1500])
+def test_a_weight_of_codes_that_a_launch_just_wrote(cuda, M):
+    """A weight whose codes are another launch's 8-bit rows: the layer behind it reads what that launch wrote."""
+    from vila_b200 import ops
+    a = ops.fp8_quantize(rand(1, M, 1024).to(cuda))
+    xs = [rand(2 + i, 640, 1024).to(cuda) for i in range(2)]
+    s = torch.rand(5, 8, device=cuda)
+    wants = []
+    for x in xs:
+        codes = ops.fp8_quantize(x).codes
+        torch.cuda.synchronize()
+        wants.append(ops.fp8_linear(a, ops.fp8_pack(codes, s)))
+    torch.cuda.synchronize()
+    for i in range(20):
+        got = ops.fp8_linear(a, ops.fp8_pack(ops.fp8_quantize(xs[i % 2]).codes, s))
+        assert torch.equal(got, wants[i % 2])
+
+
 @pytest.mark.parametrize("M", [1, 20, 40])
 def test_a_long_launch_before_takes_no_tries(cuda, monkeypatch, M):
     """The launch before lets this one begin and runs for milliseconds: waits are counted from its end."""

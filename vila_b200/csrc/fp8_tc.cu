@@ -19,7 +19,8 @@
 // its sums to the CTAs that finish them, by rows, and these add them in rank order.
 //
 // A launch may begin before the one before it has ended: TMEM and the first weights are asked for while that one ends, everything else comes
-// behind griddepcontrol.wait.  (Weights come from launches that do not let others begin early.)
+// behind griddepcontrol.wait.  So what writes a weight must not let the next launch begin before its own end: the weights' quantisation is
+// launched so, and the Python class has such a launch behind codes of another origin.
 #include "../../include/vila_b200.h"
 #include "common.cuh"
 #include "fp8.cuh"

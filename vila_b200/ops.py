@@ -1527,6 +1527,10 @@ class Fp8:
         self._ldc, self._lds = _fp8_ldc_of(codes), _fp8_lds_of(scales, block_rows)
         _fp8_check(self._lds > 0, "the scales do not lie as the kernels read them (fp8_pack copies those that do not)")
         _fp8_check(self._ldc > 0, "rows of codes must start on 16-byte boundaries and have whole 16 bytes of memory (fp8_pack copies those that do not)")
+        if block_rows == FP8_BLOCK and codes.is_cuda:
+            # A linear layer asks for its first weights while the launch before it ends.  What wrote these codes may be a launch that lets others
+            # begin before its end (rows' quantisation is): one that does not comes between.
+            scales.new_zeros(1)
 
     @classmethod
     def _alloc(cls, like: torch.Tensor, rows: int, cols: int, block_rows: int) -> "Fp8":
