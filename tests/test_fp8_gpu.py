@@ -758,3 +758,14 @@ def test_prompts_in_8_bits_are_the_operators_in_turn(cuda):
     layer, eights = llm.model.layers[0], llm._fp8_weights()[0]
     h, x = ops.fp8_rmsnorm(x, layer.input_layernorm.weight, llm.config.rms_norm_eps)
     check_product(ops.fp8_linear(h, eights[0], layer._qkv_b), R.values(h.codes.cpu(), h.scales.cpu()), R.values(*(t.cpu() for t in (eights[0].codes, eights[0].scales)), 128), layer._qkv_b)
+
+
+def test_weights_in_one_form_are_not_put_into_the_other(cuda):
+    from vila_b200.model import quantize_weights
+    import importlib
+    T = importlib.import_module("tests.test_nibelix_gpu")
+    _, model = T.build(next(iter(T.CONFIGS)), BF, seed=3)
+    quantize_weights(model, to="fp8")
+    quantize_weights(model, to="fp8")
+    with pytest.raises(ValueError, match="held in 8 bits already"):
+        quantize_weights(model, to="mx4")

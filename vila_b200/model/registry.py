@@ -63,6 +63,9 @@ def quantize_weights(model, to: str = "mx4"):
         raise ValueError(f"{type(model).__name__} does not hold weights in {WEIGHT_BITS[to]} bits (those that do: {sorted(MX4_WEIGHTS)})")
     if model.dtype != torch.bfloat16:
         raise ValueError(f"{WEIGHT_BITS[to]}-bit weights go with bfloat16 activations, not {model.dtype}")
+    other = ops.Fp8 if to == "mx4" else ops.Mx4
+    if any(isinstance(getattr(layer, name, None), other) for layer in model.layers for name in names):
+        raise ValueError(f"the weights are held in {WEIGHT_BITS['fp8' if to == 'mx4' else 'mx4']} bits already")
     if torch.device(model.device).type == "cuda":
         torch.cuda.synchronize(model.device)      # no step that reads the replaced weights is under way, on whichever stream
     model.weights_version = getattr(model, "weights_version", 0) + 1
