@@ -760,6 +760,70 @@ def test_prompts_in_8_bits_are_the_operators_in_turn(cuda):
     check_product(ops.fp8_linear(h, eights[0], layer._qkv_b), R.values(h.codes.cpu(), h.scales.cpu()), R.values(*(t.cpu() for t in (eights[0].codes, eights[0].scales)), 128), layer._qkv_b)
 
 
+def test_weights_that_come_to_lie_where_others_were(cuda):
+    """Other tensors at the former ones' addresses, of the same version, are not taken for them."""
+    llm, emb = qwen(layers=1).prefill_in_fp8(), rand(4, 90, 512).to(BF).to(cuda)
+    layer = llm.model.layers[0]
+    first = hidden(llm, emb)
+    for i in range(4):
+        v = rand(50 + i, 512, 1104).to(BF).to(cuda) / 32
+        layer.mlp.down_proj.weight = None      # freed, if nothing else holds it
+        layer.mlp.down_proj.weight = torch.nn.Parameter(v.clone(), requires_grad=False)
+        got = hidden(llm, emb)
+        want = hidden(llm.prefill_in_fp8(), emb)      # quantised anew
+        assert torch.equal(got, want) and not torch.equal(got, first)
+        first = got
+
+
+def test_captured_prompts_keep_the_8_bit_weights(cuda):
+    """A caller's own capture: refused where the weights would be made in it; behind a change the graph reads the new ones."""
+    llm, other, emb = qwen(layers=2).prefill_in_fp8(), qwen(seed=1, layers=2), rand(4, 90, 512).to(BF).to(cuda)
+    cache = llm.new_cache(90)
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="outside of a capture"):
+        with torch.cuda.graph(g):
+            llm.prefill_hidden(emb, cache)
+    torch.cuda.synchronize()
+    want = hidden(llm, emb)
+    cache, g = llm.new_cache(90), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = llm.prefill_hidden(emb, cache)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    with torch.no_grad():
+        for p, q in zip(llm.state_dict().values(), other.state_dict().values()):
+            p.copy_(q)
+    want = hidden(llm, emb)
+    junk = [torch.full((1 << 20,), 0x7f, dtype=torch.uint8, device=cuda) for _ in range(16)]      # over what the change has freed
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and len(junk) == 16
+    # behind a write that torch does not count: called again
+    llm.model.layers[0].mlp.down_proj.weight.data.mul_(2)
+    want = hidden(llm.prefill_in_fp8(), emb)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_prompts_in_8_bits_on_two_streams(cuda):
+    """The first prompt behind a change makes the weights; one on another stream at once reads them made."""
+    llm, other, emb = qwen(layers=2).prefill_in_fp8(), qwen(seed=1, layers=2).prefill_in_fp8(), rand(4, 300, 512).to(BF).to(cuda)
+    want = hidden(other, emb)
+    hidden(llm, emb)
+    with torch.no_grad():
+        for p, q in zip(llm.state_dict().values(), other.state_dict().values()):
+            p.copy_(q)
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(2):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got.append(hidden(llm, emb))
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want) and torch.equal(got[1], want)
+
+
 def test_weights_in_one_form_are_not_put_into_the_other(cuda):
     from vila_b200.model import quantize_weights
     import importlib

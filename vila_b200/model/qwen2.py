@@ -155,7 +155,7 @@ class Qwen2ForCausalLM(nn.Module):
         self.generation_config = None
         self._decoder = None
         self._prefill_graphs = {}
-        self._fp8 = None      # prefill_in_fp8: per layer (qkv, o, gate / up, down) as ops.Fp8, and the versions of what they were made from
+        self._fp8 = None      # prefill_in_fp8: per layer (qkv, o, gate / up, down) as ops.Fp8, addresses and versions of what they were made from, and that
 
     # ---- HF-style accessors ----
     @property
@@ -176,9 +176,12 @@ class Qwen2ForCausalLM(nn.Module):
     def prefill_in_fp8(self, on: bool = True) -> "Qwen2ForCausalLM":
         """Run prompts' projections in 8 bits: weights held a second time as e4m3 numbers with a scale per 128 x 128, rows quantised by the norm
         before them, by the gated unit, or (the attention's output) by the projection itself.  Attention, cache, residual stream and decoded
-        tokens' steps stay bf16.  Changed weights are quantised anew at the next prompt.  Sequence-parallel prompts stay bf16.  In place; -> self."""
+        tokens' steps stay bf16.  Sequence-parallel prompts stay bf16.  In place; -> self.
+        The 8-bit weights are made at the first prompt, not within a graph's capture, and anew, in the same memory, at the first one behind a change
+        that torch counts: other tensors, or writes in place.  Behind writes that it does not count (through .data, or to tensors made in
+        inference mode) call this again, not while a prompt runs."""
         self._prefill_graphs.clear()
-        self._fp8 = ([], None) if on else None
+        self._fp8 = ([] if self._fp8 is None else self._fp8[0], None, None) if on else None
         return self
 
     def _fp8_weights(self):
@@ -188,8 +191,23 @@ class Qwen2ForCausalLM(nn.Module):
         held = [(layer._qkv_w, layer.self_attn.o_proj.weight, layer._gu_w, layer.mlp.down_proj.weight) for layer in self.model.layers]
         now = [(w.data_ptr(), None if w.is_inference() else w._version) for ws in held for w in ws]
         if self._fp8[1] != now:
-            self._prefill_graphs.clear()      # they read the former ones
-            self._fp8 = ([tuple(ops.fp8_quantize(w, block_rows=ops.FP8_BLOCK) for w in ws) for ws in held], now)
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the layers' 8-bit weights are made at a prompt outside of a capture: run one before")
+            torch.cuda.synchronize(self.device)      # prompts that read the former ones, on whichever stream
+            self._prefill_graphs.clear()
+            olds, eights = self._fp8[0], []
+            for li, ws in enumerate(held):
+                qs = []
+                for i, w in enumerate(ws):
+                    q, old = ops.fp8_quantize(w, block_rows=ops.FP8_BLOCK), olds[li][i] if olds else None
+                    if old is not None and (old.shape, old.device) == (q.shape, q.device):
+                        old._held().copy_(q._held())      # a caller's captured graph reads it where it is
+                        q = old
+                    qs.append(q)
+                eights.append(tuple(qs))
+            torch.cuda.synchronize(self.device)      # the next prompt may come on another stream
+            # The tensors themselves are held, too: others that come to lie where they were would be taken for them.
+            self._fp8 = (eights, now, [w.detach() for ws in held for w in ws])
         return self._fp8[0]
 
     def new_cache(self, max_tokens: int, page_order=None) -> PagedKVCache:
