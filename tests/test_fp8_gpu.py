@@ -420,6 +420,31 @@ def test_refusals(cuda):
     assert (out == 7).all()
 
 
+def test_offsets_past_32_bits(cuda):
+    """2^31 bytes of codes and more, as rows and as a weight.  Numbers are +-448, their scales 1, so that every sum is a multiple of 448^2 and exact in
+    fp32 in whatever order: what lies at the end is what it is by itself, bit by bit."""
+    from vila_b200 import ops
+    rows, cols, tail = 66048, 33000, 300
+    x = torch.empty(rows, cols, dtype=BF, device=cuda)
+    for i in range(0, rows, 8192):
+        x[i:i + 8192] = torch.randint(0, 2, x[i:i + 8192].shape, dtype=torch.int8, device=cuda)
+    x.mul_(2).sub_(1).mul_(448)
+    end = x[-tail:].clone()
+    q, w = ops.fp8_quantize(x), ops.fp8_quantize(x, block_rows=128)
+    assert q.codes.numel() > 1 << 31 and (q.scales == 1).all() and (w.scales == 1).all()
+    assert torch.equal(q.codes[-tail:].to(BF), end) and torch.equal(w.codes[-tail:].to(BF), end)
+    assert torch.equal(ops.fp8_dequantize(q)[-tail:], end)
+    few = ops.fp8_quantize(x[:640].clone(), block_rows=128)
+    a = ops.fp8_quantize(end)
+    assert torch.equal(ops.fp8_linear(q, few)[-tail:], ops.fp8_linear(a, few))
+    w_end = ops.fp8_quantize(x[-512:].clone(), block_rows=128)
+    for M in (1, 40, 300):
+        b = ops.fp8_quantize(x[:M].clone())
+        assert torch.equal(ops.fp8_linear(b, w)[:, -512:], ops.fp8_linear(b, w_end))
+    _, total = ops.fp8_rmsnorm(x[:, :32768], None, 1e-6, residual=x[:, :32768])
+    assert torch.equal(total[-tail:], 2 * end[:, :32768])
+
+
 # ---- streams, graphs, waits that run out ---------------------------------------------------------------------
 KERNELS = [(1, 300, 700), (1, 300, 9000), (20, 300, 700), (40, 300, 700), (100, 300, 9000), (300, 770, 520), (1500, 1300, 800), (2000, 2400, 800)]
 

@@ -1776,7 +1776,8 @@ def fp8_linear(a, w: Fp8, bias: Optional[torch.Tensor] = None, *, act: int = ACT
     flags = (1 if swiglu else 0) | (4 if glu_clamp is not None else 0) | (FLAG_GEGLU if geglu else 0)
     _fp8_check(act != ACT_XIELU or act_params is not None, "ACT_XIELU takes act_params")
     n_out = N // 2 if flags else N
-    _fp8_check(n_out > 0, f"a gated unit has an even number of weight rows (N={N})")
+    if n_out == 0:
+        raise RuntimeError(f"vila_b200.ops: a gated unit has an even number of weight rows (N={N})")
     if bias is not None:
         _chk(bias, "bias")
         _mx4_here(bias, "bias")
