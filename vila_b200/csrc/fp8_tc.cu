@@ -64,7 +64,7 @@ template <int BN, bool kSwap> struct Shape {
   static constexpr size_t kSmem = 1024 + static_cast<size_t>(kStages) * kStage + (2 * kTogether * kTokens + BN * (kRows + (kSwap ? 0 : 8))) * 4 + 256;
   static_assert(kCols == 64 || kCols == 128 || kCols == 256 || kCols == 512, "TMEM");
   // Clusters of two launches, each with a CTA that holds TMEM and one that waits for what the other holds, would not end.  Those that fit on an SM
-  // together never ask for more than 512 columns: kernels here whose CTAs wait for one another take 165 KB or more where they take 512.
+  // together never ask for more than 512 columns: kernels here whose CTAs wait for one another take over 128 KB of shared memory where they take 512.
   static_assert(kCols * kPerSm <= 512, "TMEM of an SM");
   static_assert((kSmem + 1024) * kPerSm <= 228 * 1024, "shared memory");
   static_assert(kTogether % kVisit == 0 && (kSwap || kColumns == 32), "");
