@@ -253,9 +253,10 @@ class Qwen2ForCausalLM(nn.Module):
         return static_out
 
     def prefill_hidden(self, inputs_embeds: torch.Tensor, cache: PagedKVCache,
-                       position_ids: Optional[torch.Tensor] = None) -> torch.Tensor:
+                       position_ids: Optional[torch.Tensor] = None, decoded: bool = False) -> torch.Tensor:
         """inputs_embeds [S, hidden] appended to `cache`; returns the final hidden states [S, hidden]
-        BEFORE the last RMSNorm (the caller norms only the rows it needs)."""
+        BEFORE the last RMSNorm (the caller norms only the rows it needs).  decoded: the rows are
+        decoded tokens, not a prompt's: prefill_in_fp8 does not concern them."""
         cfg = self.config
         S = inputs_embeds.shape[0]
         Hq, Hkv, D = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
@@ -269,7 +270,7 @@ class Qwen2ForCausalLM(nn.Module):
         fused_rope = D == 128 and 0 < S <= 384
         # cos / sin once per request (shared by all layers and heads)
         table = ops.rope_table(position_ids, D, self.inv_freq) if S > 0 and D % 16 == 0 else None
-        eights, y = self._fp8_weights() if S > 0 else None, None      # y: what the next norm adds to x
+        eights, y = self._fp8_weights() if S > 0 and not decoded else None, None      # y: what the next norm adds to x
         for li, layer in enumerate(self.model.layers):
             qkv = None
             if eights is not None:
@@ -556,7 +557,7 @@ class Qwen2ForCausalLM(nn.Module):
             if tok in eos_ids:
                 break
             e = self.model.embed_tokens(torch.tensor([tok], device=self.device))
-            hid = self.prefill_hidden(e, cache)
+            hid = self.prefill_hidden(e, cache, decoded=True)
             logits = self.logits_from_hidden(hid)[0]
         ops.check_waits()   # the tokens have been read from the device: they are of complete launches
         return ids
