@@ -62,3 +62,27 @@ def test_sampled_and_constrained_decoding_stays_bf16(llm, how):
     eight, plain = [n for name, n in llm.calls if name == "fp8"], [n for name, n in llm.calls if name == "bf16"]
     assert eight == [7] * 8                       # the prompt: four projections a layer
     assert plain == [1] * 8 * 4                   # every decoded token
+
+
+@pytest.mark.parametrize("first, then", [("inference", "plain"), ("inference", "no_grad"), ("plain", "inference"), ("inference", "inference")])
+def test_8_bit_weights_follow_a_change_in_either_mode(llm, first, then):
+    """Weights made at a prompt in inference mode are made anew, in the same memory, at one outside of it, and the other way round."""
+    modes = dict(inference=torch.inference_mode, plain=torch.enable_grad, no_grad=torch.no_grad)
+    llm.prefill_in_fp8()
+    emb = torch.randn(3, 64).bfloat16()
+
+    def prompt(mode):
+        del llm.calls[:]
+        with modes[mode]():
+            llm.forward(inputs_embeds=emb[None])
+        return [name for name, _ in llm.calls].count("quantise"), [q for qs in llm._fp8_weights() for q in qs]
+
+    made, held = prompt(first)
+    assert made == 8 and not any(q._held().is_inference() for q in held)
+    assert prompt(first)[0] == prompt(then)[0] == 0
+    with torch.no_grad():
+        llm.model.layers[1].mlp.down_proj.weight.mul_(2)
+    made, again = prompt(then)
+    assert made == 8 and [q._held().data_ptr() for q in again] == [q._held().data_ptr() for q in held]
+    assert prompt(then)[0] == prompt(first)[0] == 0
+    assert prompt(first)[0] == 0 and llm.prefill_in_fp8() is llm and prompt(then)[0] == 8

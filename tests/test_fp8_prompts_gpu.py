@@ -27,3 +27,18 @@ def test_constrained_decoding_is_bf16_behind_an_8_bit_prompt(cuda, S):
     for i, tok in enumerate(toks):
         assert torch.equal(llm.logits_from_hidden(hid[-1:])[0].float(), seen[i])
         hid = llm.prefill_hidden(llm.model.embed_tokens(torch.tensor([tok], device=cuda)), cache)
+
+
+@pytest.mark.parametrize("mode", [torch.enable_grad, torch.no_grad, torch.inference_mode])
+def test_weights_made_by_generate_are_made_anew_by_forward(cuda, mode):
+    llm, emb = qwen(layers=2).prefill_in_fp8(), rand(4, 90, 512).to(BF).to(cuda)
+    llm.generate(inputs_embeds=emb[None], max_new_tokens=2, eos_token_id=None)      # in inference mode
+    with torch.no_grad():
+        llm.model.layers[1].mlp.down_proj.weight.mul_(2)
+    with mode():
+        got = llm.forward(inputs_embeds=emb[None]).logits
+    assert torch.equal(llm.forward(inputs_embeds=emb[None]).logits, got)
+    other = qwen(layers=2)
+    with torch.no_grad():
+        other.model.layers[1].mlp.down_proj.weight.mul_(2)
+    assert torch.equal(other.prefill_in_fp8().forward(inputs_embeds=emb[None]).logits, got)

@@ -179,7 +179,8 @@ class Qwen2ForCausalLM(nn.Module):
         tokens' steps stay bf16.  Sequence-parallel prompts stay bf16.  In place; -> self.
         The 8-bit weights are made at the first prompt, not within a graph's capture, and anew, in the same memory, at the first one behind a change
         that torch counts: other tensors, or writes in place.  Behind writes that it does not count (through .data, or to tensors made in
-        inference mode) call this again, not while a prompt runs."""
+        inference mode) call this again, not while a prompt runs.
+        on=False gives their memory back: a caller's graph of prompts in 8 bits is not replayed behind it."""
         self._prefill_graphs.clear()
         self._fp8 = ([] if self._fp8 is None else self._fp8[0], None, None) if on else None
         return self
@@ -196,15 +197,17 @@ class Qwen2ForCausalLM(nn.Module):
             torch.cuda.synchronize(self.device)      # prompts that read the former ones, on whichever stream
             self._prefill_graphs.clear()
             olds, eights = self._fp8[0], []
-            for li, ws in enumerate(held):
-                qs = []
-                for i, w in enumerate(ws):
-                    q, old = ops.fp8_quantize(w, block_rows=ops.FP8_BLOCK), olds[li][i] if olds else None
-                    if old is not None and (old.shape, old.device) == (q.shape, q.device):
-                        old._held().copy_(q._held())      # a caller's captured graph reads it where it is
-                        q = old
-                    qs.append(q)
-                eights.append(tuple(qs))
+            # Tensors made in inference mode cannot be written outside of it, and the first prompt is often a generate's.
+            with torch.inference_mode(False), torch.no_grad():
+                for li, ws in enumerate(held):
+                    qs = []
+                    for i, w in enumerate(ws):
+                        q, old = ops.fp8_quantize(w, block_rows=ops.FP8_BLOCK), olds[li][i] if olds else None
+                        if old is not None and (old.shape, old.device) == (q.shape, q.device):
+                            old._held().copy_(q._held())      # a caller's captured graph reads it where it is
+                            q = old
+                        qs.append(q)
+                    eights.append(tuple(qs))
             torch.cuda.synchronize(self.device)      # the next prompt may come on another stream
             # The tensors themselves are held, too: others that come to lie where they were would be taken for them.
             self._fp8 = (eights, now, [w.detach() for ws in held for w in ws])
