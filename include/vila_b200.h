@@ -989,9 +989,8 @@ int vila_fp8_rmsnorm(const vila_fp8_rmsnorm_params* p, void* stream);
  * blocks (K over a cluster: each CTA's, then the CTAs').  Scales are finite, not negative, or NaN.  bias bf16 or NULL.  act, flags and their parameters as in
  * vila_mx4_linear; with a gated unit the result has N / 2 columns.  The result goes to out in bf16 (row stride ldo), or, with out NULL,
  * unrounded to o_codes and o_scales (block_rows 1).  Rows as they come: x (VILA_DT_*, row stride ldx) instead of a_codes and a_scales, quantised
- * into the scratch first.  w_codes may be read while the launch before this one ends.  Where a launch that lets others begin before its own end
- * (griddepcontrol; vila_fp8_quantize with block_rows 1, vila_fp8_linear) wrote them, one that does not has to come between: a copy, say, or
- * vila_fp8_quantize with block_rows 128. */
+ * into the scratch first.  VILA_FLAG_STATIC_W in flags: w_codes may be fetched while launches before this one are under way.  Set it where the host
+ * has waited for whatever wrote them. */
 typedef struct vila_fp8_linear_params {
   const void* x;
   int64_t ldx;

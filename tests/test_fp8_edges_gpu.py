@@ -1,0 +1,74 @@
+"""GPU: linear layers on 8-bit rows where launches follow one another closely, and at the ends of their numbers' range."""
+import ctypes as C
+
+import pytest
+import torch
+
+from tests.test_fp8_gpu import KERNELS, nothing_left_behind, rand, rows8, weight  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+
+
+@pytest.mark.parametrize("rows", ["codes", "bf16"])
+@pytest.mark.parametrize("M, N, K", KERNELS)
+def test_a_weight_written_in_place_right_before(cuda, M, N, K, rows):
+    """The layer reads what the launch before wrote into its weight, whether rows are quantised between the two or not."""
+    from vila_b200 import ops
+    w, x = ops.fp8_quantize(rand(1, N, K).to(cuda), block_rows=128), rand(2, M, K).to(BF).to(cuda)
+    a = x if rows == "bf16" else ops.fp8_quantize(x)
+    xs = [rand(3 + i, N, K).to(cuda) for i in range(2)]
+    forms = [ops.fp8_quantize(t, block_rows=128) for t in xs]
+    torch.cuda.synchronize()
+    wants = [ops.fp8_linear(a, q) for q in forms]
+    torch.cuda.synchronize()
+    assert not torch.equal(*wants) and not w.static_w
+    for i in range(20):
+        w._held().copy_(forms[i % 2]._held())
+        assert torch.equal(ops.fp8_linear(a, w), wants[i % 2])
+        assert torch.equal(ops.fp8_linear(a, ops.fp8_quantize(xs[i % 2], block_rows=128)), wants[i % 2])
+    w.static_w = True      # behind a synchronisation the same numbers
+    torch.cuda.synchronize()
+    assert torch.equal(ops.fp8_linear(a, w), wants[1])
+
+
+def test_a_flag_that_a_layer_does_not_know_is_refused(cuda):
+    from vila_b200 import _lib, ops
+    (q, _), (a, _) = weight(1, 64, 64, cuda), rows8(rand(2, 3, 64), cuda)
+    out = torch.full((3, 64), 7.0, dtype=BF, device=cuda)
+    codes, scales = a._ptrs()
+    w_codes, w_scales = q._ptrs()
+    for flags, ok in ((2, True), (16, False), (18, False), (-1, False), (2 | 1 | 8, False)):
+        p = _lib.Fp8LinearParams(a_codes=codes, lda=64, a_scales=scales, ld_as=4, w_codes=w_codes, ldw=64, w_scales=w_scales, ld_ws=1, out=out.data_ptr(), ldo=64,
+                                 M=3, N=64, K=64, flags=flags)
+        torch.cuda.synchronize()
+        assert (_lib.load().vila_fp8_linear(C.byref(p), None) == 0) == ok
+    torch.cuda.synchronize()
+    assert torch.equal(out, ops.fp8_linear(a, q))
+
+
+@pytest.mark.parametrize("tries", [0, 1, -2, -3, -4, -5])
+@pytest.mark.parametrize("M, N, K", [(1, 300, 9000), (20, 300, 700), (100, 300, 9000), (300, 770, 520)])
+def test_waits_that_run_out_with_weights_fetched_ahead(cuda, monkeypatch, M, N, K, tries):
+    """What was fetched ahead has landed before the launch ends, whoever gave up; the next status says so once, and the call after that is right."""
+    from vila_b200 import _lib, ops
+    w, a = ops.fp8_quantize(rand(1, N, K).to(cuda), block_rows=128), ops.fp8_quantize(rand(2, M, K).to(cuda))
+    want = ops.fp8_linear(a, w)
+    torch.cuda.synchronize()
+    w.static_w = True
+    ops.check_waits()
+    lib = _lib.load()
+    with monkeypatch.context() as m:
+        m.setattr(lib, "vila_fp8_linear", lambda p, stream: lib.vila_fp8_linear_tries(p, tries, stream))
+        out = ops.fp8_linear(a, w)
+        torch.cuda.synchronize()
+    if tries <= 0 or not torch.equal(out, want):
+        with pytest.raises(RuntimeError, match="ran out of tries"):
+            ops.check_waits()
+    else:
+        try:      # a warp may have given up behind the last wait that its output needs
+            ops.check_waits()
+        except RuntimeError:
+            pass
+    ops.check_waits()
+    assert torch.equal(ops.fp8_linear(a, w), want)

@@ -86,3 +86,38 @@ def test_8_bit_weights_follow_a_change_in_either_mode(llm, first, then):
     assert made == 8 and [q._held().data_ptr() for q in again] == [q._held().data_ptr() for q in held]
     assert prompt(then)[0] == prompt(first)[0] == 0
     assert prompt(first)[0] == 0 and llm.prefill_in_fp8() is llm and prompt(then)[0] == 8
+
+
+def test_only_weights_that_were_waited_for_are_fetched_ahead(llm, monkeypatch):
+    """A layer asks for its weight ahead of what the launch before wrote only where the weight says so: those of a model behind a synchronisation."""
+    from types import SimpleNamespace
+    weight = ops.Fp8(torch.zeros(64, 64).to(torch.float8_e4m3fn), torch.ones(1, 1), 128)
+    kept = ops.Fp8Kept(ops.Fp8(torch.zeros(64, 64).to(torch.float8_e4m3fn), torch.ones(1, 1), 128), torch.zeros(8, 64).bfloat16())
+    x, asked = torch.zeros(3, 64).bfloat16(), []
+    monkeypatch.undo()
+    monkeypatch.setattr(ops, "_mx4_here", lambda t, name: None)
+    monkeypatch.setattr(ops, "_chk", lambda t, name: None)
+    monkeypatch.setattr(ops, "_stream", lambda: 0)
+    lib = SimpleNamespace(vila_fp8_linear_scratch=lambda p: 0, vila_fp8_linear=lambda p, stream: asked.append(p._obj.flags & 2) or 0)
+    monkeypatch.setattr(ops._lib, "load", lambda: lib)
+    monkeypatch.setattr(ops, "linear", lambda x, w, bias, static_w, out: asked.append(2 * static_w))
+    for call in (lambda: ops.fp8_linear(x, weight), lambda: ops.linear_any(x, weight)):
+        weight.static_w = False
+        call()
+        weight.static_w = True
+        call()
+    assert asked == [0, 2, 0, 2]
+    ops.linear_any(x, kept)
+    kept.static_w = True
+    ops.linear_any(x, kept)
+    assert asked[4:] == [0, 0, 2, 2]
+    assert not ops.Fp8._alloc(x, 4, 64, 128).static_w and not ops.Fp8(weight.codes, weight.scales, 128).static_w
+
+
+def test_a_prompts_weights_are_fetched_ahead_once_they_were_waited_for(llm, monkeypatch):
+    waited, made = [], []
+    quantise = ops.fp8_quantize
+    monkeypatch.setattr(ops, "fp8_quantize", lambda w, block_rows: made.append(quantise(w, block_rows=block_rows)) or made[-1])
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda *a: waited.append((len(made), any(q.static_w for q in made))))
+    eights = llm.prefill_in_fp8()._fp8_weights()
+    assert waited == [(0, False), (8, False)] and all(q.static_w for qs in eights for q in qs)

@@ -26,7 +26,7 @@ int fp8_linear(const vila_fp8_linear_params& given, cudaStream_t stream, int tri
   if (wait_status()) return 1;   // an earlier launch gave up: nothing is built on its output
   VB_CHECK(p.M >= 0 && p.N > 0 && p.K > 0 && p.M <= (1 << 30) && p.N <= (1 << 30) && p.K <= (1 << 30), "fp8_linear: M=%d N=%d K=%d", p.M, p.N, p.K);
   const int gated = p.flags & kGluFlags;
-  VB_CHECK((p.flags & ~kGluFlags) == 0 && (gated & (gated - 1)) == 0, "fp8_linear: flags=%d (one gated unit at most)", p.flags);
+  VB_CHECK((p.flags & ~(kGluFlags | VILA_FLAG_STATIC_W)) == 0 && (gated & (gated - 1)) == 0, "fp8_linear: flags=%d (one gated unit at most)", p.flags);
   VB_CHECK(gated == 0 || p.N % 2 == 0, "fp8_linear: a gated unit has an even number of weight rows (N=%d)", p.N);
   VB_CHECK(gated == 0 || p.act == VILA_ACT_NONE, "fp8_linear: a gated unit takes no other activation (act=%d)", p.act);
   VB_CHECK(p.act == VILA_ACT_NONE || p.act == VILA_ACT_GELU_TANH || p.act == VILA_ACT_GELU_ERF || p.act == VILA_ACT_SILU ||

@@ -18,9 +18,9 @@
 // A CTA takes one tile, or, where the tiles leave SMs idle, a share of its blocks: a cluster of up to 8 CTAs splits K, every CTA sends
 // its sums to the CTAs that finish them, by rows, and these add them in rank order.
 //
-// A launch may begin before the one before it has ended: TMEM and the first weights are asked for while that one ends, everything else comes
-// behind griddepcontrol.wait.  So what writes a weight must not let the next launch begin before its own end: the weights' quantisation is
-// launched so, and the Python class has such a launch behind codes of another origin.
+// A launch may begin before the one before it has ended: TMEM is asked for while that one ends, and so are the first weights where the caller says
+// that the host has waited for what wrote them (VILA_FLAG_STATIC_W).  Everything else comes behind griddepcontrol.wait: that alone promises that
+// what the launch before wrote can be seen, even where that one lets none begin before its own end.
 #include "../../include/vila_b200.h"
 #include "common.cuh"
 #include "fp8.cuh"
@@ -180,7 +180,8 @@ fp8_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ C
 
   if (split > 1) cluster_arrive();      // this CTA runs: others may write to its shared memory
   const uint32_t bytes = S::kPBytes + bn * 128;                                // of a stage
-  const int ahead = limit.quits == 0 ? 0 : min(ST, kb1 - kb0);                 // stages whose weights are asked for before the launch before has ended
+  // stages whose weights are asked for before the launch before has ended
+  const int ahead = (p.flags & VILA_FLAG_STATIC_W) == 0 || limit.quits == 0 ? 0 : min(ST, kb1 - kb0);
   if (warp == S::kTma) {
     if (lane == 0) {
       tma_prefetch_desc(&tmap_p);

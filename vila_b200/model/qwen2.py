@@ -208,7 +208,9 @@ class Qwen2ForCausalLM(nn.Module):
                             q = old
                         qs.append(q)
                     eights.append(tuple(qs))
-            torch.cuda.synchronize(self.device)      # the next prompt may come on another stream
+            torch.cuda.synchronize(self.device)      # the next prompt may come on another stream, and fetches them ahead
+            for q in (q for qs in eights for q in qs):
+                q.static_w = True
             # The tensors themselves are held, too: others that come to lie where they were would be taken for them.
             self._fp8 = (eights, now, [w.detach() for ws in held for w in ws])
         return self._fp8[0]

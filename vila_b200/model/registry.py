@@ -78,6 +78,12 @@ def quantize_weights(model, to: str = "mx4"):
                 if first > 0:
                     keep = w.shape[0] - first
                     setattr(layer, name, ops.mx4_quantize(w, keep=keep) if to == "mx4" else ops.fp8_quantize(w, block_rows=ops.FP8_BLOCK, keep=keep))
+    if to == "fp8":
+        if torch.device(model.device).type == "cuda":
+            torch.cuda.synchronize(model.device)
+        for q in (getattr(layer, name, None) for layer in model.layers for name in names):
+            if isinstance(q, ops.Fp8):
+                q.static_w = True
     return model
 
 

@@ -1515,7 +1515,9 @@ class Fp8:
     """A matrix of e4m3 numbers with an fp32 scale per block of 128 columns of one row (block_rows 1: activations) or of 128 rows (block_rows
     128: weights).  Made by fp8_quantize, fp8_rmsnorm and fp8_linear(to8=True), or by fp8_pack from a checkpoint's tensors."""
 
-    __slots__ = ("rows", "cols", "block_rows", "_codes", "_ldc", "_scales", "_lds", "_both", "_at")
+    # static_w: a layer may fetch this weight while launches before it are under way (VILA_FLAG_STATIC_W).  Set by who has waited on the host for
+    # what wrote it, and writes it no more (or waits again behind that); the models do.
+    __slots__ = ("rows", "cols", "block_rows", "static_w", "_codes", "_ldc", "_scales", "_lds", "_both", "_at")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, block_rows: int):
         """codes [rows, cols] float8_e4m3fn, rows a multiple of 16 bytes apart, on a 16-byte boundary; scales fp32, with block_rows 128
@@ -1523,20 +1525,16 @@ class Fp8:
         rows, columns a multiple of 4 apart (and that much memory to the end), on a 16-byte boundary."""
         _fp8_shape(codes, scales, block_rows)
         self.rows, self.cols = codes.shape
-        self.block_rows, self._codes, self._scales, self._both, self._at = block_rows, codes, scales, None, 0
+        self.block_rows, self.static_w, self._codes, self._scales, self._both, self._at = block_rows, False, codes, scales, None, 0
         self._ldc, self._lds = _fp8_ldc_of(codes), _fp8_lds_of(scales, block_rows)
         _fp8_check(self._lds > 0, "the scales do not lie as the kernels read them (fp8_pack copies those that do not)")
         _fp8_check(self._ldc > 0, "rows of codes must start on 16-byte boundaries and have whole 16 bytes of memory (fp8_pack copies those that do not)")
-        if block_rows == FP8_BLOCK and codes.is_cuda:
-            # A linear layer asks for its first weights while the launch before it ends.  What wrote these codes may be a launch that lets others
-            # begin before its end (rows' quantisation is): one that does not comes between.
-            scales.new_zeros(1)
 
     @classmethod
     def _alloc(cls, like: torch.Tensor, rows: int, cols: int, block_rows: int) -> "Fp8":
         """Uninitialised, codes and scales in one piece of memory on the device of `like`: the views of it are made when they are asked for."""
         q = cls.__new__(cls)
-        q.rows, q.cols, q.block_rows, q._codes, q._scales = rows, cols, block_rows, None, None
+        q.rows, q.cols, q.block_rows, q.static_w, q._codes, q._scales = rows, cols, block_rows, False, None, None
         q._ldc = (cols + 15) // 16 * 16
         blocks = (cols + 127) // 128
         if block_rows == 1:
@@ -1596,6 +1594,14 @@ class Fp8Kept(Fp8):
     def __init__(self, part: Fp8, kept: torch.Tensor):
         self.part, self.kept = part, kept
         self.rows, self.cols, self.block_rows = part.rows + kept.shape[0], part.cols, part.block_rows
+
+    @property
+    def static_w(self) -> bool:
+        return self.part.static_w
+
+    @static_w.setter
+    def static_w(self, on: bool) -> None:
+        self.part.static_w = on
 
     def _held(self) -> torch.Tensor:
         return self.part._held()
@@ -1754,8 +1760,8 @@ def fp8_linear(a, w: Fp8, bias: Optional[torch.Tensor] = None, *, act: int = ACT
                swiglu: bool = False, geglu: bool = False, glu_clamp: Optional[Tuple[float, float]] = None, out: Optional[torch.Tensor] = None,
                to8: bool = False):
     """act(a [M, K] . w[N, K]^T + bias) in bf16, or with to8 as Fp8 rows (quantised unrounded: what the next layer reads).  a: Fp8 with
-    block_rows 1, or bf16 / fp32 rows, which are quantised first; w: Fp8 with block_rows 128.  fp32 sums.  Activations and gated units as
-    in linear / glinear."""
+    block_rows 1, or bf16 / fp32 rows, which are quantised first; w: Fp8 with block_rows 128, fetched ahead where w.static_w says so.  fp32
+    sums.  Activations and gated units as in linear / glinear."""
     if not isinstance(w, Fp8) or w.block_rows != FP8_BLOCK or not (isinstance(a, torch.Tensor) or (isinstance(a, Fp8) and a.block_rows == 1)):
         raise RuntimeError("vila_b200.ops: a must be Fp8 rows (block_rows 1) or a tensor, w an Fp8 weight (block_rows 128)")
     held = w._held()
@@ -1808,7 +1814,7 @@ def fp8_linear(a, w: Fp8, bias: Optional[torch.Tensor] = None, *, act: int = ACT
         rest, to = None if bias is None else bias[n:], out[:, cut:]
         if (act == ACT_NONE and not flags and K % 8 == 0 and (N - n) % 8 == 0 and a.stride(0) % 8 == 0 and a.stride(0) >= K and a.data_ptr() % 16 == 0
                 and to.stride(0) % 8 == 0 and to.data_ptr() % 16 == 0):
-            linear(a, w.kept, rest, static_w=True, out=to)
+            linear(a, w.kept, rest, static_w=w.static_w, out=to)
         else:      # with an activation: glinear rounds once, behind it, as the 8-bit rows' kernels do
             glinear(a, w.kept, out=to, bias=rest, **more)
         return out
@@ -1816,7 +1822,7 @@ def fp8_linear(a, w: Fp8, bias: Optional[torch.Tensor] = None, *, act: int = ACT
     pos, neg = act_params if act_params is not None else (0.0, 0.0)
     w_codes, w_scales = w._ptrs()
     p = _lib.Fp8LinearParams(x_ptr, ldx, a_codes, lda, a_scales, ld_as, w_codes, w._ldc, w_scales, w._lds, None if bias is None else bias.data_ptr(), o_ptr,
-                             ldo, o_codes, ld_oc, o_scales, ld_os, alpha, limit, pos, neg, M, N, K, act, flags, x_dt)
+                             ldo, o_codes, ld_oc, o_scales, ld_os, alpha, limit, pos, neg, M, N, K, act, flags | (2 if w.static_w else 0), x_dt)
     lib = _lib.load()
     if to8 or x_ptr is not None:      # a workspace of the call's own: a captured graph keeps its own, too
         n = lib.vila_fp8_linear_scratch(C.byref(p))
