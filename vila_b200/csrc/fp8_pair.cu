@@ -191,13 +191,13 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
       for (int i = 0; i < 128; ++i) z[i] = 0.f;
       float sa_now[kAhead], sa_next[kAhead];
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) sa_now[j] = j < nkb ? __ldg(sa + j * p.ld_as) : 0.f;
+      for (int j = 0; j < kAhead; ++j) sa_now[j] = j < nkb ? sa[j * p.ld_as] : 0.f;
       float w32 = 0.f;                        // of 32 blocks, one a lane
 #pragma unroll 1
       for (int kb = 0; kb < nkb && ok; kb += kAhead) {
-        if ((kb & 31) == 0) w32 = kb + lane < nkb ? __ldg(sw + kb + lane) : 0.f;
+        if ((kb & 31) == 0) w32 = kb + lane < nkb ? sw[kb + lane] : 0.f;
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) sa_next[j] = kb + kAhead + j < nkb ? __ldg(sa + (kb + kAhead + j) * p.ld_as) : 0.f;
+        for (int j = 0; j < kAhead; ++j) sa_next[j] = kb + kAhead + j < nkb ? sa[(kb + kAhead + j) * p.ld_as] : 0.f;
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
           if (kb + j < nkb && ok) {

@@ -289,7 +289,8 @@ fp8_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ C
     __syncwarp();
   } else if (warp == S::kScale) {
     griddep_wait();
-    // a lane takes four tokens; a row of scales is a multiple of 4 long, and behind the last token nothing counts
+    // a lane takes four tokens; a row of scales is a multiple of 4 long, and behind the last token nothing counts.  Plain loads: the launch before may
+    // still write what this one reads, and the read-only path is for what no launch writes meanwhile.
     const int most = kSwap ? bn : kRows;
     const bool there = lane * 4 < most && t0 + lane * 4 < p.ld_as;
     const float* sa = p.a_scales + (there ? t0 + lane * 4 : 0);
@@ -301,8 +302,8 @@ fp8_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ C
 #pragma unroll
       for (int i = 0; i < S::kTogether; ++i) {
         const bool in = there && kb + i < kb1;
-        a[i] = in ? __ldg(reinterpret_cast<const float4*>(sa + (kb + i) * p.ld_as)) : make_float4(0.f, 0.f, 0.f, 0.f);
-        w[i] = in ? __ldg(sw + kb + i) : 0.f;
+        a[i] = in ? *reinterpret_cast<const float4*>(sa + (kb + i) * p.ld_as) : make_float4(0.f, 0.f, 0.f, 0.f);
+        w[i] = in ? sw[kb + i] : 0.f;
       }
       ok = mx4_warp_wait(&scale_free[g & 1], ((g >> 1) & 1) ^ 1, gave_up, limit.tries);      // the first two pass
       if (!ok) break;
