@@ -10,8 +10,7 @@
 //   scale warp      the products of both scales, a group of blocks at a time, into shared memory
 //   epilogue warps  two blocks at a time: scales times accumulators, added up
 //
-// Up to 32 tokens (kSwap): weight rows are the 128 lanes of a tile, tokens its columns, of which there are only as many as needed; bound by the
-// weights' bytes.  More tokens: these are the lanes, 64 or 128 weight rows the columns, so that a thread's scale is one number a block (as one a column
+// Up to 32 tokens (kSwap): weight rows are the 128 lanes of a tile, tokens its 16 or 32 columns; bound by the weights' bytes.  More tokens: these are the lanes, 64 or 128 weight rows the columns, so that a thread's scale is one number a block (as one a column
 // it took four loads from shared memory per 16 columns, in line with the loads from TMEM: 0.43 us a block instead of 0.3).  There a block
 // costs what an epilogue warp does for it one after another: a wait takes 150 - 250 clocks even if it is over, 16 columns of TMEM 70.
 //
@@ -150,11 +149,11 @@ __device__ __forceinline__ void finish_rows(const vila_fp8_linear_params& p, con
   });
 }
 
-// bn: columns of a tile, with kSwap a multiple of 16, at most BN.  split: CTAs of a cluster, which share a tile and cut K.
+// split: CTAs of a cluster, which share a tile and cut K.
 template <int BN, bool kSwap>
 __global__ void __launch_bounds__(Shape<BN, kSwap>::kThreads, Shape<BN, kSwap>::kPerSm)
 fp8_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ CUtensorMap tmap_q, const vila_fp8_linear_params p, const vila_glinear_ext x,
-           float* out32, const int bn, const int split, const WaitLimit limit, volatile unsigned int* failed) {
+           float* out32, const int split, const WaitLimit limit, volatile unsigned int* failed) {
   using S = Shape<BN, kSwap>;
   constexpr int ST = S::kStages;
   extern __shared__ uint8_t smem_raw[];
@@ -175,11 +174,10 @@ fp8_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ C
   const int p_tiles = ((kSwap ? p.N : p.M) + kRows - 1) / kRows, nkb = fp8_blocks(p.K);
   const int tile = static_cast<int>(blockIdx.x) / split, rank = static_cast<int>(blockIdx.x) - tile * split;
   const int kb0 = static_cast<int>(static_cast<long long>(nkb) * rank / split), kb1 = static_cast<int>(static_cast<long long>(nkb) * (rank + 1) / split);
-  const int qt = tile / p_tiles, p0 = (tile - qt * p_tiles) * kRows, q0 = qt * bn;      // tiles that run together share their columns' rows
+  const int qt = tile / p_tiles, p0 = (tile - qt * p_tiles) * kRows, q0 = qt * BN;      // tiles that run together share their columns' rows
   const int t0 = kSwap ? q0 : p0, n0 = kSwap ? p0 : q0;                                 // first token, first weight row
 
   if (split > 1) cluster_arrive();      // this CTA runs: others may write to its shared memory
-  const uint32_t bytes = S::kPBytes + bn * 128;                                // of a stage
   // stages whose weights are asked for before the launch before has ended
   const int ahead = (p.flags & VILA_FLAG_STATIC_W) == 0 || limit.quits == 0 ? 0 : min(ST, kb1 - kb0);
   if (warp == S::kTma) {
@@ -200,7 +198,7 @@ fp8_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ C
       *gave_up = 0;
       fence_barrier_init();
       for (int i = 0; i < ahead; ++i) {
-        mbar_arrive_expect_tx(&full_bar[i], bytes);
+        mbar_arrive_expect_tx(&full_bar[i], S::kStage);
         tma_load_2d(smem + i * S::kStage + (kSwap ? 0 : S::kPBytes), kSwap ? &tmap_p : &tmap_q, &full_bar[i], (kb0 + i) * 128, n0);
       }
     }
@@ -236,7 +234,7 @@ fp8_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ C
       if (one) {
         uint8_t* st = smem + s * S::kStage;
         if (!first) {
-          mbar_arrive_expect_tx(&full_bar[s], bytes);
+          mbar_arrive_expect_tx(&full_bar[s], S::kStage);
           tma_load_2d(st + w_at, tw, &full_bar[s], kb * 128, n0);
         }
         tma_load_2d(st + a_at, ta, &full_bar[s], kb * 128, t0);
@@ -259,7 +257,7 @@ fp8_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ C
     // The whole warp walks the loop and one lane issues: what the instructions are given stays in uniform registers.
     const bool one = elect_one();
     const uint64_t pd0 = make_smem_desc(smem_u32(smem), 16, 1024, kLayoutSW128), qd0 = make_smem_desc(smem_u32(smem) + S::kPBytes, 16, 1024, kLayoutSW128);
-    const uint32_t idesc = fp8_idesc(kRows, bn);
+    constexpr uint32_t idesc = fp8_idesc(kRows, BN);
     griddep_wait();                       // or the tries of the first wait would be spent on the launch before
     int s = 0, v = 0;                     // stage, visits of the epilogue warps so far
     uint32_t ph = 0;
@@ -291,8 +289,7 @@ fp8_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ C
     griddep_wait();
     // a lane takes four tokens; a row of scales is a multiple of 4 long, and behind the last token nothing counts.  Plain loads: the launch before may
     // still write what this one reads, and the read-only path is for what no launch writes meanwhile.
-    const int most = kSwap ? bn : kRows;
-    const bool there = lane * 4 < most && t0 + lane * 4 < p.ld_as;
+    const bool there = lane * 4 < S::kTokens && t0 + lane * 4 < p.ld_as;
     const float* sa = p.a_scales + (there ? t0 + lane * 4 : 0);
     const float* sw = p.w_scales + (n0 / kFp8Block) * p.ld_ws;
     int g = 0;
@@ -379,7 +376,7 @@ fp8_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ C
 #pragma unroll 1
             for (int i = lane; i < S::kColumns * 8; i += 32) {
               const int c = c0 + i / 8, r = quad * 32 + 4 * (i % 8);
-              if (c < bn) finish<decltype(epi)::value>(p, x, out32, ld32, wide, t0 + c, n0 + r, *reinterpret_cast<const float4*>(sums + c * kRows + r));
+              finish<decltype(epi)::value>(p, x, out32, ld32, wide, t0 + c, n0 + r, *reinterpret_cast<const float4*>(sums + c * kRows + r));
             }
           });
         } else {
@@ -409,7 +406,7 @@ fp8_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ C
     cluster_wait();
     const int share = kRows / split;
     if constexpr (kSwap) {
-      const int fours = share / 4, items = min(bn, p.M - q0) * fours;
+      const int fours = share / 4, items = min(BN, p.M - q0) * fours;
       mx4_with_epilogue(p, [&](auto epi) {
 #pragma unroll 1
         for (int i = tid; i < items; i += S::kThreads) {
@@ -480,10 +477,9 @@ int launch(const vila_fp8_linear_params& p, const vila_glinear_ext& x, float* ou
   using S = Shape<BN, kSwap>;
   static PerDeviceOnce once;
   VB_ALLOW_SMEM(once, fp8_kernel<BN, kSwap>, static_cast<int>(S::kSmem));
-  const int bn = kSwap ? (p.M + 15) / 16 * 16 : BN;
   CUtensorMap tw, ta;
   if (int rc = make_tmap_2d_u8(&tw, p.w_codes, p.N, p.K, p.ldw, kSwap ? kRows : BN, 128, 128)) return rc;
-  if (int rc = make_tmap_2d_u8(&ta, p.a_codes, p.M, p.K, p.lda, kSwap ? bn : kRows, 128, 128)) return rc;
+  if (int rc = make_tmap_2d_u8(&ta, p.a_codes, p.M, p.K, p.lda, S::kTokens, 128, 128)) return rc;
   const long long tiles = kSwap ? (p.N + kRows - 1) / kRows : static_cast<long long>((p.N + BN - 1) / BN) * ((p.M + kRows - 1) / kRows);
   VB_CHECK(tiles < (1LL << 27), "fp8_linear: too many tiles (M=%d N=%d)", p.M, p.N);
   static Mx4Clusters clusters;
@@ -495,7 +491,7 @@ int launch(const vila_fp8_linear_params& p, const vila_glinear_ext& x, float* ou
   for (int l = 1; l <= 3 && (1 << l) <= limit && tiles <= static_cast<long long>(S::kPerSm) * clusters.of(fp8_kernel<BN, kSwap>, l, S::kThreads, S::kSmem); ++l)
     split = 1 << l;
   VB_CUDA(launch_pdl_cluster(fp8_kernel<BN, kSwap>, dim3(static_cast<unsigned>(tiles * split)), dim3(S::kThreads), S::kSmem, stream, dim3(split),
-                             kSwap ? tw : ta, kSwap ? ta : tw, p, x, out32, bn, split, wait_limit(tries), failed_word()));
+                             kSwap ? tw : ta, kSwap ? ta : tw, p, x, out32, split, wait_limit(tries), failed_word()));
   return 0;
 }
 
