@@ -985,8 +985,9 @@ typedef struct vila_fp8_rmsnorm_params {
 } vila_fp8_rmsnorm_params;
 int vila_fp8_rmsnorm(const vila_fp8_rmsnorm_params* p, void* stream);
 /* vila_fp8_linear: out[m, n] = epi(sum_k a[m, k] w[n, k] + bias[n]), a [M, K] with block_rows 1, w [N, K] with block_rows 128.  Products of a
- * block's numbers and their sum in fp32, times the product of both scales (fp32, cut at fp32's largest number), added in fp32 in the order of the
- * blocks (K over a cluster: each CTA's, then the CTAs').  Scales are finite, not negative, or NaN.  bias bf16 or NULL.  act, flags and their parameters as in
+ * block's numbers and their sum in fp32, times the product of both scales, added in fp32 in the order of the blocks (K over a cluster: each CTA's,
+ * then the CTAs').  The scales' product is an fp32 number, below 2^-126 with as many bits as fp32 has there; where it is past fp32's largest one, zero sums stay
+ * zero, and others are what fp32 holds of the whole.  Scales are finite, not negative, or NaN.  bias bf16 or NULL.  act, flags and their parameters as in
  * vila_mx4_linear; with a gated unit the result has N / 2 columns.  The result goes to out in bf16 (row stride ldo), or, with out NULL,
  * unrounded to o_codes and o_scales (block_rows 1).  Rows as they come: x (VILA_DT_*, row stride ldx) instead of a_codes and a_scales, quantised
  * into the scratch first.  VILA_FLAG_STATIC_W in flags: w_codes may be fetched while launches before this one are under way.  Set it where the host

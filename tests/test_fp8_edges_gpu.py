@@ -4,10 +4,12 @@ import ctypes as C
 import pytest
 import torch
 
-from tests.test_fp8_gpu import KERNELS, nothing_left_behind, rand, rows8, weight  # noqa: F401
+from tests import fp8_reference as R
+from tests.test_fp8_gpu import KERNELS, check_rows8, nothing_left_behind, rand, rows8, weight  # noqa: F401
+from tests.test_mx4_gpu import check_product
 
 pytestmark = pytest.mark.gpu
-BF = torch.bfloat16
+BF, E4M3 = torch.bfloat16, torch.float8_e4m3fn
 
 
 @pytest.mark.parametrize("rows", ["codes", "bf16"])
@@ -72,3 +74,42 @@ def test_waits_that_run_out_with_weights_fetched_ahead(cuda, monkeypatch, M, N, 
             pass
     ops.check_waits()
     assert torch.equal(ops.fp8_linear(a, w), want)
+
+
+@pytest.mark.parametrize("to8", [False, True])
+@pytest.mark.parametrize("M, N, K", KERNELS + [(32, 130, 300), (128, 130, 1300), (129, 300, 700)])
+def test_products_of_scales_past_fp32(cuda, M, N, K, to8):
+    """Blocks whose scales' product is past fp32's largest number: sums that make it finite again are what they are, sums of zero count nothing, and tokens
+    beside them whose product is an ordinary one are what they were."""
+    from vila_b200 import ops
+    blocks, tiny = -(-K // 128), torch.tensor([0.0, 2.0 ** -9, -2.0 ** -9, 2.0 ** -8])
+    pick = torch.Generator().manual_seed(5)
+    codes, scales = R.quantise(rand(1, N, K), 128)
+    a_codes, a_scales = R.quantise(rand(2, M, K))
+    codes[:, 128:256] = tiny[torch.randint(4, (N, 128), generator=pick)].double()
+    a_codes[:, 128:256] = tiny[torch.randint(4, (M, 128), generator=pick)].double()
+    scales[:, 1] = 1.5 * 2.0 ** 65
+    a_scales[:, 1] = torch.where(torch.arange(M) % 3 == 0, 1.25 * 2.0 ** 66, 2.0 ** -20)      # sums up to 128 x 2^-16: 2^123
+    a_codes[:, 256:384], a_scales[:, 2] = 0, 3e38
+    scales[:, 2] = 3e38
+    assert blocks > 2 and (a_scales[0, 1].double() * scales[0, 1].double()) > 3.5e38
+    q, a = ops.fp8_pack(codes.to(E4M3).to(cuda), scales.to(cuda)), ops.fp8_pack(a_codes.to(E4M3).to(cuda), a_scales.to(cuda), block_rows=1)
+    got, x, w = ops.fp8_linear(a, q, to8=to8), R.values(a_codes, a_scales), R.values(codes, scales, 128)
+    (check_rows8 if to8 else check_product)(got, x, w, None)
+
+
+@pytest.mark.parametrize("M, N, K", KERNELS + [(32, 130, 300), (128, 130, 1300)])
+def test_what_fp32_cannot_hold_is_an_infinity(cuda, M, N, K):
+    from vila_b200 import ops
+    codes, scales = R.quantise(rand(1, N, K), 128)
+    a_codes, a_scales = R.quantise(rand(2, M, K))
+    plain = ops.fp8_linear(ops.fp8_pack(a_codes.to(E4M3).to(cuda), a_scales.to(cuda), block_rows=1), ops.fp8_pack(codes.to(E4M3).to(cuda), scales.to(cuda)))
+    a_codes[:, 128:256] = 0
+    base = ops.fp8_linear(ops.fp8_pack(a_codes.to(E4M3).to(cuda), a_scales.to(cuda), block_rows=1), ops.fp8_pack(codes.to(E4M3).to(cuda), scales.to(cuda)))
+    m, sign = M // 2, (torch.arange(N) % 3 - 1).double()
+    a_codes[m, 133], a_scales[m, 1], scales[:, 1] = 1.0, 3e38, 4.0
+    codes[:, 133] = sign
+    got = ops.fp8_linear(ops.fp8_pack(a_codes.to(E4M3).to(cuda), a_scales.to(cuda), block_rows=1), ops.fp8_pack(codes.to(E4M3).to(cuda), scales.to(cuda)))
+    want = base.clone()
+    want[m] = torch.where(sign.to(cuda) == 0, base[m], (sign * torch.inf).to(cuda).to(BF))
+    assert torch.equal(got, want) and not torch.equal(plain, base)

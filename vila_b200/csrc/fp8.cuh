@@ -64,10 +64,27 @@ __device__ __forceinline__ void fp8_fma2(float& d0, float& d1, float a0, float a
       : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
 }
 
-// Both scales of a block's products.  Their product is cut at fp32's largest number: sums that are zero stay zero.  A NaN stays one.
+// Both scales of a block's products, which are finite and not negative, or NaN.  A product past fp32's largest number is given as minus its 2^-128th:
+// the sums that it is for go through fp8_widen first, so that sums of zero stay zero and what fp32 can hold is what it is.
 __device__ __forceinline__ float fp8_both_scales(float a, float b) {
   const float s = a * b;
-  return s > 3.40282347e38f ? 3.40282347e38f : s;
+  return s > 3.40282347e38f ? -(a * 0x1p-64f * (b * 0x1p-64f)) : s;
+}
+__device__ __forceinline__ bool fp8_is_wide(float both) { return both < 0.f; }
+// A block's sums of a warp's lanes in TMEM, `columns` from `at` on, times -2^128 where both(column) is wide.  In place and by a short loop: on the
+// registers that the sums go to behind it, it made the kernel of CTA pairs spill.
+template <typename F>
+__device__ __forceinline__ void fp8_widen(uint32_t at, int columns, F&& both) {
+#pragma unroll 1
+  for (int c = 0; c < columns; c += 8) {
+    float r[8];
+    tmem_ld_32x32b_x8(at + c, reinterpret_cast<uint32_t*>(r));
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = fp8_is_wide(both(c + i)) ? r[i] * 0x1p64f * -0x1p64f : r[i];
+    tmem_st_32x32b_x8(at + c, reinterpret_cast<uint32_t*>(r));
+  }
+  tmem_st_wait();
 }
 
 }  // namespace vb

@@ -192,21 +192,28 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
       float sa_now[kAhead], sa_next[kAhead];
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) sa_now[j] = j < nkb ? sa[j * p.ld_as] : 0.f;
-      float w32 = 0.f;                        // of 32 blocks, one a lane
+      float w_now = lane < nkb ? sw[lane] : 0.f;      // of 32 blocks, one a lane
+      // a block's factor, and whether any lane's is wide: made while the block before is fetched from TMEM
+      float both = fp8_both_scales(sa_now[0], __shfl_sync(0xffffffffu, w_now, 0));
+      bool any_wide = __any_sync(0xffffffffu, fp8_is_wide(both));
 #pragma unroll 1
       for (int kb = 0; kb < nkb && ok; kb += kAhead) {
-        if ((kb & 31) == 0) w32 = kb + lane < nkb ? sw[kb + lane] : 0.f;
+        float w_next = w_now;
+        if (((kb + kAhead) & 31) == 0) w_next = kb + kAhead + lane < nkb ? sw[kb + kAhead + lane] : 0.f;
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) sa_next[j] = kb + kAhead + j < nkb ? sa[(kb + kAhead + j) * p.ld_as] : 0.f;
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
           if (kb + j < nkb && ok) {
-            const float both = fp8_both_scales(sa_now[j], __shfl_sync(0xffffffffu, w32, (kb + j) & 31));
             ok = mx4_warp_wait(&done_bar[s], ph, gave_up, limit.tries);
             if (ok) {
               tc_fence_after();
+              if (any_wide) fp8_widen(lanes + a * kN, 128, [&](int) { return both; });
               float r[2][16];
               tmem_ld_32x32b_x16(lanes + a * kN, reinterpret_cast<uint32_t*>(r[0]));
+              const float both_next = fp8_both_scales(j + 1 < kAhead ? sa_now[(j + 1) % kAhead] : sa_next[0],
+                                                      __shfl_sync(0xffffffffu, j + 1 < kAhead ? w_now : w_next, (kb + j + 1) & 31));
+              any_wide = __any_sync(0xffffffffu, fp8_is_wide(both_next));
 #pragma unroll
               for (int c = 0; c < 8; ++c) {      // a chunk is fetched under the sums of the one before
                 tmem_ld_wait();
@@ -222,9 +229,11 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
                 s = 0;
                 ph ^= 1;
               }
+              both = both_next;
             }
           }
         }
+        w_now = w_next;
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) sa_now[j] = sa_next[j];
       }

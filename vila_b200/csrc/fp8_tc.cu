@@ -169,6 +169,7 @@ fp8_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ C
   uint64_t* drain_bar = scale_free + 2;
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(drain_bar + 1);
   volatile int* gave_up = reinterpret_cast<int*>(tmem_ptr + 1);
+  int* wides = reinterpret_cast<int*>(tmem_ptr + 2);      // [2]: whether a token's scales in a group of blocks are fp8_is_wide
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int p_tiles = ((kSwap ? p.N : p.M) + kRows - 1) / kRows, nkb = fp8_blocks(p.K);
@@ -304,14 +305,23 @@ fp8_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ C
       }
       ok = mx4_warp_wait(&scale_free[g & 1], ((g >> 1) & 1) ^ 1, gave_up, limit.tries);      // the first two pass
       if (!ok) break;
-      if (lane * 4 < S::kTokens) {
+      bool wide_x = false, wide_y = false, wide_z = false, wide_w = false;
 #pragma unroll
-        for (int i = 0; i < S::kTogether; ++i)
-          *reinterpret_cast<float4*>(scales + ((g & 1) * S::kTogether + i) * S::kTokens + lane * 4) =
-              make_float4(fp8_both_scales(a[i].x, w[i]), fp8_both_scales(a[i].y, w[i]), fp8_both_scales(a[i].z, w[i]), fp8_both_scales(a[i].w, w[i]));
+      for (int i = 0; i < S::kTogether; ++i) {
+        const float4 f = make_float4(fp8_both_scales(a[i].x, w[i]), fp8_both_scales(a[i].y, w[i]), fp8_both_scales(a[i].z, w[i]), fp8_both_scales(a[i].w, w[i]));
+        wide_x |= fp8_is_wide(f.x);
+        wide_y |= fp8_is_wide(f.y);
+        wide_z |= fp8_is_wide(f.z);
+        wide_w |= fp8_is_wide(f.w);
+        if (lane * 4 < S::kTokens) *reinterpret_cast<float4*>(scales + ((g & 1) * S::kTogether + i) * S::kTokens + lane * 4) = f;
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&scale_full[g & 1]);
+      const int t = t0 + lane * 4;
+      const bool any = __any_sync(0xffffffffu, (wide_x && t < p.M) || (wide_y && t + 1 < p.M) || (wide_z && t + 2 < p.M) || (wide_w && t + 3 < p.M));
+      if (lane == 0) {
+        wides[g & 1] = any;
+        mbar_arrive(&scale_full[g & 1]);
+      }
     }
   } else {
     griddep_wait();
@@ -319,6 +329,7 @@ fp8_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ C
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quad * 32) << 16) + c0;
     constexpr int kChunks = S::kColumns / 16;
     int v = 0, g = 0;                     // visits, groups of blocks so far
+    bool any_wide = false;
     float sum[S::kColumns];
 #pragma unroll
     for (int i = 0; i < S::kColumns; ++i) sum[i] = 0.f;
@@ -332,6 +343,7 @@ fp8_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ C
         }
         ok = mx4_warp_wait(&scale_full[g & 1], (g >> 1) & 1, gave_up, limit.tries);
         if (!ok) break;
+        any_wide = wides[g & 1] != 0;
       }
       const float* both = scales + ((g & 1) * S::kTogether + in_group) * S::kTokens + (kSwap ? c0 : row);
       float mine[kVisit];
@@ -340,6 +352,11 @@ fp8_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ C
       ok = mx4_warp_wait(&acc_full[v & 1], (v >> 1) & 1, gave_up, limit.tries);
       if (!ok) break;
       tc_fence_after();
+      if (any_wide) {      // ahead of the loop: between its blocks the branch alone would keep one's sums from the next one's loads
+#pragma unroll 1
+        for (int i = 0; i < kVisit && kb + i < kb1; ++i)
+          fp8_widen(lanes + ((v & 1) * kVisit + i) * BN, S::kColumns, [&](int c) { return both[i * S::kTokens + (kSwap ? c : 0)]; });
+      }
 #pragma unroll
       for (int i = 0; i < kVisit; ++i) {
         if (kb + i < kb1) {
