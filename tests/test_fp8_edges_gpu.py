@@ -113,3 +113,52 @@ def test_what_fp32_cannot_hold_is_an_infinity(cuda, M, N, K):
     want = base.clone()
     want[m] = torch.where(sign.to(cuda) == 0, base[m], (sign * torch.inf).to(cuda).to(BF))
     assert torch.equal(got, want) and not torch.equal(plain, base)
+
+
+def one_term(M, N, K, z, cuda):
+    """Rows and a weight whose sum of token m is z[m] times +-1 (columns' turn), exact in fp32: one number each, z a power of two."""
+    from vila_b200 import ops
+    codes, a_codes = torch.zeros(N, K), torch.zeros(M, K)
+    codes[:, K // 2], a_codes[:, K // 2] = torch.where(torch.arange(N) % 2 == 0, 1.0, -1.0), 1.0
+    a_scales = torch.full((M, -(-K // 128)), 0.5)
+    a_scales[:, K // 2 // 128] = z
+    a = ops.fp8_pack(a_codes.to(E4M3).to(cuda), a_scales.to(cuda), block_rows=1)
+    return a, ops.fp8_pack(codes.to(E4M3).to(cuda), torch.ones(-(-N // 128), a_scales.shape[1], device=cuda)), torch.outer(z.double(), codes[:, K // 2].double())
+
+
+@pytest.mark.parametrize("M, N, K", KERNELS)
+def test_small_numbers_through_xielu(cuda, M, N, K):
+    """z down to -+2^-40.  e^z - 1 - z is a_neg = 0.4 times, and near 0 the result is about z / 2.  Above -1/16 the series leaves out z^5 / 120, 2^-22 of that; from there
+    on __expf is off by at most 2 units of 2^-24 and two roundings by half a one each: 3 x 0.4 x 2^-24 of 2^-5 and more, below 2^-18; the sum's own roundings are 2^-23.
+    Then half a step of its type: bf16 2^-8, or e4m3's 2^-4 and 2^-10 of its block's scale."""
+    from vila_b200 import ops
+    z = torch.exp2(-(torch.arange(M) % 41).float())
+    a, w, sums = one_term(M, N, K, z, cuda)
+    want = torch.where(sums > 0, 0.7 * sums * sums + sums / 2, 0.4 * (torch.expm1(sums) - sums) + sums / 2)
+    args = dict(act=ops.ACT_XIELU, act_params=(0.7, 0.4))
+    got = ops.fp8_linear(a, w, **args).double().cpu()
+    assert ((got - want).abs() <= want.abs() * (2.0 ** -8 + 2.0 ** -18)).all()
+    q = ops.fp8_linear(a, w, to8=True, **args)
+    v, s = ops.fp8_dequantize(q, out_dtype=torch.float32).double().cpu(), R.per_element(q.scales.cpu(), 1, M, N)
+    assert ((v - want).abs() <= torch.maximum(want.abs() * 2.0 ** -4, s * 2.0 ** -10) * (1 + 2.0 ** -16) + want.abs() * 2.0 ** -18).all()
+
+
+@pytest.mark.parametrize("M, N, K", KERNELS)
+def test_far_negative_gates(cuda, M, N, K):
+    """silu of -16, -32, -64 and their positive ones, times u = minus the same.  __expf(x) is off by 2 + 1.2 |x| units of 2^-23, the division by 2 more and the products by half
+    one each: (5 + 1.2 |x|) 2^-23; then half a step of the result's type."""
+    from vila_b200 import ops
+    N = N // 4 * 4
+    z = torch.exp2(4.0 + torch.arange(M) % 3)
+    a, w, sums = one_term(M, N, K, z, cuda)      # gates z, ups -z
+    codes = w.codes.clone()
+    codes[2::4], codes[3::4] = codes[3::4].clone(), codes[2::4].clone()      # and the other way round
+    sums[:, 2::4], sums[:, 3::4] = -sums[:, 2::4], -sums[:, 3::4]
+    g, u = sums[:, 0::2], sums[:, 1::2]
+    want = g * torch.sigmoid(g) * u
+    more = want.abs() * (5 + 1.2 * g.abs()) * 2.0 ** -23
+    got = ops.fp8_linear(a, ops.fp8_pack(codes, w.scales), swiglu=True).double().cpu()
+    assert (want[0] != 0).all() and ((got - want).abs() <= want.abs() * 2.0 ** -8 * (1 + 2.0 ** -16) + more).all()
+    q = ops.fp8_linear(a, ops.fp8_pack(codes, w.scales), swiglu=True, to8=True)
+    v, s = ops.fp8_dequantize(q, out_dtype=torch.float32).double().cpu(), R.per_element(q.scales.cpu(), 1, *want.shape)
+    assert ((v - want).abs() <= torch.maximum(want.abs() * 2.0 ** -4, s * 2.0 ** -10) * (1 + 2.0 ** -15) + more).all()

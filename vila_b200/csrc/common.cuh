@@ -69,7 +69,8 @@ __device__ __forceinline__ float warp_max(float v) {
 }
 
 // ---- activations (shared by the GEMM / GEMV epilogues).  They divide with __fdividef, which costs less than
-// the correctly rounded division; every result is rounded to bf16 right after.
+// the correctly rounded division; every result is rounded right after, to bf16 or (8-bit rows, some by way of fp32) to e4m3.
+// __expf(x) is off by (2 + 1.2 |x|) 2^-23 of itself: 2^-16 under a gate of -80.  Gates below -87 give zero for what is less than 2^-119.
 __device__ __forceinline__ float silu_f(float x) { return __fdividef(x, 1.0f + __expf(-x)); }
 __device__ __forceinline__ float gelu_tanh_f(float x) {
   // gelu_pytorch_tanh: 0.5 x (1 + tanh( sqrt(2/pi) (x + 0.044715 x^3) ))
@@ -82,11 +83,19 @@ __device__ __forceinline__ float gelu_tanh_f(float x) {
 __device__ __forceinline__ float xielu_f(float z, float a_pos, float a_neg) {
   return z > 0.f ? fmaf(a_pos * z, z, 0.5f * z) : fmaf(a_neg, expm1f(z) - z, 0.5f * z);
 }
-// the same for epilogues whose result is rounded to bf16 right after: fast exponential, no branch
+// the same for epilogues whose result is rounded to bf16 right after: fast exponential, no branch.  Off by up to a_neg 2^-22: of small negative z, whose
+// result is about z / 2, that is more than bf16's rounding.
 __device__ __forceinline__ float xielu_fast_f(float z, float a_pos, float a_neg) {
   const float zn = fminf(z, 0.f);
   const float neg = a_neg * (__expf(zn) - 1.0f - zn), pos = a_pos * z * z;
   return fmaf(0.5f, z, z > 0.f ? pos : neg);
+}
+// the same where small negative z count, too: e^z - 1 - z by its series from -1/16 on.  Of the result, which is about z / 2 there, what the series leaves out is
+// a_neg 2^-22 at most, and __expf's error below -1/16 a_neg 2^-17.
+__device__ __forceinline__ float xielu_near_f(float z, float a_pos, float a_neg) {
+  float y = __expf(z) - 1.0f - z;
+  if (z > -0.0625f) y = 0.5f * z * z * fmaf(z, fmaf(z, 1.f / 12, 1.f / 3), 1.f);
+  return fmaf(0.5f, z, z > 0.f ? a_pos * z * z : a_neg * y);
 }
 // clamped gated unit: g = min(zg, limit), u = clamp(zu, +-limit): g sigmoid(alpha g) (u + 1)
 __device__ __forceinline__ float glu_clamp_fast_f(float zg, float zu, float alpha, float limit) {

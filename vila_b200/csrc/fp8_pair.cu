@@ -263,7 +263,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
           uint32_t top = 0;
 #pragma unroll
           for (int i = 0; i < kOut; ++i) {
-            const float v = kGated ? mx4_glu<EPI>(z[2 * i % 128], z[(2 * i + 1) % 128], x) : mx4_act<EPI>(z[i], x);
+            const float v = kGated ? mx4_glu<EPI>(z[2 * i % 128], z[(2 * i + 1) % 128], x) : mx4_act<EPI, true>(z[i], x);
             z[i] = o0 + i < cols ? v : 0.f;
             top = max(top, __float_as_uint(z[i]) & 0x7fffffffu);
           }

@@ -71,7 +71,7 @@ template <int BN, bool kSwap> struct Shape {
 };
 
 // kSwap: what becomes of the sums of token m, weight rows n .. n + 3 (n a multiple of 4).  out32: unrounded, rows of ld32 columns.  `wide`: four
-// results of out lie on an 8-byte boundary.  The fast exponentials are off by some 2^-21, under either rounding that follows.
+// results of out lie on an 8-byte boundary.  The fast exponentials' error is under either rounding that follows (common.cuh has it).
 template <int EPI>
 __device__ __forceinline__ void finish(const vila_fp8_linear_params& p, const vila_glinear_ext& x, float* out32, int ld32, bool wide, int m, int n, float4 sums) {
   constexpr bool kGated = EPI >= kMx4Gated;
@@ -85,7 +85,7 @@ __device__ __forceinline__ void finish(const vila_fp8_linear_params& p, const vi
       if (n + j < p.N) z[j] += __bfloat162float(bias[j]);
   }
 #pragma unroll
-  for (int j = 0; j < kOut; ++j) z[j] = kGated ? mx4_glu<EPI>(z[2 * j % 4], z[(2 * j + 1) % 4], x) : mx4_act<EPI>(z[j], x);
+  for (int j = 0; j < kOut; ++j) z[j] = kGated ? mx4_glu<EPI>(z[2 * j % 4], z[(2 * j + 1) % 4], x) : mx4_act<EPI, true>(z[j], x);
   const int cols = kGated ? p.N / 2 : p.N, o = kGated ? n / 2 : n;
   if (out32 != nullptr) {
 #pragma unroll
@@ -120,7 +120,7 @@ __device__ __forceinline__ void finish_rows(const vila_fp8_linear_params& p, con
       for (int i = 0; i < 32; ++i) z[i] += n + i < p.N ? __bfloat162float(bias[n + i]) : 0.f;
     }
 #pragma unroll
-    for (int i = 0; i < kOut; ++i) z[i] = kGated ? mx4_glu<EPI>(z[2 * i % 32], z[(2 * i + 1) % 32], x) : mx4_act<EPI>(z[i], x);
+    for (int i = 0; i < kOut; ++i) z[i] = kGated ? mx4_glu<EPI>(z[2 * i % 32], z[(2 * i + 1) % 32], x) : mx4_act<EPI, true>(z[i], x);
     if (out32 == nullptr && wide && o + kOut <= cols) {
       if (m < end) {
         uint32_t h[kOut / 2];
@@ -475,7 +475,7 @@ fp8_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ C
 #pragma unroll
               for (int j = 0; j < (kGated ? 2 : 1); ++j) z[j] += __bfloat162float(bias[kGated ? 2 * o + j : o]);
             }
-            const float v = kGated ? mx4_glu<EPI>(z[0], z[1], x) : mx4_act<EPI>(z[0], x);
+            const float v = kGated ? mx4_glu<EPI>(z[0], z[1], x) : mx4_act<EPI, true>(z[0], x);
             if (out32 != nullptr) out32[static_cast<size_t>(m) * ld32 + o] = v;
             else static_cast<__nv_bfloat16*>(p.out)[static_cast<size_t>(m) * p.ldo + o] = __float2bfloat16_rn(v);
           }

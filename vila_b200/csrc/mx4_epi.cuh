@@ -1,5 +1,6 @@
 // What the tcgen05 kernels on microscaled rows do with their sums: bias, activation or gated unit, bf16.
 #pragma once
+#include <type_traits>
 #include "../../include/vila_b200.h"
 #include "common.cuh"
 #include "glinear_epi.cuh"
@@ -25,12 +26,13 @@ __device__ __forceinline__ void mx4_with_epilogue(const P& p, F&& f) {      // P
 }
 
 // The activations with __expf and __fdividef: their results are rounded to bf16 right after, and under the unpacking of weights
-// or a few clocks of products per output the exact ones showed (2048 x 37888 x 3584 with a gated unit: 545 us).
-template <int EPI>
+// or a few clocks of products per output the exact ones showed (2048 x 37888 x 3584 with a gated unit: 545 us).  kNear: small negative z count
+// by themselves (layers on 8-bit rows, whose result may have a scale of its own).
+template <int EPI, bool kNear = false>
 __device__ __forceinline__ float mx4_act(float z, const vila_glinear_ext& x) {
   if (EPI == VILA_ACT_SILU) return silu_f(z);
   if (EPI == VILA_ACT_GELU_TANH) return gelu_tanh_f(z);
-  if (EPI == VILA_ACT_XIELU) return xielu_fast_f(z, x.act_pos, x.act_neg);
+  if (EPI == VILA_ACT_XIELU) return kNear ? xielu_near_f(z, x.act_pos, x.act_neg) : xielu_fast_f(z, x.act_pos, x.act_neg);
   return activate(z, EPI, x);
 }
 template <int EPI>
@@ -49,7 +51,7 @@ __device__ __forceinline__ void mx4_stg32(void* p, const uint32_t* h) {
 // Lane = output row (token), 32 columns n .. n + 31 of the sums.  `wide`: rows of out start on 32-byte boundaries.
 template <int EPI, typename P>
 __device__ __forceinline__ void mx4_store_row(const P& p, const vila_glinear_ext& x, float (&z)[32], int m, int n, bool wide) {
-  constexpr bool kGated = EPI >= kMx4Gated;
+  constexpr bool kGated = EPI >= kMx4Gated, kNear = !std::is_same<P, vila_mx4_linear_params>::value;
   constexpr int kWords = kGated ? 8 : 16;
   if (p.bias != nullptr) {
     const __nv_bfloat16* bias = static_cast<const __nv_bfloat16*>(p.bias);
@@ -62,7 +64,7 @@ __device__ __forceinline__ void mx4_store_row(const P& p, const vila_glinear_ext
 #pragma unroll
   for (int i = 0; i < kWords; ++i) {
     if constexpr (kGated) h[i] = pack_bf16(mx4_glu<EPI>(z[4 * i], z[4 * i + 1], x), mx4_glu<EPI>(z[4 * i + 2], z[4 * i + 3], x));
-    else h[i] = pack_bf16(mx4_act<EPI>(z[2 * i], x), mx4_act<EPI>(z[2 * i + 1], x));
+    else h[i] = pack_bf16(mx4_act<EPI, kNear>(z[2 * i], x), mx4_act<EPI, kNear>(z[2 * i + 1], x));
   }
   const int o = kGated ? n / 2 : n, end = kGated ? p.N / 2 : p.N;
   __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out) + static_cast<size_t>(m) * p.ldo + o;
