@@ -3,6 +3,7 @@ llava.Image / llava.Video / text -> model.generate_content(prompt, response_form
 import argparse
 import importlib.util
 import os
+import warnings
 
 import llava
 from llava import conversation as clib
@@ -35,7 +36,7 @@ def main(argv=None) -> str:
     parser.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
     parser.add_argument("--weights", choices=["mx4", "fp8"], default=None,
                         help="hold the layers' weights in microscaled 4-bit numbers, or in 8-bit floating point; for a VILA "
-                             "checkpoint fp8 runs prompts in 8 bits")
+                             "checkpoint fp8 runs prompts in 8 bits and mx4 does nothing")
     parser.add_argument("--temperature", type=float, default=0.0, help="0: greedy")
     parser.add_argument("--top-k", type=int, default=0)
     parser.add_argument("--top-p", type=float, default=1.0)
@@ -62,7 +63,7 @@ def main(argv=None) -> str:
         response_format = ResponseFormat(type="json_schema", json_schema=JsonSchemaResponseFormat(
             schema=get_schema_from_python_path(args.json_schema)))
     if args.weights == "mx4":
-        raise SystemExit("--weights mx4 is for token-id language models")
+        warnings.warn("--weights mx4 is for token-id language models: this checkpoint's weights stay bfloat16")
     model = llava.load(args.model_path, model_base=None)
     if args.weights == "fp8":
         model.llm.prefill_in_fp8()

@@ -121,3 +121,20 @@ def test_a_prompts_weights_are_fetched_ahead_once_they_were_waited_for(llm, monk
     monkeypatch.setattr(torch.cuda, "synchronize", lambda *a: waited.append((len(made), any(q.static_w for q in made))))
     eights = llm.prefill_in_fp8()._fp8_weights()
     assert waited == [(0, False), (8, False)] and all(q.static_w for qs in eights for q in qs)
+
+
+@pytest.mark.parametrize("weights, asked, told", [(None, 0, False), ("fp8", 1, False), ("mx4", 0, True)])
+def test_weights_of_a_vision_language_checkpoint(monkeypatch, tmp_path, capsys, weights, asked, told):
+    """fp8 runs its prompts in 8 bits; mx4, which it never had, is accepted as it always was, and says that it does nothing."""
+    import warnings
+    from types import SimpleNamespace
+    from llava.cli import infer
+    calls = []
+    fake = SimpleNamespace(llm=SimpleNamespace(prefill_in_fp8=lambda: calls.append("fp8")), config=SimpleNamespace(),
+                           generate_content=lambda prompt, response_format=None: "an answer")
+    monkeypatch.setattr(infer.llava, "load", lambda path, model_base=None: fake)
+    with warnings.catch_warnings(record=True) as seen:
+        warnings.simplefilter("always")
+        got = infer.main(["--model-path", str(tmp_path), "--text", "hello"] + (["--weights", weights] if weights else []))
+    assert got == "an answer" and "an answer" in capsys.readouterr().out
+    assert calls == ["fp8"] * asked and any("token-id language models" in str(w.message) for w in seen) == told
