@@ -138,3 +138,13 @@ def test_weights_of_a_vision_language_checkpoint(monkeypatch, tmp_path, capsys, 
         got = infer.main(["--model-path", str(tmp_path), "--text", "hello"] + (["--weights", weights] if weights else []))
     assert got == "an answer" and "an answer" in capsys.readouterr().out
     assert calls == ["fp8"] * asked and any("token-id language models" in str(w.message) for w in seen) == told
+
+
+def test_weights_are_copied_whole():
+    import copy
+    part = ops.Fp8(torch.zeros(64, 64).to(torch.float8_e4m3fn), torch.ones(1, 1), 128)
+    for w in (part, ops.Fp8Kept(part, torch.zeros(8, 64).bfloat16())):
+        w.static_w = True
+        for other in (copy.deepcopy(w), copy.copy(w)):
+            assert type(other) is type(w) and other.shape == w.shape and other.static_w
+            assert torch.equal(getattr(other, "part", other).codes.float(), part.codes.float())

@@ -1593,15 +1593,7 @@ class Fp8Kept(Fp8):
 
     def __init__(self, part: Fp8, kept: torch.Tensor):
         self.part, self.kept = part, kept
-        self.rows, self.cols, self.block_rows = part.rows + kept.shape[0], part.cols, part.block_rows
-
-    @property
-    def static_w(self) -> bool:
-        return self.part.static_w
-
-    @static_w.setter
-    def static_w(self, on: bool) -> None:
-        self.part.static_w = on
+        self.rows, self.cols, self.block_rows, self.static_w = part.rows + kept.shape[0], part.cols, part.block_rows, part.static_w
 
     def _held(self) -> torch.Tensor:
         return self.part._held()
@@ -1810,6 +1802,7 @@ def fp8_linear(a, w: Fp8, bias: Optional[torch.Tensor] = None, *, act: int = ACT
         _fp8_check(not flags or (n % 2 == 0 and N % 2 == 0), "a gated unit has an even number of weight rows, in 8 bits and kept")
         cut = n // 2 if flags else n
         more = dict(act=act, act_params=act_params, swiglu=swiglu, geglu=geglu, glu_clamp=glu_clamp)
+        w.part.static_w = w.static_w
         fp8_linear(a, w.part, None if bias is None else bias[:n], out=out[:, :cut], **more)
         rest, to = None if bias is None else bias[n:], out[:, cut:]
         if (act == ACT_NONE and not flags and K % 8 == 0 and (N - n) % 8 == 0 and a.stride(0) % 8 == 0 and a.stride(0) >= K and a.data_ptr() % 16 == 0
