@@ -960,10 +960,10 @@ int vila_mx4_linear_tries(const vila_mx4_linear_params* p, int tries, void* stre
  * vila_fp8_quantize: x [rows, cols] (VILA_DT_*, row stride ldx elements) -> codes, scales.  Per block with largest magnitude m: scale =
  *   max(m / 448, 2^-126), code = x * (1 / scale) rounded to the nearest e4m3 number, ties to even (quotients and product rounded to fp32).  A
  *   block with an infinity or a NaN: a NaN for its scale, codes 0.
- * vila_fp8_dequantize: out[r, c] = number of the code * scale, rounded once to out_dtype (code 0x7f or 0xff: NaN).
+ * vila_fp8_dequantize: out[r, c] = number of the code * scale in fp32, rounded to out_dtype (code 0x7f or 0xff: NaN).
  * vila_fp8_rmsnorm: the norm before a layer whose rows are 8-bit numbers.  s = x + residual, rounded to x's type (residual NULL: s = x); codes
  *   and scales (block_rows 1) of s / sqrt(mean(s^2) + eps) * w, unrounded fp32 (w NULL: 1).  With a residual s is written to sum (x's type, row
- *   stride ld_sum; it may be x itself, in place).  At most 32768 columns. */
+ *   stride ld_sum; it may be x itself, in place, and does not overlap x or residual otherwise).  At most 32768 columns. */
 int vila_fp8_quantize(const void* x, int x_dtype, int64_t ldx, void* codes, int64_t ldc, float* scales, int64_t lds, int rows, int cols,
                       int block_rows, void* stream);
 int vila_fp8_dequantize(const void* codes, int64_t ldc, const float* scales, int64_t lds, void* out, int out_dtype, int64_t ldo, int rows,

@@ -4,8 +4,8 @@
 // block of a row: its largest magnitude takes three shuffles, and the numbers wait in registers for it.  Data are read once.
 //
 // Rows of 16470 x 3584 bf16: 31.4 us in a captured graph, 27.3 at the rate of a copy; a weight of 37888 x 3584: 62.3 us, 62.3 at that rate.
-// The norm issues on 71 % of its clocks and writes most: 16470 x 3584 with a residual 67 us, 6.1 TB/s; of 2048 rows 12.1 us, 7.9 at a copy's
-// rate.  A single row is 1.3 us, and the call 13: the host's.
+// The norm of 16470 x 3584 with a residual 67 us, 6.1 TB/s; of 2048 rows 12.1 us, 7.9 at a copy's rate: 2.3 rounds of CTAs, which each load x and the
+// residual, meet, and then load the norm's weights.  A single row is 1.3 us, and the call 13: the host's.
 #include "../../include/vila_b200.h"
 #include "fp8.cuh"
 #include "dtype_any.cuh"

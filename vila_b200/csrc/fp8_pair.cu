@@ -8,8 +8,8 @@
 // instructions, and what a warp does for a block one after another some 900 - 1000: a wait 150 - 250 even if it is over, 16 columns of
 // TMEM 70.
 //
-// 2048 x 37888 x 3584 runs at 1.69 PFLOP/s over seconds, 8192 x 8192 x 8192 at 1.81, both at some 1.5 GHz under the power limit (a copy that
-// fetched no sums, for timing: 2.07 and 2.20 at 1.4 GHz, so that at most a fifth is left).  Tried and slower or even: registers moved to the
+// 2048 x 37888 x 3584 runs at 1.71 PFLOP/s over seconds, 8192 x 8192 x 8192 at 1.84, both at some 1.5 - 1.6 GHz under the power limit (a copy that
+// fetched no sums, for timing: 2.05 and 2.21, so that at most a fifth is left).  Tried and slower or even: registers moved to the
 // epilogue (by 8 %), 16 epilogue warps, 32 columns a TMEM load, scales staged by warps of their own, lane 0 alone polling (116 us for 75).
 //
 // A result in 8 bits is made in the epilogue: a thread has 128 columns of a row, a block of it, or behind a gated unit half a block, and learns
@@ -193,7 +193,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) sa_now[j] = j < nkb ? sa[j * p.ld_as] : 0.f;
       float w_now = lane < nkb ? sw[lane] : 0.f;      // of 32 blocks, one a lane
-      // a block's factor, and whether any lane's is wide: made while the block before is fetched from TMEM
+      // a block's factor, and whether any lane's is wide: made while the block before is fetched from TMEM (in line with it the test took 3 - 4 %)
       float both = fp8_both_scales(sa_now[0], __shfl_sync(0xffffffffu, w_now, 0));
       bool any_wide = __any_sync(0xffffffffu, fp8_is_wide(both));
 #pragma unroll 1
@@ -320,7 +320,8 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
 
 }  // namespace
 
-// By rounds through the GPU: of 3584 columns a round of pairs takes 17.5 us, one of single CTAs' tiles of 128 x 128 (fp8_tc.cu) 13.4, us against us:
+// By rounds through the GPU, rows of padding counted as rows; measured at 3584 columns only.  There a round of pairs takes 17.5 us, one of single CTAs'
+// tiles of 128 x 128 (fp8_tc.cu) 13.4, us against us:
 // 600 rows of 1152 weight rows 19.6 and 11.6, 512 of 4608 20.5 and 14.7 (one round each), 600 of 4608 20.8 and 26.7 (one and two), 300 of 18944
 // 39.3 and 43.5, 1536 of 3584 37.2 and 40.5 (two and three), 1024 of 18944 73.6 and 112.8.
 bool fp8_pair_takes(const vila_fp8_linear_params& p) {

@@ -501,7 +501,7 @@ int launch(const vila_fp8_linear_params& p, const vila_glinear_ext& x, float* ou
   VB_CHECK(tiles < (1LL << 27), "fp8_linear: too many tiles (M=%d N=%d)", p.M, p.N);
   static Mx4Clusters clusters;
   // As many CTAs a tile, a power of two up to 8, as the GPU holds clusters for at once.  The occupancy that CUDA reports counts one CTA an SM
-  // where two fit (15 clusters of 8); the GPU holds both (64 rows of 3584 x 18944 by 8: 25.5 us, by 4, as reported, 33.6).
+  // where two fit (15 clusters of 8); the GPU holds both (64 rows of 3584 x 18944 by 4: 25.5 us, by 2, as reported, 33.6).
   // Of 4 blocks a cluster's joint end costs what it saves (77 rows of 1157 x 512: 7.2 us by two, 6.2 alone; x 1024 by 4 7.1, by 2 8.0).
   const int blocks = fp8_blocks(p.K), limit = blocks < 8 ? 1 : blocks / 2;
   int split = 1;
